@@ -316,10 +316,18 @@ def causal_conv1d(x, weight, bias=None, activation="silu", initial_state=None):
 
 
 # ---- attention -------------------------------------------------------------
-def softmax_attention(q, k, v, scale=None, causal=True, q_offset: int = 0, window=None):
+def softmax_attention(q, k, v, scale=None, causal=True, q_offset: int = 0, window=None, *, softcap=None, slopes=None, key_first=None,
+                      key_stop=None):
+    """Grouped-query attention, q ``[B,Tq,Hq,D]`` on k / v ``[B,Tk,Hkv,D]``.  The options cap the scores, bias them by distance and limit the keys that a
+    query sees (packed documents, prefixes, padding): :mod:`.scored_attn`."""
+    if softcap is not None or slopes is not None or key_first is not None or key_stop is not None:
+        return scored_attention(q, k, v, scale, causal, q_offset, window, softcap, slopes, key_first, key_stop)
     if _cuda(q):
         return _K().flash_attention(q, k, v, scale, causal, q_offset, window)
     return R.softmax_attention(q, k, v, scale, causal, q_offset, window)
+
+
+from .scored_attn import document_first, prefix_stop, scored_attention   # noqa: E402,F401
 
 
 # ---- packed-row operators (serving only) -----------------------------------------------------------

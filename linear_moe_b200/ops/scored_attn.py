@@ -1,0 +1,188 @@
+"""Softmax attention with capped scores, a bias by distance and a range of visible keys per query.
+
+    x_ij = cap tanh(scale q_i k_j / cap) - slope_h |p_i - j|        p_i = q_offset + i
+    o_i  = sum_j softmax_j(x_ij) v_j   over the keys  key_first_i <= j < key_stop_i  that causality and the window leave too
+
+A query that sees no key gives zeros and passes no gradient.  One interval per query describes packed documents
+(:func:`document_first`), prefixes that see themselves whole and padded batches (:func:`prefix_stop`).
+
+bf16 and fp16 CUDA tensors with heads of up to 128, in multiples of 8, run the tcgen05 kernels of ``csrc/flash_attn_tc.cuh``; others (fp32, CPU,
+wider heads) run the eager definition :func:`linear_moe_b200.ref.ops.softmax_attention`.  Slopes and ranges get no gradient.  Hidden keys and
+values have to be finite, as for the eager form: a weight of zero times NaN is NaN.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from ..ref import ops as R
+
+MAX_QUERIES = 1 << 20          # what the dk / dv kernel's list of query tiles holds
+
+
+def on_device(t: torch.Tensor):
+    """Launches go to the current device's stream: makes it the tensor's device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+# ---- ranges ---------------------------------------------------------------------------------------------------------------------
+def document_first(tokens: torch.Tensor, end_token: int) -> torch.Tensor:
+    """First token of every position's document, int32 ``[B, T]``, where ``end_token`` closes a document (its own position belongs to the
+    document that it ends): ``key_first`` of causal attention inside documents."""
+    T = tokens.shape[-1]
+    at = torch.arange(T, device=tokens.device, dtype=torch.int32)
+    starts = torch.where(tokens == end_token, at + 1, torch.zeros_like(at))
+    first = torch.cummax(starts, dim=-1).values
+    return torch.cat([torch.zeros_like(first[..., :1]), first[..., :-1]], dim=-1).contiguous()
+
+
+def prefix_stop(T: int, prefix: Sequence[int], lengths: Optional[Sequence[int]] = None, device=None) -> torch.Tensor:
+    """Key behind the last visible one, int32 ``[B, T]``, for sequences whose first ``prefix[b]`` tokens see one another and whose later tokens
+    are causal (``causal=False``, the range says it all).  Positions from ``lengths[b]`` on are padding: they see nothing and nobody sees
+    them."""
+    at = torch.arange(T, device=device, dtype=torch.int32)[None]
+    p = torch.as_tensor(prefix, dtype=torch.int32, device=device)[:, None]
+    stop = torch.maximum(at + 1, p)
+    if lengths is not None:
+        n = torch.as_tensor(lengths, dtype=torch.int32, device=device)[:, None]
+        stop = torch.where(at < n, torch.minimum(stop, n), torch.zeros_like(stop))
+    return stop.contiguous()
+
+
+def _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, key_stop):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("attention takes q [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")
+    if k.shape[:3] != v.shape[:3] or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not go together")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"{q.shape[2]} query heads do not share {k.shape[2]} key/value heads evenly")
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise ValueError("q, k and v have one type and lie on one device")
+    _check_scores(q, q.shape[2], scale, softcap, slopes)
+    if window is not None and not (causal and window >= 1):
+        raise ValueError("a window is a positive number of keys of causal attention")
+    for name, r in (("key_first", key_first), ("key_stop", key_stop)):
+        if r is None:
+            continue
+        if r.dtype != torch.int32 or r.shape != q.shape[:2] or r.device != q.device:
+            raise ValueError(f"{name} is an int32 tensor [B, Tq] = {tuple(q.shape[:2])} on {q.device}")
+
+
+def _check_scores(q, heads, scale, softcap, slopes):
+    if scale is not None and not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale {scale}")
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise ValueError(f"soft cap {softcap}")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or slopes.device != q.device or slopes.requires_grad):
+        raise ValueError(f"slopes are {heads} fp32 numbers on {q.device} without a gradient, one per query head")
+
+
+# ---- binding --------------------------------------------------------------------------------------------------------------------
+class _Ranges(ctypes.Structure):
+    _fields_ = ([("first", ctypes.c_void_p), ("stop", ctypes.c_void_p), ("first_b", ctypes.c_longlong), ("stop_b", ctypes.c_longlong)] +
+                [("slopes", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("cap", ctypes.c_float), ("causal", ctypes.c_int), ("d", ctypes.c_int)])
+
+
+_SIZES = [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "q_offset", "window")] + [("scale", ctypes.c_float), ("err", ctypes.c_void_p), ("x", _Ranges)]
+
+
+class _Args(ctypes.Structure):
+    _fields_ = [("out", ctypes.c_void_p), ("lse", ctypes.c_void_p)] + _SIZES
+
+
+class _BwdArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("lse", "delta", "dq", "dk", "dv")] + _SIZES
+
+
+def _strides(t: torch.Tensor):
+    """Element strides (batch, token, head) of a tensor that a tensor map can describe, or None.  The stride of a dimension of one is
+    never used, whatever the tensor says: it gets the one of a dense tensor."""
+    if t.stride(3) != 1 or t.data_ptr() % 16:
+        return None
+    out, dense = [0, 0, 0], t.shape[3]
+    for i in (2, 1, 0):
+        s = t.stride(i) if t.shape[i] > 1 else dense
+        if s <= 0 or s % 8 or s >= 1 << 38:
+            return None
+        out[i], dense = s, dense * t.shape[i]
+    return (ctypes.c_longlong * 3)(*out)
+
+
+def _laid_out(t: torch.Tensor):
+    s = _strides(t)
+    if s is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = _strides(t)
+    return t, s
+
+
+def _fill(a, q, k, cfg, first, stop, slopes, tiles):
+    from . import gemm
+    scale, causal, q_offset, window, cap = cfg
+    a.B, a.Tq, a.Hq, a.Tk, a.Hkv = q.shape[0], q.shape[1], q.shape[2], k.shape[1], k.shape[2]
+    a.q_offset, a.window, a.scale, a.err = q_offset, window, scale, gemm._err(q.device).data_ptr()
+    x = a.x
+    if first is not None:
+        x.first, x.first_b = first.data_ptr(), first.stride(0)
+    if stop is not None:
+        x.stop, x.stop_b = stop.data_ptr(), stop.stride(0)
+    if slopes is not None:
+        x.slopes = slopes.data_ptr()
+    x.tiles, x.cap, x.causal, x.d = tiles.data_ptr(), cap, causal, q.shape[3]
+
+
+class ScoredAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, first, stop, slopes, cfg):
+        from . import cuda as K
+        B, Tq, Hq, D = q.shape
+        (q, qs), (k, ks), (v, vs) = _laid_out(q), _laid_out(k), _laid_out(v)
+        out = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device)
+        tiles = torch.empty(B, -(-Tq // 128), 4, dtype=torch.int32, device=q.device)
+        a = _Args()
+        a.out, a.lse = out.data_ptr(), lse.data_ptr()
+        _fill(a, q, k, cfg, first, stop, slopes, tiles)
+        f = K.lib().lmoe_scored_attn_fwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_fwd_fp16
+        with on_device(q):
+            K._check(f(K._p(q), qs, K._p(k), ks, K._p(v), vs, ctypes.byref(a), K._st()), "scored_attn_fwd")
+        ctx.save_for_backward(q, k, v, first, stop, slopes, out, lse, tiles)
+        ctx.cfg = cfg
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        from . import cuda as K
+        q, k, v, first, stop, slopes, out, lse, tiles = ctx.saved_tensors
+        d_out = d_out.contiguous()
+        if d_out.data_ptr() % 16:
+            d_out = d_out.clone()
+        dq, delta = torch.empty_like(out), torch.empty_like(lse)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dv = torch.empty_like(dk)
+        a = _BwdArgs()
+        a.lse, a.delta, a.dq, a.dk, a.dv = lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        _fill(a, q, k, ctx.cfg, first, stop, slopes, tiles)
+        f = K.lib().lmoe_scored_attn_bwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_bwd_fp16
+        with on_device(q):
+            K._check(f(K._p(q), _strides(q), K._p(k), _strides(k), K._p(v), _strides(v), K._p(out), K._p(d_out), K._p(delta), ctypes.byref(a), K._st()),
+                     "scored_attn_bwd", 3)
+        return dq, dk, dv, None, None, None, None
+
+
+def scored_attention(q, k, v, scale=None, causal: bool = True, q_offset: int = 0, window: Optional[int] = None, softcap: Optional[float] = None,
+                     slopes: Optional[torch.Tensor] = None, key_first: Optional[torch.Tensor] = None, key_stop: Optional[torch.Tensor] = None):
+    """See the module; what ``ops.softmax_attention`` calls when it is given one of the last four."""
+    _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, key_stop)
+    D = q.shape[3]
+    kernel = (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and v.shape[3] == D and D <= 128 and D % 8 == 0 and q.shape[1] <= MAX_QUERIES)
+    if not kernel or min(q.numel(), k.numel()) == 0:
+        return R.softmax_attention(q, k, v, scale, causal, q_offset, window, softcap, slopes, key_first, key_stop)
+    row = lambda r: None if r is None else r if r.stride(1) == 1 or r.shape[1] == 1 else r.contiguous()       # noqa: E731
+    cfg = (float(scale) if scale is not None else D ** -0.5, int(bool(causal)), int(q_offset), int(window or 0), float(softcap or 0.0))
+    return ScoredAttention.apply(q, k, v, row(key_first), row(key_stop), None if slopes is None else slopes.contiguous(), cfg)

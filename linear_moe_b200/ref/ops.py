@@ -139,10 +139,13 @@ def apply_rope(x, cos, sin, interleaved: bool = False):
 
 # ---- softmax attention -----------------------------------------------------
 def softmax_attention(q, k, v, scale: Optional[float] = None, causal: bool = True, q_offset: int = 0,
-                      window: Optional[int] = None):
+                      window: Optional[int] = None, softcap: Optional[float] = None, slopes=None, key_first=None, key_stop=None):
     """Naive attention with GQA.  q ``[B,Tq,Hq,D]``, k/v ``[B,Tk,Hkv,D(v)]``.  ``q_offset`` is the
     absolute position of q[0] relative to k[0] (sequence-parallel ranks hold a suffix of the keys'
-    positions; dot_product_attention.py:139-183 is the unfused form this replaces)."""
+    positions; dot_product_attention.py:139-183 is the unfused form this replaces).
+
+    ``softcap``: scores become ``cap tanh(score / cap)``; ``slopes`` ``[Hq]``: minus slope times the distance of query and key; ``key_first`` /
+    ``key_stop`` int ``[B, Tq]``: query i sees keys ``first <= j < stop`` at most, and zeros come out where that leaves none."""
     B, Tq, Hq, D = q.shape
     Tk, Hkv = k.shape[1], k.shape[2]
     scale = D ** -0.5 if scale is None else scale
@@ -150,14 +153,29 @@ def softmax_attention(q, k, v, scale: Optional[float] = None, causal: bool = Tru
     kf = k.float().repeat_interleave(rep, dim=2)
     vf = v.float().repeat_interleave(rep, dim=2)
     s = torch.einsum("bihd,bjhd->bhij", q.float() * scale, kf)
+    i = torch.arange(Tq, device=q.device)[:, None] + q_offset
+    j = torch.arange(Tk, device=q.device)[None, :]
+    if softcap is not None:
+        s = softcap * torch.tanh(s / softcap)
+    if slopes is not None:
+        s = s - slopes.float()[:, None, None] * (i - j).abs().float()
     if causal:
-        i = torch.arange(Tq, device=q.device)[:, None] + q_offset
-        j = torch.arange(Tk, device=q.device)[None, :]
         m = j <= i
         if window is not None:
             m = m & (j > i - window)
         s = s.masked_fill(~m, float("-inf"))
-    p = torch.softmax(s, dim=-1)
+    if key_first is None and key_stop is None and softcap is None and slopes is None:
+        p = torch.softmax(s, dim=-1)
+        return torch.einsum("bhij,bjhd->bihd", p, vf).to(q.dtype)
+    if key_first is not None:
+        s = s.masked_fill((j < key_first[:, :, None])[:, None], float("-inf"))
+    if key_stop is not None:
+        s = s.masked_fill((j >= key_stop[:, :, None])[:, None], float("-inf"))
+    if Tk == 0:
+        return torch.einsum("bhij,bjhd->bihd", s, vf).to(q.dtype)
+    top = s.detach().amax(-1, keepdim=True)
+    e = (s - top.masked_fill(top == float("-inf"), 0.0)).exp()
+    p = e / e.sum(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).tiny)
     return torch.einsum("bhij,bjhd->bihd", p, vf).to(q.dtype)
 
 
