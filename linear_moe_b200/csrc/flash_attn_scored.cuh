@@ -19,7 +19,7 @@ static int scored_fwd_any(const void* q, const long long* qs, const void* k, con
 template <bool H>
 static int scored_bwd_any(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const void* o,
                           const void* d_o, float* delta, const BwdArgs& a, cudaStream_t st) {
-    if (!scored_args_ok(a.x, a.B, a.Tq, a.Tk, a.Hq, a.Hkv)) return -1;
+    if (!scored_args_ok(a.x, a.B, a.Tq, a.Tk, a.Hq, a.Hkv) || a.x.low == nullptr) return -1;
     if (a.x.cap > 0.f) return scored_bwd<SCORE_CAP, H>(q, qs, k, ks, v, vs, o, d_o, delta, a, st);
     if (a.x.slopes != nullptr) return scored_bwd<SCORE_BIAS, H>(q, qs, k, ks, v, vs, o, d_o, delta, a, st);
     return scored_bwd<SCORE_PLAIN, H>(q, qs, k, ks, v, vs, o, d_o, delta, a, st);

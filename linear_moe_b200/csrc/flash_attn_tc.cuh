@@ -42,6 +42,7 @@ struct Ranges {
     const int *first, *stop;              // [B, Tq] with strides (first_b, 1), (stop_b, 1); null: 0 and Tk
     long long first_b, stop_b;
     const float* slopes;                  // [Hq]; null: no bias
+    bf16* low;                            // [B, Tq, Hq, d]: what the output's rounding took away, rounded itself; null: not wanted
     int4* tiles;                          // [B, query tiles]: union of the rows' intervals, then their intersection
     float cap;
     int causal, d;                        // d: head size, a multiple of 8 up to D (tensor maps fill the rest with zeros)
@@ -66,6 +67,10 @@ template <class F> __device__ __forceinline__ uint32_t pack16(float a, float b) 
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     } else return pack_bf16(a, b);
+}
+template <class F> __device__ __forceinline__ float2 unpack16(uint32_t x) {
+    if constexpr (F::HALF) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
 }
 // operand types of the instruction descriptor: bits 7 and 10 set for bf16, clear for fp16
 template <class F, bool B_MN, int N> __host__ __device__ constexpr uint32_t idesc_of() {
@@ -399,7 +404,7 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (row < a.Tq) {
             const float inv = l > 0.f ? 1.f / l : 0.f;
             const int d = F::RANGES ? a.x.d : D;
-            bf16* og = a.out + (((long long)b * a.Tq + row) * a.Hq + h) * d + quarter * OW;
+            const long long at = (((long long)b * a.Tq + row) * a.Hq + h) * d + quarter * OW;
 #pragma unroll
             for (int c = 0; c < OW; c += 8) {
                 if (F::RANGES && quarter * OW + c >= d) break;
@@ -408,7 +413,20 @@ fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 y.y = pack16<F>(o[c + 2] * inv, o[c + 3] * inv);
                 y.z = pack16<F>(o[c + 4] * inv, o[c + 5] * inv);
                 y.w = pack16<F>(o[c + 6] * inv, o[c + 7] * inv);
-                *reinterpret_cast<uint4*>(og + c) = y;
+                *reinterpret_cast<uint4*>(a.out + at + c) = y;
+                if constexpr (F::RANGES) {
+                    // delta = do . o is subtracted from dp, nearly its equal where one weight is large: with the rounded o alone dq and dk were off by 0.0042
+                    // at scores of 6 in root mean square, with this part 0.0025 (their own rounding: 0.0017)
+                    if (a.x.low != nullptr) {
+                        const float2 y0 = unpack16<F>(y.x), y1 = unpack16<F>(y.y), y2 = unpack16<F>(y.z), y3 = unpack16<F>(y.w);
+                        uint4 z;
+                        z.x = pack16<F>(o[c] * inv - y0.x, o[c + 1] * inv - y0.y);
+                        z.y = pack16<F>(o[c + 2] * inv - y1.x, o[c + 3] * inv - y1.y);
+                        z.z = pack16<F>(o[c + 4] * inv - y2.x, o[c + 5] * inv - y2.y);
+                        z.w = pack16<F>(o[c + 6] * inv - y3.x, o[c + 7] * inv - y3.y);
+                        *reinterpret_cast<uint4*>(a.x.low + at + c) = z;
+                    }
+                }
             }
             const float unit = F::SCORE == SCORE_PLAIN ? a.scale : 1.f / LOG2E;
             if (quarter == 0) a.lse[((long long)b * a.Hq + h) * a.Tq + row] = l > 0.f ? mm * unit + logf(l) : -INFINITY;
@@ -939,29 +957,42 @@ fa_bwd_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
 }
 
-// delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d].  Bound by reading both tensors once: D / 8 lanes take a row 16 bytes at a time, and a thread asks
-// for its pieces of four rows before it uses the first (a warp per row with 4-byte loads had too little in flight).
+// delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d] (with RANGES (O + low)).  Bound by reading the tensors once: D / 8 lanes take a row 16 bytes at a time, and a thread
+// asks for its pieces of four rows before it uses the first (a warp per row with 4-byte loads had too little in flight).
 template <int D, class F>
-__global__ void __launch_bounds__(256) fa_delta_tc_kernel(const bf16* __restrict__ o, const bf16* __restrict__ d_o, float* __restrict__ delta, int B, int Tq, int Hq, int d) {
+__global__ void __launch_bounds__(256) fa_delta_tc_kernel(const bf16* __restrict__ o, const bf16* __restrict__ low, const bf16* __restrict__ d_o,
+                                                          float* __restrict__ delta, int B, int Tq, int Hq, int d) {
     constexpr int LANES = D / 8, PER = 256 / LANES, U = 4;       // lanes of a row, rows of a block at a time
     const int l = threadIdx.x % LANES;
     const long long rows = (long long)B * Tq * Hq, row0 = (long long)blockIdx.x * (PER * U) + threadIdx.x / LANES;
-    Vec<bf16> x[U], y[U];
+    uint4 x[U], y[U], z[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (F::RANGES && l * 8 >= d) { x[u].raw = y[u].raw = make_uint4(0, 0, 0, 0); continue; }
+        x[u] = y[u] = z[u] = make_uint4(0, 0, 0, 0);
+        if (F::RANGES && l * 8 >= d) continue;
         const long long at = min(row0 + u * PER, rows - 1) * (F::RANGES ? d : D) + l * 8;
-        x[u].load(o + at);
-        y[u].load(d_o + at);
+        x[u] = *reinterpret_cast<const uint4*>(o + at);
+        y[u] = *reinterpret_cast<const uint4*>(d_o + at);
+        if constexpr (F::RANGES) z[u] = *reinterpret_cast<const uint4*>(low + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const long long row = row0 + u * PER;
         float s = 0.f;
+        const uint32_t* xs = reinterpret_cast<const uint32_t*>(&x[u]);
+        const uint32_t* ys = reinterpret_cast<const uint32_t*>(&y[u]);
+        const uint32_t* zs = reinterpret_cast<const uint32_t*>(&z[u]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (F::HALF) s += __half2float(reinterpret_cast<const __half*>(&x[u].raw)[e]) * __half2float(reinterpret_cast<const __half*>(&y[u].raw)[e]);
-            else s += x[u].get(e) * y[u].get(e);
+        for (int e = 0; e < 4; ++e) {
+            const float2 p = unpack16<F>(xs[e]), g = unpack16<F>(ys[e]);
+            if constexpr (F::RANGES) {
+                const float2 r = unpack16<F>(zs[e]);
+                s += (p.x + r.x) * g.x;
+                s += (p.y + r.y) * g.y;
+            } else {
+                s += p.x * g.x;
+                s += p.y * g.y;
+            }
         }
 #pragma unroll
         for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
@@ -1009,7 +1040,7 @@ static int launch_bwd(const void* q, const long long* qs, const void* k, const l
     if (rc) return -11;
     const long long rows = (long long)a.B * a.Tq * a.Hq;
     constexpr int per_block = 4 * 256 / (D / 8);
-    fa_delta_tc_kernel<D, F><<<(unsigned)((rows + per_block - 1) / per_block), 256, 0, st>>>((const bf16*)o, (const bf16*)d_o, delta, a.B, a.Tq, a.Hq, d);
+    fa_delta_tc_kernel<D, F><<<(unsigned)((rows + per_block - 1) / per_block), 256, 0, st>>>((const bf16*)o, a.x.low, (const bf16*)d_o, delta, a.B, a.Tq, a.Hq, d);
     constexpr int dq_smem = sizeof(SmemDq<D>), dkv_smem = sizeof(SmemDkv<D, F::RANGES>);
     rc = (int)cudaFuncSetAttribute(fa_bwd_dq_tc_kernel<D, F>, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem);
     if (rc) return rc;

@@ -84,7 +84,7 @@ def _check_scores(q, heads, scale, softcap, slopes):
 # ---- binding --------------------------------------------------------------------------------------------------------------------
 class _Ranges(ctypes.Structure):
     _fields_ = ([("first", ctypes.c_void_p), ("stop", ctypes.c_void_p), ("first_b", ctypes.c_longlong), ("stop_b", ctypes.c_longlong)] +
-                [("slopes", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("cap", ctypes.c_float), ("causal", ctypes.c_int), ("d", ctypes.c_int)])
+                [("slopes", ctypes.c_void_p), ("low", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("cap", ctypes.c_float), ("causal", ctypes.c_int), ("d", ctypes.c_int)])
 
 
 _SIZES = [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "q_offset", "window")] + [("scale", ctypes.c_float), ("err", ctypes.c_void_p), ("x", _Ranges)]
@@ -120,7 +120,7 @@ def _laid_out(t: torch.Tensor):
     return t, s
 
 
-def _fill(a, q, k, cfg, first, stop, slopes, tiles):
+def _fill(a, q, k, cfg, first, stop, slopes, low, tiles):
     from . import gemm
     scale, causal, q_offset, window, cap = cfg
     a.B, a.Tq, a.Hq, a.Tk, a.Hkv = q.shape[0], q.shape[1], q.shape[2], k.shape[1], k.shape[2]
@@ -132,6 +132,8 @@ def _fill(a, q, k, cfg, first, stop, slopes, tiles):
         x.stop, x.stop_b = stop.data_ptr(), stop.stride(0)
     if slopes is not None:
         x.slopes = slopes.data_ptr()
+    if low is not None:
+        x.low = low.data_ptr()
     x.tiles, x.cap, x.causal, x.d = tiles.data_ptr(), cap, causal, q.shape[3]
 
 
@@ -144,13 +146,14 @@ class ScoredAttention(torch.autograd.Function):
         out = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
         lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device)
         tiles = torch.empty(B, -(-Tq // 128), 4, dtype=torch.int32, device=q.device)
+        low = torch.empty_like(out) if any(ctx.needs_input_grad[:3]) else None
         a = _Args()
         a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        _fill(a, q, k, cfg, first, stop, slopes, tiles)
+        _fill(a, q, k, cfg, first, stop, slopes, low, tiles)
         f = K.lib().lmoe_scored_attn_fwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_fwd_fp16
         with on_device(q):
             K._check(f(K._p(q), qs, K._p(k), ks, K._p(v), vs, ctypes.byref(a), K._st()), "scored_attn_fwd")
-        ctx.save_for_backward(q, k, v, first, stop, slopes, out, lse, tiles)
+        ctx.save_for_backward(q, k, v, first, stop, slopes, out, low, lse, tiles)
         ctx.cfg = cfg
         return out
 
@@ -158,7 +161,7 @@ class ScoredAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         from . import cuda as K
-        q, k, v, first, stop, slopes, out, lse, tiles = ctx.saved_tensors
+        q, k, v, first, stop, slopes, out, low, lse, tiles = ctx.saved_tensors
         d_out = d_out.contiguous()
         if d_out.data_ptr() % 16:
             d_out = d_out.clone()
@@ -167,7 +170,7 @@ class ScoredAttention(torch.autograd.Function):
         dv = torch.empty_like(dk)
         a = _BwdArgs()
         a.lse, a.delta, a.dq, a.dk, a.dv = lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        _fill(a, q, k, ctx.cfg, first, stop, slopes, tiles)
+        _fill(a, q, k, ctx.cfg, first, stop, slopes, low, tiles)
         f = K.lib().lmoe_scored_attn_bwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_bwd_fp16
         with on_device(q):
             K._check(f(K._p(q), _strides(q), K._p(k), _strides(k), K._p(v), _strides(v), K._p(out), K._p(d_out), K._p(delta), ctypes.byref(a), K._st()),
