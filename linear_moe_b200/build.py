@@ -24,7 +24,7 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 # sources whose fp32 instantiations serve models in true 32-bit: IEEE division and the accurate exp / tanh
 PRECISE = {"chunk_attn.cu", "parallel_block.cu", "packed_attn.cu", "sandwich_block.cu", "moe_rows.cu", "post_norm.cu", "retention.cu", "ssd.cu",
-           "delta_rule.cu"}
+           "delta_rule.cu", "paged_step_any.cu"}
 # what serving a model of the listed kind needs (``build_serving``); everything else is training, communication and fp8
 SERVING = {"parallel_block": ("chunk_attn.cu", "chunk_attn_step.cu", "chunk_attn_tc.cu", "parallel_block.cu", "gemm_dense.cu", "gemm_skinny.cu"),
            "sandwich_block": ("packed_attn.cu", "packed_attn_step.cu", "packed_attn_tc.cu", "latent_step.cu", "moe_rows.cu", "sandwich_block.cu",

@@ -179,6 +179,34 @@ def softmax_attention(q, k, v, scale: Optional[float] = None, causal: bool = Tru
     return torch.einsum("bhij,bjhd->bihd", p, vf).to(q.dtype)
 
 
+def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, window=None, softcap=None, slopes=None, k_new=None, v_new=None):
+    """One query per request over its pages: q ``[B,H,D]``, pages ``[P,page,G,D]``, table ``[B,n]``, lengths ``[B]`` (the new token counted; its row goes to
+    the cache first)."""
+    B, H, D = q.shape
+    P, page, G = k_pages.shape[:3]
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.zeros(B, H, v_pages.shape[3], dtype=q.dtype, device=q.device)
+    for b, n in enumerate(lengths.tolist()):
+        if not 0 <= n <= table.shape[1] * page:
+            raise ValueError(f"request {b}: a length of {n} in a table of {table.shape[1]} pages of {page}")
+        at = table[b, : -(-n // page)].long()
+        if n and not 0 <= int(at.min()) <= int(at.max()) < P:
+            raise ValueError(f"request {b}: a page outside the {P} that there are")
+        if n == 0:
+            continue
+        if k_new is not None:
+            k_pages[at[-1], (n - 1) % page], v_pages[at[-1], (n - 1) % page] = k_new[b], v_new[b]
+        lo = max(0, n - window) if window is not None else 0
+        k, v = (t[at].flatten(0, 1)[lo:n].float() for t in (k_pages, v_pages))
+        x = torch.einsum("grd,jgd->grj", q[b].float().reshape(G, H // G, D) * scale, k)
+        if softcap is not None:
+            x = softcap * torch.tanh(x / softcap)
+        if slopes is not None:
+            x = x - slopes.float().reshape(G, H // G, 1) * torch.arange(n - 1 - lo, -1, -1, device=q.device).float()
+        out[b] = torch.einsum("grj,jgd->grd", torch.softmax(x, -1), v).reshape(H, -1).to(q.dtype)
+    return out
+
+
 # ---- short convolution -----------------------------------------------------
 def causal_conv1d(x, weight, bias=None, activation: Optional[str] = "silu",
                   initial_state: Optional[torch.Tensor] = None):
