@@ -20,6 +20,7 @@ from linear_moe_b200.config.arguments import parse_args                         
 from linear_moe_b200.data.tokenizer import build_tokenizer                        # noqa: E402
 from linear_moe_b200.dist.mesh import init_distributed, single_process_mesh       # noqa: E402
 from linear_moe_b200.infer.generation import GPTPredictor                         # noqa: E402
+from linear_moe_b200.infer.paged_cache import PagedCache                          # noqa: E402
 from linear_moe_b200.models.registry import load_model                           # noqa: E402
 from linear_moe_b200.models.transformer import CausalLM                           # noqa: E402
 
@@ -49,18 +50,20 @@ if __name__ == "__main__":
             load_sharded(tc.load, [model], cfg, mesh, None, layer_offsets=[mesh.pp_rank * per])
         else:
             load_checkpoint(tc.load, [model], None, None, mesh, load_rng=False)
+    if args.paged_kv_cache and not (model.packed_rows or PagedCache.supported(model)):
+        raise SystemExit("--paged-kv-cache is for models of softmax and linear layers (no latent attention, no context parallelism)")
     port = int(os.environ.get("LMOE_SERVE_PORT", "0"))
     if port:
         # HTTP endpoint (PUT /api, the request fields of Megatron's text-generation server): rank 0 serves, the other
         # ranks of a parallel replica join every generation call
         from linear_moe_b200.infer.server import build_app, serve_followers
-        graph = getattr(args, "cuda_graph_decode", False)
+        graph, paged = getattr(args, "cuda_graph_decode", False), getattr(args, "paged_kv_cache", False)
         if mesh.rank == 0:
             import uvicorn
-            uvicorn.run(build_app(model.eval(), tok, cuda_graph=graph), host=os.environ.get("LMOE_SERVE_HOST", "127.0.0.1"),
+            uvicorn.run(build_app(model.eval(), tok, cuda_graph=graph, paged=paged), host=os.environ.get("LMOE_SERVE_HOST", "127.0.0.1"),
                         port=port, log_level="warning")
         else:
-            serve_followers(model.eval(), tok, cuda_graph=graph)
+            serve_followers(model.eval(), tok, cuda_graph=graph, paged=paged)
         sys.exit(0)
     outs = GPTPredictor(model, tok, args).predict()
     if mesh.rank == 0:

@@ -47,7 +47,7 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--num-query-groups", "--n-head-kv", type=int, default=None, dest="num_query_groups")
     _flag(g, "--max-position-embeddings", type=int, default=4096)
     _flag(g, "--position-embedding-type", type=str, default="rope",
-          choices=["learned_absolute", "rope", "none"])
+          choices=["learned_absolute", "rope", "none", "alibi"])
     _flag(g, "--use-rotary-position-embeddings", action="store_true")
     _flag(g, "--no-position-embedding", action="store_true")
     _flag(g, "--rotary-base", type=float, default=10000.0)
@@ -70,6 +70,7 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--hidden-dropout", type=float, default=0.0)
     _flag(g, "--qk-layernorm", action="store_true")
     _flag(g, "--sliding-window", type=int, default=None)
+    _flag(g, "--attn-logit-softcapping", type=float, default=None, help="cap the attention scores: cap * tanh(scores / cap)")
     _flag(g, "--window-size", type=str, default=None, metavar="LEFT,RIGHT",
           help="Megatron's spelling of the attention window: LEFT earlier tokens plus the current one (RIGHT must be 0 for "
                "causal attention); the same as --sliding-window LEFT+1")
@@ -252,6 +253,9 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--recompute-granularity", type=str, default=None, choices=["full", "selective"])
     _flag(g, "--recompute-method", type=str, default=None, choices=["uniform", "block"])
     _flag(g, "--recompute-num-layers", type=int, default=1)
+    _flag(g, "--paged-kv-cache", action="store_true",
+          help="generation keeps the softmax layers' keys and values in pages: nothing is concatenated, --cuda-graph-decode captures these layers too, and beam search "
+               "runs one token a step")
     _flag(g, "--cuda-graph-decode", action="store_true",
           help="generation: replay one-token steps from a CUDA graph (models with fixed-size caches)")
     _flag(g, "--cpu-offloading", action="store_true")
@@ -336,6 +340,8 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--epochs", type=int, default=None)
     _flag(g, "--keep-last", action="store_true")
     _flag(g, "--eod-mask-loss", action="store_true")
+    _flag(g, "--reset-attention-mask", action="store_true", help="tokens attend inside their document only (documents end at the end-of-document token)")
+    _flag(g, "--reset-position-ids", action="store_true", help="rotary positions start again at every document")
     _flag(g, "--tokenizer-type", type=str, default="NullTokenizer")
     _flag(g, "--patch-tokenizer-type", type=str, default="NullTokenizer", choices=list(_TOKENIZERS))
     _flag(g, "--tokenizer-model", "--load-tokenizer", type=str, default=None, dest="tokenizer_model")
@@ -428,7 +434,7 @@ def configs_from_args(args: argparse.Namespace) -> Tuple[ModelConfig, ParallelCo
         tie_embeddings=not args.untie_embeddings_and_output_weights,
         init_method_std=args.init_method_std, hidden_dropout=args.hidden_dropout,
         attention_dropout=args.attention_dropout, qk_layernorm=args.qk_layernorm,
-        sliding_window=args.sliding_window, position_embedding_type=pos,
+        sliding_window=args.sliding_window, attn_logit_softcapping=args.attn_logit_softcapping, position_embedding_type=pos,
         rotary_base=args.rotary_base, rotary_percent=args.rotary_percent,
         rotary_interleaved=args.rotary_interleaved, rotary_scaling_factor=args.rotary_scaling_factor,
         rotary_seq_len_interpolation_factor=args.rotary_seq_len_interpolation_factor,
@@ -547,6 +553,7 @@ def configs_from_args(args: argparse.Namespace) -> Tuple[ModelConfig, ParallelCo
         train_data=args.train_data, valid_data=args.valid_data, split=args.split,
         max_padding_length=args.max_padding_length, num_workers=args.num_workers, epochs=args.epochs,
         keep_last=args.keep_last, eod_mask_loss=args.eod_mask_loss,
+        reset_attention_mask=args.reset_attention_mask, reset_position_ids=args.reset_position_ids,
         heartbeat_interval_s=args.heartbeat_interval_s, heartbeat_timeout_s=args.heartbeat_timeout_s,
     )
     if getattr(args, "preset", None):

@@ -60,8 +60,9 @@ class ModelConfig:
     attention_dropout: float = 0.0
     qk_layernorm: bool = False
     sliding_window: Optional[int] = None
+    attn_logit_softcapping: Optional[float] = None    # softmax layers: scores become cap * tanh(scores / cap)
     # ---- positional -----------------------------------------------------
-    position_embedding_type: str = "rope"         # rope | none | learned (layer-list designs: table of max_position_embeddings rows)
+    position_embedding_type: str = "rope"         # rope | none | alibi (softmax layers: minus a slope per head times the distance) | learned (layer-list designs: table of max_position_embeddings rows)
     rotary_base: float = 10000.0
     rotary_percent: float = 1.0
     rotary_interleaved: bool = False
@@ -186,6 +187,10 @@ class ModelConfig:
             raise ValueError(f"a width of {self.hidden_size} has no {self.norm_groups} equal parts")
         if self.logit_softcap is not None and not self.logit_softcap > 0:
             raise ValueError(f"soft cap {self.logit_softcap}")
+        if self.attn_logit_softcapping is not None and not self.attn_logit_softcapping > 0:
+            raise ValueError(f"soft cap {self.attn_logit_softcapping}")
+        if (self.attn_logit_softcapping is not None or self.position_embedding_type == "alibi") and (self.base_model == "deepseek_v2" or self.layers is not None):
+            raise ValueError("capped scores and the distance bias are options of grouped-query softmax layers (latent attention and the layer-list designs have their own)")
         if self.base_model not in BASE_MODELS:
             raise ValueError(f"unknown base model {self.base_model!r}")
         if self.la_module is not None and self.la_module not in LA_MODULES:
@@ -322,7 +327,7 @@ class TrainConfig:
     exit_duration_in_mins: Optional[float] = None
     optimizer: str = "adam"                       # adam | sgd
     sgd_momentum: float = 0.9
-    eod_token: Optional[int] = None               # the tokenizer's end-of-document id, for --eod-mask-loss
+    eod_token: Optional[int] = None               # the tokenizer's end-of-document id, for --eod-mask-loss and --reset-*
     moe_per_layer_logging: bool = False           # the auxiliary losses of every MoE layer in the log line and TensorBoard
     rampup_batch_size: Optional[Tuple[int, int, int]] = None     # --rampup-batch-size start increment ramp-up-samples
     override_opt_param_scheduler: bool = False
@@ -351,5 +356,7 @@ class TrainConfig:
     epochs: Optional[int] = None
     keep_last: bool = False
     eod_mask_loss: bool = False
+    reset_attention_mask: bool = False            # packed documents do not attend to one another (softmax layers)
+    reset_position_ids: bool = False              # rotary positions start again at every document
     heartbeat_interval_s: float = 0.0             # >0 starts the host watchdog
     heartbeat_timeout_s: float = 60.0

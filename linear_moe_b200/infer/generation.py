@@ -21,7 +21,9 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
+from .. import ops
 from . import parallel_forward as PF
+from .paged_cache import PagedCache
 
 
 def modify_logits_for_top_k(logits: torch.Tensor, k: int) -> torch.Tensor:
@@ -112,7 +114,7 @@ class GraphedDecodeStep:
     is captured once and replayed: the token is copied into a static buffer, the graph runs the whole forward, and the
     new states go over the state buffers that the graph reads: the one-token kernels of the decayed mixers write them there, others are
     copied back.  Softmax-attention layers whose KV cache grows by one
-    row per token are not supported and fall back to eager decoding.  A ``SlotCache`` is updated in place by the step, so
+    row per token are not supported and fall back to eager decoding; those of a ``PagedCache`` store into its pages.  A ``SlotCache`` is updated in place by the step, so
     nothing is copied back; ``rows`` then holds the requests' positions and slots in device tensors that the caller fills."""
 
     def __init__(self, model, caches: List[dict], batch: int, device, rows=None):
@@ -128,7 +130,7 @@ class GraphedDecodeStep:
             return False
         if getattr(model, "packed_rows", False):
             return True
-        if any(s.mixer in ("attn", "mla") for s in model.specs):              # KV caches grow with every token
+        if any(s.mixer in ("attn", "mla") for s in model.specs) and not isinstance(caches, PagedCache):      # KV caches grow with every token
             return False
         return all(all(torch.is_tensor(v) for v in c.values()) for c in caches)   # nested caches (MoM) decode eagerly
 
@@ -178,10 +180,11 @@ def generate_tokens(model, tokens: torch.Tensor, lengths: torch.Tensor, *, eod: 
                     top_p: float = 0.0, temperature: float = 1.0, repetition_penalty: float = 1.0,
                     return_log_probs: bool = False, use_eod_for_early_termination: bool = True,
                     stop_on_double_eol: bool = False, stop_on_eol: bool = False, generator=None,
-                    cuda_graph: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+                    cuda_graph: bool = False, paged: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """Fill ``tokens [B, L]`` from the shortest prompt length to L.  Returns (tokens, generated lengths, log-probs).
     ``cuda_graph``: replay the one-token steps from a CUDA graph (``GraphedDecodeStep``) when the model allows it; the
-    prefill and the first two one-token steps run eagerly (they also serve as the warm-up before the capture)."""
+    prefill and the first two one-token steps run eagerly (they also serve as the warm-up before the capture).
+    ``paged``: softmax layers keep their keys and values in pages (``PagedCache``) instead of concatenating them for every token, and their steps are captured too."""
     model.eval()
     if getattr(model, "packed_rows", False):
         return _generate_packed(model, tokens, lengths, eod if use_eod_for_early_termination else None,
@@ -189,13 +192,15 @@ def generate_tokens(model, tokens: torch.Tensor, lengths: torch.Tensor, *, eod: 
                                 repetition_penalty, return_log_probs, cuda_graph)
     B, L = tokens.shape
     min_len = int(lengths.min())
-    caches = model.new_cache()
+    caches = PagedCache(model, B, L) if paged else model.new_cache()
     done = torch.zeros(B, dtype=torch.bool, device=tokens.device)
     gen_len = torch.full((B,), L, dtype=torch.long, device=tokens.device)
     logps = torch.zeros(B, L - 1, dtype=torch.float32, device=tokens.device) if return_log_probs else None
     prev = 0
     graphed, single_steps = None, 0
     for ctx in range(min_len, L):
+        if paged:
+            caches.advance(ctx - prev)
         if ctx - prev == 1:
             single_steps += 1
         if cuda_graph and ctx - prev == 1 and single_steps > 2:
@@ -313,25 +318,44 @@ class BeamHypotheses:
         return self.worst >= best_sum_logprobs / (cur_len ** self.length_penalty)
 
 
+def can_page_beams(model) -> bool:
+    """Can a beam search of this model run one token a step, on caches that follow the beams?  (The memories of a mixture are not kept by row.)"""
+    return PagedCache.supported(model) and model.mesh.pp == 1 and not str(model.cfg.la_module or "").startswith("mom_")
+
+
 @torch.no_grad()
 def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int, eod: int, length_penalty: float = 1.0,
-                num_return: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Beam search for one prompt ``[1, P]`` (``beam_search_and_return_on_first_stage``).  The whole beam is re-scored
-    from its tokens each step (beams reorder, so per-beam recurrent caches are not reused)."""
+                num_return: int = 1, paged: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Beam search for one prompt ``[1, P]`` (``beam_search_and_return_on_first_stage``).  The whole beam is re-scored from its tokens each step; with
+    ``paged`` a step runs the new token of every beam alone, on caches whose states and pages follow the beams (``PagedCache.reorder``)."""
     model.eval()
     device = prompt.device
     P = prompt.shape[1]
+    caches = None
+    if paged:
+        if not can_page_beams(model):
+            raise ValueError("a paged beam search is for models of softmax and linear layers on one pipeline stage, without a mixture of memories")
+        caches = PagedCache(model, beam_size, P + max_new_tokens, live=1)
     beams = prompt.repeat(beam_size, 1)
     scores = torch.zeros(beam_size, device=device)
     scores[1:] = -1e9                                   # all beams start identical: keep one alive
     hyps = BeamHypotheses(beam_size, length_penalty)
+    next_b: List[int] = []
     for step in range(max_new_tokens):
-        logits = PF.full_logits(model, beams, last_only=True)[:, -1]
-        lp = F.log_softmax(logits, -1)
-        V = lp.shape[-1]
-        cand = (scores[:, None] + lp).reshape(-1)
-        top_s, top_i = torch.topk(cand, 2 * beam_size)
-        b_idx, t_idx = top_i // V, top_i % V
+        if caches is None:
+            logits = PF.full_logits(model, beams, last_only=True)[:, -1]
+        elif step == 0:                                    # the prompt once, then a row per beam
+            caches.advance(P)
+            logits = PF.stage_forward(model, prompt, caches, 0)[:, -1].expand(beam_size, -1)
+            if not caches.reorderable():
+                raise ValueError("a layer of this model keeps states that do not follow a beam")
+            caches.reorder([0] * beam_size)
+        else:
+            caches.reorder(next_b)
+            caches.advance(1)
+            logits = PF.stage_forward(model, beams[:, -1:], caches, P + step - 1)[:, -1]
+        V = logits.shape[-1]
+        top_s, b_idx, t_idx = (t[0] for t in ops.beam_select(logits.float()[None], scores[None], min(2 * beam_size, logits.shape[0] * V)))
         next_b, next_t, next_s = [], [], []
         for s, b, t in zip(top_s.tolist(), b_idx.tolist(), t_idx.tolist()):
             if t == eod:
@@ -358,7 +382,7 @@ def generate_and_post_process(model, tokenizer, prompts: Sequence[str], tokens_t
                               return_output_log_probs: bool = False, top_k_sampling: int = 0, top_p_sampling: float = 0.0,
                               temperature: float = 1.0, add_BOS: bool = False, use_eod_token_for_early_termination: bool = True,
                               repetition_penalty: float = 1.0, random_seed: int = -1, device=None,
-                              cuda_graph: bool = False):
+                              cuda_graph: bool = False, paged: bool = False):
     """Strings in, strings out (api.py:25-111): returns (texts, token lists, log-probs or None)."""
     device = device or next(model.parameters()).device
     gen = None
@@ -372,7 +396,7 @@ def generate_and_post_process(model, tokenizer, prompts: Sequence[str], tokens_t
                                           top_p=top_p_sampling, temperature=temperature,
                                           repetition_penalty=repetition_penalty, return_log_probs=return_output_log_probs,
                                           use_eod_for_early_termination=use_eod_token_for_early_termination, generator=gen,
-                                          cuda_graph=cuda_graph)
+                                          cuda_graph=cuda_graph, paged=paged)
     out_tokens = [tokens[i, : int(gen_len[i])].tolist() for i in range(tokens.shape[0])]
     texts = [tokenizer.decode(t) for t in out_tokens]
     return texts, out_tokens, lp
@@ -401,7 +425,8 @@ class GPTPredictor:
             texts, _, _ = generate_and_post_process(self.model, self.tok, [p], tokens_to_generate=a.out_seq_length,
                                                     top_k_sampling=a.top_k, top_p_sampling=a.top_p,
                                                     temperature=a.temperature, repetition_penalty=a.repetition_penalty,
-                                                    cuda_graph=getattr(a, "cuda_graph_decode", False))
+                                                    cuda_graph=getattr(a, "cuda_graph_decode", False),
+                                                    paged=getattr(a, "paged_kv_cache", False))
             outs.append(texts[0])
         if a.text_generate_output_file and getattr(getattr(self.model, "mesh", None), "rank", 0) == 0:
             with open(a.text_generate_output_file, "a", encoding="utf-8") as f:

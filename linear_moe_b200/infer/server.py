@@ -18,7 +18,7 @@ from typing import List, Optional
 
 import torch
 
-from .generation import beam_search, generate_and_post_process
+from .generation import beam_search, can_page_beams, generate_and_post_process
 
 MAX_PROMPTS = 128
 MAX_TOKENS = 4096
@@ -57,20 +57,20 @@ def _validate(req: dict) -> Optional[str]:
     return None
 
 
-def run_request(model, tokenizer, req: dict, cuda_graph: bool = False) -> dict:
+def run_request(model, tokenizer, req: dict, cuda_graph: bool = False, paged: bool = False) -> dict:
     """One validated request -> response body (the collective part: every rank of a parallel model calls this)."""
     if req.get("beam_width"):
         device = next(model.parameters()).device
         ids = torch.tensor([tokenizer.tokenize(req["prompts"][0])], dtype=torch.long, device=device)
         toks, scores = beam_search(model, ids, req["beam_width"], req.get("tokens_to_generate", 64), tokenizer.eod,
-                                   length_penalty=req.get("length_penalty", 1.0), num_return=req.get("beam_width"))
+                                   length_penalty=req.get("length_penalty", 1.0), num_return=req.get("beam_width"), paged=paged and can_page_beams(model))
         return {"text": [tokenizer.decode(t) for t in toks.tolist()], "tokens": toks.tolist(), "score": scores.tolist()}
     texts, tokens, lp = generate_and_post_process(
         model, tokenizer, req["prompts"], tokens_to_generate=req.get("tokens_to_generate", 64),
         return_output_log_probs=bool(req.get("logprobs", False)), top_k_sampling=req.get("top_k", 0),
         top_p_sampling=req.get("top_p", 0.0), temperature=req.get("temperature", 1.0), add_BOS=bool(req.get("add_BOS", False)),
         use_eod_token_for_early_termination=bool(req.get("use_eod_token_for_early_termination", True)),
-        repetition_penalty=req.get("repetition_penalty", 1.0), random_seed=req.get("random_seed", -1), cuda_graph=cuda_graph)
+        repetition_penalty=req.get("repetition_penalty", 1.0), random_seed=req.get("random_seed", -1), cuda_graph=cuda_graph, paged=paged)
     out = {"text": texts, "tokens": tokens}
     if lp is not None:
         out["logprobs"] = [row[: max(len(t) - 1, 0)] for row, t in zip(lp.tolist(), tokens)]
@@ -84,7 +84,7 @@ def _broadcast_request(req: Optional[dict], group) -> Optional[dict]:
     return box[0]
 
 
-def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False):
+def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False, paged: bool = False):
     """Ranks other than 0 of a tensor- / pipeline-parallel replica: wait for rank 0's requests and join each generation
     call; a broadcast ``None`` ends the loop."""
     while True:
@@ -92,10 +92,10 @@ def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False):
         if req is None:
             return
         with torch.no_grad():
-            run_request(model, tokenizer, req, cuda_graph)
+            run_request(model, tokenizer, req, cuda_graph, paged)
 
 
-def build_app(model, tokenizer, cuda_graph: bool = False, group=None):
+def build_app(model, tokenizer, cuda_graph: bool = False, group=None, paged: bool = False):
     from fastapi import FastAPI, Request
     from fastapi.responses import JSONResponse
     import torch.distributed as dist
@@ -125,7 +125,7 @@ def build_app(model, tokenizer, cuda_graph: bool = False, group=None):
         with lock, torch.no_grad():
             if parallel:
                 _broadcast_request(req, group)
-            return run_request(model, tokenizer, req, cuda_graph)
+            return run_request(model, tokenizer, req, cuda_graph, paged)
 
     @app.get("/health")
     async def health():

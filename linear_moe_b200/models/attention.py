@@ -92,8 +92,39 @@ class SelfAttention(nn.Module):
             # shared by all heads, applied to this rank's heads: the optimizer sums the partial gradients over TP
             self.q_layernorm.weight.tp_partial_grad = self.k_layernorm.weight.tp_partial_grad = True
         self.rope = RotaryCache(cfg, D) if cfg.position_embedding_type == "rope" else None
+        self._slopes: Optional[torch.Tensor] = None        # this rank's heads; made on first use (a buffer would change its type with the model)
 
-    def forward(self, x, cache: Optional[dict] = None, position_offset: int = 0, **_):
+    def _scores(self, device) -> dict:
+        """Options of the layer's scores: ``ops.softmax_attention`` and ``ops.paged_attention`` take the same ones."""
+        cfg = self.cfg
+        out = {}
+        if cfg.attn_logit_softcapping is not None:
+            out["softcap"] = cfg.attn_logit_softcapping
+        if cfg.position_embedding_type == "alibi":
+            if self._slopes is None or self._slopes.device != device:
+                n = self.Gl * self.qpg
+                self._slopes = ops.alibi_slopes(self.H)[self.mesh.tp_rank * n:(self.mesh.tp_rank + 1) * n].to(device)
+            out["slopes"] = self._slopes
+        return out
+
+    def _from_pages(self, q, k, v, cache: dict, position_offset: int):
+        """Attention of this call's tokens on a paged cache (``infer/paged_cache.py``), which gets their rows."""
+        cfg = self.cfg
+        kp, vp, table, lengths = cache["k_pages"], cache["v_pages"], cache["table"], cache["lengths"]
+        T = q.shape[1]
+        if T == 1:
+            return ops.paged_attention(q[:, 0], kp, vp, table, lengths, None, cfg.sliding_window, k_new=k[:, 0], v_new=v[:, 0], **self._scores(q.device))[:, None]
+        page = kp.shape[1]
+        at = torch.arange(position_offset, position_offset + T, device=q.device)
+        rows = table[:, at // page].long()
+        kp[rows, at % page], vp[rows, at % page] = k, v
+        if position_offset:                                # a portion: what the pages hold in front of it comes first
+            n = position_offset + T
+            k, v = (t[table[:, : -(-n // page)].long()].flatten(1, 2)[:, :n] for t in (kp, vp))
+        return ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, position_offset, cfg.sliding_window, **self._scores(q.device))
+
+    def forward(self, x, cache: Optional[dict] = None, position_offset: int = 0, key_first=None, positions=None, **_):
+        """``key_first`` int32 ``[B,T]``: first token that a token may attend to (packed documents); ``positions`` ``[B,T]``: rotary positions."""
         cfg = self.cfg
         qkv = self.linear_qkv(x)
         B, T = qkv.shape[:2]
@@ -107,16 +138,29 @@ class SelfAttention(nn.Module):
         past = cache["k"].shape[1] if (cache is not None and "k" in cache) else 0
         # position_offset is the absolute position of this call's first token (the cache length when decoding)
         pos0 = position_offset + (cp.rank * T if not cp.is_trivial else 0)
-        if self.rope is not None:
+        paged = cache is not None and "table" in cache
+        if self.rope is not None and paged and T == 1:     # the positions are on the device: a captured step goes on from them
+            at = cache["lengths"][:, None].long() - 1
+            q = ops.apply_rope_at(q.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
+            k = ops.apply_rope_at(k.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
+        elif self.rope is not None and positions is not None:
+            cos, sin = self.rope.get(T, 0, x.device)
+            q = ops.apply_rope_at(q.contiguous(), cos, sin, positions, cfg.rotary_interleaved)
+            k = ops.apply_rope_at(k.contiguous(), cos, sin, positions, cfg.rotary_interleaved)
+        elif self.rope is not None:
             cos, sin = self.rope.get(T, pos0, x.device)
             q = ops.apply_rope(q.contiguous(), cos, sin, cfg.rotary_interleaved)
             k = ops.apply_rope(k.contiguous(), cos, sin, cfg.rotary_interleaved)
+        if paged:
+            o = self._from_pages(q, k, v, cache, position_offset)
+            return self.linear_proj(o.reshape(B, T, -1))
         k, v, q_off = _kv_cache_update(cache, k, v)
         if not cp.is_trivial:
             k = C.all_gather(k.contiguous(), cp, dim=1)
             v = C.all_gather(v.contiguous(), cp, dim=1)
             q_off = cp.rank * T
-        o = ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, q_off, cfg.sliding_window)
+        o = ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, q_off, cfg.sliding_window, key_first=key_first,
+                                  **self._scores(x.device))
         return self.linear_proj(o.reshape(B, T, -1))
 
     @torch.no_grad()

@@ -122,12 +122,14 @@ class Block(nn.Module):
     def _mixer_norm(self):
         return getattr(self, "norm", None) or getattr(self, "input_layernorm", None)
 
-    def forward(self, x, residual, cache: Optional[dict] = None, position_offset: int = 0, lower_bound=None):
-        """x: output of the previous sub-layer (not yet added to the stream), residual: the stream."""
+    def forward(self, x, residual, cache: Optional[dict] = None, position_offset: int = 0, lower_bound=None, attend: Optional[dict] = None):
+        """x: output of the previous sub-layer (not yet added to the stream), residual: the stream; ``attend``: what limits attention (``SelfAttention``)."""
         mixer = self._mixer()
         if mixer is not None:
             h, residual = self._mixer_norm().add_norm(x, residual)
             kw = {"lower_bound": lower_bound} if lower_bound is not None else {}
+            if attend is not None:
+                kw.update(attend)
             x = self._drop(mixer(h, cache=cache, position_offset=position_offset, **kw))
         if self.spec.ffn is not None:
             h, residual = self.pre_mlp_layernorm.add_norm(x, residual)
@@ -227,7 +229,7 @@ class CausalLM(nn.Module):
             return new_slot_cache(self, slots, tokens)
         return [dict() for _ in self.decoder.layers]
 
-    def _run_blocks(self, x, residual, caches, position_offset):
+    def _run_blocks(self, x, residual, caches, position_offset, attend=None):
         cfg = self.cfg
         layers = self.decoder.layers
         full_recompute = cfg.recompute_granularity == "full" and self.training and caches is None
@@ -244,12 +246,12 @@ class CausalLM(nn.Module):
                 # backward: its parameter gradients are final and their reduction may start
                 x.register_hook(lambda g, i=i: ready(i))
             if full_recompute and self._should_recompute(i):
-                x, residual = ckpt.checkpoint(blk, x, residual, None, position_offset, lb_i, use_reentrant=False)
+                x, residual = ckpt.checkpoint(blk, x, residual, None, position_offset, lb_i, attend, use_reentrant=False)
             elif self.offload is not None and self.training and caches is None and torch.is_grad_enabled():
                 with self.offload.layer(i):
-                    x, residual = blk(x, residual, cache, position_offset, lb_i)
+                    x, residual = blk(x, residual, cache, position_offset, lb_i, attend)
             else:
-                x, residual = blk(x, residual, cache, position_offset, lb_i)
+                x, residual = blk(x, residual, cache, position_offset, lb_i, attend)
         return x, residual
 
     def _should_recompute(self, i: int) -> bool:
@@ -263,8 +265,11 @@ class CausalLM(nn.Module):
     def forward(self, input_ids: Optional[torch.Tensor] = None, labels: Optional[torch.Tensor] = None, *,
                 hidden_in: Optional[torch.Tensor] = None, caches: Optional[List[dict]] = None,
                 position_offset: int = 0, parallel_output: bool = False, return_hidden: bool = False, batch=None,
-                logit_rows: Optional[torch.Tensor] = None):
-        """``batch`` (``ops.row_batch.RowBatch``; models that run packed rows): ``input_ids`` are the packed tokens of its
+                logit_rows: Optional[torch.Tensor] = None, key_first: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None):
+        """``key_first`` int32 ``[B,T]`` (``ops.document_first``): a token attends to the tokens from there on; ``positions`` ``[B,T]``: rotary positions other than 0, 1, ...
+        Both are for whole sequences through models of softmax layers.
+
+        ``batch`` (``ops.row_batch.RowBatch``; models that run packed rows): ``input_ids`` are the packed tokens of its
         requests and the result has one row per token, or per entry of ``logit_rows``."""
         if self.packed_rows:
             return forward_rows(self, input_ids, labels, caches, position_offset, batch, logit_rows, return_hidden)
@@ -273,7 +278,12 @@ class CausalLM(nn.Module):
         else:
             x = hidden_in
         residual = None
-        x, residual = self._run_blocks(x, residual, caches, position_offset)
+        attend = None
+        if key_first is not None or positions is not None:
+            if caches is not None or not self.mesh["cp"].is_trivial or any(s.mixer not in ("attn", None) for s in self.specs):
+                raise ValueError("document ranges and positions are for softmax layers, on whole sequences without a cache (linear layers carry their state over a document's end)")
+            attend = {"key_first": key_first, "positions": positions}
+        x, residual = self._run_blocks(x, residual, caches, position_offset, attend)
         if not self.post_process:
             return x if residual is None else x + residual
         h, _ = self.decoder.final_layernorm.add_norm(x, residual)

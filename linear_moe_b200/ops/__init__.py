@@ -329,7 +329,7 @@ def softmax_attention(q, k, v, scale=None, causal=True, q_offset: int = 0, windo
 
 from .beam import beam_select, copy_pages_, reorder_states   # noqa: E402,F401
 from .paged_attn import paged_attention   # noqa: E402,F401
-from .scored_attn import document_first, prefix_stop, scored_attention   # noqa: E402,F401
+from .scored_attn import alibi_slopes, document_first, prefix_stop, scored_attention   # noqa: E402,F401
 
 
 # ---- packed-row operators (serving only) -----------------------------------------------------------

@@ -31,9 +31,13 @@ def _eager_select(logits, scores, n):
     x = x - x.amax(-1, keepdim=True)                       # NaN in beams of nothing but minus infinity
     total = x + (scores.double()[..., None] - x.exp().sum(-1, keepdim=True).log())
     total = torch.nan_to_num(total, nan=float("-inf"), posinf=float("inf"), neginf=float("-inf")).flatten(1)
-    best, at = torch.sort(total, dim=-1, descending=True, stable=True)
     V = logits.shape[2]
-    return best[:, :n].float(), at[:, :n] // V, at[:, :n] % V
+    best, at = torch.empty(len(total), n, dtype=torch.float64, device=x.device), torch.empty(len(total), n, dtype=torch.int64, device=x.device)
+    for i, row in enumerate(total):
+        place = (row >= row.topk(n).values[-1]).nonzero()[:, 0]          # in order of place, so that a stable sort leaves ties there
+        s, o = torch.sort(row[place], descending=True, stable=True)
+        best[i], at[i] = s[:n], place[o[:n]]
+    return best.float(), at // V, at % V
 
 
 @torch.no_grad()

@@ -53,6 +53,14 @@ def prefix_stop(T: int, prefix: Sequence[int], lengths: Optional[Sequence[int]] 
     return stop.contiguous()
 
 
+def alibi_slopes(heads: int) -> torch.Tensor:
+    """Slopes of the distance bias, fp32 ``[heads]`` (Press et al., "Train Short, Test Long"): a geometric series from 2^(-8/n) on for n heads, a power of two; other
+    numbers of heads take the series of the next lower power and every second slope of the next higher one's."""
+    n = 1 << (heads.bit_length() - 1)
+    s = [2.0 ** (-8.0 * (i + 1) / n) for i in range(n)] + [2.0 ** (-8.0 * (i + 1) / (2 * n)) for i in range(0, 2 * n, 2)]
+    return torch.tensor(s[:heads], dtype=torch.float32)
+
+
 def _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, key_stop):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes q [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")

@@ -25,6 +25,7 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
+from .. import ops
 from ..config.model_config import ModelConfig, ParallelConfig, TrainConfig
 from ..data.datasets import BatchIterator, SyntheticTokenDataset
 from ..dist import collectives as C
@@ -81,6 +82,12 @@ class Trainer:
         if cfg.layers is not None:
             raise ValueError("layer-list models (packed rows) serve only: their kernels have no backward pass")
         self.cfg, self.par, self.tc = cfg, par, tc
+        if tc.reset_attention_mask or tc.reset_position_ids:
+            if tc.eod_token is None:
+                raise ValueError("--reset-attention-mask and --reset-position-ids need the end-of-document token")
+            if par.context_parallel_size > 1 or any(s.mixer not in ("attn", None) for s in cfg.layer_types()):
+                raise ValueError("--reset-attention-mask and --reset-position-ids are for models of softmax layers without context parallelism "
+                                 "(linear layers carry their state over a document's end)")
         self.mesh = mesh or single_process_mesh()
         self.device = device or (torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available()
                                  else torch.device("cpu"))
@@ -160,7 +167,7 @@ class Trainer:
     def forward_step(self, batch, model: CausalLM, hidden_in):
         if self.custom_forward_step is not None:
             return self.custom_forward_step(batch, model, hidden_in)
-        out = model(batch["tokens"], batch["labels"] if model.post_process else None, hidden_in=hidden_in)
+        out = model(batch["tokens"], batch["labels"] if model.post_process else None, hidden_in=hidden_in, **self._documents(batch["tokens"]))
         mesh = self.mesh
 
         def loss_fn(per_token):
@@ -169,6 +176,15 @@ class Trainer:
                 raise FloatingPointError(f"rank {mesh.rank}: non-finite loss at iteration {self.iteration}")
             return loss, {"lm loss": log_loss}
         return out, loss_fn
+
+    def _documents(self, tokens) -> dict:
+        """What keeps packed documents apart (``--reset-attention-mask``, ``--reset-position-ids``)."""
+        tc = self.tc
+        if not (tc.reset_attention_mask or tc.reset_position_ids):
+            return {}
+        first = ops.document_first(tokens, tc.eod_token)
+        at = torch.arange(tokens.shape[1], device=tokens.device)
+        return {"key_first": first if tc.reset_attention_mask else None, "positions": at - first if tc.reset_position_ids else None}
 
     def _run_schedule(self, forward_only: bool = False, data_iter=None):
         tc, mesh = self.tc, self.mesh
@@ -531,7 +547,7 @@ def pretrain(argv=None, dataset_provider: Optional[Callable] = None, model_provi
     print_rank_0(f"> mesh: {mesh.describe()}")
     mem = compute_weight_and_optimizer_memory(cfg, par, verbose=mesh.rank == 0)
     train_ds, valid_ds = (dataset_provider or build_datasets)(args, cfg, tc)
-    if tc.eod_mask_loss and tc.eod_token is None:
+    if (tc.eod_mask_loss or tc.reset_attention_mask or tc.reset_position_ids) and tc.eod_token is None:
         # --eod-mask-loss: no loss on the token that follows an end-of-document token; the id comes from the tokenizer
         from ..data.tokenizer import build_tokenizer
         tok, _ = build_tokenizer(args.patch_tokenizer_type, args.tokenizer_model, cfg.vocab_size, args.extra_vocab_size)
