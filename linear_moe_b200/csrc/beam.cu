@@ -1,9 +1,10 @@
 // One step of a beam search.
 //
 // Selection: the best n of  s_b + x_bt - lse_b  over the beams b and the vocabulary t of every prompt, ties to the lowest b V + t.  Bound by reading the logits once.
-//   beam_parts_kernel   a CTA holds 4096 logits of one beam in registers: their maximum and sum of exponentials, and their n best.  The n-th largest of the
-//                       256 threads' maxima is a bound that at least n logits reach and few others do; those go to shared memory, and each finds its rank by counting.
-//                       Where too many reach it (equal logits) the n best are taken out one by one instead.
+//   beam_parts_kernel   a CTA goes through a part of one beam's logits, 4096 at a time in registers, with the next ones on their way: their maximum and sum of exponentials, and their n
+//                       best.  The threads' maxima of the first chunk give a bound that n logits reach and few others do; those go to shared memory, their n-th best
+//                       is the bound of the chunks behind, and in the end each candidate finds its rank by counting.  Where too many reach the bound a closer one is searched, and where
+//                       many are equal the n best are taken out one by one.
 //   beam_join_kernel    a CTA per prompt does the same with the parts' candidates.  Candidates of different beams can lie next to one another, so their scores are
 //                       compared in 64 bits and rounded once.
 // Inside a beam the order of the logits is the order of the scores, so no part needs another one's sum.
@@ -26,10 +27,11 @@ struct Args {
     int* at;                              //          [N K, parts, n] their tokens,
     double* sum;                          //          [N K, parts] sums
     long long s_n, s_k, c_n, c_k;         // strides of logits and of scores
-    int N, K, V, n, parts;
+    int N, K, V, n, parts, length;        // length: numbers of a part, a multiple of 8
 };
 
-constexpr int THREADS = 256, PER = 16, PART = THREADS * PER, HOLD = 1024, MOST = 128;      // MOST: largest n; HOLD: candidates that fit shared memory
+constexpr int THREADS = 256, PER = 16, CHUNK = THREADS * PER, HOLD = 1024, MOST = 128;      // MOST: largest n; HOLD: candidates that fit shared memory
+constexpr int MANY = 512;                                    // candidates from which on a closer bound is worth its search
 
 template <typename T> __device__ __forceinline__ float number(T x);
 template <> __device__ __forceinline__ float number(float x) { return x; }
@@ -37,149 +39,300 @@ template <> __device__ __forceinline__ float number(bf16 x) { return __bfloat162
 template <> __device__ __forceinline__ float number(__half x) { return __half2float(x); }
 
 // Candidates in shared memory: keys and places (negative: none).  Better: larger key, or the lower place.
-template <typename Key> struct Pool {
+template <typename Key, int BLOCK> struct Pool {
     Key key[HOLD];
     int at[HOLD];
-    Key tmax[THREADS];
-    Key bound;
+    Key last[BLOCK];                          // (one by one) a thread's best
+    int bound[BLOCK / 32], some[2][BLOCK / 32];
     int count;
-    int winner;
 };
 template <typename Key> __device__ __forceinline__ bool better(Key a, int ia, Key b, int ib) { return a > b || (a == b && ia < ib); }
+// fp32 numbers in the order of signed integers, and back
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(x);
+    return i ^ (i >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ long long ordered64(double x) {
+    const long long i = __double_as_longlong(x);
+    return i ^ (i >> 63 & 0x7fffffffffffffffLL);
+}
+__device__ __forceinline__ double number64_of(long long i) { return __longlong_as_double(i ^ (i >> 63 & 0x7fffffffffffffffLL)); }
+__device__ __forceinline__ float number_of(int i) { return __int_as_float(i ^ (i >> 31 & 0x7fffffff)); }
 
-// The n best of every thread's `mine` candidates (key(i), place(i)), in order, given to put(rank, key, place); `total` of them are real, and at least min(n, total) are given.
-// best: the thread's largest key (minus infinity: none).  The whole block calls it.
-template <typename Key, int BLOCK, typename KeyOf, typename PlaceOf, typename Put>
-__device__ __forceinline__ void best_of(Pool<Key>& sm, int n, int total, int mine, Key best, KeyOf key, PlaceOf place, Put put) {
+// Where more than MANY keys reach the first bound: the largest bound that n keys reach, by halving, then its keys into shared memory.  Keys are read from memory again: out of line, this
+// costs the usual path no registers.  hi: one above the largest.
+template <typename Key, int BLOCK, typename Keys>
+__device__ __noinline__ int closer(Pool<Key, BLOCK>& sm, int n, int lo, int most, const Keys ks) {
+    constexpr int W = BLOCK / 32;
     const int t = threadIdx.x;
-    sm.tmax[t] = best;
+    long long low = lo, hi = (long long)most + 1;            // n keys or more reach low, fewer than n reach hi
+    for (int step = 0; hi - low > 1; ++step) {
+        const int mid = (int)((low + hi) >> 1);
+        int c = 0;
+        for (int i = t; i < ks.count; i += BLOCK) c += ks.place(i) >= 0 && ordered(ks.near(i)) >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (t % 32 == 0) sm.some[step & 1][t >> 5] = c;
+        __syncthreads();
+        c = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) c += sm.some[step & 1][i];
+        if (c >= n) low = mid;
+        else hi = mid;
+    }
+    __syncthreads();                                         // the count so far has been read
     if (t == 0) sm.count = 0;
     __syncthreads();
-    // the n-th largest of the maxima (with fewer real candidates than threads: minus infinity lets all pass)
-    int rank = 0;
-    for (int i = 0; i < BLOCK; ++i) rank += better<Key>(sm.tmax[i], i, best, t);
-    if (rank == min(n, BLOCK) - 1) sm.bound = n <= BLOCK ? best : (Key)-INFINITY;
-    __syncthreads();
-    const Key bound = sm.bound;
-    for (int i = 0; i < mine; ++i)
-        if (place(i) >= 0 && key(i) >= bound) {
+    for (int i = t; i < ks.count; i += BLOCK)
+        if (ks.place(i) >= 0 && ordered(ks.near(i)) >= (int)low) {
             const int c = atomicAdd(&sm.count, 1);
-            if (c < HOLD) sm.key[c] = key(i), sm.at[c] = place(i);
+            if (c < HOLD) sm.key[c] = ks.key(i), sm.at[c] = ks.place(i);
         }
     __syncthreads();
-    const int count = sm.count;
-    if (count <= HOLD) {
-        for (int c = t; c < count; c += BLOCK) {
-            const Key x = sm.key[c];
-            const int at = sm.at[c];
-            int r = 0;
-            for (int i = 0; i < count; ++i) r += better<Key>(sm.key[i], sm.at[i], x, at);
-            if (r < n) put(r, x, at);
-        }
-        return;
-    }
-    // many equal keys: one after the other, each the best of those behind the last
-    Key last = (Key)INFINITY;
+    return sm.count;
+}
+template <typename Key> struct Top;                          // a key above all and one below all
+template <> struct Top<float> {
+    static __device__ float value() { return INFINITY; }
+    static __device__ float none() { return -INFINITY; }
+};
+template <> struct Top<long long> {
+    static __device__ long long value() { return 0x7fffffffffffffffLL; }
+    static __device__ long long none() { return -0x7fffffffffffffffLL - 1; }
+};
+// Many equal keys: one after the other, each the best of those behind the last.
+template <typename Key, int BLOCK, typename Keys, typename Put>
+__device__ __noinline__ void one_by_one(Pool<Key, BLOCK>& sm, int n, const Keys ks, const Put put) {
+    const int t = threadIdx.x;
+    Key last = Top<Key>::value();
     int last_at = -1;
-    for (int r = 0; r < min(n, total); ++r) {
-        Key bk = (Key)-INFINITY;
+    for (int r = 0; r < n; ++r) {
+        Key bk = Top<Key>::none();
         int ba = 0x7fffffff;
-        for (int i = 0; i < mine; ++i) {
-            const Key x = key(i);
-            const int at = place(i);
+        for (int i = t; i < ks.count; i += BLOCK) {
+            const Key x = ks.key(i);
+            const int at = ks.place(i);
             if (at >= 0 && (x < last || (x == last && at > last_at)) && better<Key>(x, at, bk, ba)) bk = x, ba = at;
         }
         __syncthreads();                                     // the winner of the round before has been read
-        sm.tmax[t] = bk;
+        sm.last[t] = bk;
         sm.at[t] = ba;
         __syncthreads();
         for (int s = BLOCK / 2; s > 0; s >>= 1) {
-            if (t < s && better<Key>(sm.tmax[t + s], sm.at[t + s], sm.tmax[t], sm.at[t])) sm.tmax[t] = sm.tmax[t + s], sm.at[t] = sm.at[t + s];
+            if (t < s && better<Key>(sm.last[t + s], sm.at[t + s], sm.last[t], sm.at[t])) sm.last[t] = sm.last[t + s], sm.at[t] = sm.at[t + s];
             __syncthreads();
         }
-        last = sm.tmax[0], last_at = sm.at[0];
+        last = sm.last[0], last_at = sm.at[0];
         if (t == 0) put(r, last, last_at);
     }
 }
 
+// A bound that at least n keys reach, and an empty pool: with w warps that have candidates, the n / w-th largest of the threads' maxima in each of them, the smallest of these.
+// best: the thread's largest key (minus infinity: none; rounding to fp32 keeps the order).  The whole block calls it.
+template <typename Key, int BLOCK>
+__device__ __forceinline__ float first_bound(Pool<Key, BLOCK>& sm, int n, float best) {
+    const int t = threadIdx.x, lane = t & 31;
+    int v = ordered(best), top = 0x80000000;
+    const int first = __reduce_max_sync(0xffffffffu, v), none = ordered(-INFINITY);
+    if (t == 0) sm.count = 0;
+    const int warps = __syncthreads_count(lane == 0 && first != none), rounds = (n + warps - 1) / max(warps, 1);
+    for (int r = 0; r < min(rounds, 33); ++r) {              // (of 32 maxima the 33rd is below all)
+        top = r == 0 ? first : __reduce_max_sync(0xffffffffu, v);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, v == top)) - 1) v = 0x80000000;
+    }
+    if (lane == 0) sm.bound[t >> 5] = first != none ? max(top, none) : 0x7fffffff;
+    __syncthreads();
+    int bound = sm.bound[0];
+#pragma unroll
+    for (int i = 1; i < BLOCK / 32; ++i) bound = min(bound, sm.bound[i]);
+    return warps == 0 ? -INFINITY : number_of(bound);
+}
+// The n best of the pool's candidates (all keys from `bound` on, none above `most`), in order, given to put(rank, key, place); of `total` candidates that there are, also in memory (ks),
+// min(n, total) are given.  The whole block calls it.
+template <typename Key, int BLOCK, typename Keys, typename Put>
+__device__ __forceinline__ void best_of(Pool<Key, BLOCK>& sm, int n, int total, float bound, float most, const Keys ks, const Put put) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    int count = sm.count;
+    if (count > MANY && total > n && bound < most) count = closer<Key, BLOCK>(sm, n, ordered(bound), ordered(most), ks);
+    if (count > HOLD) return one_by_one<Key, BLOCK>(sm, min(n, total), ks, put);
+    for (int c = t; c < count; c += BLOCK) {
+        const Key x = sm.key[c];
+        const int at = sm.at[c];
+        int r = 0;
+        for (int i = 0; i < count; ++i) r += better<Key>(sm.key[i], sm.at[i], x, at);
+        if (r < n) put(r, x, at);
+    }
+}
+// The largest number of the block's threads' ones.
+template <int BLOCK> __device__ __forceinline__ float block_top(float x, float* red) {
+    x = warp_max(x);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = red[0];
+#pragma unroll
+    for (int i = 1; i < BLOCK / 32; ++i) x = fmaxf(x, red[i]);
+    return x;
+}
+template <typename Key, int BLOCK> __device__ __forceinline__ void keep(Pool<Key, BLOCK>& sm, Key k, int at) {
+    const int c = atomicAdd(&sm.count, 1);
+    if (c < HOLD) sm.key[c] = k, sm.at[c] = at;
+}
+
+template <typename T> __device__ __forceinline__ T nothing();
+template <> __device__ __forceinline__ float nothing() { return -INFINITY; }
+template <> __device__ __forceinline__ bf16 nothing() { return __ushort_as_bfloat16(0xff80); }
+template <> __device__ __forceinline__ __half nothing() { return __ushort_as_half(0xfc00); }
+template <typename T> struct PartKeys {                      // the tokens [lo, lo + count) of a row
+    const T* x;
+    int lo, count;
+    __device__ float key(int i) const { return fmaxf(number<T>(x[lo + i]), -INFINITY); }
+    __device__ float near(int i) const { return key(i); }
+    __device__ int place(int i) const { return lo + i; }
+};
+struct PartPut {
+    float* key;
+    int* at;
+    __device__ void operator()(int r, float k, int p) const { key[r] = k; at[r] = p; }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS) beam_parts_kernel(Args a) {
-    constexpr int VN = 16 / sizeof(T);
-    __shared__ Pool<float> sm;
+__global__ void __launch_bounds__(THREADS, 4) beam_parts_kernel(Args a) {
+    constexpr int VN = 16 / sizeof(T), VECS = PER / VN;
+    __shared__ Pool<float, THREADS> sm;
     __shared__ float red[THREADS / 32];
-    __shared__ double dred[THREADS / 32];
+    __shared__ double sums[THREADS / 32];
+    __shared__ float closer_bound;
     const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x, w = t >> 5, lane = t & 31;
     const T* x = (const T*)a.logits + row / a.K * a.s_n + row % a.K * a.s_k;
     // vectors lie on 16-byte boundaries: the part begins up to VN - 1 numbers early, and those belong to nobody
     const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int base = part * PART - skew;                     // token of the part's first number
-    const int lo = max(base, 0), hi = min(base + PART, a.V);
-    float v[PER];
+    const int base = part * a.length - skew;                 // token of the part's first number
+    const int lo = max(base, 0), hi = min(base + a.length, a.V), total = max(hi - lo, 0), chunks = (a.length + CHUNK - 1) / CHUNK;
+    const long long slot = (long long)row * a.parts + part;
+    const PartPut put{a.key + slot * a.n, a.at + slot * a.n};
+    auto load = [&](int c, uint4 (&raw)[VECS]) {
 #pragma unroll
-    for (int i = 0; i < PER / VN; ++i) {
-        const int at = base + (i * THREADS + t) * VN;
-        if (at >= lo && at + VN <= hi) {
-            const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + at));
-            const T* p = reinterpret_cast<const T*>(&raw);
+        for (int i = 0; i < VECS; ++i) {
+            const int at = base + c * CHUNK + (i * THREADS + t) * VN;
+            if (at >= lo && at + VN <= hi) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + at));
+            else {
+                T* p = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+                for (int e = 0; e < VN; ++e) p[e] = at + e >= lo && at + e < hi ? x[at + e] : nothing<T>();
+            }
+        }
+    };
+    uint4 raw[VECS];
+    load(0, raw);
+    float top = -INFINITY, s = 0.f, bound = -INFINITY;       // the thread's largest logit so far, its sum in units of that
+    for (int c = 0; c < chunks; ++c) {
+        float v[PER];
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+            const T* p = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
             for (int e = 0; e < VN; ++e) v[i * VN + e] = fmaxf(number<T>(p[e]), -INFINITY);      // NaN -> -inf
-        } else {
+        }
+        if (c + 1 < chunks) load(c + 1, raw);                // on its way while this chunk is looked at
+        float best = v[0];
 #pragma unroll
-            for (int e = 0; e < VN; ++e) v[i * VN + e] = at + e >= lo && at + e < hi ? fmaxf(number<T>(x[at + e]), -INFINITY) : -INFINITY;
+        for (int i = 1; i < PER; ++i) best = fmaxf(best, v[i]);
+        if (best > top) {
+            s *= top == -INFINITY ? 0.f : __expf(top - best);
+            top = best;
+        }
+        if (top != -INFINITY)
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) s += (__expf(v[i] - top) + __expf(v[i + 1] - top)) + (__expf(v[i + 2] - top) + __expf(v[i + 3] - top));
+        if (c == 0) bound = first_bound<float, THREADS>(sm, a.n, best);
+        if (best >= bound) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (v[i] >= bound) {
+                    const int p = base + c * CHUNK + (i / VN * THREADS + t) * VN + i % VN;
+                    if (p >= lo && p < hi) keep(sm, v[i], p);
+                }
+        }
+        if (c == 0 && chunks > 1) {                          // what the chunks behind this one have to reach: its own n-th best
+            __syncthreads();
+            const int count = sm.count;
+            if (t == 0) closer_bound = bound;
+            __syncthreads();
+            if (count <= HOLD)
+                for (int i = t; i < count; i += THREADS) {
+                    int r = 0;
+                    for (int j = 0; j < count; ++j) r += better<float>(sm.key[j], sm.at[j], sm.key[i], sm.at[i]);
+                    if (r == a.n - 1) closer_bound = sm.key[i];
+                }
+            __syncthreads();
+            bound = closer_bound;
         }
     }
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
-    const float mine = top;
-    top = warp_max(top);
-    if (lane == 0) red[w] = top;
-    __syncthreads();
-    top = red[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) top = fmaxf(top, red[i]);
-    float s = 0.f;
-    const float unit = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int i = 0; i < PER; i += 4) s += (__expf(v[i] - unit) + __expf(v[i + 1] - unit)) + (__expf(v[i + 2] - unit) + __expf(v[i + 3] - unit));
+    pdl_trigger();
+    const float most = block_top<THREADS>(top, red);
+    s = top == -INFINITY ? 0.f : s * __expf(top - most);
     s = warp_sum(s);
-    if (lane == 0) dred[w] = (double)s;
-    __syncthreads();
-    const long long slot = (long long)row * a.parts + part;
-    if (t == 0) {
+    if (lane == 0) sums[w] = (double)s;
+    for (int r = total + t; r < a.n; r += THREADS) put.at[r] = -1;            // fewer tokens than candidates
+    best_of<float, THREADS>(sm, a.n, total, bound, most, PartKeys<T>{x, lo, total}, put);
+    if (t == 0) {                                            // behind best_of's barriers
         double d = 0.;
-        for (int i = 0; i < THREADS / 32; ++i) d += dred[i];
-        a.top[slot] = top;
+        for (int i = 0; i < THREADS / 32; ++i) d += sums[i];
+        a.top[slot] = most;
         a.sum[slot] = d;
     }
-    const int total = max(hi - lo, 0);
-    float* key = a.key + slot * a.n;
-    int* at = a.at + slot * a.n;
-    for (int r = total + t; r < a.n; r += THREADS) at[r] = -1;            // fewer tokens than candidates
-    best_of<float, THREADS>(
-        sm, a.n, total, PER, mine, [&](int i) { return v[i]; },
-        [&](int i) {
-            const int p = base + (i / VN * THREADS + t) * VN + i % VN;
-            return p >= lo && p < hi ? p : -1;
-        },
-        [&](int r, float k, int p) { key[r] = k; at[r] = p; });
 }
 
-constexpr int JOIN = 256;
+// The parts' candidates of a prompt, with their scores in 64 bits (as integers of the same order: the ranks are counted with integer comparisons).
+struct JoinKeys {
+    const float* logit;
+    const int* token;
+    const double* add;
+    const float* tops;
+    int per_beam, V, count;
+    __device__ double score(float x, int c) const {
+        const int b = c / per_beam;
+        const double k = ((double)x - tops[b]) + add[b];
+        return k == k ? k : -INFINITY;
+    }
+    __device__ long long key(int c) const { return ordered64(score(logit[c], c)); }
+    __device__ float near(int c) const { return (float)score(logit[c], c); }
+    __device__ int place(int c) const { return token[c] < 0 ? -1 : c / per_beam * V + token[c]; }
+};
+struct JoinPut {
+    float* out;
+    long long *beam, *token;
+    int V;
+    __device__ void operator()(int r, long long k, int p) const { out[r] = (float)number64_of(k); beam[r] = p / V; token[r] = p % V; }
+};
+constexpr int JOIN = 512, CANDS = 8;                         // candidates that a thread holds at a time
 __global__ void __launch_bounds__(JOIN) beam_join_kernel(Args a) {
-    __shared__ Pool<double> sm;
+    __shared__ Pool<long long, JOIN> sm;
     __shared__ double add[MOST];                             // s_b - log of the sum in units of the largest logit, which the candidates are measured from too:
     __shared__ float tops[MOST];                             // logits of the type's lowest value would lose the rest
+    __shared__ __align__(16) float heads[JOIN];
+    __shared__ float red[JOIN / 32], head_bound;
     pdl_wait();
     const int prompt = blockIdx.x, t = threadIdx.x, w = t >> 5, lane = t & 31;
+    const int per_beam = a.parts * a.n, all = a.K * per_beam, lists = a.K * a.parts;
+    const long long c0 = (long long)prompt * all, o0 = (long long)prompt * a.n;
+    const JoinKeys ks{a.key + c0, a.at + c0, add, tops, per_beam, a.V, all};
+    float logit[CANDS];
+    int token[CANDS];
+#pragma unroll
+    for (int i = 0; i < CANDS; ++i) {
+        const int c = t + i * JOIN;
+        logit[i] = c < all ? ks.logit[c] : -INFINITY;
+        token[i] = c < all ? ks.token[c] : -1;
+    }
     for (int b = w; b < a.K; b += JOIN / 32) {
         const long long r0 = ((long long)prompt * a.K + b) * a.parts;
         float top = -INFINITY;
-        for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, __ldcg(a.top + r0 + i));
+        for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, a.top[r0 + i]);
         top = warp_max(top);
         double s = 0.;
         if (top != -INFINITY)
-            for (int i = lane; i < a.parts; i += 32) s += __ldcg(a.sum + r0 + i) * exp((double)(__ldcg(a.top + r0 + i) - top));
+            for (int i = lane; i < a.parts; i += 32) s += a.sum[r0 + i] * (double)__expf(a.top[r0 + i] - top);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) {
@@ -187,27 +340,46 @@ __global__ void __launch_bounds__(JOIN) beam_join_kernel(Args a) {
             tops[b] = top == -INFINITY ? 0.f : top;
         }
     }
+    if (t == 0) sm.count = 0;
     __syncthreads();
-    const int per_beam = a.parts * a.n, all = a.K * per_beam, mine = t < all ? (all - t + JOIN - 1) / JOIN : 0;
-    const long long c0 = (long long)prompt * all;
-    auto key = [&](int i) -> double {
-        const int c = t + i * JOIN;
-        const double k = ((double)__ldcg(a.key + c0 + c) - tops[c / per_beam]) + add[c / per_beam];
-        return k == k ? k : -INFINITY;
-    };
-    auto place = [&](int i) -> int {
-        const int c = t + i * JOIN, p = __ldcg(a.at + c0 + c);
-        return p < 0 ? -1 : c / per_beam * a.V + p;
-    };
-    double best = -INFINITY;
-    for (int i = 0; i < mine; ++i)
-        if (place(i) >= 0) best = fmax(best, key(i));
-    best_of<double, JOIN>(sm, a.n, a.n, mine, best, key, place, [&](int r, double k, int p) {
-        const long long o = (long long)prompt * a.n + r;
-        a.out[o] = (float)k;
-        a.beam[o] = p / a.V;
-        a.token[o] = p % a.V;
-    });
+    // A bound that n candidates reach: the n-th largest of the parts' best ones (their first `deep` each), if these are few enough to be counted
+    const int deep = (a.n + lists - 1) / lists, m = lists * deep;
+    double k[CANDS], best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < CANDS; ++i) {
+        k[i] = token[i] >= 0 ? ks.score(logit[i], t + i * JOIN) : -INFINITY;
+        best = fmax(best, k[i]);
+    }
+    float bound;
+    if (m <= JOIN) {
+        const int c = t / deep * a.n + t % deep;
+        const float mine = t < m && ks.token[c] >= 0 ? ks.near(c) : -INFINITY;
+        heads[t] = mine;
+        __syncthreads();
+        int r = 0;
+        for (int i = 0; i < m; i += 4) {
+            const float4 y = load4(heads + i);
+            r += better<float>(y.x, i, mine, t) + better<float>(y.y, i + 1, mine, t) + better<float>(y.z, i + 2, mine, t) + better<float>(y.w, i + 3, mine, t);
+        }
+        if (t < m && r == a.n - 1) head_bound = mine;        // (behind the m-th are only minus infinities of higher places)
+        __syncthreads();
+        bound = head_bound;
+    } else {
+        for (int c = t + CANDS * JOIN; c < all; c += JOIN)
+            if (ks.token[c] >= 0) best = fmax(best, (double)ks.near(c));
+        bound = first_bound<long long, JOIN>(sm, a.n, (float)best);
+    }
+    // candidates beyond the held ones (larger vocabularies, wider beams) are read again
+#pragma unroll
+    for (int i = 0; i < CANDS; ++i)
+        if (token[i] >= 0 && (float)k[i] >= bound) keep(sm, ordered64(k[i]), (t + i * JOIN) / per_beam * a.V + token[i]);
+    for (int c = t + CANDS * JOIN; c < all; c += JOIN)
+        if (ks.token[c] >= 0 && ks.near(c) >= bound) {
+            best = fmax(best, (double)ks.near(c));
+            keep(sm, ks.key(c), ks.place(c));
+        }
+    const float most = block_top<JOIN>((float)best, red);
+    best_of<long long, JOIN>(sm, a.n, 0x7fffffff, bound, most, ks, JoinPut{a.out + o0, a.beam + o0, a.token + o0, a.V});
 }
 
 template <typename T>
@@ -228,7 +400,7 @@ struct Rows {
     int tensors;
     int* err;
 };
-constexpr int CHUNK = 32768;                                 // bytes of a row that a CTA takes
+constexpr int SLAB = 32768;                                 // bytes of a row that a CTA takes
 template <typename V>
 __device__ __forceinline__ void copy_as(const char* src, char* dst, long long n) {
     const V* s = reinterpret_cast<const V*>(src);
@@ -247,12 +419,12 @@ __device__ __forceinline__ void copy_as(const char* src, char* dst, long long n)
 }
 __global__ void __launch_bounds__(THREADS) copy_rows_kernel(const __grid_constant__ Rows a) {
     const int k = blockIdx.z;
-    const long long off = (long long)blockIdx.x * CHUNK, n = min(a.bytes[k] - off, (long long)CHUNK);
+    const long long off = (long long)blockIdx.x * SLAB, n = min(a.bytes[k] - off, (long long)SLAB);
     if (n <= 0) return;
     for (long long r = blockIdx.y; r < a.count; r += gridDim.y) {
         const long long from = __ldg(a.from + r), to = a.to != nullptr ? __ldg(a.to + r) : r;
         if (from < 0 || from >= a.rows[k] || (a.to != nullptr && (to < 0 || to >= a.rows[k]))) {
-            if (threadIdx.x == 0) atomicCAS(a.err, 0, 0xb300);
+            if (threadIdx.x == 0) atomicCAS(a.err, 0, 0x13000);
             continue;
         }
         const char* s = (const char*)a.src[k] + from * a.bytes[k] + off;
@@ -273,7 +445,8 @@ LMOE_API int lmoe_beam_select(const lmoe::beam::Args* ap, int type, cudaStream_t
     using namespace lmoe::beam;
     const Args& a = *ap;
     if (a.N <= 0 || a.K <= 0 || a.K > MOST || a.V <= 0 || a.n <= 0 || a.n > MOST || (long long)a.N * a.K > 65535 || (long long)a.K * a.V > 0x7fffffff ||
-        (long long)a.K * a.V < a.n || (long long)a.parts * PART < (long long)a.V + 7 || (long long)a.K * a.parts * a.n > 0x7fffffff) return -1;
+        (long long)a.K * a.V < a.n || a.length <= 0 || a.length % 8 != 0 ||
+        (long long)a.parts * a.length < (long long)a.V + 7 || (long long)a.K * a.parts * a.n > 0x7fffffff) return -1;
     return type == 0 ? select<float>(a, st) : type == 1 ? select<lmoe::bf16>(a, st) : select<__half>(a, st);
 }
 
@@ -283,7 +456,7 @@ LMOE_API int lmoe_copy_rows(const lmoe::beam::Rows* ap, cudaStream_t st) {
     if (a.tensors < 1 || a.tensors > TENSORS || a.count < 1) return -1;
     long long most = 1;
     for (int i = 0; i < a.tensors; ++i) most = a.bytes[i] > most ? a.bytes[i] : most;
-    const long long chunks = (most + CHUNK - 1) / CHUNK;
+    const long long chunks = (most + SLAB - 1) / SLAB;
     if (chunks > 0x7fffffff) return -1;
     copy_rows_kernel<<<dim3((unsigned)chunks, (unsigned)(a.count < 65535 ? a.count : 65535), a.tensors), THREADS, 0, st>>>(a);
     return (int)cudaGetLastError();

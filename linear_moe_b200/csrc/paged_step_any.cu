@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) paged_step_any_kernel(const Ar
     const T *q = (const T*)a.q + b * a.q_b + h * a.q_h, *kn = (const T*)a.k_new + b * a.n_b + hk * a.n_h, *vn = (const T*)a.v_new + b * a.m_b + hk * a.m_h;
     T *kc = (T*)a.k + hk * a.k_head, *vc = (T*)a.v + hk * a.v_head;
     const Share sh = share_of(a, b);
-    if (threadIdx.x == 0 && h == 0 && a.lengths[b] != sh.len) atomicCAS(a.err, 0, 0xb100);
+    if (threadIdx.x == 0 && h == 0 && a.lengths[b] != sh.len) atomicCAS(a.err, 0, 0x11000);
     const bool fresh = a.k_new != nullptr;
     if (fresh && h % (a.H / a.G) == 0 && sh.len > 0) {
         const int key = sh.len - 1, page = a.table[b * a.table_ld + key / a.page];
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) paged_step_any_kernel(const Ar
     for (int key = sh.lo + w; key < sh.len; key += ANY_WARPS) {
         const int page = a.table[b * a.table_ld + key / a.page];
         if (page < 0 || page >= a.pages) {
-            if (lane == 0) atomicCAS(a.err, 0, 0xb200);
+            if (lane == 0) atomicCAS(a.err, 0, 0x12000);
             continue;
         }
         const bool mine = fresh && key == sh.len - 1;

@@ -12,13 +12,13 @@ import torch
 
 from .scored_attn import on_device
 
-PART, MOST, TENSORS = 4096, 128, 64                       # csrc/beam.cu
+CHUNK, MOST, TENSORS = 4096, 128, 64                      # csrc/beam.cu
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class _Args(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "scores", "out", "beam", "token", "key", "top", "at", "sum")] +
-                [(n, ctypes.c_longlong) for n in ("s_n", "s_k", "c_n", "c_k")] + [(n, ctypes.c_int) for n in ("N", "K", "V", "n", "parts")])
+                [(n, ctypes.c_longlong) for n in ("s_n", "s_k", "c_n", "c_k")] + [(n, ctypes.c_int) for n in ("N", "K", "V", "n", "parts", "length")])
 
 
 class _Rows(ctypes.Structure):
@@ -40,70 +40,73 @@ def _eager_select(logits, scores, n):
     return best.float(), at // V, at % V
 
 
-@torch.no_grad()
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``logits [N, K, V]`` (fp32, bf16 or fp16) and ``scores [N, K]`` (fp32) of N prompts with K beams: ``(scores fp32, beam int64, token int64)``, each ``[N, n]``,
-    best first."""
-    if logits.dim() != 3 or scores.shape != logits.shape[:2] or logits.dtype not in _TYPES or scores.dtype != torch.float32:
+    best first.  No gradient."""
+    kind, shape, dev = _TYPES.get(logits.dtype), logits.shape, logits.device
+    if len(shape) != 3 or scores.shape != shape[:2] or kind is None or scores.dtype != torch.float32:
         raise ValueError("beam selection takes logits [N, K, V] in fp32, bf16 or fp16 and fp32 scores [N, K]")
-    if scores.device != logits.device:
+    if scores.device != dev:
         raise ValueError("logits and scores lie on one device")
-    N, K, V = logits.shape
+    N, K, V = shape
     if not 1 <= n <= K * V:
         raise ValueError(f"{n} continuations of {K} beams over a vocabulary of {V}")
     if not logits.is_cuda or n > MOST or K > MOST or N * K > 65535 or K * V >= 1 << 31 or N == 0:      # wider searches than the kernels hold
-        return _eager_select(logits, scores, n)
+        with torch.no_grad():
+            return _eager_select(logits, scores, n)
     from . import cuda as Kn
-    dev = logits.device
-    logits = logits if logits.stride(2) == 1 or V == 1 else logits.contiguous()
-    out, ids = torch.empty(N, n, dtype=torch.float32, device=dev), torch.empty(2, N, n, dtype=torch.int64, device=dev)
-    parts = -(-(V + 7) // PART)                            # rows may begin up to seven numbers behind a 16-byte boundary
+    s_n, s_k, s_v = logits.stride()
+    if s_v != 1 and V > 1:
+        logits = logits.contiguous()
+        s_n, s_k, s_v = logits.stride()
+    out, beam, token = torch.empty((N, n), dtype=torch.float32, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev)
+    # rows may begin up to seven numbers behind a 16-byte boundary; a chunk to a part, or parts for one wave of four CTAs per SM
+    parts = max(1, min(-(-(V + 7) // CHUNK), 4 * Kn.num_sms() // (N * K)))
     rows = N * K * parts
-    work = torch.empty(rows * 3 + rows * n * 2, dtype=torch.float32, device=dev)      # sums (64 bits), maxima, candidates
-    a, p = _Args(), work.data_ptr()
-    a.logits, a.scores, a.out, a.beam, a.token = logits.data_ptr(), scores.data_ptr(), out.data_ptr(), ids.data_ptr(), ids[1].data_ptr()
-    a.sum, a.top, a.key, a.at = p, p + rows * 8, p + rows * 12, p + rows * (12 + 4 * n)
-    a.s_n, a.s_k, a.c_n, a.c_k = logits.stride(0), logits.stride(1), scores.stride(0), scores.stride(1)
-    a.N, a.K, a.V, a.n, a.parts = N, K, V, n, parts
+    work = torch.empty(rows * (3 + 2 * n), dtype=torch.float32, device=dev)      # sums (64 bits), maxima, candidates
+    p = work.data_ptr()
+    c_n, c_k = scores.stride()
+    a = _Args(logits.data_ptr(), scores.data_ptr(), out.data_ptr(), beam.data_ptr(), token.data_ptr(), p + rows * 12, p + rows * 8, p + rows * (12 + 4 * n), p, s_n, s_k,
+              c_n, c_k, N, K, V, n, parts, -(-(V + 7) // (parts * 8)) * 8)
     with on_device(logits):
-        Kn._check(Kn.lib().lmoe_beam_select(ctypes.byref(a), ctypes.c_int(_TYPES[logits.dtype]), Kn._st()), "beam_select", 2)
-    return out, ids[0], ids[1]
+        Kn._check(Kn.lib().lmoe_beam_select(ctypes.byref(a), kind, Kn._st()), "beam_select", 2)
+    return out, beam, token
 
 
 def _copy_rows(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], rows: int, from_, to):
     from . import cuda as K
-    from . import gemm
     a = _Rows()
-    a.from_, a.to, a.count, a.err = from_.data_ptr(), K._ptr(to), rows, gemm._err(from_.device).data_ptr()
+    a.from_, a.to, a.count, a.err = from_.data_ptr(), K._ptr(to), rows, K.error_word(from_.device)
     with on_device(from_):
         for first in range(0, len(src), TENSORS):
             some = src[first:first + TENSORS]
-            for i, (s, d) in enumerate(zip(some, dst[first:first + TENSORS])):
-                a.src[i], a.dst[i], a.rows[i] = s.data_ptr(), d.data_ptr(), s.shape[0]
-                a.bytes[i] = s.numel() // max(s.shape[0], 1) * s.element_size()
-            a.tensors = len(some)
+            n = len(some)
+            a.src[:n], a.dst[:n] = [t.data_ptr() for t in some], [t.data_ptr() for t in dst[first:first + TENSORS]]
+            a.rows[:n] = counts = [t.shape[0] for t in some]
+            a.bytes[:n] = [t.nbytes // max(r, 1) for t, r in zip(some, counts)]
+            a.tensors = n
             K._check(K.lib().lmoe_copy_rows(ctypes.byref(a), K._st()), "copy_rows")
 
 
-@torch.no_grad()
 def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor) -> List[torch.Tensor]:
     """``[t[parents] for t in states]`` for states with one row per beam and ``parents`` int64 ``[rows]``.  A number that is no row raises on the CPU; on CUDA its row is left
-    undefined and the kernels' error word is set."""
+    undefined and the kernels' error word is set.  No gradient."""
     if parents.dtype != torch.int64 or parents.dim() != 1:
         raise ValueError("parents is an int64 tensor [rows]")
+    dev, n = parents.device, parents.shape[0]
     for t in states:
-        if t.dim() < 1 or t.device != parents.device:
+        if t.dim() < 1 or t.device != dev:
             raise ValueError("a state has a row per beam and lies where the parents are")
     if not parents.is_cuda:
-        return [t.index_select(0, parents) for t in states]
-    out = [torch.empty(parents.shape[0], *t.shape[1:], dtype=t.dtype, device=t.device) for t in states]
-    work = [(t if t.is_contiguous() else t.contiguous(), o) for t, o in zip(states, out) if o.numel()]
-    if work:
-        _copy_rows([s for s, _ in work], [d for _, d in work], parents.shape[0], parents.contiguous(), None)
+        with torch.no_grad():
+            return [t.index_select(0, parents) for t in states]
+    out = [torch.empty((n, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
+    some = [(t if t.is_contiguous() else t.contiguous(), o) for t, o in zip(states, out) if o.numel()]
+    if some:
+        _copy_rows([t for t, _ in some], [o for _, o in some], n, parents if parents.is_contiguous() else parents.contiguous(), None)
     return out
 
 
-@torch.no_grad()
 def copy_pages_(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]):
     """``pool[dst[i]] = pool[src[i]]`` in every pool ``[pages, ...]``.  The pages written are all different and none of them is read."""
     if len(src) != len(dst) or len(set(dst)) != len(dst) or set(dst) & set(src):
@@ -118,7 +121,8 @@ def copy_pages_(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
         return
     at = torch.tensor([list(src), list(dst)], dtype=torch.int64, device=pools[0].device)
     if not pools[0].is_cuda:
-        for t in pools:
-            t[at[1]] = t[at[0]]
+        with torch.no_grad():
+            for t in pools:
+                t[at[1]] = t[at[0]]
         return
     _copy_rows(pools, pools, len(src), at[0], at[1])

@@ -102,6 +102,23 @@ def _check(rc: int, name: str, n: int = 1):
     launch_count += n
 
 
+_ERROR_WORDS: dict = {}
+
+
+def error_word(device) -> int:
+    """Address of the kernels' error word on ``device``: ``gemm._err``, or on a device that it does not lie on a word of that device's own
+    (``gemm.check_error`` reads them all)."""
+    t = _ERROR_WORDS.get(device)
+    if t is None:
+        from . import gemm
+        t = gemm._err(device)
+        if t.device != device:
+            t = torch.zeros(1, dtype=torch.int32, device=device)
+            gemm.OTHER_WORDS.append(t)
+        _ERROR_WORDS[device] = t
+    return t.data_ptr()
+
+
 _i64, _i32, _f32 = ctypes.c_int64, ctypes.c_int, ctypes.c_float
 
 

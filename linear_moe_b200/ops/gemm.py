@@ -43,12 +43,19 @@ def _err(device) -> torch.Tensor:
     return _ERR
 
 
+OTHER_WORDS: list = []          # error words of devices that the status tensor does not lie on (``cuda.error_word``)
+
+
 def check_error():
-    if _ERR is not None:
-        v = int(_ERR.item())
+    for word in ([] if _ERR is None else [_ERR]) + OTHER_WORDS:
+        v = int(word.item())
         if v != 0:
-            _ERR.zero_()
-            raise RuntimeError(f"tcgen05 GEMM: bounded wait expired (code {v:#x})")
+            word.zero_()
+            raise RuntimeError(f"tcgen05 GEMM: bounded wait expired (code {v:#x})" if v < 0x10000 else _ERRORS.get(v & 0xff000, f"kernel error {v:#x}") + f" (code {v:#x})")
+
+
+_ERRORS = {0x11000: "one-token attention: a length outside the page table", 0x12000: "one-token attention: a page number outside the pool",
+           0x13000: "reordering: a row that is none", 0x14000: "one-token attention: a bounded wait expired"}
 
 
 def _ok(t: torch.Tensor) -> bool:

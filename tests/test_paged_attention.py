@@ -114,14 +114,16 @@ def test_refusals():
 
 
 def test_split_rule():
-    """At least one CTA, none of fewer than 256 keys of a long request, about twenty per SM at most."""
+    """At least one part, none of fewer than 128 keys of a long request; one wave of CTAs, or two parts."""
     for B in (1, 2, 8, 64, 1000):
         for G in (1, 2, 8):
             for heads in (1, 8, 9, 33):
-                for keys in (0, 1, 256, 257, 5000, 1 << 20):
-                    n = PA.splits_of(B, G, heads, keys)
-                    assert 1 <= n <= max(1, -(-keys // 256))
-                    assert n == 1 or (n - 1) * B * G < 21 * 148
+                for D in (64, 128):
+                    for keys in (0, 1, 256, 257, 5000, 1 << 20):
+                        n, first = PA.splits_of(B, G, heads, D, keys)
+                        assert 1 <= n <= max(1, -(-keys // 128))
+                        assert n <= 2 or n * B * G <= 4 * 148
+                        assert not first or 1 < B <= 128
 
 
 # ---- on the GPU -----------------------------------------------------------------------------------------------------------------
@@ -156,7 +158,7 @@ def test_windows_and_pages(window, page):
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
 def test_any_number_of_splits(splits, monkeypatch):
     """The parts of a request, more CTAs than it has keys for among them, give the whole."""
-    monkeypatch.setattr(PA, "splits_of", lambda *a: splits)
+    monkeypatch.setattr(PA, "splits_of", lambda *a: (splits, splits % 2))
     s = make([0, 5, 256, 257, 2000, 4097], 8, 2, 128, size=4.0)
     check(s, cap=50.0)
     check(s, 1000)
@@ -199,7 +201,7 @@ def test_pages_and_lengths_that_are_none():
         s["table"][0, 1], s["table"][1, 3] = s["k"].shape[0], -1       # in the middle; the page of the new token
         k0, v0 = s["k"].clone(), s["v"].clone()
         got = ops.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lengths"], k_new=s["k_new"], v_new=s["v_new"])
-        with pytest.raises(RuntimeError, match="0xb200"):
+        with pytest.raises(RuntimeError, match="0x12000"):
             gemm.check_error()
         gemm.check_error()
         assert torch.isfinite(got).all()
@@ -217,13 +219,13 @@ def test_pages_and_lengths_that_are_none():
         s["table"][0] = torch.tensor([0, 1, 2], device="cuda")
         s["lengths"][0] = 10 ** 9
         got = ops.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lengths"])
-        with pytest.raises(RuntimeError, match="0xb100"):
+        with pytest.raises(RuntimeError, match="0x11000"):
             gemm.check_error()
         s["lengths"][0] = 192
         assert torch.equal(got, ops.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lengths"]))
         s["lengths"][0] = -5
         assert (ops.paged_attention(s["q"], s["k"], s["v"], s["table"], s["lengths"]) == 0).all()
-        with pytest.raises(RuntimeError, match="0xb100"):
+        with pytest.raises(RuntimeError, match="0x11000"):
             gemm.check_error()
 
 
