@@ -100,8 +100,9 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor) -> Lis
     if not parents.is_cuda:
         with torch.no_grad():
             return [t.index_select(0, parents) for t in states]
-    out = [torch.empty((n, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
-    some = [(t if t.is_contiguous() else t.contiguous(), o) for t, o in zip(states, out) if o.numel()]
+    states = [t if t.is_contiguous() else t.contiguous() for t in states]
+    out = [torch.empty_like(t) if t.shape[0] == n else torch.empty((n, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
+    some = [(t, o) for t, o in zip(states, out) if o.numel()]
     if some:
         _copy_rows([t for t, _ in some], [o for _, o in some], n, parents if parents.is_contiguous() else parents.contiguous(), None)
     return out

@@ -125,7 +125,8 @@ _KIND = {torch.bfloat16: 0, torch.float16: 1}
 def paged_attention(q, k_pages, v_pages, table, lengths, scale: Optional[float] = None, window: Optional[int] = None, *, softcap: Optional[float] = None,
                     slopes: Optional[torch.Tensor] = None, k_new=None, v_new=None):
     """``[B, H, D]``; see the module.  Forward only."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_pages, v_pages, k_new, v_new)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (k_new is not None and k_new.requires_grad)
+                                    or (v_new is not None and v_new.requires_grad)):
         raise ValueError("one-token attention has no backward pass: use ops.softmax_attention")
     if not q.is_cuda:
         _check(q, k_pages, v_pages, table, lengths, scale, window, softcap, slopes, k_new, v_new)

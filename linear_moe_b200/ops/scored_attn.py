@@ -15,7 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
-from typing import Optional, Sequence
+from typing import Dict, Optional, Sequence
 
 import torch
 
@@ -109,7 +109,7 @@ class _BwdArgs(ctypes.Structure):
 def _strides(t: torch.Tensor):
     """Element strides (batch, token, head) of a tensor that a tensor map can describe, or None.  The stride of a dimension of one is
     never used, whatever the tensor says: it gets the one of a dense tensor."""
-    if t.stride(3) != 1 or t.data_ptr() % 16:
+    if t.stride(3) != 1:
         return None
     out, dense = [0, 0, 0], t.shape[3]
     for i in (2, 1, 0):
@@ -120,80 +120,124 @@ def _strides(t: torch.Tensor):
     return (ctypes.c_longlong * 3)(*out)
 
 
-def _laid_out(t: torch.Tensor):
-    s = _strides(t)
-    if s is None:
-        t = t.clone(memory_format=torch.contiguous_format)
-        s = _strides(t)
-    return t, s
+def _laid_out(t: torch.Tensor) -> torch.Tensor:
+    """The tensor, or a dense copy where no tensor map can describe it."""
+    return t if _strides(t) is not None and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _fill(a, q, k, cfg, first, stop, slopes, low, tiles):
-    from . import gemm
-    scale, causal, q_offset, window, cap = cfg
-    a.B, a.Tq, a.Hq, a.Tk, a.Hkv = q.shape[0], q.shape[1], q.shape[2], k.shape[1], k.shape[2]
-    a.q_offset, a.window, a.scale, a.err = q_offset, window, scale, gemm._err(q.device).data_ptr()
+class _Plan:
+    """What follows from shapes, strides, types and options alone: the arguments without their addresses."""
+    __slots__ = ("eager", "args", "bwd", "qs", "ks", "vs", "ranges", "lse", "tiles", "low", "fwd_fn", "bwd_fn", "copy")
+
+
+_PLANS: Dict[tuple, _Plan] = {}
+
+
+def _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop) -> _Plan:
+    from . import cuda as K
+    _check_options(q, k, v, scale, causal, window, softcap, slopes, first, stop)
+    p, (B, Tq, Hq, D) = _Plan(), q.shape
+    p.eager = (not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float16) or v.shape[3] != D or D > 128 or D % 8 != 0 or Tq > MAX_QUERIES
+               or min(q.numel(), k.numel()) == 0)
+    if p.eager:
+        return p
+    p.qs, p.ks, p.vs = _strides(q), _strides(k), _strides(v)
+    p.ranges = all(r is None or r.stride(-1) == 1 or r.shape[-1] == 1 for r in (first, stop, slopes))
+    p.copy = None in (p.qs, p.ks, p.vs) or not p.ranges
+    fwd, bwd = _Args(), _BwdArgs()
+    for a in (fwd, bwd):
+        a.B, a.Tq, a.Hq, a.Tk, a.Hkv = B, Tq, Hq, k.shape[1], k.shape[2]
+        a.q_offset, a.window, a.scale = int(q_offset), int(window or 0), float(scale) if scale is not None else D ** -0.5
+        a.x.cap, a.x.causal, a.x.d = float(softcap or 0.0), int(bool(causal)), D
+        a.x.first_b, a.x.stop_b = (0 if r is None else r.stride(0) for r in (first, stop))
+    p.args, p.bwd = bytes(fwd), bytes(bwd)
+    p.lse, p.tiles, p.low = B * Hq * Tq * 4, B * -(-Tq // 128) * 16, q.numel() * 2       # bytes
+    half = q.dtype == torch.float16
+    p.fwd_fn = K.lib().lmoe_scored_attn_fwd_fp16 if half else K.lib().lmoe_scored_attn_fwd
+    p.bwd_fn = K.lib().lmoe_scored_attn_bwd_fp16 if half else K.lib().lmoe_scored_attn_bwd
+    return p
+
+
+def _addresses(a, dev, first, stop, slopes, stats: int, low: int, tiles: int):
+    """What a launch reads beside q, k and v: ranges, slopes, and the forward kernel's notes (row statistics, low parts of the output, intervals of the query tiles)."""
+    from . import cuda as K
     x = a.x
     if first is not None:
-        x.first, x.first_b = first.data_ptr(), first.stride(0)
+        x.first = first.data_ptr()
     if stop is not None:
-        x.stop, x.stop_b = stop.data_ptr(), stop.stride(0)
+        x.stop = stop.data_ptr()
     if slopes is not None:
         x.slopes = slopes.data_ptr()
-    if low is not None:
-        x.low = low.data_ptr()
-    x.tiles, x.cap, x.causal, x.d = tiles.data_ptr(), cap, causal, q.shape[3]
+    a.lse, x.low, x.tiles, a.err = stats, low, tiles, K.error_word(dev)
+
+
+def _round16(n: int) -> int:
+    return (n + 15) & ~15
 
 
 class ScoredAttention(torch.autograd.Function):
+    """q, k and v as tensor maps take them (``_Plan.copy`` is false, bases on 16-byte boundaries)."""
+
     @staticmethod
-    def forward(ctx, q, k, v, first, stop, slopes, cfg):
+    def forward(ctx, q, k, v, first, stop, slopes, p):
         from . import cuda as K
-        B, Tq, Hq, D = q.shape
-        (q, qs), (k, ks), (v, vs) = _laid_out(q), _laid_out(k), _laid_out(v)
-        out = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device)
-        tiles = torch.empty(B, -(-Tq // 128), 4, dtype=torch.int32, device=q.device)
-        low = torch.empty_like(out) if any(ctx.needs_input_grad[:3]) else None
-        a = _Args()
-        a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        _fill(a, q, k, cfg, first, stop, slopes, low, tiles)
-        f = K.lib().lmoe_scored_attn_fwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_fwd_fp16
+        dev = q.device
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        train = any(ctx.needs_input_grad[:3])
+        at_tiles = _round16(p.lse)
+        at_low = at_tiles + p.tiles
+        notes = torch.empty(at_low + (p.low if train else 0), dtype=torch.uint8, device=dev)
+        base = notes.data_ptr()
+        a = _Args.from_buffer_copy(p.args)
+        a.out = out.data_ptr()
+        _addresses(a, dev, first, stop, slopes, base, base + at_low if train else 0, base + at_tiles)
         with on_device(q):
-            K._check(f(K._p(q), qs, K._p(k), ks, K._p(v), vs, ctypes.byref(a), K._st()), "scored_attn_fwd")
-        ctx.save_for_backward(q, k, v, first, stop, slopes, out, low, lse, tiles)
-        ctx.cfg = cfg
+            K._check(p.fwd_fn(K._p(q), p.qs, K._p(k), p.ks, K._p(v), p.vs, ctypes.byref(a), K._st()), "scored_attn_fwd")
+        if train:
+            ctx.save_for_backward(q, k, v, first, stop, slopes, out, notes)
+            ctx.plan = p
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         from . import cuda as K
-        q, k, v, first, stop, slopes, out, low, lse, tiles = ctx.saved_tensors
+        q, k, v, first, stop, slopes, out, notes = ctx.saved_tensors
+        p, dev = ctx.plan, q.device
         d_out = d_out.contiguous()
         if d_out.data_ptr() % 16:
             d_out = d_out.clone()
-        dq, delta = torch.empty_like(out), torch.empty_like(lse)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dv = torch.empty_like(dk)
-        a = _BwdArgs()
-        a.lse, a.delta, a.dq, a.dk, a.dv = lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        _fill(a, q, k, ctx.cfg, first, stop, slopes, low, tiles)
-        f = K.lib().lmoe_scored_attn_bwd if q.dtype == torch.bfloat16 else K.lib().lmoe_scored_attn_bwd_fp16
+        dq = torch.empty_like(out)
+        dk, dv = torch.empty(k.shape, dtype=k.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
+        delta = torch.empty(p.lse, dtype=torch.uint8, device=dev)
+        base, at_tiles = notes.data_ptr(), _round16(p.lse)
+        a = _BwdArgs.from_buffer_copy(p.bwd)
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        _addresses(a, dev, first, stop, slopes, base, base + at_tiles + p.tiles, base + at_tiles)
         with on_device(q):
-            K._check(f(K._p(q), _strides(q), K._p(k), _strides(k), K._p(v), _strides(v), K._p(out), K._p(d_out), K._p(delta), ctypes.byref(a), K._st()),
-                     "scored_attn_bwd", 3)
+            K._check(p.bwd_fn(K._p(q), p.qs, K._p(k), p.ks, K._p(v), p.vs, K._p(out), K._p(d_out), K._p(delta), ctypes.byref(a), K._st()), "scored_attn_bwd", 3)
         return dq, dk, dv, None, None, None, None
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad)
 
 
 def scored_attention(q, k, v, scale=None, causal: bool = True, q_offset: int = 0, window: Optional[int] = None, softcap: Optional[float] = None,
                      slopes: Optional[torch.Tensor] = None, key_first: Optional[torch.Tensor] = None, key_stop: Optional[torch.Tensor] = None):
     """See the module; what ``ops.softmax_attention`` calls when it is given one of the last four."""
-    _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, key_stop)
-    D = q.shape[3]
-    kernel = (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and v.shape[3] == D and D <= 128 and D % 8 == 0 and q.shape[1] <= MAX_QUERIES)
-    if not kernel or min(q.numel(), k.numel()) == 0:
+    # checks, strides and sizes are worked out once per layout
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, scale, causal, q_offset, window, softcap,
+           _meta(slopes), _meta(key_first), _meta(key_stop))
+    p = _PLANS.get(key)
+    if p is None:
+        p = _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, key_first, key_stop)
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _PLANS[key] = p
+    if p.eager:
         return R.softmax_attention(q, k, v, scale, causal, q_offset, window, softcap, slopes, key_first, key_stop)
-    row = lambda r: None if r is None else r if r.stride(1) == 1 or r.shape[1] == 1 else r.contiguous()       # noqa: E731
-    cfg = (float(scale) if scale is not None else D ** -0.5, int(bool(causal)), int(q_offset), int(window or 0), float(softcap or 0.0))
-    return ScoredAttention.apply(q, k, v, row(key_first), row(key_stop), None if slopes is None else slopes.contiguous(), cfg)
+    if p.copy or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        row = lambda r: None if r is None else r.contiguous()       # noqa: E731
+        return scored_attention(_laid_out(q), _laid_out(k), _laid_out(v), scale, causal, q_offset, window, softcap, row(slopes), row(key_first), row(key_stop))
+    return ScoredAttention.apply(q, k, v, key_first, key_stop, slopes, p)
