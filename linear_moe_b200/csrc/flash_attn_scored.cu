@@ -1,13 +1,14 @@
-// Attention with key ranges, capped scores and a bias by distance over bf16: see flash_attn_tc.cuh.
+// Attention with key ranges, capped scores and a bias by distance over bf16: see flash_attn_scored.cuh.  (A source per type, so that they compile side by side.)
 #include "flash_attn_scored.cuh"
 
 using namespace lmoe::fatc;
 
-LMOE_API int lmoe_scored_attn_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
-                                 const Args* ap, cudaStream_t st) {
-    return scored_fwd_any<false>(q, qs, k, ks, v, vs, *ap, st);
+// q [B,Tq,Hq,d], k / v [B,Tk,Hkv,d] with element strides; ap->x.tiles [B, ceil(Tq / 128)] is written by the forward and read by the backward pass.
+LMOE_API int lmoe_scored_attn_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const Args* ap,
+                                 cudaStream_t st) {
+    return scored_fwd<false>(q, qs, k, ks, v, vs, *ap, st);
 }
-LMOE_API int lmoe_scored_attn_bwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
-                                 const void* o, const void* d_o, float* delta, const BwdArgs* ap, cudaStream_t st) {
-    return scored_bwd_any<false>(q, qs, k, ks, v, vs, o, d_o, delta, *ap, st);
+LMOE_API int lmoe_scored_attn_bwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const void* o,
+                                 const void* d_o, float* delta, const BwdArgs* ap, cudaStream_t st) {
+    return scored_bwd<false>(q, qs, k, ks, v, vs, o, d_o, delta, *ap, st);
 }

@@ -11,11 +11,15 @@ import os
 
 import torch
 
-from .scored_attn import _Args, _BwdArgs
-
 _ENABLED = os.environ.get("LMOE_FLASH_ATTN", "1") != "0"
 _TCGEN05_FWD = os.environ.get("LMOE_FLASH_TCGEN05", "1") != "0"      # forward on tcgen05/TMEM (csrc/flash_attn_tc.cu)
 _TCGEN05_BWD = os.environ.get("LMOE_FLASH_TCGEN05_BWD", "1") != "0"  # backward on tcgen05/TMEM (two kernels: dQ, dK/dV)
+
+
+class _FaTcBwdArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("lse", "delta", "dq", "dk", "dv")] +
+                [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "q_offset", "window")] +
+                [("scale", ctypes.c_float), ("err", ctypes.c_void_p)])
 
 
 def _backward_tcgen05(q, k, v, out, d_out, lse, scale, q_offset, window):
@@ -26,7 +30,7 @@ def _backward_tcgen05(q, k, v, out, d_out, lse, scale, q_offset, window):
     dk = torch.empty(B, k.shape[1], k.shape[2], D, dtype=q.dtype, device=q.device)
     dv = torch.empty_like(dk)
     delta = torch.empty_like(lse)
-    a = _BwdArgs()
+    a = _FaTcBwdArgs()
     a.lse, a.delta, a.dq, a.dk, a.dv = lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     a.B, a.Tq, a.Hq, a.Tk, a.Hkv = B, Tq, Hq, k.shape[1], k.shape[2]
     a.q_offset, a.window, a.scale = int(q_offset), int(window or 0), float(scale)
@@ -37,10 +41,16 @@ def _backward_tcgen05(q, k, v, out, d_out, lse, scale, q_offset, window):
     return dq, dk, dv
 
 
+class _FaTcArgs(ctypes.Structure):
+    _fields_ = ([("out", ctypes.c_void_p), ("lse", ctypes.c_void_p)] +
+                [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "q_offset", "window")] +
+                [("scale", ctypes.c_float), ("err", ctypes.c_void_p)])
+
+
 def _forward_tcgen05(q, k, v, out, lse, scale, q_offset, window):
     from . import cuda as K
     from . import gemm
-    a = _Args()
+    a = _FaTcArgs()
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     a.B, a.Tq, a.Hq = q.shape[0], q.shape[1], q.shape[2]
     a.Tk, a.Hkv = k.shape[1], k.shape[2]

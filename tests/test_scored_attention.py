@@ -7,6 +7,7 @@ to 2^-24 of their terms, 2e-7 of the cap in tanh, exp2 to 2^-22.
 In fp16 a number below 2^-14 is rounded by up to 2^-25 whatever its size: half the distance 2^-24 of the subnormals.  Weights are rounded in units of a maximum that is at
 most the row's sum, so a normalised weight is off by at most max(u p, 2^-25) and ds by max(u ds, 2^-25): the bounds get 2^-25 times the sums of the
 magnitudes of the visible v, k, q and do.  (A key whose weights all lie below 2^-14 has a dv of which u times its terms is less than that.)
+In bf16 the same holds for 2^-126, below which 32-bit numbers are flushed to zero (weights of far keys under a steep bias).
 The bounds by magnitudes would let a wrong key among hundreds pass, so the relative error in the 2-norm is held to 2 u and 4 u as well: errors of single roundings have no common
 sign and their squares add up to less."""
 import math
@@ -69,7 +70,7 @@ def formulas(q, k, v, do, scale, cap, slopes, seen, dist):
 
 def check(got, res, mag, low, dtype, names=("o", "dq", "dk", "dv")):
     u = torch.finfo(dtype).eps / 2
-    tiny = torch.finfo(dtype).smallest_normal * u              # the largest rounding of a number below the normal ones
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
     for name, g, w, m, z in zip(names, got, res, mag, low):
         n = 2 if name in ("o", "dv") else 4
         assert g.dtype == dtype and g.shape == w.shape
@@ -256,6 +257,26 @@ def test_ranges_of_any_kind():
     none = torch.zeros(3, T, dtype=torch.int32, device="cuda")
     got = compare(q, k, v, do, causal=False, stop=none + 130)
     assert (got[2][:, 130:] == 0).all() and (got[3][:, 130:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,D,heads,cap,bias", [(torch.bfloat16, 128, (16, 4), 30.0, False), (torch.bfloat16, 64, (24, 12), None, True), (torch.float16, 128, (12, 2), 50.0, True),
+                                                    (torch.bfloat16, 96, (20, 20), None, False)])
+def test_more_tiles_than_ctas(dtype, D, heads, cap, bias):
+    """Several hundred tiles of queries, which the CTAs work through: none to twelve key tiles each, in turns, so that every ring and phase meets every other one; key heads with shares of four, two and
+    one CTAs."""
+    B, T = 3, 1500
+    q, k, v, do = inputs(B, T, T, *heads, D, dtype, size=3.0)
+    first = packed(B, T, [[700, 3, 120, 40], [128, 256, 1, 127], [1500]])
+    stop = torch.full((B, T), T, dtype=torch.int32, device="cuda")
+    stop[0, 128:384] = 0                                       # whole tiles that see nothing
+    stop[1, ::2] = 0
+    stop[2, 1408:] = 700
+    sl = slope_table(heads[0]) if bias else None
+    a = compare(q, k, v, do, cap=cap, slopes=sl, first=first, stop=stop)
+    for _ in range(3):
+        b = run(q, k, v, do, softcap=cap, slopes=sl, key_first=first, key_stop=stop)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 @gpu
