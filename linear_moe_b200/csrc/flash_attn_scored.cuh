@@ -134,6 +134,28 @@ template <class F, int N> __device__ __forceinline__ void scored(uint32_t (&v)[N
 }
 
 
+// Bounded waits.  (Without the time hint of mbar_wait_suspend.)
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+    if (try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+        if (try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_CYCLES) break;
+    }
+    *abort_flag = 1;
+    atomicCAS(err, 0, code);
+    return false;
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+    return __all_sync(0xffffffffu, wait_for(bar, parity, abort_flag, err, code));
+}
+
 // ---- work ----------------------------------------------------------------------------------------------------------------------------
 // Which tile a CTA takes: the last (longest) tiles of a sequence first, over `group` (batch, head) pairs at a time, whose streamed rows share the L2.
 struct TileOf { int rank, pair; };
@@ -161,56 +183,47 @@ __device__ __forceinline__ int work_of(const void* answer) {
     return (int)id;
 }
 // The tiles that a CTA works through, two slots: warp 3 fills one while the other is worked on.
+struct Item { int q0, h, b, hk, nb_lo, n_it; int2 every; };      // n_it: key tiles, from nb_lo on (-1: no more work); inside `every` no row masks anything
 struct Work {
     uint64_t full[2], empty[2], asked;
     __align__(16) uint4 answer;
-    int4 range[2];                        // union and intersection of the tile's intervals
-    int index[2];                         // -1: no more
+    __align__(16) Item item[2];
 };
-struct Item { int q0, h, b, hk, nb_lo, n_it; int2 every; };
-template <class A> __device__ __forceinline__ Item item_of(const A& a, const Work& w, int slot, int group) {
-    const int n_qb = (a.Tq + BM - 1) / BM;
-    const TileOf t = longest_first(w.index[slot], n_qb, a.B * a.Hq, group);
-    const int4 r = w.range[slot];
-    Item i;
-    i.q0 = (n_qb - 1 - t.rank) * BM;
-    i.h = t.pair % a.Hq, i.b = t.pair / a.Hq, i.hk = i.h / (a.Hq / a.Hkv);
-    i.nb_lo = min(r.x, r.y) / BN;
-    i.n_it = max((r.y + BN - 1) / BN - i.nb_lo, 0);
-    i.every = make_int2(r.z, r.w);
-    return i;
-}
 __device__ __forceinline__ void init_work(Work& w, int readers) {      // readers of a slot: loads, products, softmax warps
     for (int s = 0; s < 2; ++s) { mbar_init(&w.full[s], 1); mbar_init(&w.empty[s], readers); }
     mbar_init(&w.asked, 1);
 }
-// Warp 3.  COMPUTE: the intervals from the ranges (and, from the first head, to memory for the backward pass), else from memory.
-template <bool COMPUTE, class A>
-__device__ __forceinline__ void hand_out(Work& w, const A& a, int group, volatile int* abort_flag, int* err, int code) {
+// Warp 3.  seen: [2][128] in shared memory for the rows' ranges, where the intervals are to be worked out (and, from the first head, noted for the backward pass); null: they are read from the notes.
+template <class A>
+__device__ __forceinline__ void hand_out(Work& w, int2 (*seen)[BM], const A& a, int group, volatile int* abort_flag, int* err, int code) {
     const int lane = threadIdx.x & 31, n_qb = (a.Tq + BM - 1) / BM;
     for (int it = 0;; ++it) {
         const int slot = it & 1;
-        if (!mbar_wait_warp(&w.empty[slot], ((it >> 1) & 1) ^ 1, abort_flag, err, code)) return;
+        if (!wait_warp(&w.empty[slot], ((it >> 1) & 1) ^ 1, abort_flag, err, code)) return;
         int index = blockIdx.x;
         if (it > 0) {                                             // not before there is room: what a CTA has asked for no other one can take
             if (lane == 0) ask_work(&w.answer, &w.asked);
             __syncwarp();
-            if (!mbar_wait_warp(&w.asked, (it - 1) & 1, abort_flag, err, code + 1)) return;
+            if (!wait_warp(&w.asked, (it - 1) & 1, abort_flag, err, code + 1)) return;
             index = work_of(&w.answer);
             __syncwarp();
         }
-        int4 t = make_int4(0, 0, 0, 0);
+        Item x;
+        x.n_it = -1;
         if (index >= 0) {
             const TileOf tile = longest_first(index, n_qb, a.B * a.Hq, group);
-            const int qb = n_qb - 1 - tile.rank, b = tile.pair / a.Hq;
-            int4* note = a.x.tiles + (long long)b * n_qb + qb;
-            if (COMPUTE) {
-                t = make_int4(0x7fffffff, 0, 0, 0x7fffffff);     // empty rows add nothing to the union and leave no intersection
+            const int qb = n_qb - 1 - tile.rank;
+            x.h = tile.pair % a.Hq, x.b = tile.pair / a.Hq, x.hk = x.h / (a.Hq / a.Hkv), x.q0 = qb * BM;
+            int4* note = a.x.tiles + (long long)x.b * n_qb + qb;
+            int4 t;
+            if (seen != nullptr) {
+                t = make_int4(0x7fffffff, 0, 0, 0x7fffffff);     // {union, intersection}: empty rows add nothing to the first and leave none of the second
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = qb * BM + lane + 32 * e;
+                    const int row = x.q0 + lane + 32 * e;
+                    const int2 r = row < a.Tq ? visible_range(a, x.b, row) : make_int2(0, 0);
+                    seen[slot][lane + 32 * e] = r;
                     if (row >= a.Tq) continue;
-                    const int2 r = visible_range(a, b, row);
                     if (r.x < r.y) t = make_int4(min(t.x, r.x), max(t.y, r.y), max(t.z, r.x), min(t.w, r.y));
                     else t.z = 0x7fffffff, t.w = 0;
                 }
@@ -218,16 +231,19 @@ __device__ __forceinline__ void hand_out(Work& w, const A& a, int group, volatil
                 t.y = __reduce_max_sync(0xffffffffu, t.y);
                 t.z = __reduce_max_sync(0xffffffffu, t.z);
                 t.w = __reduce_min_sync(0xffffffffu, t.w);
-                if (tile.pair % a.Hq == 0 && lane == 0) *note = t;
+                if (x.h == 0 && lane == 0) *note = t;
             } else t = __ldg(note);
+            x.nb_lo = min(t.x, t.y) / BN;
+            x.n_it = max((t.y + BN - 1) / BN - x.nb_lo, 0);
+            x.every = make_int2(t.z, t.w);
         }
+        __syncwarp();
         if (lane == 0) {
-            w.index[slot] = index;
-            w.range[slot] = t;
+            w.item[slot] = x;
             mbar_arrive(&w.full[slot]);
         }
         __syncwarp();
-        if (index < 0) return;
+        if (x.n_it < 0) return;
     }
 }
 // All softmax warps: do they all want to go on?  (A barrier; what it decides is the same for all.)
@@ -296,7 +312,7 @@ struct __align__(1024) SmemFwd {
     Work work;
     float mx[2][2][2][BM];                                    // [parity of the group's tile][group][half of the columns]
     float ls[2][2][2][BM], ms[2][2][BM];                      // sums and maxima at the end, [parity of the tile of queries][group]
-    int2 seen[2][4][BM];                                      // [slot][quarter]: a thread's visible keys
+    int2 seen[2][BM];                                         // [slot]: the rows' visible keys
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -354,22 +370,23 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             int c0 = 0, c1 = 0;
             for (int it = 0, qi = 0;; ++it) {
                 const int slot = it & 1;
-                if (!mbar_wait_suspend(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x21000 | slot) || sm.work.index[slot] < 0) break;
-                const Item w = item_of(a, sm.work, slot, group);
+                if (!wait_for(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x21000 | slot)) break;
+                const Item w = sm.work.item[slot];
+                if (w.n_it < 0) break;
                 mbar_arrive(&sm.work.empty[slot]);
                 if (w.n_it == 0) continue;
                 const int qs = qi & 1;
-                if (!mbar_wait_suspend(&sm.q_empty[qs], ((qi >> 1) & 1) ^ 1, abort_flag, err, 0x21010 | qs)) break;
+                if (!wait_for(&sm.q_empty[qs], ((qi >> 1) & 1) ^ 1, abort_flag, err, 0x21010 | qs)) break;
                 mbar_expect_tx(&sm.q_full[qs], BM * D * 2);
                 load_tile<D>(sm.q[qs], &tmQ, &sm.q_full[qs], w.h, w.q0, w.b);
                 bool ok = true;
                 for (int j = 0; j < w.n_it; ++j) {
                     const int s = j & 1, c = s == 0 ? c0++ : c1++, sk = c % (KS / 2) * 2 + s, key0 = (w.nb_lo + j) * BN;
-                    ok = mbar_wait_suspend(&sm.k_empty[sk], ((c / (KS / 2)) & 1) ^ 1, abort_flag, err, 0x21020 | sk);
+                    ok = wait_for(&sm.k_empty[sk], ((c / (KS / 2)) & 1) ^ 1, abort_flag, err, 0x21020 | sk);
                     if (!ok) break;
                     mbar_expect_tx(&sm.k_full[sk], BN * D * 2);
                     load_tile<D>(sm.k[sk], &tmK, &sm.k_full[sk], w.hk, key0, w.b);
-                    ok = mbar_wait_suspend(&sm.v_empty[s], (c & 1) ^ 1, abort_flag, err, 0x21030 | s);
+                    ok = wait_for(&sm.v_empty[s], (c & 1) ^ 1, abort_flag, err, 0x21030 | s);
                     if (!ok) break;
                     mbar_expect_tx(&sm.v_full[s], BN * D * 2);
                     // MN-major operand: per 64 keys, D / 64 boxes of {64 d, 64 keys} (8 KiB each)
@@ -389,9 +406,9 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool ok = true;
         for (int it = 0, qi = 0, c = 0; ok; ++it) {
             const int slot = it & 1;
-            ok = mbar_wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x22000 | slot);
-            if (!ok || (int)uniform(sm.work.index[slot]) < 0) break;
-            const int n_it = uniform(item_of(a, sm.work, slot, group).n_it);
+            ok = wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x22000 | slot);
+            const int n_it = uniform(sm.work.item[slot].n_it);
+            if (!ok || n_it < 0) break;
             if (lane == 0) mbar_arrive(&sm.work.empty[slot]);
             __syncwarp();
             if (n_it == 0) continue;
@@ -401,9 +418,9 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const uint32_t ph = c & 1;
                 const bool first = j == g;
                 // the scores go over the group's last P: its product has to complete
-                ok = (!first || mbar_wait_warp(&sm.q_full[qs], (qi >> 1) & 1, abort_flag, err, 0x22010 | qs)) &&
-                     mbar_wait_warp(&sm.k_full[sk], (c / (KS / 2)) & 1, abort_flag, err, 0x22020 | sk) &&
-                     (c == 0 || mbar_wait_warp(&sm.pv_done[g], ph ^ 1, abort_flag, err, 0x22030));
+                ok = (!first || wait_warp(&sm.q_full[qs], (qi >> 1) & 1, abort_flag, err, 0x22010 | qs)) &&
+                     wait_warp(&sm.k_full[sk], (c / (KS / 2)) & 1, abort_flag, err, 0x22020 | sk) &&
+                     (c == 0 || wait_warp(&sm.pv_done[g], ph ^ 1, abort_flag, err, 0x22030));
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -417,7 +434,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     umma_commit(&sm.s_full[g]);
                 }
                 // (the first product of a tile of queries goes over the output of the one before, which the softmax warps have all read ahead of these weights)
-                ok = mbar_wait_warp(&sm.v_full[g], ph, abort_flag, err, 0x22040 | g) && mbar_wait_warp(&sm.p_ready[g], ph, abort_flag, err, 0x22050 | g);
+                ok = wait_warp(&sm.v_full[g], ph, abort_flag, err, 0x22040 | g) && wait_warp(&sm.p_ready[g], ph, abort_flag, err, 0x22050 | g);
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -435,7 +452,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             ++qi;
         }
     } else if (warp == 3) {
-        hand_out<true>(sm.work, a, group, abort_flag, err, 0x23000);
+        hand_out(sm.work, sm.seen, a, group, abort_flag, err, 0x23000);
     } else {
         const int qd = warp & 3, quarter = (warp - 4) >> 2, grp = quarter >> 1, part = quarter & 1;
         const int r = qd * 32 + lane;                         // query row inside the tile
@@ -447,25 +464,18 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         int done[2] = {0, 0};                                 // key tiles of the groups so far
         for (int it = 0, qi = 0;; ++it) {
             const int slot = it & 1;
-            if (ok) ok = mbar_wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x24000 | slot);
+            if (ok) ok = wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x24000 | slot);
             if (!all_softmax(ok)) break;
-            if (sm.work.index[slot] < 0) break;
-            const volatile int4& every = reinterpret_cast<const volatile int4&>(sm.work.range[slot]);
-            int n_it, qi_at;
+            const int n_it = sm.work.item[slot].n_it;
+            if (n_it < 0) break;
             float m = -INFINITY, l = 0.f;
-            ScoreOf so;
-            {
-                const Item w = item_of(a, sm.work, slot, group);
-                n_it = w.n_it;
-                qi_at = a.q_offset + w.q0 + r;
-                so = score_of<F>(a.scale, a.x, w.h);
-                sm.seen[slot][quarter][r] = w.q0 + r < a.Tq ? visible_range(a, w.b, w.q0 + r) : make_int2(0, 0);      // its own thread's only
-            }
+            const ScoreOf so = score_of<F>(a.scale, a.x, sm.work.item[slot].h);
             const float sc = so.unit;
             for (int j = grp, c = grp == 0 ? done[0] : done[1]; j < n_it; j += 2, ++c) {
-                if (ok) ok = mbar_wait_warp(&sm.s_full[grp], c & 1, abort_flag, err, 0x24010 | grp);
-                const int tile_key0 = (min(every.x, every.y) / BN + j) * BN, key0 = tile_key0 + part * 64;
-                const bool need_mask = tile_key0 < every.z || tile_key0 + BN > every.w;
+                if (ok) ok = wait_warp(&sm.s_full[grp], c & 1, abort_flag, err, 0x24010 | grp);
+                const volatile Item& w = sm.work.item[slot];
+                const int tile_key0 = (w.nb_lo + j) * BN, key0 = tile_key0 + part * 64;
+                const bool need_mask = tile_key0 < w.every.x || tile_key0 + BN > w.every.y;
                 tc_fence_after();
                 if constexpr (F::SCORE == SCORE_BOUND) {
                     if (!ok) continue;
@@ -477,7 +487,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         tmem_ld_wait();
                         tanh_of(v, so.a);
                         if (need_mask) {
-                            const int2 range = sm.seen[slot][quarter][r];
+                            const int2 range = sm.seen[slot][r];
                             const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;       // visible: lo < i <= hi
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -497,9 +507,9 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     uint32_t v[64];
                     tmem_ld64(s_addr, v);
                     tmem_ld_wait();
-                    scored<F>(v, so, a.x, (float)(key0 - qi_at));
+                    scored<F>(v, so, a.x, (float)(key0 - a.q_offset - w.q0 - r));
                     if (need_mask) {
-                        const int2 range = sm.seen[slot][quarter][r];
+                        const int2 range = sm.seen[slot][r];
                         const int hi = range.y - 1 - key0, lo = range.x - 1 - key0;
 #pragma unroll
                         for (int i = 0; i < 64; ++i)
@@ -524,7 +534,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (grow) m = mx;
                     l *= corr;
                     if (__any_sync(0xffffffffu, scaled)) {        // not at the group's first tile; these scores were issued behind the last product of the group
-                        ok = mbar_wait_warp(&sm.pv_done[grp], (c & 1) ^ 1, abort_flag, err, 0x24020 | grp);
+                        ok = wait_warp(&sm.pv_done[grp], (c & 1) ^ 1, abort_flag, err, 0x24020 | grp);
                         if (!ok) continue;
                         tc_fence_after();
 #pragma unroll
@@ -562,7 +572,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_ready[grp]);
             }
-            const Item w = item_of(a, sm.work, slot, group);
+            const Item w = sm.work.item[slot];
             const int row = w.q0 + r, d = a.x.d;
             const long long out0 = (((long long)w.b * a.Tq + w.q0 + qd * 32) * a.Hq + w.h) * d + quarter * OW, row_stride = (long long)a.Hq * d;
             const int rows = min(32, a.Tq - w.q0 - qd * 32), cols = d - quarter * OW;
@@ -599,7 +609,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 if (n_it <= g) continue;
-                if (ok) ok = mbar_wait_warp(&sm.pv_done[g], (done[g] + (n_it - g - 1) / 2) & 1, abort_flag, err, 0x24030 | g);     // the group's last tile
+                if (ok) ok = wait_warp(&sm.pv_done[g], (done[g] + (n_it - g - 1) / 2) & 1, abort_flag, err, 0x24030 | g);     // the group's last tile
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t x[OW];
@@ -667,8 +677,8 @@ __device__ __forceinline__ void derive(uint32_t (&v)[32], float2 (&p)[16], const
 
 template <int D>
 struct __align__(1024) SmemDq {
-    uint8_t q[BM * D * 2], g[BM * D * 2], k[3][BM * D * 2], v[2][BM * D * 2];      // K: read by a tile's first and last product
-    uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], dp_full, ds_ready, dq_done, all_done;
+    uint8_t q[BM * D * 2], g[BM * D * 2], k[3][BM * D * 2], v[2][BM * D * 2];      // K: read by a tile's first and last product; g in the end: dq on its way to memory
+    uint64_t q_full, q_empty, g_full, g_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], dp_full, ds_ready, dq_done, all_done;
     Work work;
     uint32_t tmem_base;
     int abort_flag;
@@ -689,7 +699,7 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     volatile int* abort_flag = &sm.abort_flag;
     int* err = a.err;
     if (threadIdx.x == 0) {
-        mbar_init(&sm.q_full, 1); mbar_init(&sm.q_empty, 1);
+        mbar_init(&sm.q_full, 1); mbar_init(&sm.q_empty, 1); mbar_init(&sm.g_full, 1); mbar_init(&sm.g_empty, 16);
         for (int s = 0; s < 3; ++s) { mbar_init(&sm.k_full[s], 1); mbar_init(&sm.k_empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&sm.v_full[s], 1); mbar_init(&sm.v_empty[s], 1); mbar_init(&sm.s_full[s], 1); }
         mbar_init(&sm.dp_full, 1); mbar_init(&sm.ds_ready, 16); mbar_init(&sm.dq_done, 1); mbar_init(&sm.all_done, 1);
@@ -708,25 +718,29 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             bool ok = true;
             for (int it = 0, qi = 0, n = 0; ok; ++it) {
                 const int slot = it & 1;
-                ok = mbar_wait_suspend(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25010 | slot);
-                if (!ok || sm.work.index[slot] < 0) break;
-                const Item w = item_of(a, sm.work, slot, group);
+                ok = wait_for(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25010 | slot);
+                if (!ok) break;
+                const Item w = sm.work.item[slot];
+                if (w.n_it < 0) break;
                 mbar_arrive(&sm.work.empty[slot]);
                 if (w.n_it == 0) continue;
                 for (int j = 0; ok && j < w.n_it; ++j, ++n) {
                     const int s = n & 1, s3 = n % 3, key0 = (w.nb_lo + j) * BN;
-                    ok = mbar_wait_suspend(&sm.k_empty[s3], ((n / 3) & 1) ^ 1, abort_flag, err, 0x25020 | s3);
+                    ok = wait_for(&sm.k_empty[s3], ((n / 3) & 1) ^ 1, abort_flag, err, 0x25020 | s3);
                     if (!ok) break;
                     mbar_expect_tx(&sm.k_full[s3], BM * D * 2);
                     load_tile<D>(sm.k[s3], &tmK, &sm.k_full[s3], w.hk, key0, w.b);
-                    if (j == 0) {                                              // behind the first K: that one needs not wait for the tile of queries before
-                        ok = mbar_wait_suspend(&sm.q_empty, (qi & 1) ^ 1, abort_flag, err, 0x25030);
+                    if (j == 0) {
+                        ok = wait_for(&sm.q_empty, (qi & 1) ^ 1, abort_flag, err, 0x25030);
                         if (!ok) break;
-                        mbar_expect_tx(&sm.q_full, 2 * BM * D * 2);
+                        mbar_expect_tx(&sm.q_full, BM * D * 2);
                         load_tile<D>(sm.q, &tmQ, &sm.q_full, w.h, w.q0, w.b);
-                        load_tile<D>(sm.g, &tmG, &sm.q_full, w.h, w.q0, w.b);
+                        ok = wait_for(&sm.g_empty, (qi & 1) ^ 1, abort_flag, err, 0x25031);
+                        if (!ok) break;
+                        mbar_expect_tx(&sm.g_full, BM * D * 2);
+                        load_tile<D>(sm.g, &tmG, &sm.g_full, w.h, w.q0, w.b);
                     }
-                    ok = mbar_wait_suspend(&sm.v_empty[s], ((n >> 1) & 1) ^ 1, abort_flag, err, 0x25040 | s);
+                    ok = wait_for(&sm.v_empty[s], ((n >> 1) & 1) ^ 1, abort_flag, err, 0x25040 | s);
                     if (!ok) break;
                     mbar_expect_tx(&sm.v_full[s], BM * D * 2);
                     load_tile<D>(sm.v[s], &tmV, &sm.v_full[s], w.hk, key0, w.b);
@@ -735,50 +749,59 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
         }
     } else if (warp == 1) {
+        int last = 0;
         auto scores = [&](int n) -> bool {
             const int s = n & 1, s3 = n % 3;
-            if (!mbar_wait_warp(&sm.k_full[s3], (n / 3) & 1, abort_flag, err, 0x25100 | s3)) return false;
+            if (!wait_warp(&sm.k_full[s3], (n / 3) & 1, abort_flag, err, 0x25100 | s3)) return false;
             tc_fence_after();
             score_product<D, F>(tmem_base + s * 128, sm.q, sm.k[s3]);
-            if (elect_one()) umma_commit(&sm.s_full[s]);
+            if (elect_one()) {
+                umma_commit(&sm.s_full[s]);
+                if (n + 1 == last) umma_commit(&sm.q_empty);              // the next Q may come: only scores read it
+            }
             return true;
         };
         auto dprobs = [&](int n) -> bool {
             const int s = n & 1;
-            if (!mbar_wait_warp(&sm.v_full[s], (n >> 1) & 1, abort_flag, err, 0x25110 | s)) return false;
+            if (!wait_warp(&sm.v_full[s], (n >> 1) & 1, abort_flag, err, 0x25110 | s)) return false;
             tc_fence_after();
             score_product<D, F>(tmem_base + DP, sm.g, sm.v[s]);
-            if (elect_one()) { umma_commit(&sm.v_empty[s]); umma_commit(&sm.dp_full); }
+            if (elect_one()) {
+                umma_commit(&sm.v_empty[s]);
+                umma_commit(&sm.dp_full);
+            }
             return true;
         };
         bool ok = true;
         for (int it = 0, qi = 0, base = 0; ok; ++it) {
             const int slot = it & 1;
-            ok = mbar_wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25120 | slot);
-            if (!ok || (int)uniform(sm.work.index[slot]) < 0) break;
-            const int n_it = uniform(item_of(a, sm.work, slot, group).n_it), last = base + n_it;
+            ok = wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25120 | slot);
+            const int n_it = uniform(sm.work.item[slot].n_it);
+            if (!ok || n_it < 0) break;
             if (lane == 0) mbar_arrive(&sm.work.empty[slot]);
             __syncwarp();
             if (n_it == 0) continue;
-            ok = mbar_wait_warp(&sm.q_full, qi & 1, abort_flag, err, 0x25130) && scores(base) && dprobs(base) && (n_it < 2 || scores(base + 1));
+            last = base + n_it;
+            ok = wait_warp(&sm.q_full, qi & 1, abort_flag, err, 0x25130) && scores(base) && wait_warp(&sm.g_full, qi & 1, abort_flag, err, 0x25131) && dprobs(base) &&
+                 (n_it < 2 || scores(base + 1));
             for (int n = base; ok && n < last; ++n) {
-                if (!mbar_wait_warp(&sm.ds_ready, n & 1, abort_flag, err, 0x25140)) { ok = false; break; }
+                if (!wait_warp(&sm.ds_ready, n & 1, abort_flag, err, 0x25140)) { ok = false; break; }
                 if (n + 1 < last && !dprobs(n + 1)) { ok = false; break; }
                 tc_fence_after();
                 grad_product<D, F>(tmem_base + DQ, tmem_base + (n & 1) * 128, sm.k[n % 3], n > base);
                 if (elect_one()) {
                     umma_commit(&sm.k_empty[n % 3]);
                     umma_commit(&sm.dq_done);
-                    if (n + 1 == last) { umma_commit(&sm.q_empty); umma_commit(&sm.all_done); }
+                    if (n + 1 == last) umma_commit(&sm.all_done);
                 }
                 // the next scores of this buffer go over dS_n: the product that reads it has to complete.  (Waited for at every tile, so that no phase is passed over.)
-                ok = mbar_wait_warp(&sm.dq_done, n & 1, abort_flag, err, 0x25150) && (n + 2 >= last || scores(n + 2));
+                ok = wait_warp(&sm.dq_done, n & 1, abort_flag, err, 0x25150) && (n + 2 >= last || scores(n + 2));
             }
             base = last;
             ++qi;
         }
     } else if (warp == 3) {
-        hand_out<false>(sm.work, a, group, abort_flag, err, 0x25160);
+        hand_out(sm.work, nullptr, a, group, abort_flag, err, 0x25160);
     } else if (warp >= 4) {
         const int qd = warp & 3, part = (warp - 4) >> 2;
         const int r = qd * 32 + lane;
@@ -787,33 +810,36 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         bool ok = true;
         for (int it = 0, qi = 0, base = 0;; ++it) {
             const int slot = it & 1;
-            if (ok) ok = mbar_wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25200 | slot);
+            if (ok) ok = wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x25200 | slot);
             if (!all_softmax(ok)) break;
-            if (sm.work.index[slot] < 0) break;
-            const Item w = item_of(a, sm.work, slot, group);
+            const Item w = sm.work.item[slot];
             __syncwarp();
+            if (w.n_it < 0) break;
             if (lane == 0) mbar_arrive(&sm.work.empty[slot]);
             const int row = w.q0 + r, qi_at = a.q_offset + row, last = base + w.n_it, d = a.x.d;
-            bf16* out = a.dq + (((long long)w.b * a.Tq + row) * a.Hq + w.h) * d + part * OW;
+            const long long row_stride = (long long)a.Hq * d;
+            bf16* out = a.dq + (((long long)w.b * a.Tq + w.q0 + qd * 32) * a.Hq + w.h) * d + part * OW;      // of the warp's first row
             if (w.n_it == 0) {
                 if (row < a.Tq)
-                    for (int c = 0; c < OW && part * OW + c < d; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < OW && part * OW + c < d; c += 8) *reinterpret_cast<uint4*>(out + lane * row_stride + c) = make_uint4(0, 0, 0, 0);
                 continue;
             }
             const ScoreOf so = score_of<F>(a.scale, a.x, w.h);
             const float sc = so.unit;
             const long long stat = ((long long)w.b * a.Hq + w.h) * a.Tq + row;
-            float lse2 = row < a.Tq ? a.lse[stat] * LOG2E : INFINITY;
-            if (lse2 == -INFINITY) lse2 = INFINITY;                          // a row that sees nothing: its weights are zero
-            const int2 range = row < a.Tq ? visible_range(a, w.b, row) : make_int2(0, 0);
-            const float dl = row < a.Tq ? a.delta[stat] : 0.f;
+            float lse2 = row < a.Tq ? a.lse[stat] : INFINITY, dl = row < a.Tq ? a.delta[stat] : 0.f;
+            int2 range = row < a.Tq ? visible_range(a, w.b, row) : make_int2(0, 0);
             for (int n = base; ok && n < last; ++n) {
                 const int s = n & 1;
                 const int tile_key0 = (w.nb_lo + n - base) * BN, key0 = tile_key0 + part * 32;
                 const bool need_mask = tile_key0 < w.every.x || tile_key0 + BN > w.every.y;
-                ok = mbar_wait_warp(&sm.s_full[s], (n >> 1) & 1, abort_flag, err, 0x25210 | s);
+                ok = wait_warp(&sm.s_full[s], (n >> 1) & 1, abort_flag, err, 0x25210 | s);
                 if (!ok) break;
                 tc_fence_after();
+                if (n == base) {                                             // the row's numbers have been on their way while the products ran
+                    asm volatile("" : "+f"(lse2), "+f"(dl), "+r"(range.x), "+r"(range.y));
+                    lse2 = lse2 == -INFINITY ? INFINITY : lse2 * LOG2E;      // a row that sees nothing: its weights are zero
+                }
                 uint32_t v[32];
                 float2 p[16];
                 tmem_ld32(lane_addr + s * 128 + part * 32, v);
@@ -831,7 +857,7 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     p[i] = F::SCORE == SCORE_CAP ? __fmul2_rn(p[i], e) : e;
                     asm volatile("" : "+f"(p[i].x), "+f"(p[i].y));                                 // here, not behind the wait
                 }
-                ok = mbar_wait_warp(&sm.dp_full, n & 1, abort_flag, err, 0x25220);
+                ok = wait_warp(&sm.dp_full, n & 1, abort_flag, err, 0x25220);
                 if (!ok) break;
                 tc_fence_after();
                 tmem_ld32(lane_addr + DP + part * 32, v);
@@ -844,24 +870,20 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 hand_over(lane_addr + s * 128 + part * 32, pk, &sm.ds_ready);
             }
-            if (ok) ok = mbar_wait_warp(&sm.all_done, qi & 1, abort_flag, err, 0x25230);
+            if (ok) ok = wait_warp(&sm.all_done, qi & 1, abort_flag, err, 0x25230);
             tc_fence_after();
             if (ok) {
-                uint32_t v[OW];
+                uint32_t v[OW], y[OW / 2];
                 tmem_ld<OW>(lane_addr + DQ + part * OW, v);
                 tmem_ld_wait();
                 tc_fence_before();                                                               // ahead of the next weights, behind which the accumulator is written again
-                if (row < a.Tq) {
 #pragma unroll
-                    for (int c = 0; c < OW; c += 8) {
-                        if (part * OW + c >= d) break;
-                        float f[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = a.scale * __uint_as_float(v[c + e]);
-                        *reinterpret_cast<uint4*>(out + c) = make_uint4(pack16<F>(f[0], f[1]), pack16<F>(f[2], f[3]), pack16<F>(f[4], f[5]), pack16<F>(f[6], f[7]));
-                    }
-                }
+                for (int c = 0; c < OW; c += 2) y[c / 2] = pack16<F>(a.scale * __uint_as_float(v[c]), a.scale * __uint_as_float(v[c + 1]));
+                rows_out<OW>(sm.g + (warp - 4) * 32 * OW * 2, y, out, row_stride, min(32, a.Tq - w.q0 - qd * 32), d - part * OW);
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                         // ahead of the next dO in this buffer
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.g_empty);
             base = last;
             ++qi;
         }
@@ -943,26 +965,26 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int it = 0; it < n_it; ++it) {
                 const int s = it & 1;
                 const int h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
-                if (!mbar_wait_suspend(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26100 | s)) break;
+                if (!wait_for(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26100 | s)) break;
                 mbar_expect_tx(&sm.q_full[s], BM * D * 2);
                 load_tile<D>(sm.q[s], &tmQ, &sm.q_full[s], h, q0, b);
-                if (!mbar_wait_suspend(&sm.g_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26120 | s)) break;
+                if (!wait_for(&sm.g_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26120 | s)) break;
                 mbar_expect_tx(&sm.g_full[s], BM * D * 2);
                 load_tile<D>(sm.g[s], &tmG, &sm.g_full[s], h, q0, b);
             }
         }
     } else if (warp == 1) {
         if (n_it > 0) {
-            bool ok = mbar_wait_warp(&sm.kv_full, 0, abort_flag, err, 0x26200);
+            bool ok = wait_warp(&sm.kv_full, 0, abort_flag, err, 0x26200);
             auto scores = [&](int it) -> bool {
-                if (!mbar_wait_warp(&sm.q_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26300 | (it & 1))) return false;
+                if (!wait_warp(&sm.q_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26300 | (it & 1))) return false;
                 tc_fence_after();
                 score_product<D, F>(tmem_base + ST, sm.k, sm.q[it & 1]);
                 if (elect_one()) umma_commit(&sm.s_full);
                 return true;
             };
             auto dprobs = [&](int it) -> bool {
-                if (!mbar_wait_warp(&sm.g_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26310 | (it & 1))) return false;
+                if (!wait_warp(&sm.g_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26310 | (it & 1))) return false;
                 tc_fence_after();
                 score_product<D, F>(tmem_base + DP, sm.v, sm.g[it & 1]);
                 if (elect_one()) umma_commit(&sm.dp_full);
@@ -970,7 +992,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             };
             if (ok) ok = scores(0) && dprobs(0);
             for (int it = 0; ok && it < n_it; ++it) {
-                if (!mbar_wait_warp(&sm.p_ready, it & 1, abort_flag, err, 0x26400)) break;
+                if (!wait_warp(&sm.p_ready, it & 1, abort_flag, err, 0x26400)) break;
                 tc_fence_after();
                 const bool more = it + 1 < n_it;
                 grad_product<D, F>(tmem_base + DV, tmem_base + ST, sm.g[it & 1], it > 0);   // dV += P^T dO
@@ -978,13 +1000,13 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (more) {
                     // the next scores go over P^T: the product that reads it has to complete
                     if (elect_one()) umma_commit(&sm.dv_done);
-                    if (!mbar_wait_warp(&sm.dv_done, it & 1, abort_flag, err, 0x26600) || !scores(it + 1)) break;
+                    if (!wait_warp(&sm.dv_done, it & 1, abort_flag, err, 0x26600) || !scores(it + 1)) break;
                 }
-                if (!mbar_wait_warp(&sm.ds_ready, it & 1, abort_flag, err, 0x26410)) break;
+                if (!wait_warp(&sm.ds_ready, it & 1, abort_flag, err, 0x26410)) break;
                 tc_fence_after();
                 grad_product<D, F>(tmem_base + DKC, tmem_base + DP, sm.q[it & 1], it > 0);  // dK += dS^T Q
                 if (elect_one()) { umma_commit(&sm.q_empty[it & 1]); umma_commit(more ? &sm.dk_done : &sm.all_done); }
-                if (more) ok = mbar_wait_warp(&sm.dk_done, it & 1, abort_flag, err, 0x26610) && dprobs(it + 1);
+                if (more) ok = wait_warp(&sm.dk_done, it & 1, abort_flag, err, 0x26610) && dprobs(it + 1);
             }
         }
     } else if (warp == 2) {                                      // log-sum-exp, delta and range of the looped queries
@@ -1002,7 +1024,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (x[e] == -INFINITY) x[e] = INFINITY;          // a row that sees nothing: its weights are zero
                 range[e] = q < a.Tq ? visible_range(a, b, q) : make_int2(0, 0);
             }
-            if (!mbar_wait_suspend(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
+            if (!wait_for(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 sm.lse2[s][lane + 32 * e] = x[e]; sm.delta[s][lane + 32 * e] = y[e];
@@ -1021,8 +1043,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool alive = n_it > 0;
         for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
             const int s = it & 1, tile = sm.list[at], tile_q0 = (tile & 0x7fff) * BM;
-            if (!mbar_wait_suspend(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
-            if (!mbar_wait_suspend(&sm.s_full, it & 1, abort_flag, err, 0x26500)) { alive = false; break; }
+            if (!wait_for(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
+            if (!wait_for(&sm.s_full, it & 1, abort_flag, err, 0x26500)) { alive = false; break; }
             tc_fence_after();
             uint32_t v[32], pk[16];
             float2 p[16];
@@ -1051,7 +1073,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 p[i + 1] = F::SCORE == SCORE_CAP ? __fmul2_rn(p[i + 1], ey) : ey;
             }
             hand_over(lane_addr + ST + part * 32, pk, &sm.p_ready);
-            if (!mbar_wait_suspend(&sm.dp_full, it & 1, abort_flag, err, 0x26520)) { alive = false; break; }
+            if (!wait_for(&sm.dp_full, it & 1, abort_flag, err, 0x26520)) { alive = false; break; }
             tc_fence_after();
             tmem_ld32(lane_addr + DP + part * 32, v);
             tmem_ld_wait();
@@ -1069,7 +1091,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (F::SCORE != SCORE_PLAIN && it + 1 < n_it) so = score_of<F>(a.scale, a.x, ++h);
             }
         }
-        if (alive) alive = mbar_wait_suspend(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
+        if (alive) alive = wait_for(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
         tc_fence_after();
         // to shared memory in fp32, units of 16 bytes at (unit ^ row % 8), so that 32 rows at a time fall into different banks
         constexpr int OW = D / SPLIT;
@@ -1171,8 +1193,10 @@ static int launch_fwd(const void* q, const long long* qs, const void* k, const l
     return (int)cudaGetLastError();
 }
 
-// CTAs that share a tile of keys
-static int key_share(int rep) { return rep % 4 == 0 ? 4 : rep % 2 == 0 ? 2 : 1; }
+// CTAs that share a tile of keys: two, each with half of the query heads, where those can be halved.  Two short ones leave less of a tail than a long one, but a CTA has its fixed costs.
+// Measured, 16 over 4 heads of 128, 8192 tokens, dk / dv kernel at one / two: documents of 4096 271 / 273 us, 1024 120 / 112 us, 256 60 / 75 us; of uneven lengths, 1024 on average, 169 / 145 us.
+// Both passes together: documents of 700 on average 428 / 386 us, a batch with prefixes 301 / 286 us, one document of 8192 with slopes 667 / 657 us.  Four were slower than two everywhere.
+static int key_share(int rep) { return rep % 2 == 0 ? 2 : 1; }
 
 // o, d_o: contiguous [B,Tq,Hq,d]; delta: scratch [B,Hq,Tq]; writes dq, dk, dv.
 template <int D, class F>
