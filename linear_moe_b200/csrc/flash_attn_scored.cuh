@@ -898,7 +898,7 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
 template <int D>
 struct __align__(1024) SmemDkv {
-    uint8_t k[BM * D * 2], v[BM * D * 2], q[2][BM * D * 2], g[2][BM * D * 2];        // q and g at the end: the sums in fp32, [dv, dk][128 rows][D]
+    uint8_t k[BM * D * 2], v[BM * D * 2], q[2][BM * D * 2], g[2][BM * D * 2];        // at the end q: the other CTA's part of the sum, g: dk and dv on their way to memory
     float lse2[2][BM], delta[2][BM];                                         // of the looped queries
     int first[2][BM], stop[2][BM];
     uint16_t list[MAX_TILES];                                                // query tiles that see a key of this tile; 0x8000: all their rows see all of it
@@ -949,6 +949,9 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         mbar_init(&sm.dv_done, 1); mbar_init(&sm.dk_done, 1); mbar_init(&sm.all_done, 1);
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mbar_expect_tx(&sm.kv_full, 2 * BM * D * 2);                          // on their way while the tensor memory is fetched and the list made
+        load_tile<D>(sm.k, &tmK, &sm.kv_full, hk, k0, b);
+        load_tile<D>(sm.v, &tmV, &sm.kv_full, hk, k0, b);
     }
     if (warp == 1) tmem_alloc_512(&sm.tmem_base);
     tc_fence_before();
@@ -956,12 +959,10 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tc_fence_after();
     const uint32_t tmem_base = uniform(sm.tmem_base);
     const int ni = uniform(sm.listed), n_it = ni * heads;
+    bool alive = n_it > 0;
 
     if (warp == 0) {
-        if (lane == 0 && n_it > 0) {
-            mbar_expect_tx(&sm.kv_full, 2 * BM * D * 2);
-            load_tile<D>(sm.k, &tmK, &sm.kv_full, hk, k0, b);
-            load_tile<D>(sm.v, &tmV, &sm.kv_full, hk, k0, b);
+        if (lane == 0) {
             for (int it = 0; it < n_it; ++it) {
                 const int s = it & 1;
                 const int h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
@@ -974,8 +975,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
         }
     } else if (warp == 1) {
+        bool ok = wait_warp(&sm.kv_full, 0, abort_flag, err, 0x26200);
         if (n_it > 0) {
-            bool ok = wait_warp(&sm.kv_full, 0, abort_flag, err, 0x26200);
             auto scores = [&](int it) -> bool {
                 if (!wait_warp(&sm.q_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26300 | (it & 1))) return false;
                 tc_fence_after();
@@ -1040,7 +1041,6 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t lane_addr = tmem_base + ((uint32_t)(qd * 32) << 16);
         ScoreOf so = score_of<F>(a.scale, a.x, h0);
         const float sc = so.unit;
-        bool alive = n_it > 0;
         for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
             const int s = it & 1, tile = sm.list[at], tile_q0 = (tile & 0x7fff) * BM;
             if (!wait_for(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
@@ -1093,18 +1093,47 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         if (alive) alive = wait_for(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
         tc_fence_after();
-        // to shared memory in fp32, units of 16 bytes at (unit ^ row % 8), so that 32 rows at a time fall into different banks
-        constexpr int OW = D / SPLIT;
-        float4* sums = reinterpret_cast<float4*>(sm.q[0]);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
+    }
+    // Two CTAs that share a tile of keys: the first one finishes dv, the second one dk.  Each warp leaves its part of the other sum in the other CTA's shared memory, where its counterpart
+    // there, which holds the same rows and columns, adds it to its own.
+    cg::cluster_group cl = cg::this_cluster();
+    constexpr int OW = D / SPLIT;
+    const uint32_t sums_at = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + ((warp - 4) >> 2) * OW;
+    float4* given = reinterpret_cast<float4*>(sm.q[0]) + (threadIdx.x - 128);                   // [unit of 4 columns][thread]
+    if (share > 1) {
+        cl.sync();                                                                              // both CTAs' products have read their tiles
+        if (warp >= 4) {
+            float4* theirs = cl.map_shared_rank(given, rank ^ 1);
             uint32_t v[OW];
-            tmem_ld<OW>(lane_addr + (x == 0 ? DV : DKC) + part * OW, v);
+            tmem_ld<OW>(sums_at + (rank == 0 ? DKC : DV), v);
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < OW; c += 4)
-                sums[(x * 128 + r) * (D / 4) + ((part * OW + c) / 4 ^ (r & 7))] =
-                    alive ? make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
+                theirs[c / 4 * 512] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+        }
+        cl.sync();
+    }
+    if (warp >= 4) {
+        const int row0 = k0 + (warp & 3) * 32, col0 = ((warp - 4) >> 2) * OW, d = a.x.d;
+        const long long at = (((long long)b * a.Tk + row0) * a.Hkv + hk) * d + col0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            if (share > 1 && rank != x) continue;
+            uint32_t v[OW], y[OW / 2];
+            tmem_ld<OW>(sums_at + (x == 0 ? DV : DKC), v);
+            tmem_ld_wait();
+            const float f = x == 0 ? 1.f : a.scale;
+#pragma unroll
+            for (int c = 0; c < OW; c += 4) {
+                float4 z = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+                if (share > 1) {
+                    const float4 o = given[c / 4 * 512];
+                    z.x += o.x; z.y += o.y; z.z += o.z; z.w += o.w;
+                }
+                y[c / 2] = alive ? pack16<F>(f * z.x, f * z.y) : 0u;                            // no query sees these keys: zeros
+                y[c / 2 + 1] = alive ? pack16<F>(f * z.z, f * z.w) : 0u;
+            }
+            rows_out<OW>(sm.g[0] + (warp - 4) * 32 * OW * 2, y, (x == 0 ? a.dv : a.dk) + at, (long long)a.Hkv * d, min(32, a.Tk - row0), d - col0);
         }
     }
     tc_fence_before();
@@ -1113,47 +1142,29 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_after();
         tmem_free_512(tmem_base);
     }
-    // the CTAs of a cluster add their sums, each for a part of the rows, in the order of the heads
-    cg::cluster_group cl = cg::this_cluster();
-    if (share > 1) cl.sync();
-    const int per = BM / share, d = a.x.d;
-    for (int i = threadIdx.x; i < 2 * per * (D / 4); i += THREADS) {
-        const int x = i / (per * (D / 4)), rem = i % (per * (D / 4)), r = rank * per + rem / (D / 4), u = rem % (D / 4);
-        if (k0 + r >= a.Tk || u * 4 >= d) continue;
-        const float4* mine = reinterpret_cast<const float4*>(sm.q[0]) + (x * 128 + r) * (D / 4) + (u ^ (r & 7));
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; c < share; ++c) {
-            const float4 z = share > 1 ? *cl.map_shared_rank(mine, c) : *mine;
-            y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-        }
-        const float f = x == 0 ? 1.f : a.scale;
-        bf16* out = (x == 0 ? a.dv : a.dk) + (((long long)b * a.Tk + k0 + r) * a.Hkv + hk) * d + u * 4;
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack16<F>(f * y.x, f * y.y), pack16<F>(f * y.z, f * y.w));
-    }
-    if (share > 1) cl.sync();                                                                   // the others have read this CTA's sums
 }
 
 // delta[b,h,t] = sum_d dO[b,t,h,d] (O + low)[b,t,h,d].  Bound by reading the tensors once: D / 8 lanes take a row 16 bytes at a time, and a thread
 // asks for its pieces of four rows before it uses the first (a warp per row with 4-byte loads had too little in flight).
 template <int D, class F>
 __global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ low, const bf16* __restrict__ d_o,
-                                                          float* __restrict__ delta, int B, int Tq, int Hq, int d) {
+                                                          float* __restrict__ delta, int Tq, int Hq, int d) {
     constexpr int LANES = D / 8, PER = 256 / LANES, U = 4;       // lanes of a row, rows of a block at a time
-    const int l = threadIdx.x % LANES;
-    const long long rows = (long long)B * Tq * Hq, row0 = (long long)blockIdx.x * (PER * U) + threadIdx.x / LANES;
+    const int l = threadIdx.x % LANES, rows = Tq * Hq;           // of a sequence: below 2^31 (64-bit divisions for every row cost more than the sums)
+    const int blocks = (rows + PER * U - 1) / (PER * U), b = blockIdx.x / blocks, row0 = (blockIdx.x - b * blocks) * (PER * U) + threadIdx.x / LANES;
     uint4 x[U], y[U], z[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         x[u] = y[u] = z[u] = make_uint4(0, 0, 0, 0);
         if (l * 8 >= d) continue;
-        const long long at = min(row0 + u * PER, rows - 1) * d + l * 8;
+        const long long at = ((long long)b * rows + min(row0 + u * PER, rows - 1)) * d + l * 8;
         x[u] = *reinterpret_cast<const uint4*>(o + at);
         y[u] = *reinterpret_cast<const uint4*>(d_o + at);
         z[u] = *reinterpret_cast<const uint4*>(low + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long row = row0 + u * PER;
+        const int row = row0 + u * PER;
         float s = 0.f;
         const uint32_t* xs = reinterpret_cast<const uint32_t*>(&x[u]);
         const uint32_t* ys = reinterpret_cast<const uint32_t*>(&y[u]);
@@ -1168,8 +1179,8 @@ __global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restric
 #pragma unroll
         for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
         if (l == 0 && row < rows) {
-            const long long bt = row / Hq;
-            delta[((bt / Tq) * Hq + row % Hq) * Tq + bt % Tq] = s;
+            const int t = row / Hq, h = row - t * Hq;
+            delta[((long long)b * Hq + h) * Tq + t] = s;
         }
     }
 }
@@ -1212,9 +1223,8 @@ static int launch_bwd(const void* q, const long long* qs, const void* k, const l
     rc |= make_map_4d(&mk, k, a.B, a.Tk, a.Hkv, d, ks[0], ks[1], ks[2], BM);
     rc |= make_map_4d(&mv, v, a.B, a.Tk, a.Hkv, d, vs[0], vs[1], vs[2], BM);
     if (rc) return -11;
-    const long long rows = (long long)a.B * a.Tq * a.Hq;
     constexpr int per_block = 4 * 256 / (D / 8);
-    scored_delta_kernel<D, F><<<(unsigned)((rows + per_block - 1) / per_block), 256, 0, st>>>((const bf16*)o, a.x.low, (const bf16*)d_o, delta, a.B, a.Tq, a.Hq, d);
+    scored_delta_kernel<D, F><<<(unsigned)((a.Tq * a.Hq + per_block - 1) / per_block) * a.B, 256, 0, st>>>((const bf16*)o, a.x.low, (const bf16*)d_o, delta, a.Tq, a.Hq, d);
     constexpr int dq_smem = sizeof(SmemDq<D>), dkv_smem = sizeof(SmemDkv<D>);
     rc = (int)cudaFuncSetAttribute(scored_dq_kernel<D, F>, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem);
     if (rc) return rc;
@@ -1251,7 +1261,7 @@ static int bwd_by_width(const void* q, const long long* qs, const void* k, const
 }
 static bool scored_args_ok(const Ranges& x, int B, int Tq, int Tk, int Hq, int Hkv) {
     return B > 0 && Tq > 0 && Tk > 0 && Hkv > 0 && Hq % Hkv == 0 && x.d > 0 && x.d <= 128 && x.d % 8 == 0 && x.tiles != nullptr &&
-           (Tq + BM - 1) / BM <= MAX_TILES;
+           (Tq + BM - 1) / BM <= MAX_TILES && Hq < 1024;               // 2^20 queries, below 2^30 rows of a sequence
 }
 template <bool H>
 static int scored_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const Args& a, cudaStream_t st) {
