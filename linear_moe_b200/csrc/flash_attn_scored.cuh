@@ -279,6 +279,23 @@ __device__ __forceinline__ void grad_product(uint32_t tmem_d, uint32_t tmem_a, c
     for (int kk = 0; kk < 128 / UMMA_K; ++kk)
         umma_ts(tmem_d, tmem_a + kk / 2 * 32 + kk % 2 * 8, bl + ((kk * 2048) >> 4), idesc_of<F, true, D>(), add || kk > 0);
 }
+// The same with 64 queries for B, and over 64 queries.  QB: bytes between the 64-column blocks of B
+template <int D, class F, int QB>
+__device__ __forceinline__ void half_product(uint32_t tmem_d, const uint8_t* A, const uint8_t* B) {
+    if (!elect_one()) return;
+    const uint32_t al = desc_lo<false>(s32(A)), bl = desc_lo<false>(s32(B));
+#pragma unroll
+    for (int kk = 0; kk < D / UMMA_K; ++kk)
+        umma_ss(tmem_d, al + (((kk / 4) * BLK + (kk % 4) * 32) >> 4), bl + (((kk / 4) * QB + (kk % 4) * 32) >> 4), idesc_of<F, false, 64>(), kk > 0);
+}
+template <int D, class F, int QB>
+__device__ __forceinline__ void half_grad(uint32_t tmem_d, uint32_t tmem_a, const uint8_t* B, bool add) {
+    if (!elect_one()) return;
+    const uint32_t bl = ((s32(B) >> 4) & 0x3FFFu) | ((uint32_t)(QB >> 4) << 16);
+#pragma unroll
+    for (int kk = 0; kk < 64 / UMMA_K; ++kk)
+        umma_ts(tmem_d, tmem_a + kk / 2 * 32 + kk % 2 * 8, bl + ((kk * 2048) >> 4), idesc_of<F, true, D>(), add || kk > 0);
+}
 // this thread's 32 columns of an operand, over scores that it has read
 __device__ __forceinline__ void hand_over(uint32_t taddr, const uint32_t (&v)[16], uint64_t* bar) {
     tmem_st16(taddr, v);
@@ -898,11 +915,13 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
 template <int D>
 struct __align__(1024) SmemDkv {
-    uint8_t k[BM * D * 2], v[BM * D * 2], q[2][BM * D * 2], g[2][BM * D * 2];        // at the end q: the other CTA's part of the sum, g: dk and dv on their way to memory
+    static constexpr int QS = 4;                                             // half tiles of Q
+    uint8_t k[BM * D * 2], v[BM * D * 2], q[QS][64 * D * 2], g[2][BM * D * 2];        // at the end q: the other CTA's part of the sum, g: dk and dv on their way to memory
     float lse2[2][BM], delta[2][BM];                                         // of the looped queries
     int first[2][BM], stop[2][BM];
     uint16_t list[MAX_TILES];                                                // query tiles that see a key of this tile; 0x8000: all their rows see all of it
-    uint64_t kv_full, q_full[2], q_empty[2], stat_full[2], g_full[2], g_empty[2], s_full, dp_full, p_ready, ds_ready, dv_done, dk_done, all_done;
+    uint64_t kv_full, q_full[QS], q_empty[QS], stat_full[2], stat_empty[2], g_full[2], g_empty[2];
+    uint64_t s_full[2], dp_full[2], p_ready[2], ds_ready[2], dv_done[2], dk_done[2], all_done;      // [half of the queries]
     uint32_t tmem_base;
     int abort_flag, listed;
 };
@@ -919,6 +938,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         return;
     }
     constexpr uint32_t ST = 0, DP = 128, DV = 256, DKC = 384;
+    constexpr int QS = SmemDkv<D>::QS;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rep = a.Hq / a.Hkv, share = rep / heads, rank = blockIdx.x % share;
     const TileOf t = longest_first(blockIdx.x / share, (a.Tk + BM - 1) / BM, a.B * a.Hkv, group);
@@ -940,13 +960,17 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (threadIdx.x == 0) {
         mbar_init(&sm.kv_full, 1);
+        for (int s = 0; s < QS; ++s) { mbar_init(&sm.q_full[s], 1); mbar_init(&sm.q_empty[s], 1); }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&sm.q_full[s], 1); mbar_init(&sm.q_empty[s], 1); mbar_init(&sm.stat_full[s], 1);
+            mbar_init(&sm.stat_full[s], 1); mbar_init(&sm.stat_empty[s], 1);
             mbar_init(&sm.g_full[s], 1); mbar_init(&sm.g_empty[s], 1);
         }
-        mbar_init(&sm.s_full, 1); mbar_init(&sm.dp_full, 1);
-        mbar_init(&sm.p_ready, 16); mbar_init(&sm.ds_ready, 16);
-        mbar_init(&sm.dv_done, 1); mbar_init(&sm.dk_done, 1); mbar_init(&sm.all_done, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sm.s_full[s], 1); mbar_init(&sm.dp_full[s], 1);
+            mbar_init(&sm.p_ready[s], 8); mbar_init(&sm.ds_ready[s], 8);
+            mbar_init(&sm.dv_done[s], 1); mbar_init(&sm.dk_done[s], 1);
+        }
+        mbar_init(&sm.all_done, 1);
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         mbar_expect_tx(&sm.kv_full, 2 * BM * D * 2);                          // on their way while the tensor memory is fetched and the list made
@@ -964,51 +988,70 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 0) {
         if (lane == 0) {
             for (int it = 0; it < n_it; ++it) {
-                const int s = it & 1;
-                const int h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
-                if (!wait_for(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26100 | s)) break;
-                mbar_expect_tx(&sm.q_full[s], BM * D * 2);
-                load_tile<D>(sm.q[s], &tmQ, &sm.q_full[s], h, q0, b);
+                const int s = it & 1, h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
+                auto half_q = [&](int half) -> bool {
+                    const int n = 2 * it + half, sq = n % QS;
+                    if (!wait_for(&sm.q_empty[sq], ((n / QS) & 1) ^ 1, abort_flag, err, 0x26100 | sq)) return false;
+                    mbar_expect_tx(&sm.q_full[sq], 64 * D * 2);
+#pragma unroll
+                    for (int kb = 0; kb < D / 64; ++kb) tma_load_4d(sm.q[sq] + kb * 8192, &tmQ, &sm.q_full[sq], kb * 64, h, q0 + half * 64, b);
+                    return true;
+                };
+                if (!half_q(0)) break;                            // in the order in which the buffers get free
                 if (!wait_for(&sm.g_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26120 | s)) break;
                 mbar_expect_tx(&sm.g_full[s], BM * D * 2);
                 load_tile<D>(sm.g[s], &tmG, &sm.g_full[s], h, q0, b);
+                if (!half_q(1)) break;
             }
         }
     } else if (warp == 1) {
         bool ok = wait_warp(&sm.kv_full, 0, abort_flag, err, 0x26200);
         if (n_it > 0) {
-            auto scores = [&](int it) -> bool {
-                if (!wait_warp(&sm.q_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26300 | (it & 1))) return false;
+            auto scores = [&](int it, int half) -> bool {
+                const int n = 2 * it + half, sq = n % QS;
+                if (!wait_warp(&sm.q_full[sq], (n / QS) & 1, abort_flag, err, 0x26300 | sq)) return false;
                 tc_fence_after();
-                score_product<D, F>(tmem_base + ST, sm.k, sm.q[it & 1]);
-                if (elect_one()) umma_commit(&sm.s_full);
+                half_product<D, F, 8192>(tmem_base + ST + half * 64, sm.k, sm.q[sq]);
+                if (elect_one()) umma_commit(&sm.s_full[half]);
                 return true;
             };
-            auto dprobs = [&](int it) -> bool {
+            auto dprobs = [&](int it, int half) -> bool {
                 if (!wait_warp(&sm.g_full[it & 1], (it >> 1) & 1, abort_flag, err, 0x26310 | (it & 1))) return false;
                 tc_fence_after();
-                score_product<D, F>(tmem_base + DP, sm.v, sm.g[it & 1]);
-                if (elect_one()) umma_commit(&sm.dp_full);
+                half_product<D, F, BLK>(tmem_base + DP + half * 64, sm.v, sm.g[it & 1] + half * 8192);
+                if (elect_one()) umma_commit(&sm.dp_full[half]);
                 return true;
             };
-            if (ok) ok = scores(0) && dprobs(0);
+            auto grad_v = [&](int it, int half) -> bool {                                         // dV += P^T dO
+                if (!wait_warp(&sm.p_ready[half], it & 1, abort_flag, err, 0x26400 | half)) return false;
+                tc_fence_after();
+                half_grad<D, F, BLK>(tmem_base + DV, tmem_base + ST + half * 64, sm.g[it & 1] + half * 8192, it > 0 || half > 0);
+                if (elect_one()) umma_commit(&sm.dv_done[half]);
+                if (half == 1 && elect_one()) umma_commit(&sm.g_empty[it & 1]);
+                return true;
+            };
+            auto grad_k = [&](int it, int half) -> bool {                                         // dK += dS^T Q
+                if (!wait_warp(&sm.ds_ready[half], it & 1, abort_flag, err, 0x26410 | half)) return false;
+                tc_fence_after();
+                const int sq = (2 * it + half) % QS;
+                half_grad<D, F, 8192>(tmem_base + DKC, tmem_base + DP + half * 64, sm.q[sq], it > 0 || half > 0);
+                if (elect_one()) umma_commit(&sm.dk_done[half]);
+                if (elect_one()) umma_commit(&sm.q_empty[sq]);
+                if (half == 1 && elect_one()) umma_commit(&sm.stat_empty[it & 1]);
+                return true;
+            };
+            // the next scores go over P^T, the next dP^T over dS^T: the products that read them have to complete (waited for at every tile, so that no phase is passed over)
+            auto free_p = [&](int it, int half) { return wait_warp(&sm.dv_done[half], it & 1, abort_flag, err, 0x26600 | half); };
+            auto free_ds = [&](int it, int half) { return wait_warp(&sm.dk_done[half], it & 1, abort_flag, err, 0x26610 | half); };
+            ok = ok && scores(0, 0) && dprobs(0, 0) && scores(0, 1) && dprobs(0, 1);
             for (int it = 0; ok && it < n_it; ++it) {
-                if (!wait_warp(&sm.p_ready, it & 1, abort_flag, err, 0x26400)) break;
-                tc_fence_after();
                 const bool more = it + 1 < n_it;
-                grad_product<D, F>(tmem_base + DV, tmem_base + ST, sm.g[it & 1], it > 0);   // dV += P^T dO
-                if (elect_one()) umma_commit(&sm.g_empty[it & 1]);
-                if (more) {
-                    // the next scores go over P^T: the product that reads it has to complete
-                    if (elect_one()) umma_commit(&sm.dv_done);
-                    if (!wait_warp(&sm.dv_done, it & 1, abort_flag, err, 0x26600) || !scores(it + 1)) break;
-                }
-                if (!wait_warp(&sm.ds_ready, it & 1, abort_flag, err, 0x26410)) break;
-                tc_fence_after();
-                grad_product<D, F>(tmem_base + DKC, tmem_base + DP, sm.q[it & 1], it > 0);  // dK += dS^T Q
-                if (elect_one()) { umma_commit(&sm.q_empty[it & 1]); umma_commit(more ? &sm.dk_done : &sm.all_done); }
-                if (more) ok = wait_warp(&sm.dk_done, it & 1, abort_flag, err, 0x26610) && dprobs(it + 1);
+                // the first half's weights and the second half's gradients of the tile before
+                ok = grad_v(it, 0) && (it == 0 || grad_k(it - 1, 1)) && free_p(it, 0) && (!more || scores(it + 1, 0)) && (it == 0 || (free_ds(it - 1, 1) && dprobs(it, 1)));
+                // the second half's weights and the first half's gradients
+                ok = ok && grad_v(it, 1) && grad_k(it, 0) && free_p(it, 1) && (!more || scores(it + 1, 1)) && free_ds(it, 0) && (!more || dprobs(it + 1, 0));
             }
+            if (ok && grad_k(n_it - 1, 1) && elect_one()) umma_commit(&sm.all_done);
         }
     } else if (warp == 2) {                                      // log-sum-exp, delta and range of the looped queries
         for (int it = 0; it < n_it; ++it) {
@@ -1025,7 +1068,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (x[e] == -INFINITY) x[e] = INFINITY;          // a row that sees nothing: its weights are zero
                 range[e] = q < a.Tq ? visible_range(a, b, q) : make_int2(0, 0);
             }
-            if (!wait_for(&sm.q_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
+            if (!wait_for(&sm.stat_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 sm.lse2[s][lane + 32 * e] = x[e]; sm.delta[s][lane + 32 * e] = y[e];
@@ -1035,7 +1078,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (lane == 0) mbar_arrive(&sm.stat_full[s]);
         }
     } else if (warp >= 4) {
-        const int qd = warp & 3, part = (warp - 4) >> 2;
+        const int qd = warp & 3, part = (warp - 4) >> 2, half = part >> 1;
         const int r = qd * 32 + lane;                            // key row inside the tile
         const int key = k0 + r;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(qd * 32) << 16);
@@ -1044,7 +1087,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
             const int s = it & 1, tile = sm.list[at], tile_q0 = (tile & 0x7fff) * BM;
             if (!wait_for(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
-            if (!wait_for(&sm.s_full, it & 1, abort_flag, err, 0x26500)) { alive = false; break; }
+            if (!wait_for(&sm.s_full[half], it & 1, abort_flag, err, 0x26500 | half)) { alive = false; break; }
             tc_fence_after();
             uint32_t v[32], pk[16];
             float2 p[16];
@@ -1072,8 +1115,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 p[i] = F::SCORE == SCORE_CAP ? __fmul2_rn(p[i], ex) : ex;
                 p[i + 1] = F::SCORE == SCORE_CAP ? __fmul2_rn(p[i + 1], ey) : ey;
             }
-            hand_over(lane_addr + ST + part * 32, pk, &sm.p_ready);
-            if (!wait_for(&sm.dp_full, it & 1, abort_flag, err, 0x26520)) { alive = false; break; }
+            hand_over(lane_addr + ST + part * 32, pk, &sm.p_ready[half]);
+            if (!wait_for(&sm.dp_full[half], it & 1, abort_flag, err, 0x26520 | half)) { alive = false; break; }
             tc_fence_after();
             tmem_ld32(lane_addr + DP + part * 32, v);
             tmem_ld_wait();
@@ -1085,7 +1128,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 pk[i] = pack16<F>(x.x, x.y);
                 pk[i + 1] = pack16<F>(y.x, y.y);
             }
-            hand_over(lane_addr + DP + part * 32, pk, &sm.ds_ready);
+            hand_over(lane_addr + DP + part * 32, pk, &sm.ds_ready[half]);
             if (++at == ni) {                                                                   // the next head
                 at = 0;
                 if (F::SCORE != SCORE_PLAIN && it + 1 < n_it) so = score_of<F>(a.scale, a.x, ++h);
@@ -1216,9 +1259,10 @@ static int launch_bwd(const void* q, const long long* qs, const void* k, const l
     const int d = a.x.d;
     a.delta = delta;
     const long long gs[3] = {(long long)a.Tq * a.Hq * d, (long long)a.Hq * d, (long long)d};
-    CUtensorMap mq, mg, mk, mv;
+    CUtensorMap mq, mqh, mg, mk, mv;
     int rc = 0;
     rc |= make_map_4d(&mq, q, a.B, a.Tq, a.Hq, d, qs[0], qs[1], qs[2], BM);
+    rc |= make_map_4d(&mqh, q, a.B, a.Tq, a.Hq, d, qs[0], qs[1], qs[2], BM / 2);
     rc |= make_map_4d(&mg, d_o, a.B, a.Tq, a.Hq, d, gs[0], gs[1], gs[2], BM);
     rc |= make_map_4d(&mk, k, a.B, a.Tk, a.Hkv, d, ks[0], ks[1], ks[2], BM);
     rc |= make_map_4d(&mv, v, a.B, a.Tk, a.Hkv, d, vs[0], vs[1], vs[2], BM);
@@ -1246,7 +1290,7 @@ static int launch_bwd(const void* q, const long long* qs, const void* k, const l
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = share > 1 ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, scored_dkv_kernel<D, F>, mq, mg, mk, mv, a, pairs_in_l2(a.B * a.Hkv, a.Tq, D, 1), rep / share);
+    cudaLaunchKernelEx(&cfg, scored_dkv_kernel<D, F>, mqh, mg, mk, mv, a, pairs_in_l2(a.B * a.Hkv, a.Tq, D, 1), rep / share);
     return (int)cudaGetLastError();
 }
 
@@ -1261,7 +1305,7 @@ static int bwd_by_width(const void* q, const long long* qs, const void* k, const
 }
 static bool scored_args_ok(const Ranges& x, int B, int Tq, int Tk, int Hq, int Hkv) {
     return B > 0 && Tq > 0 && Tk > 0 && Hkv > 0 && Hq % Hkv == 0 && x.d > 0 && x.d <= 128 && x.d % 8 == 0 && x.tiles != nullptr &&
-           (Tq + BM - 1) / BM <= MAX_TILES && Hq < 1024;               // 2^20 queries, below 2^30 rows of a sequence
+           (Tq + BM - 1) / BM <= MAX_TILES && Hq < 1024;               // (below 2^30 rows of a sequence)
 }
 template <bool H>
 static int scored_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const Args& a, cudaStream_t st) {
