@@ -24,7 +24,7 @@ struct Ranges {
     const int *first, *stop;              // [B, Tq] with strides (first_b, 1), (stop_b, 1); null: 0 and Tk
     long long first_b, stop_b;
     const float* slopes;                  // [Hq]; null: no bias
-    bf16* low;                            // [B, Tq, Hq, d]: what the output's rounding took away, rounded itself; null: not wanted
+    int8_t* low;                          // [B, Tq, Hq, d rounded up to 16]: the next eight bits of the output (residue); null: not wanted
     int4* tiles;                          // [B, query tiles]: union of the rows' intervals, then their intersection
     float cap;
     int causal, d;                        // d: head size, a multiple of 8 up to D (tensor maps fill the rest with zeros)
@@ -67,6 +67,22 @@ template <class F> __device__ __forceinline__ float2 unpack16(uint32_t x) {
     if constexpr (F::HALF) return __half22float2(*reinterpret_cast<const __half2*>(&x));
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
 }
+// What the output's rounding took away.  delta = do . o is subtracted from dp, nearly its equal where one weight is large: with the rounded o alone dq and dk were off by 0.0042 at scores
+// of 6 in root mean square, with eight bits more 0.0025 (their own rounding: 0.0017).  Both numbers have the same sign, so their patterns differ by an integer: at most half a step, 2^15
+// (fp16: 2^12; 2^15 after a shift), of which the upper eight bits are kept.  Four numbers and the two pairs that they were rounded to -> four bytes.
+template <class F> __device__ __forceinline__ uint32_t residues(float a, float b, float c, float d, uint32_t ab, uint32_t cd) {
+    const float2 x = unpack16<F>(ab), y = unpack16<F>(cd);
+    int e[4] = {__float_as_int(a) - __float_as_int(x.x), __float_as_int(b) - __float_as_int(x.y), __float_as_int(c) - __float_as_int(y.x), __float_as_int(d) - __float_as_int(y.y)};
+    if constexpr (F::HALF) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = min(max(e[i], -4096), 4096) * 8;                       // (in fp16's subnormals a step is more)
+    }
+    uint32_t p, q;
+    asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(p) : "r"(e[1]), "r"(e[0]));
+    asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(q) : "r"(e[3]), "r"(e[2]));
+    return __byte_perm(p, q, 0x7531);
+}
+template <class F> __device__ __forceinline__ float with_residue(float kept, int r) { return __int_as_float(__float_as_int(kept) + r * (F::HALF ? 32 : 256)); }
 // operand types of the instruction descriptor: bits 7 and 10 set for bf16, clear for fp16
 template <class F, bool B_MN, int N> __host__ __device__ constexpr uint32_t idesc_of() {
     return F::HALF ? idesc_bf16<B_MN, N>() & ~((1u << 7) | (1u << 10)) : idesc_bf16<B_MN, N>();
@@ -330,10 +346,19 @@ struct __align__(1024) SmemFwd {
     float mx[2][2][2][BM];                                    // [parity of the group's tile][group][half of the columns]
     float ls[2][2][2][BM], ms[2][2][BM];                      // sums and maxima at the end, [parity of the tile of queries][group]
     int2 seen[2][BM];                                         // [slot]: the rows' visible keys
+    __align__(1024) uint8_t low[BM * D];
     uint32_t tmem_base;
     int abort_flag;
 };
 
+// N units of 16 bytes of a row, from unit `at` on, where a tensor map that swizzles rows of W bytes (64 or 128) expects them
+template <int W, int N>
+__device__ __forceinline__ void stage_units(uint8_t* tile, int row, int at, const uint32_t (&y)[4 * N]) {
+    const int key = row * W / 128 & (W / 16 - 1);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+        *reinterpret_cast<uint4*>(tile + row * W + ((at + u ^ key) << 4)) = make_uint4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
+}
 // 32 rows x OW columns of a warp (lane = row) through 32 x OW x 2 bytes of shared memory to rows of `d` numbers: a store then covers whole pieces of rows, not 16 bytes of 32 rows.
 template <int OW>
 __device__ __forceinline__ void rows_out(uint8_t* stage, const uint32_t (&y)[OW / 2], bf16* out, long long row_stride, int rows, int cols) {
@@ -355,7 +380,8 @@ __device__ __forceinline__ void rows_out(uint8_t* stage, const uint32_t (&y)[OW 
 
 template <int D, class F>
 __global__ void __launch_bounds__(THREADS, 1)
-scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a, int group) {
+scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmL, const Args a, int group) {
     extern __shared__ uint8_t smem_raw[];
     SmemFwd<D>& sm = *reinterpret_cast<SmemFwd<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int KS = SmemFwd<D>::KS, DK = D / 64;
@@ -366,7 +392,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (threadIdx.x == 0) {
         for (int s = 0; s < KS; ++s) { mbar_init(&sm.k_full[s], 1); mbar_init(&sm.k_empty[s], 1); }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&sm.q_full[s], 1); mbar_init(&sm.q_empty[s], 16);
+            mbar_init(&sm.q_full[s], 1); mbar_init(&sm.q_empty[s], 4);
             mbar_init(&sm.v_full[s], 1); mbar_init(&sm.v_empty[s], 1);
             mbar_init(&sm.s_full[s], 1); mbar_init(&sm.pv_done[s], 1);
             mbar_init(&sm.p_ready[s], 8);
@@ -479,6 +505,16 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool ok = true;                                       // after a wait that ran out only the barriers are kept up with
         // (What the loop over key tiles does not need at every turn is left in shared memory: the 64 scores of a thread leave few registers.)
         int done[2] = {0, 0};                                 // key tiles of the groups so far
+        int owed = -1;                                        // (quarter 0) buffer of Q from which rows are still on their way
+        auto settle = [&]() {
+            if (owed < 0) return;
+            if (lane == 0) {
+                tma_store_wait_read();
+                mbar_arrive(&sm.q_empty[owed]);
+            }
+            __syncwarp();
+            owed = -1;
+        };
         for (int it = 0, qi = 0;; ++it) {
             const int slot = it & 1;
             if (ok) ok = wait_warp(&sm.work.full[slot], (it >> 1) & 1, abort_flag, err, 0x24000 | slot);
@@ -589,6 +625,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_ready[grp]);
             }
+            settle();
             const Item w = sm.work.item[slot];
             const int row = w.q0 + r, d = a.x.d;
             const long long out0 = (((long long)w.b * a.Tq + w.q0 + qd * 32) * a.Hq + w.h) * d + quarter * OW, row_stride = (long long)a.Hq * d;
@@ -598,10 +635,11 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (lane == 0) mbar_arrive(&sm.work.empty[slot]);
             if (n_it == 0) {                                  // nothing to see: zeros
                 if (row < a.Tq) {
-                    for (int c = 0; c < OW && c < cols; c += 8) {
-                        *reinterpret_cast<uint4*>(a.out + out0 + lane * row_stride + c) = make_uint4(0, 0, 0, 0);
-                        if (a.x.low != nullptr) *reinterpret_cast<uint4*>(a.x.low + out0 + lane * row_stride + c) = make_uint4(0, 0, 0, 0);
-                    }
+                    for (int c = 0; c < OW && c < cols; c += 8) *reinterpret_cast<uint4*>(a.out + out0 + lane * row_stride + c) = make_uint4(0, 0, 0, 0);
+                    const int wide = (d + 15) & ~15;
+                    if (a.x.low != nullptr)
+                        for (int c = quarter * OW; c < (quarter + 1) * OW && c < wide; c += 16)
+                            *reinterpret_cast<uint4*>(a.x.low + (((long long)w.b * a.Tq + row) * a.Hq + w.h) * wide + c) = make_uint4(0, 0, 0, 0);
                     if (quarter == 0) *lse = -INFINITY;
                 }
                 continue;
@@ -641,28 +679,37 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 uint32_t y[OW / 2];
 #pragma unroll
                 for (int c = 0; c < OW; c += 2) y[c / 2] = pack16<F>(o[c] * inv, o[c + 1] * inv);
-                uint8_t* stage = sm.q[qi & 1] + (warp - 4) * 32 * OW * 2;            // both groups' products of this tile are done
-                rows_out<OW>(stage, y, a.out + out0, row_stride, rows, cols);
+                // Both groups' products of this tile are done: the rows go through Q's buffer, by bulk copies, which go on while the warps turn to the next tile.  The four warps of 32 rows
+                // join theirs: copies of 128 bytes a row are three times as fast as of 64 and 32.
+                uint8_t* stage = sm.q[qi & 1];
+                if constexpr (D == 128) stage_units<128, 4>(stage + (quarter >> 1) * BLK, r, (quarter & 1) * 4, y);
+                else stage_units<128, 2>(stage, r, quarter * 2, y);
                 if (a.x.low != nullptr) {
-                    // delta = do . o is subtracted from dp, nearly its equal where one weight is large: with the rounded o alone dq and dk were off by 0.0042
-                    // at scores of 6 in root mean square, with this part 0.0025 (their own rounding: 0.0017)
+                    uint32_t z[OW / 4];
 #pragma unroll
-                    for (int c = 0; c < OW; c += 2) {
-                        const float2 z = unpack16<F>(y[c / 2]);
-                        y[c / 2] = pack16<F>(o[c] * inv - z.x, o[c + 1] * inv - z.y);
-                    }
-                    rows_out<OW>(stage, y, a.x.low + out0, row_stride, rows, cols);
+                    for (int c = 0; c < OW; c += 4) z[c / 4] = residues<F>(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv, y[c / 2], y[c / 2 + 1]);
+                    stage_units<D, OW / 16>(sm.low, r, quarter * (OW / 16), z);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            asm volatile("bar.sync %0, 128;" :: "r"(11 + qd) : "memory");
+            if (quarter == 0) {
+                if (ok && lane == 0 && rows > 0) {
+#pragma unroll
+                    for (int kb = 0; kb < D / 64; ++kb)
+                        if (kb * 64 < d) tma_store_4d(&tmO, sm.q[qi & 1] + kb * BLK + qd * 4096, kb * 64, w.h, w.q0 + qd * 32, w.b);
+                    if (a.x.low != nullptr) tma_store_4d(&tmL, sm.low + qd * 32 * D, 0, w.h, w.q0 + qd * 32, w.b);
+                    tma_store_commit();
                 }
                 const float unit = F::SCORE == SCORE_PLAIN ? a.scale : F::SCORE == SCORE_BIAS ? 1.f / LOG2E : a.x.cap;
-                if (quarter == 0 && row < a.Tq) *lse = l > 0.f ? mm * unit + logf(l) : -INFINITY;
+                if (row < a.Tq) *lse = l > 0.f ? mm * unit + logf(l) : -INFINITY;
+                owed = qi & 1;
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // ahead of the next Q in this buffer
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.q_empty[qi & 1]);
             done[0] += (n_it + 1) / 2;
             done[1] += n_it / 2;
             ++qi;
         }
+        if (lane == 0) tma_store_wait();
     }
     tc_fence_before();
     __syncthreads();
@@ -1187,23 +1234,24 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
 }
 
-// delta[b,h,t] = sum_d dO[b,t,h,d] (O + low)[b,t,h,d].  Bound by reading the tensors once: D / 8 lanes take a row 16 bytes at a time, and a thread
+// delta[b,h,t] = sum_d dO[b,t,h,d] O[b,t,h,d], O with its residue.  Bound by reading the tensors once: D / 8 lanes take a row 16 bytes at a time, and a thread
 // asks for its pieces of four rows before it uses the first (a warp per row with 4-byte loads had too little in flight).
 template <int D, class F>
-__global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ low, const bf16* __restrict__ d_o,
+__global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restrict__ o, const int8_t* __restrict__ low, const bf16* __restrict__ d_o,
                                                           float* __restrict__ delta, int Tq, int Hq, int d) {
     constexpr int LANES = D / 8, PER = 256 / LANES, U = 4;       // lanes of a row, rows of a block at a time
     const int l = threadIdx.x % LANES, rows = Tq * Hq;           // of a sequence: below 2^31 (64-bit divisions for every row cost more than the sums)
     const int blocks = (rows + PER * U - 1) / (PER * U), b = blockIdx.x / blocks, row0 = (blockIdx.x - b * blocks) * (PER * U) + threadIdx.x / LANES;
-    uint4 x[U], y[U], z[U];
+    uint4 x[U], y[U];
+    uint2 z[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        x[u] = y[u] = z[u] = make_uint4(0, 0, 0, 0);
+        x[u] = y[u] = make_uint4(0, 0, 0, 0), z[u] = make_uint2(0, 0);
         if (l * 8 >= d) continue;
-        const long long at = ((long long)b * rows + min(row0 + u * PER, rows - 1)) * d + l * 8;
+        const long long row = (long long)b * rows + min(row0 + u * PER, rows - 1), at = row * d + l * 8;
         x[u] = *reinterpret_cast<const uint4*>(o + at);
         y[u] = *reinterpret_cast<const uint4*>(d_o + at);
-        z[u] = *reinterpret_cast<const uint4*>(low + at);
+        z[u] = *reinterpret_cast<const uint2*>(low + row * ((d + 15) & ~15) + l * 8);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1211,13 +1259,12 @@ __global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restric
         float s = 0.f;
         const uint32_t* xs = reinterpret_cast<const uint32_t*>(&x[u]);
         const uint32_t* ys = reinterpret_cast<const uint32_t*>(&y[u]);
-        const uint32_t* zs = reinterpret_cast<const uint32_t*>(&z[u]);
+        const int8_t* zs = reinterpret_cast<const int8_t*>(&z[u]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 p = unpack16<F>(xs[e]), g = unpack16<F>(ys[e]);
-            const float2 r = unpack16<F>(zs[e]);
-            s += (p.x + r.x) * g.x;
-            s += (p.y + r.y) * g.y;
+            s += with_residue<F>(p.x, zs[2 * e]) * g.x;
+            s += with_residue<F>(p.y, zs[2 * e + 1]) * g.y;
         }
 #pragma unroll
         for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
@@ -1229,6 +1276,18 @@ __global__ void __launch_bounds__(256) scored_delta_kernel(const bf16* __restric
 }
 
 // ---- launches: strides in elements (batch, token, head); 16-byte aligned bases, strides multiples of 8 ---------------------------
+// Contiguous [B, T, H, d] bytes: boxes of 32 rows of D
+template <int D>
+static int make_map_low(CUtensorMap* map, const void* ptr, int B, int T, int H, int d) {
+    EncodeTiledFn enc = get_encode();
+    if (enc == nullptr) return -10;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
+    const cuuint64_t strides[3] = {(cuuint64_t)d, (cuuint64_t)d * H, (cuuint64_t)d * H * T};
+    const cuuint32_t box[4] = {D, 1, 32, 1}, estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -11;
+}
 template <int D, class F>
 static int launch_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const Args& a, cudaStream_t st) {
     const int d = a.x.d;
@@ -1239,11 +1298,18 @@ static int launch_fwd(const void* q, const long long* qs, const void* k, const l
     if (rc) return rc;
     rc = make_map_4d(&mv, v, a.B, a.Tk, a.Hkv, d, vs[0], vs[1], vs[2], 64);
     if (rc) return rc;
+    CUtensorMap mo, ml;
+    rc = make_map_4d(&mo, a.out, a.B, a.Tq, a.Hq, d, (long long)a.Tq * a.Hq * d, (long long)a.Hq * d, d, 32);
+    if (rc) return rc;
+    const int wide = (d + 15) & ~15;
+    rc = a.x.low != nullptr ? make_map_low<D>(&ml, a.x.low, a.B, a.Tq, a.Hq, wide) : 0;
+    if (rc) return rc;
+    if (a.x.low == nullptr) ml = mo;                             // not read
     const unsigned grid = (unsigned)((a.Tq + BM - 1) / BM) * a.Hq * a.B;
     const size_t smem = sizeof(SmemFwd<D>) + 1024;
     rc = (int)cudaFuncSetAttribute(scored_fwd_kernel<D, F>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (rc) return rc;
-    scored_fwd_kernel<D, F><<<grid, THREADS, smem, st>>>(mq, mk, mv, a, pairs_in_l2(a.B * a.Hq, a.Tk, D, a.Hq / a.Hkv));
+    scored_fwd_kernel<D, F><<<grid, THREADS, smem, st>>>(mq, mk, mv, mo, ml, a, pairs_in_l2(a.B * a.Hq, a.Tk, D, a.Hq / a.Hkv));
     return (int)cudaGetLastError();
 }
 

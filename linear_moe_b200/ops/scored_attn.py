@@ -151,7 +151,7 @@ def _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop
         a.x.cap, a.x.causal, a.x.d = float(softcap or 0.0), int(bool(causal)), D
         a.x.first_b, a.x.stop_b = (0 if r is None else r.stride(0) for r in (first, stop))
     p.args, p.bwd = bytes(fwd), bytes(bwd)
-    p.lse, p.tiles, p.low = B * Hq * Tq * 4, B * -(-Tq // 128) * 16, q.numel() * 2       # bytes
+    p.lse, p.tiles, p.low = B * Hq * Tq * 4, B * -(-Tq // 128) * 16, B * Tq * Hq * _round16(D)      # bytes
     half = q.dtype == torch.float16
     p.fwd_fn = K.lib().lmoe_scored_attn_fwd_fp16 if half else K.lib().lmoe_scored_attn_fwd
     p.bwd_fn = K.lib().lmoe_scored_attn_bwd_fp16 if half else K.lib().lmoe_scored_attn_bwd
@@ -159,7 +159,7 @@ def _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop
 
 
 def _addresses(a, dev, first, stop, slopes, stats: int, low: int, tiles: int):
-    """What a launch reads beside q, k and v: ranges, slopes, and the forward kernel's notes (row statistics, low parts of the output, intervals of the query tiles)."""
+    """What a launch reads beside q, k and v: ranges, slopes, and the forward kernel's notes (row statistics, next bits of the output, intervals of the query tiles)."""
     from . import cuda as K
     x = a.x
     if first is not None:
