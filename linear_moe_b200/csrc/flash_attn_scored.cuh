@@ -134,21 +134,31 @@ template <int N> __device__ __forceinline__ void tanh_of(uint32_t (&v)[N], float
         for (int i = 0; i < N; ++i) v[i] = __float_as_uint(1.f - 2.f * rcp(ex2(__uint_as_float(v[i]) * a2) + 1.f));
     }
 }
-// ... minus the bias of N neighbouring keys (queries), the first of them `dist` away
-template <int N> __device__ __forceinline__ void biased(uint32_t (&v)[N], const ScoreOf& s, float dist) {
+// v -> a v - the bias of N neighbouring keys (queries), the first of them `dist` away.  Where no one is on the other side for any row of the warp (all but a causal sequence's diagonal tiles)
+// the distance needs no absolute value: a product with the column's number and one for two scores, instead of a sum, a product and another one for each.  8192 queries x 16 heads, window of
+// 2048: forward 218 / 212 us, dq 177 / 159 us, dk / dv 267 / 257 us.
+template <int N> __device__ __forceinline__ void biased(uint32_t (&v)[N], float a, float slope, float dist) {
+    const bool before = dist <= 1 - N;
+    if (__all_sync(0xffffffffu, before) || __all_sync(0xffffffffu, dist >= 0.f)) {
+        const float t = before ? slope : -slope, base = t * dist;
+        const float2 a2 = make_float2(a, a);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) - s.sl * fabsf(dist + i));
-}
-template <class F, int N> __device__ __forceinline__ void scored(uint32_t (&v)[N], const ScoreOf& s, const Ranges& x, float dist) {
-    if constexpr (F::SCORE == SCORE_BIAS) {
+        for (int i = 0; i < N; i += 2) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), a2, make_float2(fmaf(t, i, base), fmaf(t, i + 1, base)));
+            v[i] = __float_as_uint(x.x), v[i + 1] = __float_as_uint(x.y);
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * s.a - s.sl * fabsf(dist + i));
-    } else if constexpr (F::SCORE == SCORE_CAP) {
-        tanh_of(v, s.a);
-        if (x.slopes != nullptr) biased(v, s, dist);
+        for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a - slope * fabsf(dist + i));
     }
 }
-
+template <class F, int N> __device__ __forceinline__ void scored(uint32_t (&v)[N], const ScoreOf& s, const Ranges& x, float dist) {
+    if constexpr (F::SCORE == SCORE_BIAS) biased(v, s.a, s.sl, dist);
+    else if constexpr (F::SCORE == SCORE_CAP) {
+        tanh_of(v, s.a);
+        if (x.slopes != nullptr) biased(v, 1.f, s.sl, dist);
+    }
+}
 
 // Bounded waits.  (Without the time hint of mbar_wait_suspend.)
 __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
@@ -735,7 +745,7 @@ __device__ __forceinline__ void derive(uint32_t (&v)[32], float2 (&p)[16], const
             const float2 t = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
             p[i] = __ffma2_rn(make_float2(-t.x, -t.y), t, make_float2(1.f, 1.f));
         }
-        if (x.slopes != nullptr) biased(v, so, dist);
+        if (x.slopes != nullptr) biased(v, 1.f, so.sl, dist);
     } else scored<F>(v, so, x, dist);
 }
 
