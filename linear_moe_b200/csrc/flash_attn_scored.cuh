@@ -57,6 +57,12 @@ constexpr float LAG = 8.f;                // how far, as a power of two, a row's
 constexpr int BLK = BM * 128;             // one 64-column block of a 128-row tile
 constexpr int MAX_TILES = 8192;           // query tiles that a dk / dv CTA can list: 2^20 queries
 
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                    "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
 template <class F> __device__ __forceinline__ uint32_t pack16(float a, float b) {
     if constexpr (F::HALF) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -567,24 +573,31 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     }
                     l += sum.x + sum.y;
                 } else {
-                    uint32_t v[64];
-                    tmem_ld64(s_addr, v);
-                    tmem_ld_wait();
-                    scored<F>(v, so, a.x, (float)(key0 - a.q_offset - w.q0 - r));
-                    if (need_mask) {
-                        const int2 range = sm.seen[slot][r];
-                        const int hi = range.y - 1 - key0, lo = range.x - 1 - key0;
+                    // Plain scores stay in registers; others, which want more of those, go back to tensor memory for as long as the maximum is looked for.
+                    constexpr bool BACK = F::SCORE != SCORE_PLAIN;
+                    constexpr int N = BACK ? 32 : 64;
+                    uint32_t v[N];
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 64; ++i)
-                            if (i > hi || i <= lo) v[i] = 0xff800000u;                                   // -inf
+                    for (int c = 0; c < 64; c += N) {
+                        if constexpr (BACK) tmem_ld32(s_addr + c, v);
+                        else tmem_ld64(s_addr, v);
+                        tmem_ld_wait();
+                        scored<F>(v, so, a.x, (float)(key0 + c - a.q_offset - w.q0 - r));
+                        if (need_mask) {
+                            const int2 range = sm.seen[slot][r];
+                            const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;
+#pragma unroll
+                            for (int i = 0; i < N; ++i)
+                                if (i > hi || i <= lo) v[i] = 0xff800000u;                               // -inf
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int i = 0; i < N; i += 8) mx4[e] = max3(mx4[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
+                        if constexpr (BACK) tmem_st32(s_addr + c, v);
                     }
-                    float mx4[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        mx4[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 4]));
-#pragma unroll
-                        for (int c = 8; c < 64; c += 8) mx4[e] = max3(mx4[e], __uint_as_float(v[c + e]), __uint_as_float(v[c + e + 4]));
-                    }
+                    if constexpr (BACK) tmem_st_wait();
                     float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                     sm.mx[c & 1][grp][part][r] = mx;
                     asm volatile("bar.sync %0, 64;" :: "r"(1 + grp * 4 + qd) : "memory");
@@ -616,10 +629,16 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                     for (int c = 0; c < 64; c += 32) {
                         uint32_t p[16];
+                        constexpr int at = BACK ? 0 : 1;
+                        if constexpr (BACK) {
+                            tmem_ld32(s_addr + c, v);
+                            tmem_ld_wait();
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float2 x01 = __ffma2_rn(make_float2(__uint_as_float(v[c + i]), __uint_as_float(v[c + i + 1])), sc2, nm2);
-                            const float2 x23 = __ffma2_rn(make_float2(__uint_as_float(v[c + i + 2]), __uint_as_float(v[c + i + 3])), sc2, nm2);
+                            const int e = at * c + i;
+                            const float2 x01 = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, nm2);
+                            const float2 x23 = __ffma2_rn(make_float2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), sc2, nm2);
                             const float p0 = exp2f(x01.x), p1 = exp2f(x01.y), p2 = exp2f(x23.x), p3 = exp2f(x23.y);
                             sum0 = __fadd2_rn(sum0, make_float2(p0, p1));
                             sum1 = __fadd2_rn(sum1, make_float2(p2, p3));
