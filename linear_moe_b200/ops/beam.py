@@ -82,8 +82,8 @@ def _copy_rows(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], rows: i
             some = src[first:first + TENSORS]
             n = len(some)
             a.src[:n], a.dst[:n] = [t.data_ptr() for t in some], [t.data_ptr() for t in dst[first:first + TENSORS]]
-            a.rows[:n] = counts = [t.shape[0] for t in some]
-            a.bytes[:n] = [t.nbytes // max(r, 1) for t, r in zip(some, counts)]
+            a.rows[:n] = [t.shape[0] for t in some]
+            a.bytes[:n] = [t.nbytes // t.shape[0] for t in dst[first:first + TENSORS]]
             a.tensors = n
             K._check(K.lib().lmoe_copy_rows(ctypes.byref(a), K._st()), "copy_rows")
 
@@ -113,8 +113,8 @@ def copy_pages_(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if len(src) != len(dst) or len(set(dst)) != len(dst) or set(dst) & set(src):
         raise ValueError("pages are copied to as many other ones, each once")
     for t in pools:
-        if not t.is_contiguous():
-            raise ValueError("a pool of pages is contiguous")
+        if not t.is_contiguous() or t.device != pools[0].device:
+            raise ValueError("pools of pages are contiguous and lie on one device")
         if any(not 0 <= p < t.shape[0] for p in (*src, *dst)):
             raise ValueError(f"a page outside the {t.shape[0]} of its pool")
     pools = [t for t in pools if t.numel()]

@@ -91,7 +91,7 @@ def _plan(q, k, v, table, lengths, scale, window, softcap, slopes, k_new, v_new)
     if k_new is not None:
         a.n_b, a.n_h, a.m_b, a.m_h = k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1)
     a.B, a.H, a.G, a.D, a.page, a.pages, a.table_n, a.table_ld = B, H, G, D, page, P, table.shape[1], table.stride(0)
-    a.window, a.scale, a.cap, a.splits = int(window or 0), float(scale) if scale is not None else D ** -0.5, float(softcap or 0.0), 1
+    a.window, a.scale, a.cap, a.splits = min(int(window or 0), (1 << 31) - 1), float(scale) if scale is not None else D ** -0.5, float(softcap or 0.0), 1
     p.flat = all(t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 for t in (q, k_new, v_new, table, lengths, slopes))
     # 16-byte rows (of q and the new token too: misaligned ones are rare and small, but a copy of the cache is out of the question)
     vec = (q.dtype != torch.float32 and D % 8 == 0 and D <= 128 and page % GROUP == 0 and P > 0 and

@@ -6,8 +6,8 @@
 A query that sees no key gives zeros and passes no gradient.  One interval per query describes packed documents
 (:func:`document_first`), prefixes that see themselves whole and padded batches (:func:`prefix_stop`).
 
-bf16 and fp16 CUDA tensors with heads of up to 128, in multiples of 8, run the tcgen05 kernels of ``csrc/flash_attn_tc.cuh``; others (fp32, CPU,
-wider heads) run the eager definition :func:`linear_moe_b200.ref.ops.softmax_attention`.  Slopes and ranges get no gradient.  Hidden keys and
+bf16 and fp16 CUDA tensors with heads of up to 128, in multiples of 8, run the tcgen05 kernels of ``csrc/flash_attn_scored.cuh``; others (fp32, CPU,
+wider heads, more than 2^20 queries or 1023 query heads) run the eager definition :func:`linear_moe_b200.ref.ops.softmax_attention`.  Slopes and ranges get no gradient.  Hidden keys and
 values have to be finite, as for the eager form: a weight of zero times NaN is NaN.
 """
 from __future__ import annotations
@@ -21,7 +21,7 @@ import torch
 
 from ..ref import ops as R
 
-MAX_QUERIES = 1 << 20          # what the dk / dv kernel's list of query tiles holds
+MAX_QUERIES, MAX_HEADS = 1 << 20, 1023        # what the dk / dv kernel's list of query tiles holds; heads for which a sequence's rows stay below 2^31
 
 
 def on_device(t: torch.Tensor):
@@ -61,7 +61,7 @@ def alibi_slopes(heads: int) -> torch.Tensor:
     return torch.tensor(s[:heads], dtype=torch.float32)
 
 
-def _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, key_stop):
+def _check_options(q, k, v, scale, causal, q_offset, window, softcap, slopes, key_first, key_stop):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention takes q [B, Tq, Hq, D], k and v [B, Tk, Hkv, D]")
     if k.shape[:3] != v.shape[:3] or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
@@ -73,6 +73,8 @@ def _check_options(q, k, v, scale, causal, window, softcap, slopes, key_first, k
     _check_scores(q, q.shape[2], scale, softcap, slopes)
     if window is not None and not (causal and window >= 1):
         raise ValueError("a window is a positive number of keys of causal attention")
+    if not abs(q_offset) < 1 << 30 or max(q.shape[1], k.shape[1]) >= 1 << 30:
+        raise ValueError(f"positions beyond 2^30: {q.shape[1]} queries from {q_offset} on, {k.shape[1]} keys")
     for name, r in (("key_first", key_first), ("key_stop", key_stop)):
         if r is None:
             continue
@@ -135,9 +137,9 @@ _PLANS: Dict[tuple, _Plan] = {}
 
 def _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop) -> _Plan:
     from . import cuda as K
-    _check_options(q, k, v, scale, causal, window, softcap, slopes, first, stop)
+    _check_options(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop)
     p, (B, Tq, Hq, D) = _Plan(), q.shape
-    p.eager = (not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float16) or v.shape[3] != D or D > 128 or D % 8 != 0 or Tq > MAX_QUERIES
+    p.eager = (not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float16) or v.shape[3] != D or D > 128 or D % 8 != 0 or Tq > MAX_QUERIES or Hq > MAX_HEADS
                or min(q.numel(), k.numel()) == 0)
     if p.eager:
         return p
@@ -147,7 +149,7 @@ def _plan(q, k, v, scale, causal, q_offset, window, softcap, slopes, first, stop
     fwd, bwd = _Args(), _BwdArgs()
     for a in (fwd, bwd):
         a.B, a.Tq, a.Hq, a.Tk, a.Hkv = B, Tq, Hq, k.shape[1], k.shape[2]
-        a.q_offset, a.window, a.scale = int(q_offset), int(window or 0), float(scale) if scale is not None else D ** -0.5
+        a.q_offset, a.window, a.scale = int(q_offset), min(int(window or 0), (1 << 31) - 1), float(scale) if scale is not None else D ** -0.5
         a.x.cap, a.x.causal, a.x.d = float(softcap or 0.0), int(bool(causal)), D
         a.x.first_b, a.x.stop_b = (0 if r is None else r.stride(0) for r in (first, stop))
     p.args, p.bwd = bytes(fwd), bytes(bwd)

@@ -169,3 +169,17 @@ def test_copy_pages(device):
         o[[0, 5, 2]] = o[[1, 1, 8]]
         assert torch.equal(p, o)
     ops.copy_pages_(pools, [], [])
+
+
+def test_pools_on_two_devices():
+    with pytest.raises(ValueError):
+        ops.copy_pages_([torch.zeros(4, 2), torch.zeros(4, 2, device="meta")], [0], [1])
+
+
+@gpu
+def test_state_without_rows():
+    """Every parent is one too many."""
+    from linear_moe_b200.ops import gemm
+    assert ops.reorder_states([torch.zeros(0, 3, device="cuda")], torch.tensor([0, 1], device="cuda"))[0].shape == (2, 3)
+    with pytest.raises(RuntimeError, match="0x13000"):
+        gemm.check_error()

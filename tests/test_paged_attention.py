@@ -283,3 +283,13 @@ def test_shared_pages_and_far_offsets():
     got = ops.paged_attention(s["q"][:1].expand(2, 4, 128), k, v, table, s["lengths"])
     assert torch.equal(got[0], got[1])
     assert torch.equal(got[0], check(s)[0])
+
+
+@gpu
+def test_window_beyond_32_bits():
+    """More keys than the cache can have: no window at all."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(*s, generator=gen, device="cuda").bfloat16() for s in ((2, 4, 64), (6, 64, 2, 64), (6, 64, 2, 64)))
+    table, lengths = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device="cuda"), torch.tensor([150, 7], dtype=torch.int32, device="cuda")
+    for x, y, z in ((q, k, v), (q.float(), k.float(), v.float())):
+        assert torch.equal(ops.paged_attention(x, y, z, table, lengths, window=1 << 40), ops.paged_attention(x, y, z, table, lengths))

@@ -347,3 +347,85 @@ def test_large_scores():
     check(pick(got), *(pick(x) for x in formulas(q, k, v, do, 0.125, 5.0, None, seen, dist)), torch.bfloat16, ("o", "dv"))
     for t in run(q, k, v, do, slopes=slope_table(2)):
         assert torch.isfinite(t).all()
+
+
+# ---- calls at the edges of what is allowed -------------------------------------------------------------------------------------------
+def test_positions_that_do_not_fit():
+    q, k, v, _ = inputs(1, 4, 4, 2, 1, 8, torch.float32, "cpu")
+    for off in (1 << 30, -(1 << 30), 1 << 40):
+        with pytest.raises(ValueError):
+            ops.softmax_attention(q, k, v, q_offset=off, softcap=5.0)
+    plain = ops.softmax_attention(q, k, v, softcap=5.0)
+    assert torch.equal(ops.softmax_attention(q, k, v, window=1 << 40, softcap=5.0), plain)
+
+
+@gpu
+def test_window_beyond_32_bits():
+    q, k, v, do = inputs(1, 200, 200, 2, 1, 64, torch.bfloat16)
+    for a, b in zip(run(q, k, v, do, window=1 << 40, softcap=5.0), run(q, k, v, do, softcap=5.0)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_more_heads_than_the_kernels_take():
+    compare(*inputs(1, 3, 3, 1024, 2, 8, torch.bfloat16), cap=20.0)
+
+
+@gpu
+def test_offsets_in_front_of_and_behind_the_keys():
+    """No query sees a key; all see all of them."""
+    q, k, v, do = inputs(2, 130, 140, 4, 2, 64, torch.bfloat16)
+    for t in run(q, k, v, do, off=-200, slopes=slope_table(4)):
+        assert (t == 0).all()
+    compare(q, k, v, do, off=100000, slopes=slope_table(4))
+
+
+@gpu
+def test_gradient_of_a_sum():
+    """The incoming gradient is one number, broadcast."""
+    q, k, v, _ = inputs(1, 140, 140, 4, 2, 72, torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(ops.softmax_attention(*leaves, softcap=20.0).sum(), leaves)
+    want = run(q, k, v, torch.ones_like(q), softcap=20.0)[1:]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    (only,) = torch.autograd.grad(ops.softmax_attention(q.detach(), k, v.detach(), softcap=20.0).sum(), (k,))
+    assert torch.equal(only, want[1])
+
+
+@gpu
+@pytest.mark.parametrize("D,Hkv", [(64, 1), (128, 2)])
+def test_long_sequence(D, Hkv):
+    """66000 queries, most of whose rows see a window in the middle of everything: pieces of the results against the formulas of the piece."""
+    T, W = 66000, 100
+    q, k, v, do = inputs(1, T, T, 2, Hkv, D, torch.bfloat16)
+    sl = slope_table(2)
+    got = run(q, k, v, do, window=W, slopes=sl)
+    for t0 in (0, 32700, T - 512):
+        cut = slice(t0, t0 + 512)
+        seen, dist = visible(512, 512, True, 0, W, None, None, "cuda")
+        parts = formulas(*(t[:, cut] for t in (q, k, v, do)), D ** -0.5, None, sl, seen, dist)
+        lo, hi = (0 if t0 == 0 else W - 1), (512 if t0 + 512 == T else 512 - W + 1)          # keys whose queries all lie in the piece, and behind them queries whose keys do
+        rows = lambda x: [x[0][:, lo:], x[1][:, lo:], x[2][:, lo:hi], x[3][:, lo:hi]]         # noqa: E731
+        check(rows([g[:, cut] for g in got]), *(rows(x) for x in parts), torch.bfloat16)
+
+
+@gpu
+def test_two_graphs_at_once():
+    """Two captured calls, replayed side by side on two streams: each has its own workspace."""
+    jobs = []
+    for seed in (1, 2):
+        held = inputs(2, 400, 400, 8, 2, 128, torch.bfloat16, seed=seed)
+        kw = dict(softcap=30.0, key_first=packed(2, 400, [[70, 150]]))
+        want = run(*held, **kw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(*held, **kw)
+        jobs.append((graph, out, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, _, _, stream in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _ in jobs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
