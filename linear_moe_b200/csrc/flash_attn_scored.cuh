@@ -49,7 +49,8 @@ struct BwdArgs {
 };
 
 // SCORE_CAP with the bias too, where there are slopes.  SCORE_BOUND: capped at 60 at most, no bias, bf16: e^x and its sums stay in fp32's and the weights in bf16's range, and
-// the forward pass needs no maximum.
+// the forward pass needs no maximum (forward, 8192 queries in packed documents, 16 heads of 128: 119 us with one, 105 without).  A large weight is then no longer one, which is exact, but rounded, so
+// the output is divided by the sum of the rounded weights (else it is off by the largest one's rounding, and dq and dk with it: 0.0034 for 0.0025 at scores of 6 in root mean square).
 enum { SCORE_PLAIN, SCORE_BIAS, SCORE_CAP, SCORE_BOUND };
 template <int S, bool H> struct Form { static constexpr bool HALF = H; static constexpr int SCORE = S; };
 constexpr float BOUND = 60.f;
@@ -166,7 +167,8 @@ template <class F, int N> __device__ __forceinline__ void scored(uint32_t (&v)[N
     }
 }
 
-// Bounded waits.  (Without the time hint of mbar_wait_suspend.)
+// Bounded waits.  (Without the time hint of mbar_wait_suspend, and with several tries between two looks at the flag and the clock: these cost the other warps' turns.  Forward kernel of a batch
+// with prefixes 92 -> 85 us.)
 __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(s32(bar)), "r"(parity) : "memory");
@@ -176,7 +178,9 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatil
     if (try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     for (;;) {
-        if (try_wait(bar, parity)) return true;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if (try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
         if (clock64() - t0 > WAIT_CYCLES) break;
     }
@@ -361,6 +365,7 @@ struct __align__(1024) SmemFwd {
     Work work;
     float mx[2][2][2][BM];                                    // [parity of the group's tile][group][half of the columns]
     float ls[2][2][2][BM], ms[2][2][BM];                      // sums and maxima at the end, [parity of the tile of queries][group]
+    float lt[2][2][2][BM];                                    // SCORE_BOUND: sums of the rounded weights
     int2 seen[2][BM];                                         // [slot]: the rows' visible keys
     __align__(1024) uint8_t low[BM * D];
     uint32_t tmem_base;
@@ -537,7 +542,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (!all_softmax(ok)) break;
             const int n_it = sm.work.item[slot].n_it;
             if (n_it < 0) break;
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f, lt = 0.f;
             const ScoreOf so = score_of<F>(a.scale, a.x, sm.work.item[slot].h);
             const float sc = so.unit;
             for (int j = grp, c = grp == 0 ? done[0] : done[1]; j < n_it; j += 2, ++c) {
@@ -548,7 +553,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 tc_fence_after();
                 if constexpr (F::SCORE == SCORE_BOUND) {
                     if (!ok) continue;
-                    float2 sum = make_float2(0.f, 0.f);
+                    float2 sum = make_float2(0.f, 0.f), taken = sum;
 #pragma unroll
                     for (int c = 0; c < 64; c += 32) {
                         uint32_t v[32], p[16];
@@ -568,10 +573,12 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                             const float2 e = make_float2(exp2f(x.x), exp2f(x.y));
                             sum = __fadd2_rn(sum, e);
                             p[i >> 1] = pack16<F>(e.x, e.y);
+                            taken = __fadd2_rn(taken, unpack16<F>(p[i >> 1]));
                         }
                         tmem_st16(s_addr + (c >> 1), p);      // over scores that have been read
                     }
                     l += sum.x + sum.y;
+                    lt += taken.x + taken.y;
                 } else {
                     // The scores are read twice, 32 at a time, and stay in tensor memory while the maximum is looked for: 64 of them and what a bias or a cap needs did not fit into 96
                     // registers (8192 queries with slopes 453 -> 367 us, plain scores 305 -> 300 us).
@@ -670,16 +677,18 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             // join the groups: every warp takes a quarter of the columns of both outputs
             const int par = qi & 1;
             sm.ls[par][grp][part][r] = l;
+            if (F::SCORE == SCORE_BOUND) sm.lt[par][grp][part][r] = lt;
             if (part == 0) sm.ms[par][grp][r] = F::SCORE == SCORE_BOUND ? 0.f : m;
             asm volatile("bar.sync 10, 512;" ::: "memory");       // behind it at most the last product of each group is outstanding
             const float mm = fmaxf(sm.ms[par][0][r], sm.ms[par][1][r]);
             float wg[2];
-            l = 0.f;
+            l = lt = 0.f;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const float mg = sm.ms[par][g][r];
                 wg[g] = mg == -INFINITY ? 0.f : exp2f((mg - mm) * sc);
                 l += wg[g] * (sm.ls[par][g][0][r] + sm.ls[par][g][1][r]);
+                if (F::SCORE == SCORE_BOUND) lt += sm.lt[par][g][0][r] + sm.lt[par][g][1][r];
             }
             float o[OW];
 #pragma unroll
@@ -698,7 +707,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             tc_fence_before();                                // ahead of the next weights, behind which the outputs are written again
             if (ok) {
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float whole = F::SCORE == SCORE_BOUND ? lt : l, inv = whole > 0.f ? 1.f / whole : 0.f;
                 uint32_t y[OW / 2];
 #pragma unroll
                 for (int c = 0; c < OW; c += 2) y[c / 2] = pack16<F>(o[c] * inv, o[c + 1] * inv);

@@ -429,3 +429,21 @@ def test_two_graphs_at_once():
     torch.cuda.synchronize()
     for _, out, want, _ in jobs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@gpu
+@pytest.mark.parametrize("cap,bias", [(None, False), (None, True), (30.0, False), (50.0, False), (80.0, False), (50.0, True)])
+def test_gradients_where_one_weight_is_large(cap, bias):
+    """dq and dk are sums of  p (dp - do . o), a difference of nearly equal terms where one weight is close to 1.  All that should be left are two roundings in a row, of ds and of the
+    result: rounding to u is off by u / sqrt(3) x sqrt(0.54) = 0.42 u in root mean square (numbers spread evenly over a power of two), twice that in squares is 0.59 u; the roundings of
+    the weights in o, which the sum of many makes small, may add half as much in squares: sqrt(0.59^2 + 0.42^2) = 0.72 u.  An o that is off by the largest weight's rounding, or that
+    is used as it was rounded, adds another 0.42 u or more to ds."""
+    u = torch.finfo(torch.bfloat16).eps / 2
+    q, k, v, do = inputs(1, 512, 512, 4, 2, 128, torch.bfloat16, size=4.0)
+    sl = slope_table(4) if bias else None
+    got = run(q, k, v, do, softcap=cap, slopes=sl, key_first=torch.zeros(1, 512, dtype=torch.int32, device="cuda"))
+    seen, dist = visible(512, 512, True, 0, None, None, None, "cuda")
+    res = formulas(q, k, v, do, 128 ** -0.5, cap, sl, seen, dist)[0]
+    for name, g, w in zip(("dq", "dk"), got[1:3], res[1:3]):
+        rel = ((g.double() - w).norm() / w.norm()).item()
+        assert rel < 0.72 * u, (name, rel / u)
