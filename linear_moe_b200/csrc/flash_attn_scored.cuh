@@ -48,13 +48,9 @@ struct BwdArgs {
     Ranges x;
 };
 
-// SCORE_CAP with the bias too, where there are slopes.  SCORE_BOUND: capped at 60 at most, no bias, bf16: e^x and its sums stay in fp32's and the weights in bf16's range, and
-// the forward pass needs no maximum (forward, 8192 queries in packed documents, 16 heads of 128: 119 us with one, 105 without).  A large weight is then no longer one, which is exact, but rounded, so
-// the output is divided by the sum of the rounded weights (else it is off by the largest one's rounding, and dq and dk with it: 0.0034 for 0.0025 at scores of 6 in root mean square).
-enum { SCORE_PLAIN, SCORE_BIAS, SCORE_CAP, SCORE_BOUND };
+// SCORE_CAP with the bias too, where there are slopes.
+enum { SCORE_PLAIN, SCORE_BIAS, SCORE_CAP };
 template <int S, bool H> struct Form { static constexpr bool HALF = H; static constexpr int SCORE = S; };
-constexpr float BOUND = 60.f;
-constexpr float LAG = 8.f;                // how far, as a power of two, a row's weights may run ahead of the maximum they are measured in
 constexpr int BLK = BM * 128;             // one 64-column block of a 128-row tile
 constexpr int MAX_TILES = 8192;           // query tiles that a dk / dv CTA can list: 2^20 queries
 
@@ -113,7 +109,6 @@ template <class F> __device__ __forceinline__ ScoreOf score_of(float scale, cons
     ScoreOf s{1.f, 0.f, scale * LOG2E};
     if constexpr (F::SCORE == SCORE_BIAS) s = {scale * LOG2E, __ldg(x.slopes + h) * LOG2E, 1.f};
     if constexpr (F::SCORE == SCORE_CAP) s = {scale / x.cap, x.slopes != nullptr ? __ldg(x.slopes + h) / x.cap : 0.f, x.cap * LOG2E};
-    if constexpr (F::SCORE == SCORE_BOUND) s = {scale / x.cap, 0.f, x.cap * LOG2E};
     return s;
 }
 // v -> tanh(a v).  The special-function pipe (16 a clock) would be the bound: two operations here and one in the softmax.  So |a v| <= 1.5 takes an odd polynomial of degree 15 on the FMA
@@ -365,7 +360,6 @@ struct __align__(1024) SmemFwd {
     Work work;
     float mx[2][2][2][BM];                                    // [parity of the group's tile][group][half of the columns]
     float ls[2][2][2][BM], ms[2][2][BM];                      // sums and maxima at the end, [parity of the tile of queries][group]
-    float lt[2][2][2][BM];                                    // SCORE_BOUND: sums of the rounded weights
     int2 seen[2][BM];                                         // [slot]: the rows' visible keys
     __align__(1024) uint8_t low[BM * D];
     uint32_t tmem_base;
@@ -542,7 +536,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (!all_softmax(ok)) break;
             const int n_it = sm.work.item[slot].n_it;
             if (n_it < 0) break;
-            float m = -INFINITY, l = 0.f, lt = 0.f;
+            float m = -INFINITY, l = 0.f;
             const ScoreOf so = score_of<F>(a.scale, a.x, sm.work.item[slot].h);
             const float sc = so.unit;
             for (int j = grp, c = grp == 0 ? done[0] : done[1]; j < n_it; j += 2, ++c) {
@@ -551,105 +545,77 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const int tile_key0 = (w.nb_lo + j) * BN, key0 = tile_key0 + part * 64;
                 const bool need_mask = tile_key0 < w.every.x || tile_key0 + BN > w.every.y;
                 tc_fence_after();
-                if constexpr (F::SCORE == SCORE_BOUND) {
-                    if (!ok) continue;
-                    float2 sum = make_float2(0.f, 0.f), taken = sum;
+                // The scores are read twice, 32 at a time, and stay in tensor memory while the maximum is looked for: 64 of them and what a bias or a cap needs did not fit into 96
+                // registers (8192 queries with slopes 453 -> 367 us, plain scores 305 -> 300 us).
+                uint32_t v[32];
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
-                        uint32_t v[32], p[16];
-                        tmem_ld32(s_addr + c, v);
-                        tmem_ld_wait();
-                        tanh_of(v, so.a);
-                        if (need_mask) {
-                            const int2 range = sm.seen[slot][r];
-                            const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;       // visible: lo < i <= hi
+                for (int c = 0; c < 64; c += 32) {
+                    tmem_ld32(s_addr + c, v);
+                    tmem_ld_wait();
+                    scored<F>(v, so, a.x, (float)(key0 + c - a.q_offset - w.q0 - r));
+                    if (need_mask) {
+                        const int2 range = sm.seen[slot][r];
+                        const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i > hi || i <= lo) v[i] = 0xff800000u;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 x = __fmul2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(sc, sc));
-                            const float2 e = make_float2(exp2f(x.x), exp2f(x.y));
-                            sum = __fadd2_rn(sum, e);
-                            p[i >> 1] = pack16<F>(e.x, e.y);
-                            taken = __fadd2_rn(taken, unpack16<F>(p[i >> 1]));
-                        }
-                        tmem_st16(s_addr + (c >> 1), p);      // over scores that have been read
+                        for (int i = 0; i < 32; ++i)
+                            if (i > hi || i <= lo) v[i] = 0xff800000u;                               // -inf
                     }
-                    l += sum.x + sum.y;
-                    lt += taken.x + taken.y;
-                } else {
-                    // The scores are read twice, 32 at a time, and stay in tensor memory while the maximum is looked for: 64 of them and what a bias or a cap needs did not fit into 96
-                    // registers (8192 queries with slopes 453 -> 367 us, plain scores 305 -> 300 us).
-                    uint32_t v[32];
-                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
-                        tmem_ld32(s_addr + c, v);
-                        tmem_ld_wait();
-                        scored<F>(v, so, a.x, (float)(key0 + c - a.q_offset - w.q0 - r));
-                        if (need_mask) {
-                            const int2 range = sm.seen[slot][r];
-                            const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;
+                    for (int e = 0; e < 4; ++e)
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i > hi || i <= lo) v[i] = 0xff800000u;                               // -inf
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8) mx4[e] = max3(mx4[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
-                        if (F::SCORE != SCORE_PLAIN || need_mask) tmem_st32(s_addr + c, v);
-                    }
-                    tmem_st_wait();
-                    float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    sm.mx[c & 1][grp][part][r] = mx;
-                    asm volatile("bar.sync %0, 64;" :: "r"(1 + grp * 4 + qd) : "memory");
-                    if (!ok) continue;
-                    mx = fmaxf(mx, sm.mx[c & 1][grp][part ^ 1][r]);
-                    // both halves of a row see the same numbers and decide alike
-                    const bool grow = (mx - m) * sc > LAG;        // also the first visible key of the row (m = -inf)
-                    const bool scaled = grow && m != -INFINITY;
-                    const float corr = scaled ? exp2f((m - mx) * sc) : 1.f;
-                    if (grow) m = mx;
-                    l *= corr;
-                    if (__any_sync(0xffffffffu, scaled)) {        // not at the group's first tile; these scores were issued behind the last product of the group
-                        ok = wait_warp(&sm.pv_done[grp], (c & 1) ^ 1, abort_flag, err, 0x24020 | grp);
-                        if (!ok) continue;
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D / 2; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o_addr + c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                            tmem_st16(o_addr + c, o);
-                        }
-                    }
-                    const float nm = m == -INFINITY ? 0.f : -m * sc;
-                    const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
-                    float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
-                        uint32_t p[16];
-                        tmem_ld32(s_addr + c, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float2 x01 = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
-                            const float2 x23 = __ffma2_rn(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2, nm2);
-                            const float p0 = exp2f(x01.x), p1 = exp2f(x01.y), p2 = exp2f(x23.x), p3 = exp2f(x23.y);
-                            sum0 = __fadd2_rn(sum0, make_float2(p0, p1));
-                            sum1 = __fadd2_rn(sum1, make_float2(p2, p3));
-                            p[i >> 1] = pack16<F>(p0, p1);
-                            p[(i >> 1) + 1] = pack16<F>(p2, p3);
-                        }
-                        tmem_st16(s_addr + (c >> 1), p);          // over scores that have been read
-                    }
-                    l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+                        for (int i = 0; i < 32; i += 8) mx4[e] = max3(mx4[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
+                    if (F::SCORE != SCORE_PLAIN || need_mask) tmem_st32(s_addr + c, v);
                 }
+                tmem_st_wait();
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                sm.mx[c & 1][grp][part][r] = mx;
+                asm volatile("bar.sync %0, 64;" :: "r"(1 + grp * 4 + qd) : "memory");
+                if (!ok) continue;
+                mx = fmaxf(mx, sm.mx[c & 1][grp][part ^ 1][r]);
+                // Both halves of a row see the same numbers and decide alike.  The maximum is followed exactly, so that the largest weight is one, without a rounding: with weights up to
+                // 2^8 above one, or capped scores (whose exponentials fit without a maximum) as they are, dq and dk of rows with one large weight were off by 0.0027 and 0.0034, not 0.0025.
+                // (Forward, 8192 queries in packed documents, 16 heads of 128: 111 us exactly and up to 2^8 behind, 105 without; a batch with prefixes of 3 x 1531: 83 / 79 us.)
+                const bool grow = mx > m;                     // also the first visible key of the row (m = -inf)
+                const bool scaled = grow && m != -INFINITY;
+                const float corr = scaled ? exp2f((m - mx) * sc) : 1.f;
+                if (grow) m = mx;
+                l *= corr;
+                if (__any_sync(0xffffffffu, scaled)) {        // not at the group's first tile; these scores were issued behind the last product of the group
+                    ok = wait_warp(&sm.pv_done[grp], (c & 1) ^ 1, abort_flag, err, 0x24020 | grp);
+                    if (!ok) continue;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < D / 2; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                        tmem_st16(o_addr + c, o);
+                    }
+                }
+                const float nm = m == -INFINITY ? 0.f : -m * sc;
+                const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+                float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t p[16];
+                    tmem_ld32(s_addr + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float2 x01 = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
+                        const float2 x23 = __ffma2_rn(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2, nm2);
+                        const float p0 = exp2f(x01.x), p1 = exp2f(x01.y), p2 = exp2f(x23.x), p3 = exp2f(x23.y);
+                        sum0 = __fadd2_rn(sum0, make_float2(p0, p1));
+                        sum1 = __fadd2_rn(sum1, make_float2(p2, p3));
+                        p[i >> 1] = pack16<F>(p0, p1);
+                        p[(i >> 1) + 1] = pack16<F>(p2, p3);
+                    }
+                    tmem_st16(s_addr + (c >> 1), p);          // over scores that have been read
+                }
+                l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -677,18 +643,16 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             // join the groups: every warp takes a quarter of the columns of both outputs
             const int par = qi & 1;
             sm.ls[par][grp][part][r] = l;
-            if (F::SCORE == SCORE_BOUND) sm.lt[par][grp][part][r] = lt;
-            if (part == 0) sm.ms[par][grp][r] = F::SCORE == SCORE_BOUND ? 0.f : m;
+            if (part == 0) sm.ms[par][grp][r] = m;
             asm volatile("bar.sync 10, 512;" ::: "memory");       // behind it at most the last product of each group is outstanding
             const float mm = fmaxf(sm.ms[par][0][r], sm.ms[par][1][r]);
             float wg[2];
-            l = lt = 0.f;
+            l = 0.f;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const float mg = sm.ms[par][g][r];
                 wg[g] = mg == -INFINITY ? 0.f : exp2f((mg - mm) * sc);
                 l += wg[g] * (sm.ls[par][g][0][r] + sm.ls[par][g][1][r]);
-                if (F::SCORE == SCORE_BOUND) lt += sm.lt[par][g][0][r] + sm.lt[par][g][1][r];
             }
             float o[OW];
 #pragma unroll
@@ -707,7 +671,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             tc_fence_before();                                // ahead of the next weights, behind which the outputs are written again
             if (ok) {
-                const float whole = F::SCORE == SCORE_BOUND ? lt : l, inv = whole > 0.f ? 1.f / whole : 0.f;
+                const float inv = l > 0.f ? 1.f / l : 0.f;
                 uint32_t y[OW / 2];
 #pragma unroll
                 for (int c = 0; c < OW; c += 2) y[c / 2] = pack16<F>(o[c] * inv, o[c + 1] * inv);
@@ -1408,8 +1372,6 @@ static bool scored_args_ok(const Ranges& x, int B, int Tq, int Tk, int Hq, int H
 template <bool H>
 static int scored_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs, const Args& a, cudaStream_t st) {
     if (!scored_args_ok(a.x, a.B, a.Tq, a.Tk, a.Hq, a.Hkv)) return -1;
-    if constexpr (!H)
-        if (a.x.cap > 0.f && a.x.cap <= BOUND && a.x.slopes == nullptr) return fwd_by_width<Form<SCORE_BOUND, H>>(q, qs, k, ks, v, vs, a, st);
     if (a.x.cap > 0.f) return fwd_by_width<Form<SCORE_CAP, H>>(q, qs, k, ks, v, vs, a, st);
     if (a.x.slopes != nullptr) return fwd_by_width<Form<SCORE_BIAS, H>>(q, qs, k, ks, v, vs, a, st);
     return fwd_by_width<Form<SCORE_PLAIN, H>>(q, qs, k, ks, v, vs, a, st);
