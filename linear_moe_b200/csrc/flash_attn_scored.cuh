@@ -550,22 +550,24 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 uint32_t v[32];
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 64; c += 32) {
-                    tmem_ld32(s_addr + c, v);
+                for (int col = 0; col < 64; col += 32) {
+                    tmem_ld32(s_addr + col, v);
                     tmem_ld_wait();
-                    scored<F>(v, so, a.x, (float)(key0 + c - a.q_offset - w.q0 - r));
+                    scored<F>(v, so, a.x, (float)(key0 + col - a.q_offset - w.q0 - r));
                     if (need_mask) {
                         const int2 range = sm.seen[slot][r];
-                        const int hi = range.y - 1 - key0 - c, lo = range.x - 1 - key0 - c;
+                        const int hi = range.y - 1 - key0 - col, lo = range.x - 1 - key0 - col;
+                        if (__any_sync(0xffffffffu, hi < 31 || lo >= 0)) {                           // most blocks of 32 x 32 in a masked tile are visible
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i > hi || i <= lo) v[i] = 0xff800000u;                               // -inf
+                            for (int i = 0; i < 32; ++i)
+                                if (i > hi || i <= lo) v[i] = 0xff800000u;                           // -inf
+                        }
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) mx4[e] = max3(mx4[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + e + 4]));
-                    if (F::SCORE != SCORE_PLAIN || need_mask) tmem_st32(s_addr + c, v);
+                    if (F::SCORE != SCORE_PLAIN || need_mask) tmem_st32(s_addr + col, v);
                 }
                 tmem_st_wait();
                 float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
@@ -586,22 +588,22 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (!ok) continue;
                     tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < D / 2; c += 16) {
+                    for (int col = 0; col < D / 2; col += 16) {
                         uint32_t o[16];
-                        tmem_ld16(o_addr + c, o);
+                        tmem_ld16(o_addr + col, o);
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                        tmem_st16(o_addr + c, o);
+                        tmem_st16(o_addr + col, o);
                     }
                 }
                 const float nm = m == -INFINITY ? 0.f : -m * sc;
                 const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int c = 0; c < 64; c += 32) {
+                for (int col = 0; col < 64; col += 32) {
                     uint32_t p[16];
-                    tmem_ld32(s_addr + c, v);
+                    tmem_ld32(s_addr + col, v);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
@@ -613,7 +615,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         p[i >> 1] = pack16<F>(p0, p1);
                         p[(i >> 1) + 1] = pack16<F>(p2, p3);
                     }
-                    tmem_st16(s_addr + (c >> 1), p);          // over scores that have been read
+                    tmem_st16(s_addr + (col >> 1), p);          // over scores that have been read
                 }
                 l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
                 tmem_st_wait();
@@ -905,7 +907,7 @@ scored_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 tmem_ld32(lane_addr + s * 128 + part * 32, v);
                 tmem_ld_wait();
                 derive<F>(v, p, so, a.x, (float)(key0 - qi_at));
-                if (need_mask) {
+                if (need_mask && __any_sync(0xffffffffu, key0 < range.x || key0 + 32 > range.y)) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (key0 + i < range.x || key0 + i >= range.y) v[i] = 0xff800000u;       // -inf -> p = 0
@@ -962,7 +964,8 @@ struct __align__(1024) SmemDkv {
     uint8_t k[BM * D * 2], v[BM * D * 2], q[QS][64 * D * 2], g[2][BM * D * 2];        // at the end q: the other CTA's part of the sum, g: dk and dv on their way to memory
     float lse2[2][BM], delta[2][BM];                                         // of the looped queries
     int first[2][BM], stop[2][BM];
-    uint16_t list[MAX_TILES];                                                // query tiles that see a key of this tile; 0x8000: all their rows see all of it
+    int2 every[2][4];                                                        // keys that 32 of them all see
+    uint16_t list[MAX_TILES];                                                // query tiles that see a key of this tile
     uint64_t kv_full, q_full[QS], q_empty[QS], stat_full[2], stat_empty[2], g_full[2], g_empty[2];
     uint64_t s_full[2], dp_full[2], p_ready[2], ds_ready[2], dv_done[2], dk_done[2], all_done;      // [half of the queries]
     uint32_t tmem_base;
@@ -996,7 +999,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const int4 r = t0 + lane < n_qb ? __ldg(a.x.tiles + (long long)b * n_qb + t0 + lane) : make_int4(0, 0, 0, 0);
             const bool sees = r.x < k1 && r.y > k0;
             const uint32_t who = __ballot_sync(0xffffffffu, sees);
-            if (sees) sm.list[n + __popc(who & ((1u << lane) - 1))] = (uint16_t)((t0 + lane) | (r.z <= k0 && r.w >= k1 ? 0x8000 : 0));
+            if (sees) sm.list[n + __popc(who & ((1u << lane) - 1))] = (uint16_t)(t0 + lane);
             n += __popc(who);
         }
         if (lane == 0) sm.listed = n;
@@ -1031,7 +1034,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 0) {
         if (lane == 0) {
             for (int it = 0; it < n_it; ++it) {
-                const int s = it & 1, h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
+                const int s = it & 1, h = h0 + it / ni, q0 = sm.list[it % ni] * BM;
                 auto half_q = [&](int half) -> bool {
                     const int n = 2 * it + half, sq = n % QS;
                     if (!wait_for(&sm.q_empty[sq], ((n / QS) & 1) ^ 1, abort_flag, err, 0x26100 | sq)) return false;
@@ -1099,7 +1102,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     } else if (warp == 2) {                                      // log-sum-exp, delta and range of the looped queries
         for (int it = 0; it < n_it; ++it) {
             const int s = it & 1;
-            const int h = h0 + it / ni, q0 = (sm.list[it % ni] & 0x7fff) * BM;
+            const int h = h0 + it / ni, q0 = sm.list[it % ni] * BM;
             const long long row = ((long long)b * a.Hq + h) * a.Tq;
             float x[4], y[4];
             int2 range[4];
@@ -1116,6 +1119,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int e = 0; e < 4; ++e) {
                 sm.lse2[s][lane + 32 * e] = x[e]; sm.delta[s][lane + 32 * e] = y[e];
                 sm.first[s][lane + 32 * e] = range[e].x; sm.stop[s][lane + 32 * e] = range[e].y;
+                const int lo = __reduce_max_sync(0xffffffffu, range[e].x), hi = __reduce_min_sync(0xffffffffu, range[e].y);
+                if (lane == 0) sm.every[s][e] = make_int2(lo, hi);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.stat_full[s]);
@@ -1128,7 +1133,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ScoreOf so = score_of<F>(a.scale, a.x, h0);
         const float sc = so.unit;
         for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
-            const int s = it & 1, tile = sm.list[at], tile_q0 = (tile & 0x7fff) * BM;
+            const int s = it & 1, tile_q0 = sm.list[at] * BM;
             if (!wait_for(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
             if (!wait_for(&sm.s_full[half], it & 1, abort_flag, err, 0x26500 | half)) { alive = false; break; }
             tc_fence_after();
@@ -1137,7 +1142,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld32(lane_addr + ST + part * 32, v);
             tmem_ld_wait();
             derive<F>(v, p, so, a.x, (float)(a.q_offset + tile_q0 + part * 32 - key));
-            if ((tile & 0x8000) == 0) {
+            const int2 every = sm.every[s][part];
+            if (k0 + qd * 32 < every.x || k0 + qd * 32 + 32 > every.y) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                     const int4 lo = *reinterpret_cast<const int4*>(&sm.first[s][part * 32 + i]), hi = *reinterpret_cast<const int4*>(&sm.stop[s][part * 32 + i]);
