@@ -447,3 +447,11 @@ def test_gradients_where_one_weight_is_large(cap, bias):
     for name, g, w in zip(("dq", "dk"), got[1:3], res[1:3]):
         rel = ((g.double() - w).norm() / w.norm()).item()
         assert rel < 0.72 * u, (name, rel / u)
+
+
+@gpu
+@pytest.mark.parametrize("cap", [2.0, 4.0, 6.0, 8.0, 12.0, 200.0])
+def test_scores_against_the_cap(cap):
+    """Scores of 1.5 in root mean square, up to 7: below three quarters of the cap, up to one and a half times, and beyond, where tanh is evaluated in different ways."""
+    compare(*inputs(1, 260, 260, 4, 2, 64, torch.bfloat16), cap=cap)
+    compare(*inputs(1, 260, 260, 4, 2, 128, torch.float16), cap=cap)
