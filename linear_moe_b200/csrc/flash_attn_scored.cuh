@@ -3,11 +3,19 @@
 //   ds_ij = p_ij (dp_ij - delta_i) (1 - tanh^2),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do
 // The products and their operands are laid out as in flash_attn_tc.cu: tcgen05 with accumulators in tensor memory, weights back into tensor memory as the A operand, sixteen softmax warps.
 // What differs is the work.  A query's visible keys are one interval, whatever it comes from; a query tile's key tiles are the union of its rows' intervals, and only tiles that are not inside
-// all of them are masked.  Packed documents leave a tile of queries few key tiles (five, for documents of 700 tokens), and then what a CTA does around its loop is most of its time: with a CTA
+// all of them are masked.  Packed documents leave a tile of queries few key tiles (five, for documents of 700 tokens), and then what a CTA does around its loop is half of its time: with a CTA
 // per query tile 2200 cycles until its tensor memory and barriers are there, 2400 for Q, 2700 for its output in pieces of 16 bytes, 1600 until the next CTA is there; a key tile takes 2500.
 // So the query-side kernels keep their CTAs: warp 3 asks the hardware for the tile of a CTA that has not started yet (clusterlaunchcontrol), one tile ahead, and works out its interval; loads,
 // products and softmax go on from tile to tile, the rings and their phases counted through.  The dk / dv kernel, whose tiles of a long document have many times the work of others, shares the
-// query heads of a key head between the CTAs of a cluster, which add their parts in distributed shared memory, in a fixed order.
+// query heads of a key head between two CTAs, each of which finishes one of the two sums.
+// Measured, kernel by kernel (one B200): (a) 2 x 4096 queries in packed documents of 700 on average, 16 over 4 heads of 128, capped at 50, (b) 8192 queries, 16 heads of 128, slopes, window
+// of 2048.  Matrix rates in TFLOP/s, with the tensor pipe's active cycles:
+//   forward  (a) 112 us, 270, 18 %  (b) 173 us, 596, 32 %     a tile's chain: scores 800 cycles, softmax 3400 (capped 5000), P V 950; two groups of warps take turns
+//   delta    16 us for 84 MB, 5.2 TB/s
+//   dq       (a) 105 us, 431, 30 %  (b) 159 us, 972, 55 %
+//   dk / dv  (a) 130 us, 464, 33 %  (b) 260 us, 793, 45 %     of 3700 cycles a tile (uncapped) 2500 are products being issued: with 64 queries at a time K and V are read twice as often
+// What is left: the forward chain, which ends only where P no longer lies over S (tensor memory is full with 128-wide heads); two query tiles in flight, one for each group of warps, with
+// everything around the loop hidden, took as long (what one group does, the other one's issue slots pay for) and lost where few tiles of queries share the GPU.
 // Every wait is bounded; the softmax warps, which meet in barriers, agree at every tile's end on whether to go on.
 #pragma once
 #include <cooperative_groups.h>
@@ -724,9 +732,12 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------------
 // Two kernels that recompute the scores, on tiles of 128 queries x 128 keys, as in flash_attn_tc.cu; a thread holds 32 columns of a row.
-//   dq       warp 1 issues S = Q K^T and dP = dO V^T, the softmax warps make dS of them (in 16 bits over S), dQ += dS K.  Persistent, as the forward kernel.
+//   dq       warp 1 issues S = Q K^T and dP = dO V^T, the softmax warps make dS of them (in 16 bits over S), dQ += dS K.  Persistent, as the forward kernel.  Its rows go out through dO's
+//            buffer: direct stores of 16 bytes of 32 rows filled the load / store pipe for 2000 cycles, behind which other warps' waits on barriers queued too.
 //   dk / dv  a CTA has 128 keys of a key head and goes through some of its query heads and, for each, the query tiles that see one of its keys:
-//            S^T = K Q^T, dP^T = V dO^T, P^T and dS^T over them, dV += P^T dO, dK += dS^T Q.
+//            S^T = K Q^T, dP^T = V dO^T, P^T and dS^T over them, dV += P^T dO, dK += dS^T Q.  In two halves of 64 queries, eight softmax warps each, half a turn apart: while one makes its
+//            weights the other makes its gradients, and their products and the next scores run meanwhile.  (Against all warps in step:
+//            documents of 4096, capped, 393 -> 336 us, a batch with prefixes 127 -> 116 us; uncapped 128-wide heads 254 -> 263 us by themselves, 642 -> 630 us with all kernels in a graph.)
 
 // The weights' exponents and (SCORE_CAP) the derivative of the cap, from 32 scores; dist: distance of the first column
 template <class F>

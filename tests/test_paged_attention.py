@@ -293,3 +293,18 @@ def test_window_beyond_32_bits():
     table, lengths = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device="cuda"), torch.tensor([150, 7], dtype=torch.int32, device="cuda")
     for x, y, z in ((q, k, v), (q.float(), k.float(), v.float())):
         assert torch.equal(ops.paged_attention(x, y, z, table, lengths, window=1 << 40), ops.paged_attention(x, y, z, table, lengths))
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(8, 2), (16, 4), (32, 2)])
+def test_only_the_result_is_rounded(heads):
+    """bf16, few keys of similar weights: the weights' roundings would be as large as the result's, u / sqrt(3) x sqrt(0.54) = 0.42 u in root mean square (numbers spread evenly over a
+    power of two), 0.6 u together.  Their remainders go into the products too, so the result's own are left."""
+    (H, G), D, n = heads, 128, 300
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(*s, generator=gen, device="cuda").bfloat16() for s in ((4, H, D), (20, 64, G, D), (20, 64, G, D)))
+    table, lengths = torch.arange(20, dtype=torch.int32, device="cuda").view(4, 5), torch.full((4,), n, dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, k, v, table, lengths).double()
+    kk, vv = (t.view(4, 320, G, D)[:, :n].double().repeat_interleave(H // G, 2) for t in (k, v))
+    want = torch.einsum("bhj,bjhd->bhd", torch.softmax(torch.einsum("bhd,bjhd->bhj", q.double(), kk) * D ** -0.5, -1), vv)
+    assert ((got - want).norm() / want.norm()).item() < 0.5 * torch.finfo(torch.bfloat16).eps / 2
