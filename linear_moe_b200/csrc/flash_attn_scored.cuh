@@ -99,13 +99,14 @@ template <class F, bool B_MN, int N> __host__ __device__ constexpr uint32_t ides
     return F::HALF ? idesc_bf16<B_MN, N>() & ~((1u << 7) | (1u << 10)) : idesc_bf16<B_MN, N>();
 }
 
-// Visible keys [lo, hi) of query `row`, clipped to the keys that there are; a query that sees nothing has lo >= hi.
+// Visible keys [lo, hi) of query `row`, clipped to the keys that there are; a query that sees nothing has lo >= hi.  Neither is negative.
 template <class A> __device__ __forceinline__ int2 visible_range(const A& a, int b, int row) {
     int lo = a.x.first != nullptr ? max(__ldg(a.x.first + b * a.x.first_b + row), 0) : 0;
     int hi = a.x.stop != nullptr ? min(__ldg(a.x.stop + b * a.x.stop_b + row), a.Tk) : a.Tk;
-    if (a.x.causal) hi = min(hi, a.q_offset + row + 1);
-    if (a.window > 0) lo = max(lo, a.q_offset + row - a.window + 1);
-    return make_int2(lo, hi);
+    const int at = a.q_offset + row;
+    if (a.x.causal) hi = min(hi, at + 1);
+    if (a.window > 0 && at >= 0) lo = max(lo, at - a.window + 1);
+    return make_int2(lo, max(hi, 0));
 }
 
 // Scores as the kernels hold them, and what they are multiplied by to be exponents of 2 (`unit`):

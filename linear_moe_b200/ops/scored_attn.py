@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 from typing import Dict, Optional, Sequence
 
 import torch
@@ -83,9 +82,9 @@ def _check_options(q, k, v, scale, causal, q_offset, window, softcap, slopes, ke
 
 
 def _check_scores(q, heads, scale, softcap, slopes):
-    if scale is not None and not (math.isfinite(scale) and scale > 0):
+    if scale is not None and not 1e-30 < scale < 1e30:           # what fp32 holds, and its quotient with a cap
         raise ValueError(f"scale {scale}")
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+    if softcap is not None and not 1e-7 < softcap < 1e7:
         raise ValueError(f"soft cap {softcap}")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or slopes.device != q.device or slopes.requires_grad):
         raise ValueError(f"slopes are {heads} fp32 numbers on {q.device} without a gradient, one per query head")

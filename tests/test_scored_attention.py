@@ -420,14 +420,14 @@ def test_two_graphs_at_once():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = run(*held, **kw)
-        jobs.append((graph, out, want, torch.cuda.Stream()))
+        jobs.append((graph, out, want, torch.cuda.Stream(), held, kw))              # (a graph reads the inputs that it was captured with)
     torch.cuda.synchronize()
     for _ in range(5):
-        for graph, _, _, stream in jobs:
+        for graph, _, _, stream, _, _ in jobs:
             with torch.cuda.stream(stream):
                 graph.replay()
     torch.cuda.synchronize()
-    for _, out, want, _ in jobs:
+    for _, out, want, _, _, _ in jobs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
@@ -455,3 +455,22 @@ def test_scores_against_the_cap(cap):
     """Scores of 1.5 in root mean square, up to 7: below three quarters of the cap, up to one and a half times, and beyond, where tanh is evaluated in different ways."""
     compare(*inputs(1, 260, 260, 4, 2, 64, torch.bfloat16), cap=cap)
     compare(*inputs(1, 260, 260, 4, 2, 128, torch.float16), cap=cap)
+
+
+def test_caps_and_scales_that_32_bits_do_not_hold():
+    q, k, v, _ = inputs(1, 4, 4, 2, 1, 8, torch.float32, "cpu")
+    for kw in (dict(softcap=1e-40), dict(softcap=1e39), dict(softcap=5.0, scale=1e-40), dict(softcap=5.0, scale=1e39)):
+        with pytest.raises(ValueError):
+            ops.softmax_attention(q, k, v, **kw)
+
+
+@gpu
+def test_ranges_at_the_ends_of_their_type():
+    """Beside rows that see something, rows whose ranges end or begin at the smallest and the largest number."""
+    q, k, v, do = inputs(1, 200, 300, 2, 1, 64, torch.bfloat16)
+    big, small = 2 ** 31 - 1, -2 ** 31
+    first = torch.tensor([[0, big, small, small, 100][i % 5] for i in range(200)], dtype=torch.int32, device="cuda")[None]
+    stop = torch.tensor([[300, big, small, big, small][i % 5] for i in range(200)], dtype=torch.int32, device="cuda")[None]
+    for causal in (False, True):
+        compare(q, k, v, do, causal=causal, off=60, first=first, stop=stop)
+    compare(q, k, v, do, off=-100, window=2 ** 31 - 1, first=first)
