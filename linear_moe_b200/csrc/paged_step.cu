@@ -11,6 +11,7 @@
 // keys) to that of its own rounding, 0.0017, and at most 0.3 us (1 x 300 keys 5.4 / 5.7 us, 64 x 8192 191 / 191 us).
 // Rows of a group that are hidden (behind the last key, in front of the window) are masked, and their values set to zero in the ring, so that nothing stale meets a weight of zero;
 // a page number outside the pool is outside the tensor map and reads as zeros.
+// A NaN score raises no maximum, so what has seen nothing is told by its sum of zero, not by its maximum: a head that sees NaN gives NaN.
 //
 // The keys of a request are shared by up to 8 CTAs of a cluster, which join their maxima, sums and outputs in distributed shared memory; long contexts with few heads take
 // more CTAs, which leave their parts in fp32 for a second launch.  (First form, cp.async into the rings by all lanes, byte permutes instead of transposing loads and always two launches:
@@ -34,6 +35,7 @@ template <bool HALF> __device__ __forceinline__ uint32_t pack2(float x, float y)
     if constexpr (HALF) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
     else { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
 }
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
 // What rounding two numbers to bf16 took away, rounded itself
 __device__ __forceinline__ uint32_t rest(float x, float y, uint32_t rounded) {
     return pack2<false>(x - __uint_as_float(rounded << 16), y - __uint_as_float(rounded & 0xffff0000u));
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
 #pragma unroll
         for (int y = 1; y < WARPS; ++y) top = fmaxf(top, part_m[y][threadIdx.x]);
 #pragma unroll
-        for (int y = 0; y < WARPS; ++y) sum += part_m[y][threadIdx.x] == -INFINITY ? 0.f : part_l[y][threadIdx.x] * ex2(part_m[y][threadIdx.x] - top);
+        for (int y = 0; y < WARPS; ++y) sum += part_l[y][threadIdx.x] == 0.f ? 0.f : part_l[y][threadIdx.x] * ex2(part_m[y][threadIdx.x] - top);
         cta_m[threadIdx.x] = top;
         cta_l[threadIdx.x] = sum;
     }
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
         if (cluster) store4(O + r * LD + d, y);
         else if (d >= a.D) continue;
         else if (a.splits == 1) {
-            const float inv = cta_l[r] > 0.f ? 1.f / cta_l[r] : 0.f;
+            const float inv = inverse(cta_l[r]);
             *reinterpret_cast<uint2*>(a.out + bh * a.D + d) = make_uint2(pack2<HALF>(y.x * inv, y.y * inv), pack2<HALF>(y.z * inv, y.w * inv));
         } else {
             store4(a.part + (bh * a.splits + split) * a.D + d, y);
@@ -317,13 +319,14 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < MAX_CLUSTER; ++c) {
-            if (ms[c] == -INFINITY) continue;
+            const float part = c < a.splits ? *cl.map_shared_rank(&cta_l[r], c) : 0.f;
+            if (part == 0.f) continue;
             const float f = ex2(ms[c] - top);
             const float4 z = load4(cl.map_shared_rank(O + r * LD + d, c));
-            sum += f * *cl.map_shared_rank(&cta_l[r], c);
+            sum += f * part;
             y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = inverse(sum);
         *reinterpret_cast<uint2*>(a.out + ((long long)b * a.H + h0 + r) * a.D + d) = make_uint2(pack2<HALF>(y.x * inv, y.y * inv), pack2<HALF>(y.z * inv, y.w * inv));
     }
     cl.sync();                                                         // the other CTAs have read this one's part
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(Args a) {
         sum += L[x];
         o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = inverse(sum);
     if (mine) *reinterpret_cast<uint2*>(a.out + (long long)bh * a.D + lane * 4) = make_uint2(pack2<HALF>(o.x * inv, o.y * inv), pack2<HALF>(o.z * inv, o.w * inv));
 }
 

@@ -62,9 +62,8 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) paged_step_any_kernel(const Ar
         s = warp_sum(s);
         if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
         s -= slope * (float)(sh.len - 1 - key);
-        const float top = fmaxf(m, s);
-        if (top == -INFINITY) continue;
-        const float f = expf(m - top), p = expf(s - top);
+        // (a NaN score raises no maximum and has a weight of NaN, which stays in the sum and the output)
+        const float top = fmaxf(m, s), f = m == top ? 1.f : expf(m - top), p = expf(s - (top == -INFINITY ? 0.f : top));
         m = top;
         l = l * f + p;
 #pragma unroll
@@ -79,14 +78,14 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) paged_step_any_kernel(const Ar
     for (int i = 1; i < ANY_WARPS; ++i) top = fmaxf(top, M[i]);
 #pragma unroll
     for (int i = 0; i < ANY_WARPS; ++i) {
-        f[i] = M[i] == -INFINITY ? 0.f : expf(M[i] - top);
+        f[i] = M[i] == -INFINITY ? 0.f : expf(M[i] - top);      // times NaN: NaN
         sum += f[i] * L[i];
     }
     for (int d = threadIdx.x; d < a.D; d += ANY_WARPS * 32) {
         float y = 0.f;
 #pragma unroll
         for (int i = 0; i < ANY_WARPS; ++i) y += f[i] * O[i][d];
-        put((T*)a.out + ((long long)b * a.H + h) * a.D + d, sum > 0.f ? y / sum : 0.f);
+        put((T*)a.out + ((long long)b * a.H + h) * a.D + d, sum == 0.f ? 0.f : y / sum);             // zero: nothing seen
     }
 }
 
