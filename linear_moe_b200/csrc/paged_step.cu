@@ -310,20 +310,20 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
     for (int i = split * WARPS * 32 + threadIdx.x; i < nh * (DP / 4); i += a.splits * WARPS * 32) {
         const int r = i / (DP / 4), d = i % (DP / 4) * 4;
         if (d >= a.D) continue;
-        float ms[MAX_CLUSTER], top = -INFINITY, sum = 0.f;
+        float ms[MAX_CLUSTER], ls[MAX_CLUSTER], top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int c = 0; c < MAX_CLUSTER; ++c) {
             ms[c] = c < a.splits ? *cl.map_shared_rank(&cta_m[r], c) : -INFINITY;
+            ls[c] = c < a.splits ? *cl.map_shared_rank(&cta_l[r], c) : 0.f;
             top = fmaxf(top, ms[c]);
         }
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < MAX_CLUSTER; ++c) {
-            const float part = c < a.splits ? *cl.map_shared_rank(&cta_l[r], c) : 0.f;
-            if (part == 0.f) continue;
+            if (ls[c] == 0.f) continue;
             const float f = ex2(ms[c] - top);
             const float4 z = load4(cl.map_shared_rank(O + r * LD + d, c));
-            sum += f * part;
+            sum += f * ls[c];
             y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
         }
         const float inv = inverse(sum);
