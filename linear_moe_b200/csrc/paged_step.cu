@@ -23,6 +23,7 @@
 #include "flash_tc_utils.cuh"
 #include "mma_utils.cuh"
 #include "paged_step.cuh"
+#include "tanh_cap.cuh"
 
 namespace lmoe {
 namespace paged {
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
 #pragma unroll
             for (int x = 0; x < 2; ++x) qa[i][kk][x] = there && kk * 16 + 8 * x < a.D ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8 * x) : 0u;
     }
-    const float pre = a.cap > 0.f ? a.scale / a.cap * 2.f * LOG2E : a.scale * LOG2E, cap = a.cap * LOG2E;
+    const float pre = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap = a.cap * LOG2E, unit = a.cap > 0.f ? cap : pre;
     float m[HR], l[HR], o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < HR; ++i) m[i] = -INFINITY, l[i] = 0.f;
@@ -187,23 +188,28 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
                 mma<HALF>(s[n], qa[0][2 * c + 1][0], HR == 2 ? qa[HR - 1][2 * c + 1][0] : 0u, qa[0][2 * c + 1][1], HR == 2 ? qa[HR - 1][2 * c + 1][1] : 0u, kb[2], kb[3]);
             }
         }
+        auto seen = [&](int e) -> bool {
+            const int key = key0 + 8 * (e >> 1) + 2 * t + (e & 1);
+            return !hidden && key >= sh.lo && key < sh.len;
+        };
         float x[HR][4];
         bool ahead = false;
 #pragma unroll
         for (int i = 0; i < HR; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(s[e >> 1][2 * i + (e & 1)]);
+            if (a.cap > 0.f) fatc::tanh_each(v, pre);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float y = s[e >> 1][2 * i + (e & 1)] * pre;
-                if (a.cap > 0.f) y = cap * (1.f - 2.f * rcp(ex2(y) + 1.f));
+                float y = __uint_as_float(v[e]) * unit;
                 if (a.slopes != nullptr) y -= slope[i] * (float)(sh.len - 1 - (key0 + 8 * (e >> 1) + 2 * t + (e & 1)));
                 x[i][e] = y;
             }
             if (edge) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + 8 * (e >> 1) + 2 * t + (e & 1);
-                    if (hidden || key < sh.lo || key >= sh.len) x[i][e] = -INFINITY;
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (!seen(e)) x[i][e] = -INFINITY;
             }
             ahead |= fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])) > m[i] + LAG;
         }
