@@ -1102,7 +1102,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (x[e] == -INFINITY) x[e] = INFINITY;          // a row that sees nothing: its weights are zero
                 range[e] = q < a.Tq ? visible_range(a, b, q) : make_int2(0, 0);
             }
-            if (!wait_for(&sm.stat_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
+            if (!wait_warp(&sm.stat_empty[s], ((it >> 1) & 1) ^ 1, abort_flag, err, 0x26110 | s)) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 sm.lse2[s][lane + 32 * e] = x[e]; sm.delta[s][lane + 32 * e] = y[e];
@@ -1122,8 +1122,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float sc = so.unit;
         for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
             const int s = it & 1, tile_q0 = sm.list[at] * BM;
-            if (!wait_for(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
-            if (!wait_for(&sm.s_full[half], it & 1, abort_flag, err, 0x26500 | half)) { alive = false; break; }
+            if (!wait_warp(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
+            if (!wait_warp(&sm.s_full[half], it & 1, abort_flag, err, 0x26500 | half)) { alive = false; break; }
             tc_fence_after();
             uint32_t v[32], pk[16];
             float2 p[16];
@@ -1153,7 +1153,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 p[i + 1] = F::SCORE == SCORE_CAP ? __fmul2_rn(p[i + 1], ey) : ey;
             }
             hand_over(lane_addr + ST + part * 32, pk, &sm.p_ready[half]);
-            if (!wait_for(&sm.dp_full[half], it & 1, abort_flag, err, 0x26520 | half)) { alive = false; break; }
+            if (!wait_warp(&sm.dp_full[half], it & 1, abort_flag, err, 0x26520 | half)) { alive = false; break; }
             tc_fence_after();
             tmem_ld32(lane_addr + DP + part * 32, v);
             tmem_ld_wait();
@@ -1171,7 +1171,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (F::SCORE != SCORE_PLAIN && it + 1 < n_it) so = score_of<F>(a.scale, a.x, ++h);
             }
         }
-        if (alive) alive = wait_for(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
+        if (alive) alive = wait_warp(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
         tc_fence_after();
     }
     // Two CTAs that share a tile of keys: the first one finishes dv, the second one dk.  Each warp leaves its part of the other sum in the other CTA's shared memory, where its counterpart

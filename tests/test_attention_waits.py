@@ -1,0 +1,24 @@
+"""Waits and shared memory of the attention kernels, as their sources have them: what happens once a bounded wait has run out cannot be tried on a GPU that others share."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(__file__), "..", "linear_moe_b200", "csrc")
+
+
+def kernel(file, name):
+    """The text of a kernel, from its parameters to the next function of the file."""
+    text = open(os.path.join(CSRC, file)).read()
+    text = text[re.search(r"\b%s\(" % name, text).end():]
+    return text[:re.search(r"^}", text, re.M).start()]
+
+
+@pytest.mark.parametrize("name", ["scored_fwd_kernel", "scored_dq_kernel", "scored_dkv_kernel"])
+def test_a_warp_leaves_a_wait_as_a_whole(name):
+    """Behind a wait come instructions of the whole warp (tcgen05.ld, reductions): only warp 0, one lane of which issues the loads, decides lane by lane."""
+    text = kernel("flash_attn_scored.cuh", name)
+    loads = re.search(r"if \(warp == 0\) \{\n\s+if \(lane == 0\) \{.*?\} else if \(warp == 1", text, re.S)
+    assert loads and "wait_for(" in loads.group()
+    assert not re.search(r"\bwait_for\(", text[:loads.start()] + text[loads.end():])
+    assert re.search(r"\bwait_warp\(", text[loads.end():])
