@@ -1017,7 +1017,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tc_fence_after();
     const uint32_t tmem_base = uniform(sm.tmem_base);
     const int ni = uniform(sm.listed), n_it = ni * heads;
-    bool alive = n_it > 0;
+    bool alive = true;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -1120,7 +1120,7 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t lane_addr = tmem_base + ((uint32_t)(qd * 32) << 16);
         ScoreOf so = score_of<F>(a.scale, a.x, h0);
         const float sc = so.unit;
-        for (int it = 0, at = 0, h = h0; alive && it < n_it; ++it) {
+        for (int it = 0, at = 0, h = h0; it < n_it; ++it) {
             const int s = it & 1, tile_q0 = sm.list[at] * BM;
             if (!wait_warp(&sm.stat_full[s], (it >> 1) & 1, abort_flag, err, 0x26510 | s)) { alive = false; break; }
             if (!wait_warp(&sm.s_full[half], it & 1, abort_flag, err, 0x26500 | half)) { alive = false; break; }
@@ -1171,13 +1171,14 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (F::SCORE != SCORE_PLAIN && it + 1 < n_it) so = score_of<F>(a.scale, a.x, ++h);
             }
         }
-        if (alive) alive = wait_warp(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
+        if (alive && n_it > 0) alive = wait_warp(&sm.all_done, 0, abort_flag, err, 0x26700);        // covers dV, which was issued before dK
         tc_fence_after();
     }
     // Two CTAs that share a tile of keys: the first one finishes dv, the second one dk.  Each warp leaves its part of the other sum in the other CTA's shared memory, where its counterpart
     // there, which holds the same rows and columns, adds it to its own.
     cg::cluster_group cl = cg::this_cluster();
     constexpr int OW = D / SPLIT;
+    constexpr uint32_t NAN16 = 0x7fff7fffu;                                                     // in both types: a wait ran out (keys that no query sees get zeros)
     const uint32_t sums_at = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + ((warp - 4) >> 2) * OW;
     float4* given = reinterpret_cast<float4*>(sm.q[0]) + (threadIdx.x - 128);                   // [unit of 4 columns][thread]
     if (share > 1) {
@@ -1189,7 +1190,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < OW; c += 4)
-                theirs[c / 4 * 512] = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+                theirs[c / 4 * 512] = alive ? make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]))
+                                            : make_float4(NAN, NAN, NAN, NAN);
         }
         cl.sync();
     }
@@ -1210,8 +1212,8 @@ scored_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     const float4 o = given[c / 4 * 512];
                     z.x += o.x; z.y += o.y; z.z += o.z; z.w += o.w;
                 }
-                y[c / 2] = alive ? pack16<F>(f * z.x, f * z.y) : 0u;                            // no query sees these keys: zeros
-                y[c / 2 + 1] = alive ? pack16<F>(f * z.z, f * z.w) : 0u;
+                y[c / 2] = n_it == 0 ? 0u : alive ? pack16<F>(f * z.x, f * z.y) : NAN16;
+                y[c / 2 + 1] = n_it == 0 ? 0u : alive ? pack16<F>(f * z.z, f * z.w) : NAN16;
             }
             rows_out<OW>(sm.g[0] + (warp - 4) * 32 * OW * 2, y, (x == 0 ? a.dv : a.dk) + at, (long long)a.Hkv * d, min(32, a.Tk - row0), d - col0);
         }

@@ -22,3 +22,13 @@ def test_a_warp_leaves_a_wait_as_a_whole(name):
     assert loads and "wait_for(" in loads.group()
     assert not re.search(r"\bwait_for\(", text[:loads.start()] + text[loads.end():])
     assert re.search(r"\bwait_warp\(", text[loads.end():])
+
+
+def test_gradients_behind_a_wait_that_ran_out_are_nan():
+    """Zeros are what keys get that nobody sees; where a CTA or its partner gave up, dk and dv must not look like that."""
+    text = kernel("flash_attn_scored.cuh", "scored_dkv_kernel")
+    out = text[text.index("given = reinterpret_cast"):]
+    assert not re.search(r"alive \? pack16<F>\([^?]*\) : 0u", out)
+    assert re.search(r"n_it == 0 \? 0u", out) and re.search(r"alive \? pack16<F>.* : NAN16", out)
+    sent = out[:out.index("rows_out")]
+    assert re.search(r"theirs\[c / 4 \* 512\] = alive \?", sent)          # the partner's half of a sum
