@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[WARPS][STAGES];
     __shared__ float part_m[WARPS][16], part_l[WARPS][16], cta_m[16], cta_l[16];
-    __shared__ int abort_flag, drain_flag, chosen;
+    __shared__ int abort_flag, drain_flag, chosen, lens[WARPS * 32];     // lens: beside the rings, whose bulk copies no fence keeps behind ordinary accesses
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int qpg = a.H / a.G, tiles = (qpg + 8 * HR - 1) / (8 * HR);
     int b = blockIdx.z;
@@ -74,7 +74,6 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_step_kernel(const __grid_
     pdl_wait();
     pdl_trigger();
     if (a.sorted) {                                                    // this CTA's request: the one with blockIdx.z longer ones (up to 128 requests)
-        int* lens = reinterpret_cast<int*>(smem);
         const int mine = threadIdx.x < a.B ? a.lengths[threadIdx.x] : 0;
         lens[threadIdx.x] = mine;
         __syncthreads();

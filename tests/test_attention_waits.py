@@ -32,3 +32,10 @@ def test_gradients_behind_a_wait_that_ran_out_are_nan():
     assert re.search(r"n_it == 0 \? 0u", out) and re.search(r"alive \? pack16<F>.* : NAN16", out)
     sent = out[:out.index("rows_out")]
     assert re.search(r"theirs\[c / 4 \* 512\] = alive \?", sent)          # the partner's half of a sum
+
+
+def test_lengths_lie_beside_the_rings():
+    """The one-token kernel's list of lengths is written and read by ordinary accesses: not where bulk copies go next without a fence between the two."""
+    text = kernel("paged_step.cu", "paged_step_kernel")
+    assert re.search(r"__shared__ int [^;]*\blens\[WARPS \* 32\]", text)
+    assert not re.search(r"int\* lens", text)
