@@ -1,6 +1,8 @@
 // One step of a beam search.
 //
 // Selection: the best n of  s_b + x_bt - lse_b  over the beams b and the vocabulary t of every prompt, ties to the lowest b V + t.  Bound by reading the logits once.
+// What is compared: inside a beam the logits; between beams 64-bit scores whose log-sums carry the error of sums of 32-bit exponentials (some 1e-7; equal rows have equal ones), so
+// candidates of different beams closer than that can come in either order.
 //   beam_parts_kernel   a CTA goes through a part of one beam's logits, 4096 at a time in registers, with the next ones on their way: their maximum and sum of exponentials, and their n
 //                       best.  The threads' maxima of the first chunk give a bound that n logits reach and few others do; those go to shared memory, their n-th best
 //                       is the bound of the chunks behind, and in the end each candidate finds its rank by counting.  Where too many reach the bound a closer one is searched, and where
@@ -197,41 +199,63 @@ struct PartPut {
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4) beam_parts_kernel(Args a) {
-    constexpr int VN = 16 / sizeof(T), VECS = PER / VN;
+    constexpr int VN = 16 / sizeof(T), VECS = PER / VN, W = sizeof(T) == 4 ? 4 : 5;       // numbers and 32-bit words of a vector, the latter with one more where numbers straddle words
     __shared__ Pool<float, THREADS> sm;
     __shared__ float red[THREADS / 32];
     __shared__ double sums[THREADS / 32];
     __shared__ float closer_bound;
     const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x, w = t >> 5, lane = t & 31;
     const T* x = (const T*)a.logits + row / a.K * a.s_n + row % a.K * a.s_k;
-    // vectors lie on 16-byte boundaries: the part begins up to VN - 1 numbers early, and those belong to nobody
-    const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int base = part * a.length - skew;                 // token of the part's first number
-    const int lo = max(base, 0), hi = min(base + a.length, a.V), total = max(hi - lo, 0), chunks = (a.length + CHUNK - 1) / CHUNK;
+    // Which thread sums up which tokens does not depend on where the row begins: equal rows have equal sums, to the bit, and their candidates tie.
+    const bool whole = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const int odd = sizeof(T) == 2 ? (int)(reinterpret_cast<uintptr_t>(x) >> 1 & 1) : 0;      // the row begins in the middle of a word
+    const int lo = part * a.length, hi = min(lo + a.length, a.V), total = max(hi - lo, 0), chunks = (a.length + CHUNK - 1) / CHUNK;
     const long long slot = (long long)row * a.parts + part;
     const PartPut put{a.key + slot * a.n, a.at + slot * a.n};
-    auto load = [&](int c, uint4 (&raw)[VECS]) {
+    auto load = [&](int c, uint32_t (&raw)[VECS][W]) {
 #pragma unroll
         for (int i = 0; i < VECS; ++i) {
-            const int at = base + c * CHUNK + (i * THREADS + t) * VN;
-            if (at >= lo && at + VN <= hi) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + at));
-            else {
-                T* p = reinterpret_cast<T*>(&raw[i]);
+            const int at = lo + c * CHUNK + (i * THREADS + t) * VN;
+            raw[i][W - 1] = 0;
+            if (whole && at + VN <= hi) {
+                const uint4 y = __ldcs(reinterpret_cast<const uint4*>(x + at));
+                raw[i][0] = y.x; raw[i][1] = y.y; raw[i][2] = y.z; raw[i][3] = y.w;
+            } else if (!whole && at >= odd && at + VN <= hi && at + VN + odd <= a.V) {           // the words that hold them, none of them outside the row
+                const uint32_t* y = reinterpret_cast<const uint32_t*>(x + at - odd);
 #pragma unroll
-                for (int e = 0; e < VN; ++e) p[e] = at + e >= lo && at + e < hi ? x[at + e] : nothing<T>();
+                for (int k = 0; k < 4; ++k) raw[i][k] = y[k];
+                if (odd) raw[i][W - 1] = y[W - 1];
+            } else {
+                T y[VN];
+#pragma unroll
+                for (int e = 0; e < VN; ++e) y[e] = at + e < hi ? x[at + e] : nothing<T>();
+                uint32_t last = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t word;
+                    memcpy(&word, y + k * (VN / 4), 4);
+                    raw[i][k] = odd ? __funnelshift_r(last, word, 16) : word;
+                    last = word;
+                }
+                if (odd) raw[i][W - 1] = last >> 16;
             }
         }
     };
-    uint4 raw[VECS];
+    uint32_t raw[VECS][W];
     load(0, raw);
     float top = -INFINITY, s = 0.f, bound = -INFINITY;       // the thread's largest logit so far, its sum in units of that
     for (int c = 0; c < chunks; ++c) {
         float v[PER];
 #pragma unroll
         for (int i = 0; i < VECS; ++i) {
-            const T* p = reinterpret_cast<const T*>(&raw[i]);
+            T y[VN];
 #pragma unroll
-            for (int e = 0; e < VN; ++e) v[i * VN + e] = fmaxf(number<T>(p[e]), -INFINITY);      // NaN -> -inf
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t word = W == 5 ? __funnelshift_r(raw[i][k], raw[i][W == 5 ? k + 1 : k], odd * 16) : raw[i][k];
+                memcpy(y + k * (VN / 4), &word, 4);
+            }
+#pragma unroll
+            for (int e = 0; e < VN; ++e) v[i * VN + e] = fmaxf(number<T>(y[e]), -INFINITY);      // NaN -> -inf
         }
         if (c + 1 < chunks) load(c + 1, raw);                // on its way while this chunk is looked at
         float best = v[0];
@@ -249,8 +273,8 @@ __global__ void __launch_bounds__(THREADS, 4) beam_parts_kernel(Args a) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (v[i] >= bound) {
-                    const int p = base + c * CHUNK + (i / VN * THREADS + t) * VN + i % VN;
-                    if (p >= lo && p < hi) keep(sm, v[i], p);
+                    const int p = lo + c * CHUNK + (i / VN * THREADS + t) * VN + i % VN;
+                    if (p < hi) keep(sm, v[i], p);
                 }
         }
         if (c == 0 && chunks > 1) {                          // what the chunks behind this one have to reach: its own n-th best
@@ -446,7 +470,7 @@ LMOE_API int lmoe_beam_select(const lmoe::beam::Args* ap, int type, cudaStream_t
     const Args& a = *ap;
     if (a.N <= 0 || a.K <= 0 || a.K > MOST || a.V <= 0 || a.n <= 0 || a.n > MOST || (long long)a.N * a.K > 65535 || (long long)a.K * a.V > 0x7fffffff ||
         (long long)a.K * a.V < a.n || a.length <= 0 || a.length % 8 != 0 ||
-        (long long)a.parts * a.length < (long long)a.V + 7 || (long long)a.K * a.parts * a.n > 0x7fffffff) return -1;
+        (long long)a.parts * a.length < a.V || (long long)a.K * a.parts * a.n > 0x7fffffff) return -1;
     return type == 0 ? select<float>(a, st) : type == 1 ? select<lmoe::bf16>(a, st) : select<__half>(a, st);
 }
 

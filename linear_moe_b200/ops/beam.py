@@ -1,7 +1,8 @@
 """One step of a beam search: the best continuations, and the beams' states in their new order (``csrc/beam.cu``; CPU tensors run the eager form).
 
-:func:`beam_select` takes the best ``n`` of ``scores[b] + log_softmax(logits[b])[t]`` over beams and vocabulary of every prompt, ties to the lowest ``b V + t``; the scores are
-compared in 64 bits and rounded once.  NaN logits count as minus infinity.  :func:`reorder_states` gives the rows ``parents`` of every state, all of them in one launch;
+:func:`beam_select` takes the best ``n`` of ``scores[b] + log_softmax(logits[b])[t]`` over beams and vocabulary of every prompt, ties to the lowest ``b V + t``.  Candidates of one beam
+are compared by their logits; those of different beams by scores in 64 bits (rounded once for the result) whose log-sums are sums of 32-bit exponentials, some 1e-7 off: nearer ones can come in
+either order on CUDA, equal rows with equal scores in the order of their beams.  NaN logits count as minus infinity.  :func:`reorder_states` gives the rows ``parents`` of every state, all of them in one launch;
 :func:`copy_pages_` copies pages inside their pools."""
 from __future__ import annotations
 
@@ -60,14 +61,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
         logits = logits.contiguous()
         s_n, s_k, s_v = logits.stride()
     out, beam, token = torch.empty((N, n), dtype=torch.float32, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev)
-    # rows may begin up to seven numbers behind a 16-byte boundary; a chunk to a part, or parts for one wave of four CTAs per SM
-    parts = max(1, min(-(-(V + 7) // CHUNK), 4 * Kn.num_sms() // (N * K)))
+    # a chunk to a part, or parts for one wave of four CTAs per SM
+    parts = max(1, min(-(-V // CHUNK), 4 * Kn.num_sms() // (N * K)))
     rows = N * K * parts
     work = torch.empty(rows * (3 + 2 * n), dtype=torch.float32, device=dev)      # sums (64 bits), maxima, candidates
     p = work.data_ptr()
     c_n, c_k = scores.stride()
     a = _Args(logits.data_ptr(), scores.data_ptr(), out.data_ptr(), beam.data_ptr(), token.data_ptr(), p + rows * 12, p + rows * 8, p + rows * (12 + 4 * n), p, s_n, s_k,
-              c_n, c_k, N, K, V, n, parts, -(-(V + 7) // (parts * 8)) * 8)
+              c_n, c_k, N, K, V, n, parts, -(-V // (parts * 8)) * 8)
     with on_device(logits):
         Kn._check(Kn.lib().lmoe_beam_select(ctypes.byref(a), kind, Kn._st()), "beam_select", 2)
     return out, beam, token
