@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(THREADS) copy_rows_kernel(const __grid_constan
 LMOE_API int lmoe_beam_select(const lmoe::beam::Args* ap, int type, cudaStream_t st) {
     using namespace lmoe::beam;
     const Args& a = *ap;
-    if (a.N <= 0 || a.K <= 0 || a.K > MOST || a.V <= 0 || a.n <= 0 || a.n > MOST || (long long)a.N * a.K > 65535 || (long long)a.K * a.V > 0x7fffffff ||
+    if (a.N <= 0 || a.K <= 0 || a.K > MOST || a.V <= 0 || a.n <= 0 || a.n > MOST || (long long)a.N * a.K > 65535 || (long long)a.K * a.V > 0x7fffffff - 4 * CHUNK ||
         (long long)a.K * a.V < a.n || a.length <= 0 || a.length % 8 != 0 ||
         (long long)a.parts * a.length < a.V || (long long)a.K * a.parts * a.n > 0x7fffffff) return -1;
     return type == 0 ? select<float>(a, st) : type == 1 ? select<lmoe::bf16>(a, st) : select<__half>(a, st);

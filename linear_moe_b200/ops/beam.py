@@ -14,6 +14,7 @@ import torch
 from .scored_attn import on_device
 
 CHUNK, MOST, TENSORS = 4096, 128, 64                      # csrc/beam.cu
+PLACES = (1 << 31) - (1 << 14)                            # places of beam and token: a part's last chunk ends behind them, still below 2^31
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -41,6 +42,17 @@ def _eager_select(logits, scores, n):
     return best.float(), at // V, at % V
 
 
+def _held(N: int, K: int, V: int, n: int) -> bool:
+    """Do the kernels hold a search of this size?"""
+    return 0 < N and n <= MOST and K <= MOST and N * K <= 65535 and K * V <= PLACES
+
+
+def _shares(N: int, K: int, V: int, slots: int) -> Tuple[int, int]:
+    """(parts of a beam's row, logits of a part): a chunk to a part, or parts for one wave."""
+    parts = max(1, min(-(-V // CHUNK), slots // (N * K)))
+    return parts, -(-V // (parts * 8)) * 8
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``logits [N, K, V]`` (fp32, bf16 or fp16) and ``scores [N, K]`` (fp32) of N prompts with K beams: ``(scores fp32, beam int64, token int64)``, each ``[N, n]``,
     best first.  No gradient."""
@@ -52,7 +64,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
     N, K, V = shape
     if not 1 <= n <= K * V:
         raise ValueError(f"{n} continuations of {K} beams over a vocabulary of {V}")
-    if not logits.is_cuda or n > MOST or K > MOST or N * K > 65535 or K * V >= 1 << 31 or N == 0:      # wider searches than the kernels hold
+    if not logits.is_cuda or not _held(N, K, V, n):
         with torch.no_grad():
             return _eager_select(logits, scores, n)
     from . import cuda as Kn
@@ -61,14 +73,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int) -> Tuple[tor
         logits = logits.contiguous()
         s_n, s_k, s_v = logits.stride()
     out, beam, token = torch.empty((N, n), dtype=torch.float32, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev), torch.empty((N, n), dtype=torch.int64, device=dev)
-    # a chunk to a part, or parts for one wave of four CTAs per SM
-    parts = max(1, min(-(-V // CHUNK), 4 * Kn.num_sms() // (N * K)))
+    parts, length = _shares(N, K, V, 4 * Kn.num_sms())                           # four CTAs per SM
     rows = N * K * parts
     work = torch.empty(rows * (3 + 2 * n), dtype=torch.float32, device=dev)      # sums (64 bits), maxima, candidates
     p = work.data_ptr()
     c_n, c_k = scores.stride()
     a = _Args(logits.data_ptr(), scores.data_ptr(), out.data_ptr(), beam.data_ptr(), token.data_ptr(), p + rows * 12, p + rows * 8, p + rows * (12 + 4 * n), p, s_n, s_k,
-              c_n, c_k, N, K, V, n, parts, -(-V // (parts * 8)) * 8)
+              c_n, c_k, N, K, V, n, parts, length)
     with on_device(logits):
         Kn._check(Kn.lib().lmoe_beam_select(ctypes.byref(a), kind, Kn._st()), "beam_select", 2)
     return out, beam, token

@@ -105,3 +105,15 @@ def test_equal_rows_at_any_place(device, dtype, V):
         at = torch.sort(total, dim=-1, descending=True, stable=True).indices[:, :36].to(device)
         assert torch.equal(b, at // V) and torch.equal(t, at % V)
         assert (s.view(2, -1, 9) == s.view(2, -1, 9)[:, :, :1]).all()
+
+
+def test_places_stay_below_32_bits():
+    """The last number that a part's chunks (and the one asked for ahead) count up to, at the largest searches that the kernels take."""
+    for N, K in ((1, 1), (1, 3), (1, 128), (4, 2), (500, 128), (60000, 1)):
+        V = BM.PLACES // K
+        assert BM._held(N, K, V, 1) and not BM._held(N, K, V + K, 1)
+        for V in (V, V - 1, V - BM.CHUNK, 5):
+            parts, length = BM._shares(N, K, V, 4 * 148)
+            assert parts * length >= V and length % 8 == 0
+            assert (parts - 1) * length + -(-length // BM.CHUNK) * BM.CHUNK < 1 << 31
+    assert not BM._held(0, 1, 10, 1) and not BM._held(1, 129, 10, 1) and not BM._held(1, 1, 1000, 129) and not BM._held(65536, 1, 10, 1)
