@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
+from ..ops import gemm
 from . import parallel_forward as PF
 from .paged_cache import PagedCache
 
@@ -235,6 +236,7 @@ def generate_tokens(model, tokens: torch.Tensor, lengths: torch.Tensor, *, eod: 
         prev = ctx
     if return_log_probs:
         logps = PF.broadcast_from_last_stage(model, logps, tuple(logps.shape), torch.float32, tokens.device)
+    gemm.check_error("generating tokens")
     return tokens, gen_len, logps
 
 
@@ -292,6 +294,7 @@ def _generate_packed(model, tokens, lengths, eod: Optional[int], draw, repetitio
             ses.finish([slots[b] for b in live if at[b] >= L])
             live, new = [live[k] for k in go], new[go]
         logits = ses.step([slots[b] for b in live], new)
+    gemm.check_error("generating tokens")
     end = max(at)
     return tokens[:, :end], torch.tensor(gen_len, device=dev), (None if logps is None else logps)
 
@@ -370,6 +373,7 @@ def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int
         scores = torch.tensor(next_s, device=device)
     for b in range(beams.shape[0]):
         hyps.add(beams[b], float(scores[b]), beams.shape[1] - P)
+    gemm.check_error("beam search")
     best = sorted(hyps.beams, key=lambda x: x[0], reverse=True)[:num_return]
     L = max(h.shape[0] for _, h in best)
     out = torch.full((len(best), L), eod, dtype=torch.long, device=device)

@@ -46,12 +46,18 @@ def _err(device) -> torch.Tensor:
 OTHER_WORDS: list = []          # error words of devices that the status tensor does not lie on (``cuda.error_word``)
 
 
-def check_error():
+def check_error(where: str = ""):
+    """Raise if a kernel has set an error word since the last check; ``fused_comm.check_status`` reads this device's with its own word."""
     for word in ([] if _ERR is None else [_ERR]) + OTHER_WORDS:
         v = int(word.item())
         if v != 0:
             word.zero_()
-            raise RuntimeError(f"tcgen05 GEMM: bounded wait expired (code {v:#x})" if v < 0x10000 else _ERRORS.get(v & 0xff000, f"kernel error {v:#x}") + f" (code {v:#x})")
+            raise RuntimeError(error_text(v, where))
+
+
+def error_text(v: int, where: str = "") -> str:
+    what = "tcgen05 GEMM: bounded wait expired" if v < 0x10000 else _ERRORS.get(v & 0xff000, "kernel error")
+    return f"{what} (code {v:#x}) {where}".rstrip()
 
 
 _ERRORS = {0x11000: "one-token attention: a length outside the page table", 0x12000: "one-token attention: a page number outside the pool",

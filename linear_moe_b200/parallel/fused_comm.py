@@ -166,14 +166,15 @@ def status_word(device) -> torch.Tensor:
 
 def check_status(where: str = ""):
     """Raise ``CommTimeout`` if any fused kernel gave up on a bounded wait since the last check, or ``RuntimeError`` if
-    a tcgen05 GEMM did (its error word is the second element of the same status tensor, so one read covers both), or if
-    a decay too strong for the gated-scan kernels was seen (third element)."""
+    another kernel did (its error word is the second element of the same status tensor, so one read covers both; words
+    of other devices are read too), or if a decay too strong for the gated-scan kernels was seen (third element)."""
     if os.environ.get("LMOE_CANARY", "0") != "0":
         verify_canaries()
     if STATUS is None:
         return
+    from ..ops import gemm
     from ..train.watchdog import raise_on_comm_status
-    vals = STATUS[:3].cpu()
+    vals = STATUS[:3].to("cpu", copy=True)
     if int(vals[2]) != 0:
         STATUS.zero_()
         raise RuntimeError("a key-channel log decay below -80 over half a chunk (32 tokens) reached the chunked gated-scan "
@@ -184,7 +185,9 @@ def check_status(where: str = ""):
         raise_on_comm_status(vals[:1], where)
     if int(vals[1]) != 0:
         STATUS.zero_()
-        raise RuntimeError(f"tcgen05 GEMM: bounded wait expired (code {int(vals[1]):#x}) {where}")
+        raise RuntimeError(gemm.error_text(int(vals[1]), where))
+    if gemm.OTHER_WORDS:
+        gemm.check_error(where)
 
 
 # Budget of every bounded wait of the fused kernels.  The default is far above ordinary rank skew (a rank that stalls on
