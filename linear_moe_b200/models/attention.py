@@ -50,6 +50,11 @@ class RotaryCache:
             self._key, self._val = key, (cos, sin)
         return self._val
 
+    def at(self, positions):
+        """cos/sin of any positions ``[B, T]``, a row each: there is no table that one could lie outside of."""
+        cfg = self.cfg
+        return R.rope_at(positions.reshape(-1), int(self.dim * cfg.rotary_percent), cfg.rotary_base, cfg.rotary_seq_len_interpolation_factor)
+
 
 def _kv_cache_update(cache: Optional[dict], k, v):
     """Append to the KV cache of a softmax layer; returns the full K, V and the query offset."""
@@ -123,8 +128,8 @@ class SelfAttention(nn.Module):
             k, v = (t[table[:, : -(-n // page)].long()].flatten(1, 2)[:, :n] for t in (kp, vp))
         return ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, position_offset, cfg.sliding_window, **self._scores(q.device))
 
-    def forward(self, x, cache: Optional[dict] = None, position_offset: int = 0, key_first=None, positions=None, **_):
-        """``key_first`` int32 ``[B,T]``: first token that a token may attend to (packed documents); ``positions`` ``[B,T]``: rotary positions."""
+    def forward(self, x, cache: Optional[dict] = None, position_offset: int = 0, key_first=None, rotary=None, **_):
+        """``key_first`` int32 ``[B,T]``: first token that a token may attend to (packed documents); ``rotary``: cos and sin of every token (``RotaryCache.at``)."""
         cfg = self.cfg
         qkv = self.linear_qkv(x)
         B, T = qkv.shape[:2]
@@ -143,10 +148,10 @@ class SelfAttention(nn.Module):
             at = cache["lengths"][:, None].long() - 1
             q = ops.apply_rope_at(q.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
             k = ops.apply_rope_at(k.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
-        elif self.rope is not None and positions is not None:
-            cos, sin = self.rope.get(T, 0, x.device)
-            q = ops.apply_rope_at(q.contiguous(), cos, sin, positions, cfg.rotary_interleaved)
-            k = ops.apply_rope_at(k.contiguous(), cos, sin, positions, cfg.rotary_interleaved)
+        elif self.rope is not None and rotary is not None:
+            if rotary[0].shape[0] != B * T:
+                raise ValueError(f"{rotary[0].shape[0]} positions for {B} x {T} tokens")
+            q, k = (ops.apply_rope(t.reshape(1, B * T, *t.shape[2:]), *rotary, cfg.rotary_interleaved).view(t.shape) for t in (q, k))
         elif self.rope is not None:
             cos, sin = self.rope.get(T, pos0, x.device)
             q = ops.apply_rope(q.contiguous(), cos, sin, cfg.rotary_interleaved)

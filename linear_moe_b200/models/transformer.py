@@ -266,7 +266,7 @@ class CausalLM(nn.Module):
                 hidden_in: Optional[torch.Tensor] = None, caches: Optional[List[dict]] = None,
                 position_offset: int = 0, parallel_output: bool = False, return_hidden: bool = False, batch=None,
                 logit_rows: Optional[torch.Tensor] = None, key_first: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None):
-        """``key_first`` int32 ``[B,T]`` (``ops.document_first``): a token attends to the tokens from there on; ``positions`` ``[B,T]``: rotary positions other than 0, 1, ...
+        """``key_first`` int32 ``[B,T]`` (``ops.document_first``): a token attends to the tokens from there on; ``positions`` ``[B,T]``: rotary positions other than 0, 1, ..., of any size.
         Both are for whole sequences through models of softmax layers.
 
         ``batch`` (``ops.row_batch.RowBatch``; models that run packed rows): ``input_ids`` are the packed tokens of its
@@ -282,7 +282,8 @@ class CausalLM(nn.Module):
         if key_first is not None or positions is not None:
             if caches is not None or not self.mesh["cp"].is_trivial or any(s.mixer not in ("attn", None) for s in self.specs):
                 raise ValueError("document ranges and positions are for softmax layers, on whole sequences without a cache (linear layers carry their state over a document's end)")
-            attend = {"key_first": key_first, "positions": positions}
+            ropes = [r for r in (getattr(blk._mixer(), "rope", None) for blk in self.decoder.layers) if r is not None] if positions is not None else []
+            attend = {"key_first": key_first, "rotary": ropes[0].at(positions) if ropes else None}       # the same for all layers
         x, residual = self._run_blocks(x, residual, caches, position_offset, attend)
         if not self.post_process:
             return x if residual is None else x + residual

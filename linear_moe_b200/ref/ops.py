@@ -86,8 +86,13 @@ ACT2FN = {
 def rope_freqs(seq_len: int, dim: int, base: float = 10000.0, offset: int = 0, device=None,
                interpolation_factor: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """cos/sin tables ``[seq_len, dim/2]`` in fp32."""
-    inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float32, device=device) / dim))
-    pos = torch.arange(offset, offset + seq_len, dtype=torch.float32, device=device)
+    return rope_at(torch.arange(offset, offset + seq_len, dtype=torch.float32, device=device), dim, base, interpolation_factor)
+
+
+def rope_at(pos, dim: int, base: float = 10000.0, interpolation_factor: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos/sin ``[n, dim/2]`` in fp32 of any positions ``[n]``."""
+    inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float32, device=pos.device) / dim))
+    pos = pos.float()
     if interpolation_factor:
         pos = pos / interpolation_factor
     ang = pos[:, None] * inv[None, :]
