@@ -85,6 +85,13 @@ class PagedCache(list):
         self.length = end
         self._lengths.fill_(end)
 
+    def expect(self, rows: int, tokens: int, position_offset: int):
+        """What a forward pass asks of its cache: as many rows, and room for its tokens (a captured step comes without its offset)."""
+        if self.paged and rows != len(self.owned):
+            raise ValueError(f"{rows} rows of tokens on a cache of {len(self.owned)} rows")
+        if self.paged and position_offset + tokens > self.length:
+            raise ValueError(f"tokens up to {position_offset + tokens} on a cache with room for {self.length}: advance() comes first")
+
     def reorder(self, parents: Sequence[int]):
         """Row i goes on from row ``parents[i]``; linear layers' states too.  Entries have to be tensors with a row per request (:meth:`reorderable`)."""
         n = len(self.owned)

@@ -273,6 +273,8 @@ class CausalLM(nn.Module):
         requests and the result has one row per token, or per entry of ``logit_rows``."""
         if self.packed_rows:
             return forward_rows(self, input_ids, labels, caches, position_offset, batch, logit_rows, return_hidden)
+        if input_ids is not None and hasattr(caches, "expect"):
+            caches.expect(*input_ids.shape, position_offset)
         if self.pre_process:
             x = self.embedding.word_embeddings(input_ids)
         else:
