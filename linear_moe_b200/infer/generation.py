@@ -326,6 +326,16 @@ def can_page_beams(model) -> bool:
     return PagedCache.supported(model) and model.mesh.pp == 1 and not str(model.cfg.la_module or "").startswith("mom_")
 
 
+def _states_by_row(model, prompt: torch.Tensor) -> bool:
+    """Do the linear layers keep tensors with a row per request?  A token of two requests tells, which the single prompt cannot: there a leading dimension of one can be anything."""
+    trial = PagedCache(model, 2, 1)
+    if len(trial.paged) == len(trial):
+        return True
+    trial.advance(1)
+    PF.stage_forward(model, prompt[:, :1].expand(2, 1), trial, 0)
+    return trial.reorderable()
+
+
 @torch.no_grad()
 def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int, eod: int, length_penalty: float = 1.0,
                 num_return: int = 1, paged: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -338,6 +348,8 @@ def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int
     if paged:
         if not can_page_beams(model):
             raise ValueError("a paged beam search is for models of softmax and linear layers on one pipeline stage, without a mixture of memories")
+        if beam_size > 1 and not _states_by_row(model, prompt):
+            raise ValueError("a layer of this model keeps states that do not follow a beam")
         caches = PagedCache(model, beam_size, P + max_new_tokens, live=1)
     beams = prompt.repeat(beam_size, 1)
     scores = torch.zeros(beam_size, device=device)
@@ -350,8 +362,6 @@ def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int
         elif step == 0:                                    # the prompt once, then a row per beam
             caches.advance(P)
             logits = PF.stage_forward(model, prompt, caches, 0)[:, -1].expand(beam_size, -1)
-            if not caches.reorderable():
-                raise ValueError("a layer of this model keeps states that do not follow a beam")
             caches.reorder([0] * beam_size)
         else:
             caches.reorder(next_b)
