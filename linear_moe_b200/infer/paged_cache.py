@@ -40,7 +40,7 @@ class PagedCache(list):
             if att.rope is not None and rope is None:
                 rope = R.rope_freqs(width * PAGE, int(att.D * cfg.rotary_percent), cfg.rotary_base, 0, dev, cfg.rotary_seq_len_interpolation_factor)
             for name in ("k_pages", "v_pages"):
-                self[i][name] = torch.zeros(len(self.free), PAGE, att.Gl, att.D, dtype=cfg.params_dtype, device=dev)
+                self[i][name] = torch.zeros(len(self.free), PAGE, att.Gl, att.D, dtype=att.linear_qkv.weight.dtype, device=dev)
             if rope is not None:
                 self[i]["cos"], self[i]["sin"] = rope
         self._bind()

@@ -32,3 +32,16 @@ def test_rows_are_the_cache_s():
         with pytest.raises(ValueError, match="rows"):
             m(tok[:, :4], caches=cache)
         m(tok[:2, :4], caches=cache)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_pages_have_the_layers_type(device):
+    """A model built in one type and brought to another one."""
+    from linear_moe_b200.infer import generation as G
+    from test_softmax_layers import EOD, prompts
+    m = model(device, params_dtype=torch.bfloat16).float()
+    base, lengths = prompts(device, L=20)
+    a, b = (G.generate_tokens(m, base.clone(), lengths, top_k=1, paged=p)[0] for p in (False, True))
+    assert torch.equal(a, b)
+    a, b = (G.beam_search(m, base[:1, :9], 3, 5, EOD, paged=p)[0] for p in (False, True))
+    assert torch.equal(a, b)
