@@ -38,17 +38,18 @@ class RotaryCache:
     def get(self, T: int, offset: int, device):
         key = (T, offset, str(device))
         if self._key != key:
-            cfg = self.cfg
-            rot = int(self.dim * cfg.rotary_percent)
-            if self.yarn and cfg.rotary_scaling_factor > 1:
-                cos, sin, m = R.yarn_freqs(T, rot, cfg.rotary_base, cfg.rotary_scaling_factor, offset=offset,
-                                           device=device, mscale=0.707, mscale_all_dim=0.707)
-                self.mscale = m
-            else:
-                cos, sin = R.rope_freqs(T, rot, cfg.rotary_base, offset, device,
-                                        cfg.rotary_seq_len_interpolation_factor)
-            self._key, self._val = key, (cos, sin)
+            with torch.inference_mode(False):                  # a later training step saves them
+                self._val = self._tables(T, offset, device)
+            self._key = key
         return self._val
+
+    def _tables(self, T: int, offset: int, device):
+        cfg = self.cfg
+        rot = int(self.dim * cfg.rotary_percent)
+        if self.yarn and cfg.rotary_scaling_factor > 1:
+            cos, sin, self.mscale = R.yarn_freqs(T, rot, cfg.rotary_base, cfg.rotary_scaling_factor, offset=offset, device=device, mscale=0.707, mscale_all_dim=0.707)
+            return cos, sin
+        return R.rope_freqs(T, rot, cfg.rotary_base, offset, device, cfg.rotary_seq_len_interpolation_factor)
 
     def at(self, positions):
         """cos/sin of any positions ``[B, T]``, a row each: there is no table that one could lie outside of."""
@@ -108,7 +109,8 @@ class SelfAttention(nn.Module):
         if cfg.position_embedding_type == "alibi":
             if self._slopes is None or self._slopes.device != device:
                 n = self.Gl * self.qpg
-                self._slopes = ops.alibi_slopes(self.H)[self.mesh.tp_rank * n:(self.mesh.tp_rank + 1) * n].to(device)
+                with torch.inference_mode(False):              # a later training step saves them
+                    self._slopes = ops.alibi_slopes(self.H)[self.mesh.tp_rank * n:(self.mesh.tp_rank + 1) * n].to(device)
             out["slopes"] = self._slopes
         return out
 
