@@ -113,7 +113,8 @@ def error_word(device) -> int:
         from . import gemm
         t = gemm._err(device)
         if t.device != device:
-            t = torch.zeros(1, dtype=torch.int32, device=device)
+            with torch.inference_mode(False):
+                t = torch.zeros(1, dtype=torch.int32, device=device)
             gemm.OTHER_WORDS.append(t)
         _ERROR_WORDS[device] = t
     return t.data_ptr()

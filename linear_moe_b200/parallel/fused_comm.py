@@ -160,7 +160,8 @@ def mark_step_sync():
 def status_word(device) -> torch.Tensor:
     global STATUS
     if STATUS is None:
-        STATUS = torch.zeros(4, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):                  # whoever checks it clears it
+            STATUS = torch.zeros(4, dtype=torch.int32, device=device)
     return STATUS
 
 

@@ -41,3 +41,27 @@ def test_generation_reads_the_words(words, which, paged):
     with pytest.raises(RuntimeError, match="a row that is none"):
         G.beam_search(m, base[:1, :9], 2, 3, EOD, paged=paged)
     G.beam_search(m, base[:1, :9], 2, 3, EOD, paged=paged)
+
+
+@pytest.mark.parametrize("other", [False, True])
+def test_words_made_under_inference_mode(monkeypatch, other):
+    """The first kernel of a process may run there; the check that finds its error may not."""
+    from linear_moe_b200.ops import cuda as K
+    monkeypatch.setattr(fused_comm, "STATUS", None)
+    monkeypatch.setattr(gemm, "_ERR", None)
+    monkeypatch.setattr(gemm, "OTHER_WORDS", [])
+    monkeypatch.setattr(K, "_ERROR_WORDS", {})
+    cpu = torch.device("cpu")
+    with torch.inference_mode():
+        if other:
+            gemm._err(torch.device("meta"))                    # the status tensor lies elsewhere
+        K.error_word(cpu)
+    word = K._ERROR_WORDS[cpu]
+    if other:
+        monkeypatch.setattr(gemm, "_ERR", None)
+        assert len(gemm.OTHER_WORDS) == 1
+    for _ in range(2):
+        word.data[0] = 0x13000
+        with pytest.raises(RuntimeError, match="a row that is none"):
+            gemm.check_error()
+        assert int(word) == 0
