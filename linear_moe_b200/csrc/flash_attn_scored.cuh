@@ -585,6 +585,7 @@ scored_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const float nm = m == -INFINITY ? 0.f : -m * sc;
                 const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+                // The product takes the weights in 16 bits, as its operands have to be (half a step of each, in no common direction); the sum, in 32 bits, takes them as they were.
 #pragma unroll
                 for (int col = 0; col < 64; col += 32) {
                     uint32_t p[16];

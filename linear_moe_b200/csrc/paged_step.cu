@@ -6,7 +6,7 @@
 // 1.4 times the GPU's rate for 8 heads), so the tensor cores have four times the work that the formula asks for and are still idle for most of the time.
 // A CTA of four warps takes one key head and a range of keys; a warp takes every fourth group of 16 keys and has a ring of three groups of its own that TMA fills
 // (128-byte swizzle, one lane issues), so no warp waits for another one until the end.  The operands come out of the ring by ldmatrix: K as it lies, V transposed.
-// Maxima lag by up to 2^8 as in the prompt kernel: unless a score runs ahead of that, which one vote tells, nothing is exchanged between lanes and nothing rescaled.
+// Maxima lag by up to 2^8: unless a score runs ahead of that, which one vote tells, nothing is exchanged between lanes and nothing rescaled.
 // Weights in bf16 have their rounding's remainder as a second operand, with up to 8 query heads in the rows of the products that no head has: it takes the output's error from 0.0024 (of 300
 // keys) to that of its own rounding, 0.0017, and at most 0.3 us (1 x 300 keys 5.4 / 5.7 us, 64 x 8192 191 / 191 us).
 // Rows of a group that are hidden (behind the last key, in front of the window) are masked, and their values set to zero in the ring, so that nothing stale meets a weight of zero;

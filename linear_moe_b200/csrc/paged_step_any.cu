@@ -1,6 +1,8 @@
 // The function of paged_step.cu for what its tensor-core kernel does not take: fp32, heads of more than 128 numbers or no multiple of 8, rows off 16-byte boundaries, pages of any
 // size.  A block per (request, query head); a warp per key, lanes along the head; fp32 throughout, compiled without approximate functions.  Every query head reads its key head's rows by
-// itself (they meet in L1 and L2).
+// itself (they meet in L1 and L2), and a request's keys are not shared out.  Bound by the chain of a key: score, sum over the warp, exponential, the output's scaling.
+// Measured, replayed, keys of one length, 32 over 8 heads of 128 in bf16 on the tensor cores / here in pages of 24 rows / here in fp32 / here with heads of 256 (bf16): 8 requests of 2048 keys 15 / 240 / 225 / 362 us,
+// 64 of 4096 172 / 1691 / 1585 / 2925; 2 of 65536 (16 over 2 heads) 31 / 7153 / 7008 / 10907; 1 of 300 (16 over 4) 5.2 / 25 / 23 / 32.  So it is what runs where nothing else does, and no more.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
