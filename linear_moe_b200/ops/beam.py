@@ -31,7 +31,9 @@ class _Rows(ctypes.Structure):
 def _eager_select(logits, scores, n):
     x = torch.nan_to_num(logits.double(), nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
     x = x - x.amax(-1, keepdim=True)                       # NaN in beams of nothing but minus infinity
-    total = x + (scores.double()[..., None] - x.exp().sum(-1, keepdim=True).log())
+    # rows padded to begin alike: how a row's sum is grouped follows its place, and equal rows have equal sums
+    sums = torch.nn.functional.pad(x, (0, -x.shape[2] % 64), value=float("-inf")).exp().sum(-1, keepdim=True)
+    total = x + (scores.double()[..., None] - sums.log())
     total = torch.nan_to_num(total, nan=float("-inf"), posinf=float("inf"), neginf=float("-inf")).flatten(1)
     V = logits.shape[2]
     best, at = torch.empty(len(total), n, dtype=torch.float64, device=x.device), torch.empty(len(total), n, dtype=torch.int64, device=x.device)

@@ -117,3 +117,14 @@ def test_places_stay_below_32_bits():
             assert parts * length >= V and length % 8 == 0
             assert (parts - 1) * length + -(-length // BM.CHUNK) * BM.CHUNK < 1 << 31
     assert not BM._held(0, 1, 10, 1) and not BM._held(1, 129, 10, 1) and not BM._held(1, 1, 1000, 129) and not BM._held(65536, 1, 10, 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [301, 4099, 20001])
+def test_equal_rows_of_a_wide_search(device, V):
+    """The same with more beams than the kernels hold."""
+    for seed in range(4):
+        row = torch.randn(V, generator=torch.Generator().manual_seed(seed)) * 3
+        s, b, t = ops.beam_select(row.to(device).expand(1, 131, V).contiguous(), torch.full((1, 131), -0.7, device=device), 262)
+        best = torch.sort(row, descending=True, stable=True).indices[:2]
+        assert b[0].tolist() == 2 * list(range(131)) and t[0].tolist() == [int(x) for x in best for _ in range(131)]
