@@ -62,7 +62,8 @@ def error_text(v: int, where: str = "") -> str:
 
 _ERRORS = {0x11000: "one-token attention: a length outside the page table", 0x12000: "one-token attention: a page number outside the pool",
            0x13000: "reordering: a row that is none", 0x14000: "one-token attention: a bounded wait expired",
-           **{0x20000 + 0x1000 * i: "attention with key ranges: a bounded wait expired" for i in range(1, 7)}}
+           **{0x20000 + 0x1000 * i: "attention with key ranges: a bounded wait expired" for i in range(1, 7)},
+           0x41000: "heads of a projection: a position outside the tables"}
 
 
 def _ok(t: torch.Tensor) -> bool:

@@ -142,6 +142,24 @@ def apply_rope(x, cos, sin, interleaved: bool = False):
     return torch.cat([o, xp], dim=-1).to(x.dtype)
 
 
+def qkv_heads(qkv, q_weight=None, k_weight=None, eps: float = 1e-6, cos=None, sin=None, positions=None, interleaved: bool = False):
+    """Queries ``[B,T,G r,D]``, keys and values ``[B,T,G,D]`` of a projection ``[B,T,G,r + 2,D]``: RMS norm of query and key heads, rotation by the tables' row ``positions [B,T]`` (default: the
+    token's place), rounded once."""
+    B, T, G, S, D = qkv.shape
+    out = []
+    for x, w in ((qkv[..., : S - 2, :].reshape(B, T, G * (S - 2), D), q_weight), (qkv[..., S - 2, :], k_weight)):
+        y = x.float()
+        if w is not None:
+            y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        if cos is not None:
+            at = torch.arange(T, device=qkv.device).expand(B, T) if positions is None else positions.long()
+            if at.numel() and not 0 <= int(at.min()) <= int(at.max()) < cos.shape[0]:
+                raise ValueError(f"a position outside the {cos.shape[0]} of the tables")
+            y = apply_rope(y.reshape(1, B * T, *y.shape[2:]), cos[at.reshape(-1)], sin[at.reshape(-1)], interleaved).reshape(y.shape)
+        out.append(y.to(qkv.dtype))
+    return out[0], out[1], qkv[..., S - 1, :].contiguous()
+
+
 # ---- softmax attention -----------------------------------------------------
 def softmax_attention(q, k, v, scale: Optional[float] = None, causal: bool = True, q_offset: int = 0,
                       window: Optional[int] = None, softcap: Optional[float] = None, slopes=None, key_first=None, key_stop=None):
