@@ -328,6 +328,7 @@ def softmax_attention(q, k, v, scale=None, causal=True, q_offset: int = 0, windo
 
 
 from .beam import beam_select, copy_pages_, reorder_states   # noqa: E402,F401
+from .int4_cache import int4_pages, paged_attention_int4, read_rows_int4, store_rows_int4   # noqa: E402,F401
 from .paged_attn import paged_attention   # noqa: E402,F401
 from .qkv_heads import qkv_heads   # noqa: E402,F401
 from .scored_attn import alibi_slopes, document_first, prefix_stop, scored_attention   # noqa: E402,F401

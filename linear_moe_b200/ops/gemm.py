@@ -63,7 +63,8 @@ def error_text(v: int, where: str = "") -> str:
 _ERRORS = {0x11000: "one-token attention: a length outside the page table", 0x12000: "one-token attention: a page number outside the pool",
            0x13000: "reordering: a row that is none", 0x14000: "one-token attention: a bounded wait expired",
            **{0x20000 + 0x1000 * i: "attention with key ranges: a bounded wait expired" for i in range(1, 7)},
-           0x41000: "heads of a projection: a position outside the tables"}
+           0x41000: "heads of a projection: a position outside the tables", 0x42000: "cache of 4 bits a number: a length outside the page table",
+           0x43000: "cache of 4 bits a number: a page number outside the pool", 0x44000: "cache of 4 bits a number: a bounded wait expired"}
 
 
 def _ok(t: torch.Tensor) -> bool:
