@@ -1,0 +1,356 @@
+// The next token of every request out of its logits and one random number:
+//   w_i = exp((x_i - max) / temperature);  tokens in the order of falling logits, equal ones by their number; a token is kept while fewer than k come before it, what comes before it is below p of the
+//   whole, and w_i >= min_p;  the token drawn is the first one, in the order of their numbers, up to which the kept weights exceed u times their sum.
+//
+// Sums of floating-point weights depend on their order, and so would the token next to a border.  So a weight is a whole number, 2^44 w rounded, from an exponential in 64 bits (a table of 32 powers of two
+// and a polynomial of degree 5 behind it, good to 2^-47; Tang, "Table-driven implementation of the exponential function", 1989), and all sums are exact: the same token however a row is shared out.
+//
+// A row is one cluster's: each CTA reads its part of the logits once and keeps it in shared memory where that holds it.  Then, if anything is cut off: a histogram over the weights' logarithms (16 bins
+// for a factor of two) with the number and the weight of each bin's tokens tells the bin in which the cut lies; histograms over the numbers inside of it tell the logit, and the equal ones are counted
+// by their numbers.  Last, the kept weights are summed up per thread, and a scan finds the thread, and the token, that the random number falls to.
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace lmoe {
+namespace sample {
+namespace cg = cooperative_groups;
+
+struct Args {
+    const void* logits;                                // [B, V], rows of `ld`
+    const float* draw;                                 // [B]
+    const float *temperature, *top_p, *min_p;          // [B] or null: the one below for all
+    const int* top_k;
+    long long* token;                                  // [B]
+    float* logp;                                       // [B]
+    long long ld;
+    int B, V, parts, len;                              // CTAs of a row, logits of each
+    int k;
+    float t, p, least;
+};
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 768, PER_OCTAVE = 16, MAX_PARTS = 8, SUB_BITS = 9;
+constexpr int BITS = 44;                               // of a weight of one: 2^19 of them stay below 2^63
+typedef unsigned long long u64;
+
+__device__ __forceinline__ float val(float x) { return x; }
+__device__ __forceinline__ float val(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float val(__half x) { return __half2float(x); }
+// NaN counts as minus infinity, zeros are equal
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x == 0.f ? 0.f : x; }
+// Whole numbers in the order of the floating-point ones
+__device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return b >> 31 ? ~b : b | 0x80000000u; }
+
+// 2^(i / 32)
+__constant__ double POWERS[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951,
+    1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+
+struct Scale { float max; double c; };                 // log2(e) / temperature
+// 2^44 exp((x - max) / temperature), rounded
+__device__ __forceinline__ u64 weight(float x, const Scale& s, const double* powers) {
+    if (x == s.max) return x == -INFINITY ? 0 : 1ull << BITS;
+    if (x == -INFINITY || s.max == INFINITY) return 0;
+    const double y = ((double)x - (double)s.max) * s.c;
+    if (!(y > -46.0)) return 0;
+    const double magic = 6755399441055744.0;           // 1.5 2^52: what is added to it is rounded to a whole number in its lower bits
+    const double shifted = y * 32.0 + magic;
+    const int n = (int)__double_as_longlong(shifted);
+    const double f = (y - (shifted - magic) * 0.03125) * 0.6931471805599453;      // up to ln 2 / 64
+    const double e = 1.0 + f * (1.0 + f * (0.5 + f * (1.0 / 6 + f * (1.0 / 24 + f * (1.0 / 120)))));
+    const double scaled = powers[n & 31] * e * __longlong_as_double((long long)(1023 + BITS + (n >> 5)) << 52);
+    return (u64)(__double_as_longlong(scaled + 6755399441055744.0) - 0x4338000000000000ll);
+}
+
+struct Bins { uint32_t count[BINS], part[3][BINS]; };  // weights in three parts of 15 bits, whose sums over a CTA's logits 32 bits hold
+struct Shared {
+    Bins bins[2];
+    double powers[32];
+    uint32_t count[WARPS];
+    u64 mass[WARPS];
+    u64 total;                                         // of this CTA, read by the others
+    uint32_t ties, top;
+    int found;
+    uint32_t at_count;
+    u64 at_mass;
+    int owner;
+    u64 rest;
+};
+
+__device__ __forceinline__ u64 up_to(u64 v) {          // inclusive over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += x;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t up_to(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += x;
+    }
+    return v;
+}
+// What comes before this thread, and in all; a barrier at the beginning and one inside.
+template <typename N> __device__ __forceinline__ N before(N v, N* warps, N& all) {
+    const N in = up_to(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31) warps[threadIdx.x >> 5] = in;
+    __syncthreads();
+    N sum = 0, ahead = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        const N x = warps[w];
+        if (w < (int)(threadIdx.x >> 5)) ahead += x;
+        sum += x;
+    }
+    all = sum;
+    return ahead + in - v;
+}
+
+template <typename T, bool HELD>                       // HELD: the part of a row lies in shared memory
+__global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
+    extern __shared__ __align__(16) unsigned char held[];
+    __shared__ Shared sm;
+    cg::cluster_group cl = cg::this_cluster();
+    const int b = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const int first = rank * a.len, n = max(0, min(a.len, a.V - first));
+    const T* row = (const T*)a.logits + b * a.ld + first;
+    T* mine = reinterpret_cast<T*>(held);
+    const T* x = HELD ? mine : row;
+    if (tid < 32) sm.powers[tid] = POWERS[tid];
+    for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[0])[i] = 0;
+
+    const float temperature = a.temperature != nullptr ? a.temperature[b] : a.t, top_p = a.top_p != nullptr ? a.top_p[b] : a.p, min_p = a.min_p != nullptr ? a.min_p[b] : a.least;
+    const bool greedy = !(temperature > 0.f);
+    int k = a.top_k != nullptr ? a.top_k[b] : a.k;
+    if (greedy) k = 1;
+    if (k <= 0 || k > a.V) k = a.V;
+    const bool by_mass = top_p < 1.f && k > 1, cut = by_mass || k < a.V;
+
+    // the part, and the largest logit
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += THREADS) {
+        const T raw = row[i];
+        if constexpr (HELD) mine[i] = raw;
+        top = fmaxf(top, clean(val(raw)));
+    }
+    top = warp_max(top);
+    if (lane == 0) sm.count[tid >> 5] = key_of(top);
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t y = 0;
+        for (int w = 0; w < WARPS; ++w) y = max(y, sm.count[w]);
+        sm.top = y;
+    }
+    cl.sync();
+    uint32_t top_key = 0;
+    for (int r = 0; r < a.parts; ++r) top_key = max(top_key, *cl.map_shared_rank(&sm.top, r));
+    Scale s;
+    s.max = __uint_as_float(top_key >> 31 ? top_key & 0x7fffffffu : ~top_key);
+    s.c = greedy ? 1.0 : 1.4426950408889634 / (double)temperature;
+
+    // the bin that the cut lies in, then the logit: tokens with keys above `edge` are kept, and `ties` of those equal to it
+    uint32_t edge = 0, ties = 0xffffffffu;
+    int turn = 0;
+    if (cut && k == 1) edge = top_key, ties = 1;
+    else if (cut) {
+        const float slope = (float)fmin(s.c * PER_OCTAVE, 1e30);
+        uint32_t lo = 0, hi = 0;                       // keys of the bin; level 0: not yet known
+        int shift = 0;
+        uint32_t ahead = 0;                            // tokens, and weight, above the bin
+        u64 ahead_mass = 0, limit = ~0ull;             // a token is kept if less than the limit comes before it
+        for (int level = 0;; ++level, turn ^= 1) {
+            Bins& h = sm.bins[turn];
+            for (int i = tid; i < n; i += THREADS) {
+                const float v = clean(val(x[i]));
+                const uint32_t key = key_of(v);
+                if (level > 0 && (key < lo || key > hi)) continue;
+                const u64 w = weight(v, s, sm.powers);
+                if (w == 0) continue;                  // never drawn
+                const int bin = level == 0 ? min((int)((s.max - v) * slope), BINS - 1) : (int)((hi - key) >> shift);
+                atomicAdd(&h.count[bin], 1u);
+                if (by_mass)
+#pragma unroll
+                    for (int j = 0; j < 3; ++j) {
+                        const uint32_t y = (uint32_t)(w >> (15 * j)) & 0x7fffu;
+                        if (y) atomicAdd(&h.part[j][bin], y);
+                    }
+            }
+            cl.sync();
+            for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[turn ^ 1])[i] = 0;
+            uint32_t count[2] = {0, 0};
+            u64 mass[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int bin = 2 * tid + j;
+                if (bin < BINS)
+                    for (int r = 0; r < a.parts; ++r) {
+                        const Bins* o = cl.map_shared_rank(&h, r);
+                        count[j] += o->count[bin];
+                        if (by_mass) mass[j] += (u64)o->part[0][bin] + ((u64)o->part[1][bin] << 15) + ((u64)o->part[2][bin] << 30);
+                    }
+            }
+            uint32_t all;
+            u64 all_mass;
+            if (tid == 0) sm.found = -1;
+            const uint32_t c0 = ahead + before(count[0] + count[1], sm.count, all);
+            const u64 m0 = ahead_mass + before(mass[0] + mass[1], sm.mass, all_mass);
+            if (level == 0 && by_mass) limit = top_p > 0.f ? max(1ull, (u64)ceil((double)top_p * (double)all_mass)) : 1ull;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t c = c0 + (j ? count[0] : 0);
+                const u64 m = m0 + (j ? mass[0] : 0);
+                if (count[j] > 0 && c < (uint32_t)k && m < limit) atomicMax(&sm.found, 2 * tid + j);
+            }
+            __syncthreads();
+            const int bin = sm.found;
+            if (bin >= 0 && bin / 2 == tid) {
+                sm.at_count = c0 + (bin & 1 ? count[0] : 0);
+                sm.at_mass = m0 + (bin & 1 ? mass[0] : 0);
+            }
+            __syncthreads();
+            if (bin < 0) break;                        // nothing above minus infinity
+            ahead = sm.at_count;
+            ahead_mass = sm.at_mass;
+            if (level == 0) {
+                if (!by_mass && all <= (uint32_t)k) break;     // no more tokens than k
+                // Keys that are certainly around the bin's (roundings are within 2^-22 of the logits), then its ends by bisection: bins fall as keys rise.
+                hi = top_key, lo = key_of(-INFINITY);
+                if (slope > 1e-20f && slope < 1e20f) {
+                    const float up = s.max - (float)bin / slope, down = bin == BINS - 1 ? -INFINITY : s.max - (float)(bin + 1) / slope;
+                    const float slack = 1e-6f * (fabsf(s.max) + fabsf(up) + (down == -INFINITY ? 0.f : fabsf(down)));
+                    hi = min(hi, key_of(clean(up + slack) == -INFINITY ? INFINITY : up + slack));
+                    lo = max(lo, key_of(clean(down - slack)));
+                }
+                auto bin_of = [&](uint32_t key) -> int {
+                    const float v = __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+                    return min((int)((s.max - v) * slope), BINS - 1);
+                };
+                uint32_t l = lo, h2 = hi;              // the largest key of this bin
+                while (l < h2) {
+                    const uint32_t mid = l + (h2 - l + 1) / 2;
+                    if (bin_of(mid) >= bin) l = mid;
+                    else h2 = mid - 1;
+                }
+                hi = l;
+                l = lo, h2 = hi;                       // the smallest one
+                while (l < h2) {
+                    const uint32_t mid = l + (h2 - l) / 2;
+                    if (bin_of(mid) <= bin) h2 = mid;
+                    else l = mid + 1;
+                }
+                lo = l;
+            } else {
+                hi -= (uint32_t)bin << shift;
+                lo = max(lo, hi - ((1u << shift) - 1));
+            }
+            if (lo == hi) {
+                edge = lo;
+                const u64 w = weight(__uint_as_float(edge >> 31 ? edge & 0x7fffffffu : ~edge), s, sm.powers);
+                ties = (uint32_t)k - ahead;
+                if (by_mass) ties = (uint32_t)min((u64)ties, (limit - ahead_mass + w - 1) / w);
+                break;
+            }
+            shift = max(0, 32 - __clz(hi - lo) - SUB_BITS);
+        }
+    }
+    __syncthreads();
+
+    // a thread's share of the part, in order: an odd number of words, so that neighbours read from different banks
+    constexpr int WORD = sizeof(T) == 4 ? 1 : 2;
+    int share = (n + THREADS - 1) / THREADS;
+    share = ((share + WORD - 1) / WORD | 1) * WORD;
+    const int from = min(n, tid * share), to = min(n, from + share);
+    // ties that lie before this thread's
+    uint32_t tied = 0;
+    if (cut && ties != 0xffffffffu) {
+        uint32_t own = 0, all;
+        for (int i = from; i < to; ++i) own += key_of(clean(val(x[i]))) == edge;
+        tied = before(own, sm.count, all);
+        if (tid == 0) sm.ties = all;
+        cl.sync();
+        for (int r = 0; r < rank; ++r) tied += *cl.map_shared_rank(&sm.ties, r);
+    }
+    const u64 least = min_p > 0.f ? (u64)ceil((double)min_p * (double)(1ull << BITS)) : 0ull;
+    // the kept weight of token i, whose predecessors among the ties are `t`
+    auto kept = [&](int i, uint32_t& t) -> u64 {
+        const float v = clean(val(x[i]));
+        if (cut) {
+            const uint32_t key = key_of(v);
+            if (key < edge || (key == edge && t++ >= ties)) return 0;
+        }
+        const u64 w = weight(v, s, sm.powers);
+        return w >= least || v == s.max ? w : 0;       // the largest ones stay whatever min_p
+    };
+    u64 sum = 0, all;
+    uint32_t t = tied;
+    for (int i = from; i < to; ++i) sum += kept(i, t);
+    u64 ahead = before(sum, sm.mass, all);
+    if (tid == 0) sm.total = all, sm.owner = -1;
+    cl.sync();
+    u64 whole = 0, parts_ahead = 0;
+    for (int r = 0; r < a.parts; ++r) {
+        const u64 y = *cl.map_shared_rank(&sm.total, r);
+        if (r < rank) parts_ahead += y;
+        whole += y;
+    }
+    ahead += parts_ahead;
+    const double u = (double)a.draw[b];
+    u64 goal = u > 0.0 ? (u64)(u * (double)whole) : 0ull;      // the token up to which the weights exceed it
+    if (whole > 0 && goal >= whole) goal = whole - 1;
+    if (sum > 0 && ahead <= goal && goal < ahead + sum) {
+        u64 upto = ahead;
+        t = tied;
+        for (int i = from; i < to; ++i) {
+            const u64 w = kept(i, t);
+            upto += w;
+            if (upto > goal) {
+                a.token[b] = first + i;
+                a.logp[b] = (float)log((double)w / (double)whole);
+                break;
+            }
+        }
+    }
+    if (whole == 0 && rank == 0 && tid == 0) a.token[b] = 0, a.logp[b] = -INFINITY;       // a row of nothing but minus infinity
+    cl.sync();                                         // the others have read this one's sums
+}
+
+template <typename T>
+static int launch(const Args& a, cudaStream_t st) {
+    const long long bytes = (long long)a.len * sizeof(T);
+    const bool held = bytes <= 160 * 1024;
+    auto kernel = held ? sample_kernel<T, true> : sample_kernel<T, false>;
+    if (held) {
+        const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (rc) return rc;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.parts, a.B);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = held ? (size_t)bytes : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, a);
+    return (int)cudaGetLastError();
+}
+
+}  // namespace sample
+}  // namespace lmoe
+
+// type: 0 fp32, 1 bf16, 2 fp16.
+LMOE_API int lmoe_sample(const lmoe::sample::Args* ap, int type, cudaStream_t st) {
+    using namespace lmoe::sample;
+    const Args& a = *ap;
+    if (a.B <= 0 || a.B > 65535 || a.V <= 0 || a.V > 1 << 19 || a.parts < 1 || a.parts > MAX_PARTS || a.len <= 0 || a.len > 1 << 16 || (long long)a.parts * a.len < a.V) return -1;
+    return type == 0 ? launch<float>(a, st) : type == 1 ? launch<lmoe::bf16>(a, st) : launch<__half>(a, st);
+}

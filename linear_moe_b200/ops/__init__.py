@@ -331,6 +331,7 @@ from .beam import beam_select, copy_pages_, reorder_states   # noqa: E402,F401
 from .int4_cache import int4_pages, paged_attention_int4, read_rows_int4, store_rows_int4   # noqa: E402,F401
 from .paged_attn import paged_attention   # noqa: E402,F401
 from .qkv_heads import qkv_heads   # noqa: E402,F401
+from .sampling import sample_tokens   # noqa: E402,F401
 from .scored_attn import alibi_slopes, document_first, prefix_stop, scored_attention   # noqa: E402,F401
 
 

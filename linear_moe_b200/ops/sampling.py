@@ -1,0 +1,124 @@
+"""The next token of every request out of its logits and one random number (``csrc/sample.cu``; CPU tensors run the eager form).
+
+    w_i = exp((x_i - max x) / temperature)
+
+Tokens are put in the order of falling logits, equal ones by their number.  A token is kept while fewer than ``top_k`` come before it, while the weight of those before it is below ``top_p`` of the whole, and
+if ``w_i >= min_p``; the first one always is.  The token drawn is the first one, in the order of the vocabulary, up to which the kept weights exceed ``draw`` times their sum.  Given the random numbers, the result is
+a function of the logits: sums are exact in units of 2^-44 of the largest weight (weights below half of that are never drawn), so it does not depend on how a row is shared out.
+
+NaN logits count as minus infinity; tokens at plus infinity share the whole weight.  A row of nothing but minus infinity gives token 0 and a log-probability of minus infinity.  A temperature that is not
+above zero takes the largest logit; ``top_k`` below 1 and ``top_p`` of 1 or more cut nothing off."""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, Tuple, Union
+
+import torch
+
+from .scored_attn import on_device
+
+MOST, PART = 1 << 19, 1 << 16                              # logits of a row, and of a CTA (csrc/sample.cu)
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+Setting = Union[int, float, torch.Tensor]
+
+
+class _Args(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "draw", "temperature", "top_p", "min_p", "top_k", "token", "logp")] + [("ld", ctypes.c_longlong)] +
+                [(n, ctypes.c_int) for n in ("B", "V", "parts", "len", "k")] + [(n, ctypes.c_float) for n in ("t", "p", "least")])
+
+
+def _check(logits, draw, temperature, top_k, top_p, min_p):
+    if logits.dim() != 2 or logits.dtype not in _TYPES or logits.shape[1] == 0:
+        raise ValueError("sampling takes logits [B, V] in fp32, bf16 or fp16")
+    B = logits.shape[0]
+    if draw.shape != (B,) or draw.dtype != torch.float32 or draw.device != logits.device:
+        raise ValueError(f"the random numbers are fp32 [{B}], where the logits lie")
+    for name, x, dtype, good in (("temperature", temperature, torch.float32, lambda v: v >= 0), ("top_k", top_k, torch.int32, lambda v: v >= 0 and v == int(v)),
+                                 ("top_p", top_p, torch.float32, lambda v: v >= 0), ("min_p", min_p, torch.float32, lambda v: 0 <= v <= 1)):
+        if torch.is_tensor(x):
+            if x.shape != (B,) or x.dtype != dtype or x.device != logits.device:
+                raise ValueError(f"{name} is a number or {dtype} [{B}], where the logits lie")
+        elif not good(x):
+            raise ValueError(f"{name} of {x}")
+
+
+def _eager(logits, draw, temperature, top_k, top_p, min_p):
+    B, V = logits.shape
+    dev = logits.device
+
+    def setting(x):
+        return (x if torch.is_tensor(x) else torch.full((B,), float(x), dtype=torch.float32, device=dev))[:, None].double()
+    t, k, p, least = (setting(x) for x in (temperature, top_k, top_p, min_p))
+    x = torch.nan_to_num(logits.double(), nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+    x, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    top = x[:, :1]
+    greedy = ~(t > 0)
+    y = torch.where(x == top, 0.0, (x - top) / torch.where(greedy, 1.0, t))
+    unit = 2.0 ** 44
+    w = torch.where(x == float("-inf"), 0.0, (y.exp() * unit).round()).to(torch.int64)      # (minus infinity over an endless temperature is NaN)
+    upto = w.cumsum(-1)
+    before, whole = upto - w, upto[:, -1:]
+    limit = torch.where(p >= 1, float(1 << 62), (p * whole.double()).ceil().clamp_min(1)).to(torch.int64)
+    keep = (torch.arange(V, device=dev) < torch.where(greedy, 1, torch.where(k >= 1, k, V))) & (before < limit)
+    keep &= (w >= (torch.nan_to_num(least, nan=0.0).clamp(0, 1) * unit).ceil().to(torch.int64)) | (x == top)
+    kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0))
+    upto = kept.cumsum(-1)
+    whole = upto[:, -1:]
+    goal = torch.minimum((torch.nan_to_num(draw, nan=0.0).clamp_min(0)[:, None].double() * whole.double()).to(torch.int64), (whole - 1).clamp_min(0))
+    token = torch.where(whole[:, 0] > 0, (upto <= goal).sum(-1), 0)
+    share = kept.gather(1, token[:, None]).double() / whole.double()
+    return token, torch.where(whole[:, 0] > 0, share[:, 0].log(), float("-inf")).float()
+
+
+def _shares(B: int, V: int, slots: int) -> Tuple[int, int]:
+    """(CTAs of a row, logits of each)."""
+    parts = 1
+    while parts < 8 and parts * PART < V:
+        parts *= 2
+    return parts, -(-V // (parts * 8)) * 8
+
+
+def _key(x):
+    return (x.shape, x.stride(), x.dtype, x.device) if torch.is_tensor(x) else x
+
+
+_PLANS: Dict[tuple, bytes] = {}
+
+
+def _plan(logits, draw, temperature, top_k, top_p, min_p) -> bytes:
+    from . import cuda as K
+    _check(logits, draw, temperature, top_k, top_p, min_p)
+    B, V = logits.shape
+    parts, length = _shares(B, V, K.num_sms())
+    def number(x):
+        return 0 if torch.is_tensor(x) else x
+    return bytes(_Args(ld=logits.stride(0), B=B, V=V, parts=parts, len=length, k=min(int(number(top_k)), MOST), t=number(temperature), p=min(float(number(top_p)), 2.0), least=number(min_p)))
+
+
+def sample_tokens(logits: torch.Tensor, draw: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0, top_p: Setting = 1.0, min_p: Setting = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``logits [B, V]``, ``draw [B]`` fp32 in [0, 1): ``(token int64 [B], log-probability fp32 [B])``, the latter among the kept tokens.  Each setting is a number or a tensor with one for every
+    request (``top_k`` int32, the others fp32).  No gradient."""
+    if not logits.is_cuda or logits.shape[-1] > MOST or logits.shape[0] > 65535:
+        _check(logits, draw, temperature, top_k, top_p, min_p)
+        with torch.no_grad():
+            return _eager(logits, draw, temperature, top_k, top_p, min_p)
+    from . import cuda as K
+    key = (_key(logits), _key(draw), _key(temperature), _key(top_k), _key(top_p), _key(min_p))
+    plan = _PLANS.get(key)
+    if plan is None:
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        plan = _PLANS[key] = _plan(logits, draw, temperature, top_k, top_p, min_p)
+    B, V = logits.shape
+    flat = [t if not torch.is_tensor(t) or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous() for t in (logits, draw, temperature, top_k, top_p, min_p)]
+    if flat[0] is not logits:
+        return sample_tokens(*flat)
+    token, logp = torch.empty(B, dtype=torch.int64, device=logits.device), torch.empty(B, dtype=torch.float32, device=logits.device)
+    if B == 0:
+        return token, logp
+    a = _Args.from_buffer_copy(plan)
+    a.logits, a.draw, a.token, a.logp = logits.data_ptr(), flat[1].data_ptr(), token.data_ptr(), logp.data_ptr()
+    a.temperature, a.top_k, a.top_p, a.min_p = (t.data_ptr() if torch.is_tensor(t) else 0 for t in flat[2:])
+    with on_device(logits):
+        K._check(K.lib().lmoe_sample(ctypes.byref(a), _TYPES[logits.dtype], K._st()), "sample")
+    return token, logp
