@@ -1,0 +1,420 @@
+// Attention of one new token per request over a paged cache of 4 bits a number (int4_cache.cuh), bf16 and fp16 queries, heads of 32, 64, 96 and 128:
+//   x_j = cap tanh(scale q k_j / cap) - slope_h (n - 1 - j),   o = sum_j softmax_j(x_j) v_j   over the keys  max(0, n - window) <= j < n
+//
+// Bound by reading the visible rows once, 5/8 byte a number.  That is less than a third of what bf16 rows take, so a key has to be worked through in a third of the time, and what is spent on it is the
+// conversion of codes; they go to the tensor cores as they are, two at a time by one mask: 128 + code is a bf16 number whose lowest bits are the code.  With t = 128 + code
+//   q k_j = sum_c size_jc (q t_j)_c + sum_c (low_jc - 128 size_jc) Q_c        c: groups of 32, Q_c the query's sum over the group
+//   o = sum_j (p_j size_jc) t_j + sum_j p_j (low_jc - 128 size_jc)
+// The first sums are products of 16-bit numbers with one result per group of a row (keys: 8 at a time, the heads are the 16 rows of an m16n8k16 product; values: 16 numbers of a group at a time, the heads are
+// its 8 columns).  The second ones are one small product each, whose other operand is the row's lows and sizes as they lie in the cache.  Q in three bf16 parts, p and p size in two, fp16 queries in two (rows 8 to
+// 15 of the products, which no head has).
+//
+// A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys; a warp takes every fourth group of 16 keys and has a ring of its own, which bulk copies fill (a lane per copy), so no warp waits
+// for another one until the end.  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
+// Rows of a group that are hidden (behind the last key, in front of the window, on a page that is none) are masked, and their values' scales set to zero in the ring, so that nothing stale meets a weight of zero.
+// A NaN score raises no maximum, so what has seen nothing is told by its sum of zero, not by its maximum: a head that sees NaN gives NaN.
+//
+// The keys of a request are shared by up to 8 CTAs of a cluster, which join their maxima, sums and outputs in distributed shared memory; long contexts with few heads take more CTAs, which leave their parts
+// in fp32 for a second launch.
+#include <cooperative_groups.h>
+#include <type_traits>
+
+#include "attn_math.cuh"
+#include "flash_tc_utils.cuh"
+#include "int4_step.cuh"
+#include "tanh_cap.cuh"
+
+namespace lmoe {
+namespace int4 {
+namespace cg = cooperative_groups;
+
+constexpr int WARPS = 4, STAGES = 4, MAX_CLUSTER = 8, HEADS = 8;
+constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
+
+__device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ float lower(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float upper(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+// What rounding two numbers to bf16 took away, rounded itself
+__device__ __forceinline__ uint32_t rest(float x, float y, uint32_t rounded) { return pack2(x - lower(rounded), y - upper(rounded)); }
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Codes i and i + 4 of eight, as 128 + code
+__device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(tc::s32(dst)), "l"(src), "r"(bytes), "r"(tc::s32(bar)) : "memory");
+}
+template <typename T> __device__ __forceinline__ uint32_t out2(float x, float y);
+template <> __device__ __forceinline__ uint32_t out2<bf16>(float x, float y) { return pack2(x, y); }
+template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+
+// N: groups of a head.  The pointers are read behind pdl_wait by plain loads: the kernel may start while the one before it runs.
+template <typename T, int N>
+__global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs a) {
+    constexpr bool TWO = sizeof(T) == 2 && !std::is_same<T, bf16>::value;      // queries in two parts
+    constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF_STAGE = CODES + SCALES, STAGE = 2 * HALF_STAGE;      // bytes
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t full[WARPS][STAGES];
+    __shared__ float part_m[WARPS][HEADS], part_l[WARPS][HEADS], cta_m[HEADS], cta_l[HEADS];
+    __shared__ int abort_flag, drain_flag, chosen, lens[WARPS * 32];
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int qpg = a.H / a.G, tiles = (qpg + HEADS - 1) / HEADS;
+    int b = blockIdx.z;
+    const int hk = blockIdx.y / tiles, tile = blockIdx.y % tiles, split = blockIdx.x;
+    const int h0 = hk * qpg + tile * HEADS, nh = min(HEADS, hk * qpg + qpg - h0);
+    if (threadIdx.x == 0) abort_flag = drain_flag = 0;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[w][s], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    if (a.sorted) {                                                    // this CTA's request: the one with blockIdx.z longer ones (up to 128 requests)
+        const int mine = threadIdx.x < a.B ? a.lengths[threadIdx.x] : 0;
+        lens[threadIdx.x] = mine;
+        __syncthreads();
+        int rank = 0;
+        for (int i = 0; i < a.B; ++i) rank += lens[i] > mine || (lens[i] == mine && i < threadIdx.x);
+        if (threadIdx.x < a.B && rank == blockIdx.z) chosen = threadIdx.x;
+        __syncthreads();
+        b = chosen;
+    }
+    const Share sh = share_of(a, b);
+    const int beg = sh.first + split * sh.per, end = min(sh.last, beg + sh.per);
+    if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0 && a.lengths[b] != sh.len) atomicCAS(a.err, 0, 0x42000);
+    if (beg >= end && a.splits > MAX_CLUSTER) return;                  // (a cluster's CTAs all stay, and one of them writes zeros where there is nothing to see)
+
+    unsigned char* ring = smem + w * STAGES * STAGE;
+    const int n_mine = beg + w < end ? (end - beg - w + WARPS - 1) / WARPS : 0;              // groups beg + w, beg + w + WARPS, ...
+    int pages_ahead = 0, bad = 0;                                      // a lane's page number; a bit per stage whose page is none
+    const long long bytes = page_bytes(a.page, D);
+    auto issue = [&](int j) {
+        if (j >= n_mine) return;
+        const int gi = beg + w + j * WARPS, st = j % STAGES;
+        if ((j & 31) == 0) pages_ahead = j + lane < n_mine ? a.table[b * a.table_ld + (gi + lane * WARPS) * GROUP / a.page] : 0;
+        const int page = __shfl_sync(0xffffffffu, pages_ahead, j & 31), row = gi * GROUP % a.page;
+        const bool there = page >= 0 && page < a.pages;
+        bad = there ? bad & ~(1 << st) : bad | 1 << st;
+        if (!there) {
+            if (lane == 0) atomicCAS(a.err, 0, 0x43000), tc::mbar_arrive(&full[w][st]);
+            return;
+        }
+        if (lane == 0) tc::mbar_expect_tx(&full[w][st], STAGE);
+        __syncwarp();
+        if (lane < 4) {                                                // codes and scales of keys, and of values
+            const unsigned char* from = (lane < 2 ? a.k : a.v) + ((long long)page * a.G + hk) * bytes + (lane & 1 ? a.page * (D / 2) + row * (D / 8) : row * (D / 2));
+            bulk_load(ring + st * STAGE + (lane >> 1) * HALF_STAGE + (lane & 1) * CODES, from, lane & 1 ? SCALES : CODES, &full[w][st]);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < STAGES - 1; ++j) issue(j);
+
+    // Queries: a lane's numbers 8 t .. 8 t + 7 of every group, in the order of `codes`; row g the head, row g + 8 what its rounding took away
+    uint32_t qa[N][4], qb[TWO ? N : 1][4], sums[3] = {0, 0, 0};
+    const bool there = g < nh;
+    const float slope = there && a.slopes != nullptr ? a.slopes[h0 + g] * LOG2E : 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = there ? val(((const T*)a.q)[b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t + i]) : 0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            qa[c][i] = pack2(q[i], q[i + 4]);
+            if constexpr (TWO) qb[c][i] = rest(q[i], q[i + 4], qa[c][i]);
+            sum += q[i] + q[i + 4];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // beside a row's lows (numbers c) and sizes (N + c), in three parts
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int at = c + i * N;
+            if (at / 2 != t) continue;
+            float x = i ? -128.f * sum : sum;
+#pragma unroll
+            for (int y = 0; y < 3; ++y) {
+                const uint32_t part = pack2(x, 0.f);
+                sums[y] |= part << (at & 1 ? 16 : 0);
+                x -= lower(part);
+            }
+        }
+    }
+    const float pre = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap = a.cap * LOG2E, unit = a.cap > 0.f ? cap : pre;
+    float m = -INFINITY, l = 0.f, o[2 * N][4], e[4] = {0.f, 0.f, 0.f, 0.f};      // o: numbers 4 g + 2 u, 4 g + 2 u + 1 of group c, heads 2 t, 2 t + 1;  e: head g, numbers 2 t, 2 t + 1 of the scales
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+    bool alive = true;
+    int j = 0;
+    for (; j < n_mine; ++j) {
+        const int st = j % STAGES, key0 = (beg + w + j * WARPS) * GROUP;
+        const bool hidden = bad >> st & 1;
+        issue(j + STAGES - 1);                                         // into the stage that was read last
+        alive = fatc::mbar_wait_warp(&full[w][st], j / STAGES & 1, &abort_flag, a.err, 0x44000 | st);
+        if (!alive) break;
+        unsigned char *K = ring + st * STAGE, *V = K + HALF_STAGE, *KS = K + CODES, *VS = V + CODES;
+        const bool edge = hidden || key0 < sh.lo || key0 + GROUP > sh.len;
+        if (edge) {                                                    // hidden rows get scales of zero
+            for (int i = lane; i < GROUP * N; i += 32) {
+                const int key = key0 + i / N;
+                if (hidden || key < sh.lo || key >= sh.len) reinterpret_cast<uint32_t*>(VS)[i] = 0;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // ahead of the next copy into this stage
+            __syncwarp();
+        }
+        uint32_t v[4];                                                 // scores: keys 8 (e >> 1) + 2 t + (e & 1)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            const int row = 8 * n + g;
+            uint32_t sc = 2 * t < 2 * N ? reinterpret_cast<const uint32_t*>(KS + row * (D / 8))[t] : 0u;
+            mma(x, sums[0], sums[2], sums[1], 0u, sc, sc);
+            float x0 = x[0] + x[2], x1 = x[1] + x[3];
+            const uint16_t* s0 = reinterpret_cast<const uint16_t*>(KS + (8 * n + 2 * t) * (D / 8)) + N;
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                const uint32_t y = reinterpret_cast<const uint32_t*>(K + row * (D / 2) + place(N, row, c) * 16)[t];
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                mma(d, qa[c][0], TWO ? qb[TWO ? c : 0][0] : 0u, qa[c][1], TWO ? qb[TWO ? c : 0][1] : 0u, codes(y, 0), codes(y, 1));
+                mma(d, qa[c][2], TWO ? qb[TWO ? c : 0][2] : 0u, qa[c][3], TWO ? qb[TWO ? c : 0][3] : 0u, codes(y, 2), codes(y, 3));
+                if constexpr (TWO) d[0] += d[2], d[1] += d[3];
+                x0 += __uint_as_float((uint32_t)s0[c] << 16) * d[0];
+                x1 += __uint_as_float((uint32_t)s0[2 * N + c] << 16) * d[1];
+            }
+            v[2 * n] = __float_as_uint(x0);
+            v[2 * n + 1] = __float_as_uint(x1);
+        }
+        if (a.cap > 0.f) fatc::tanh_each(v, pre);
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 8 * (i >> 1) + 2 * t + (i & 1);
+            x[i] = __uint_as_float(v[i]) * unit;
+            if (a.slopes != nullptr) x[i] -= slope * (float)(sh.len - 1 - key);
+            if (edge && (hidden || key < sh.lo || key >= sh.len)) x[i] = -INFINITY;
+        }
+        const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__any_sync(0xffffffffu, most > m + LAG)) {                 // the first visible keys too
+            float mx = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx = fmaxf(mx, m);
+            const float corr = m == -INFINITY ? 1.f : ex2(m - mx);     // nothing has been summed up in front of the first one
+            m = mx;
+            l *= corr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] *= corr;
+            const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);      // of heads 2 t, 2 t + 1
+#pragma unroll
+            for (int i = 0; i < 2 * N; ++i) o[i][0] *= c0, o[i][1] *= c1, o[i][2] *= c0, o[i][3] *= c1;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - base);
+        l += (x[0] + x[1]) + (x[2] + x[3]);
+        // the weights' sums of lows and sizes
+        {
+            const uint32_t p0 = pack2(x[0], x[1]), p1 = pack2(x[2], x[3]);
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(VS) + g;
+            uint32_t b0 = 0, b1 = 0;
+            if (g < 2 * N) {
+                b0 = s[2 * t * 2 * N] | (uint32_t)s[(2 * t + 1) * 2 * N] << 16;
+                b1 = s[(2 * t + 8) * 2 * N] | (uint32_t)s[(2 * t + 9) * 2 * N] << 16;
+            }
+            mma(e, p0, rest(x[0], x[1], p0), p1, rest(x[2], x[3], p1), b0, b1);
+        }
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = x[i] * __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(VS + (8 * (i >> 1) + 2 * t + (i & 1)) * (D / 8))[N + c] << 16);
+            const uint32_t h0_ = pack2(y[0], y[1]), h1_ = pack2(y[2], y[3]), r0 = rest(y[0], y[1], h0_), r1 = rest(y[2], y[3], h1_);
+            uint32_t z[4];                                             // four codes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 8 * (i >> 1) + 2 * t + (i & 1);
+                z[i] = reinterpret_cast<const uint16_t*>(V + row * (D / 2) + place(N, row, c) * 16)[g];
+            }
+            const uint32_t z0 = z[0] | z[1] << 16, z1 = z[2] | z[3] << 16;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t a0 = codes(z0, 2 * u), a1 = codes(z0, 2 * u + 1), a2 = codes(z1, 2 * u), a3 = codes(z1, 2 * u + 1);
+                mma(o[2 * c + u], a0, a1, a2, a3, h0_, h1_);
+                mma(o[2 * c + u], a0, a1, a2, a3, r0, r1);
+            }
+        }
+        __syncwarp();                                                  // the stage is read; the next issue() fills it
+    }
+    if (!alive)                                                        // after a wait that ran out: copies in flight, again within a limit
+        for (int i = j; i < min(j + STAGES, n_mine); ++i) fatc::mbar_wait_suspend(&full[w][i % STAGES], i / STAGES & 1, &drain_flag, a.err, 0x44010);
+
+    // the warps' parts meet in shared memory
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) part_m[w][g] = m, part_l[w][g] = l;
+    __syncthreads();
+    constexpr int LD = D + 4;
+    float *O = reinterpret_cast<float*>(smem), *E = O + WARPS * HEADS * LD;      // [WARPS][HEADS][LD], [WARPS][HEADS][8], over the rings
+    auto factor = [&](int head) -> float {
+        float top = part_m[0][head];
+#pragma unroll
+        for (int y = 1; y < WARPS; ++y) top = fmaxf(top, part_m[y][head]);
+        return part_m[w][head] == -INFINITY ? 0.f : ex2(part_m[w][head] - top);
+    };
+    const float f0 = factor(2 * t), f1 = factor(2 * t + 1), fg = factor(g);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        const int d = i / 2 * 32 + 4 * g + 2 * (i & 1);
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t) * LD + d) = make_float2(f0 * o[i][0], f0 * o[i][2]);
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t + 1) * LD + d) = make_float2(f1 * o[i][1], f1 * o[i][3]);
+    }
+    *reinterpret_cast<float2*>(E + (w * HEADS + g) * 8 + 2 * t) = make_float2(fg * (e[0] + e[2]), fg * (e[1] + e[3]));
+    if (threadIdx.x < HEADS) {
+        float top = part_m[0][threadIdx.x], sum = 0.f;
+#pragma unroll
+        for (int y = 1; y < WARPS; ++y) top = fmaxf(top, part_m[y][threadIdx.x]);
+#pragma unroll
+        for (int y = 0; y < WARPS; ++y) sum += part_l[y][threadIdx.x] == 0.f ? 0.f : part_l[y][threadIdx.x] * ex2(part_m[y][threadIdx.x] - top);
+        cta_m[threadIdx.x] = top;
+        cta_l[threadIdx.x] = sum;
+    }
+    __syncthreads();
+    const bool cluster = a.splits > 1 && a.splits <= MAX_CLUSTER;
+    for (int i = threadIdx.x; i < nh * (D / 4); i += WARPS * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4, c = d / 32;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float rest_ = 0.f;
+#pragma unroll
+        for (int x = 0; x < WARPS; ++x) {
+            const float4 z = load4(O + (x * HEADS + r) * LD + d);
+            y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            rest_ += E[(x * HEADS + r) * 8 + c] - 128.f * E[(x * HEADS + r) * 8 + N + c];
+        }
+        y.x += rest_; y.y += rest_; y.z += rest_; y.w += rest_;
+        const long long bh = (long long)b * a.H + h0 + r;
+        if (cluster) store4(O + r * LD + d, y);                        // (only this thread reads what lies there)
+        else if (a.splits == 1) {
+            const float inv = inverse(cta_l[r]);
+            *reinterpret_cast<uint2*>((T*)a.out + bh * D + d) = make_uint2(out2<T>(y.x * inv, y.y * inv), out2<T>(y.z * inv, y.w * inv));
+        } else {
+            store4(a.part + (bh * a.splits + split) * D + d, y);
+            if (d == 0) *reinterpret_cast<float2*>(a.ml + (bh * a.splits + split) * 2) = make_float2(cta_m[r], cta_l[r]);
+        }
+    }
+    if (!cluster) return;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (int i = split * WARPS * 32 + threadIdx.x; i < nh * (D / 4); i += a.splits * WARPS * 32) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float ms[MAX_CLUSTER], ls[MAX_CLUSTER], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+            ms[c] = c < a.splits ? *cl.map_shared_rank(&cta_m[r], c) : -INFINITY;
+            ls[c] = c < a.splits ? *cl.map_shared_rank(&cta_l[r], c) : 0.f;
+            top = fmaxf(top, ms[c]);
+        }
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+            if (ls[c] == 0.f) continue;
+            const float f = ex2(ms[c] - top);
+            const float4 z = load4(cl.map_shared_rank(O + r * LD + d, c));
+            sum += f * ls[c];
+            y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+        }
+        const float inv = inverse(sum);
+        *reinterpret_cast<uint2*>((T*)a.out + ((long long)b * a.H + h0 + r) * D + d) = make_uint2(out2<T>(y.x * inv, y.y * inv), out2<T>(y.z * inv, y.w * inv));
+    }
+    cl.sync();                                                         // the other CTAs have read this one's part
+}
+
+// The parts of a request's CTAs: a block per (request, query head), a warp per part, a lane per four numbers.
+constexpr int JOIN_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) {
+    __shared__ float4 O[JOIN_WARPS][32];
+    __shared__ float L[JOIN_WARPS];
+    pdl_wait();
+    const int bh = blockIdx.x, b = bh / a.H, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Share sh = share_of(a, b);
+    const int n = (sh.last - sh.first + sh.per - 1) / sh.per;
+    const float* ml = a.ml + (long long)bh * a.splits * 2;
+    const float* part = a.part + (long long)bh * a.splits * a.D + lane * 4;
+    const bool mine = lane * 4 < a.D;
+    float top = -INFINITY;                                             // of all parts, first: then no part waits for the one before it
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[2 * s]);
+    top = warp_max(top);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = w; s < n; s += JOIN_WARPS) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
+        const float4 y = mine ? load4(part + (long long)s * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
+        l += x.y * f;
+        o.x += y.x * f; o.y += y.y * f; o.z += y.z * f; o.w += y.w * f;
+    }
+    O[w][lane] = o;
+    if (lane == 0) L[w] = l;
+    __syncthreads();
+    if (w > 0) return;
+    float sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < JOIN_WARPS; ++x) {
+        const float4 y = O[x][lane];
+        sum += L[x];
+        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    }
+    const float inv = inverse(sum);
+    if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * a.D + lane * 4) = make_uint2(out2<T>(o.x * inv, o.y * inv), out2<T>(o.z * inv, o.w * inv));
+}
+
+template <typename T, int N>
+static int launch(const StepArgs& a, cudaStream_t st) {
+    constexpr int D = 32 * N, ring = WARPS * STAGES * 2 * GROUP * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
+    int rc = (int)cudaFuncSetAttribute(int4_step_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc) return rc;
+    const int tiles = (a.H / a.G + HEADS - 1) / HEADS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.splits, a.G * tiles, a.B);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.splits > 1 && a.splits <= MAX_CLUSTER ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, int4_step_kernel<T, N>, a);
+    rc = (int)cudaGetLastError();
+    if (rc || a.splits <= MAX_CLUSTER) return rc;
+    return launch_early(int4_join_kernel<T>, (int64_t)a.B * a.H, JOIN_WARPS * 32, st, a);
+}
+template <typename T>
+static int by_width(const StepArgs& a, cudaStream_t st) {
+    switch (a.D / 32) {
+        case 1: return launch<T, 1>(a, st);
+        case 2: return launch<T, 2>(a, st);
+        case 3: return launch<T, 3>(a, st);
+        default: return launch<T, 4>(a, st);
+    }
+}
+
+}  // namespace int4
+}  // namespace lmoe
+
+// half: fp16, else bf16.  Heads of up to 128.
+LMOE_API int lmoe_int4_step(const lmoe::int4::StepArgs* ap, int half, cudaStream_t st) {
+    using namespace lmoe::int4;
+    const StepArgs& a = *ap;
+    if (!fits(a) || a.D > 128 || (a.sorted && a.B > WARPS * 32) || (long long)a.G * ((a.H / a.G + HEADS - 1) / HEADS) > 65535 || (a.splits > MAX_CLUSTER && (a.part == nullptr || a.ml == nullptr))) return -1;
+    return half ? by_width<__half>(a, st) : by_width<lmoe::bf16>(a, st);
+}

@@ -166,7 +166,21 @@ def read_rows_int4(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Te
 
 
 # ---- attention of one token -------------------------------------------------------------------------------------------------------
+HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 16                  # csrc/int4_step.cu, .cuh
+
+
+def splits_of(B: int, G: int, heads: int, D: int, keys: int) -> Tuple[int, int]:
+    """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first): parts for one wave, of 256 keys at least."""
+    from . import cuda as K
+    work, slots = max(1, B * G * -(-heads // HEADS)), 4 * K.num_sms()
+    n = slots // work if 2 * work <= slots else 2 if work < 4 * slots else 1
+    n = min(n, -(-keys // (GROUP * MIN_GROUPS)))
+    n = MAX_CLUSTER if MAX_CLUSTER < n < 16 else max(n, 1)
+    return n, int(1 < B <= 128 and work * n > slots)
+
+
 def _step_plan(q, k_pages, v_pages, table, lengths, scale, window, softcap, slopes):
+    """(Arguments without their addresses, floats of the parts' outputs and of their maxima and sums; on the tensor cores?)"""
     if q.dim() != 3 or q.dtype not in _TYPES or q.device != k_pages.device:
         raise ValueError("queries are [B, H, D] in fp32, bf16 or fp16, where the pools lie")
     B, H, D = q.shape
@@ -177,8 +191,14 @@ def _step_plan(q, k_pages, v_pages, table, lengths, scale, window, softcap, slop
     if window is not None and window < 1:
         raise ValueError(f"a window of {window}")
     _check_scores(q, H, scale, softcap, slopes)
-    return bytes(_Step(q_b=q.stride(0), q_h=q.stride(1), table_ld=table.stride(0), B=B, H=H, G=G, D=D, page=page, pages=k_pages.shape[0], table_n=table.shape[1],
-                       window=min(int(window or 0), (1 << 31) - 1), splits=1, sorted=0, scale=float(scale) if scale is not None else D ** -0.5, cap=float(softcap or 0.0)))
+    a = _Step(q_b=q.stride(0), q_h=q.stride(1), table_ld=table.stride(0), B=B, H=H, G=G, D=D, page=page, pages=k_pages.shape[0], table_n=table.shape[1],
+              window=min(int(window or 0), (1 << 31) - 1), splits=1, sorted=0, scale=float(scale) if scale is not None else D ** -0.5, cap=float(softcap or 0.0))
+    tensor = q.dtype != torch.float32 and D <= 128 and G * -(-(H // G) // HEADS) <= 65535
+    part = 0
+    if tensor and q.is_cuda:
+        a.splits, a.sorted = splits_of(B, G, H // G, D, table.shape[1] * page)
+        part = B * H * a.splits * D if a.splits > MAX_CLUSTER else 0
+    return bytes(a), part, tensor, a.splits
 
 
 def paged_attention_int4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: Optional[int] = None, *,
@@ -190,7 +210,7 @@ def paged_attention_int4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
         _step_plan(q, k_pages, v_pages, table, lengths, scale, window, softcap, slopes)
         return R.paged_attention(q, k_pages, v_pages, table, lengths, scale, window, softcap, slopes)
     from . import cuda as K
-    plan = _planned(("step", _key(q), _key(k_pages), _key(v_pages), _key(table), _key(lengths), scale, window, softcap, _key(slopes), slopes is not None and slopes.requires_grad,
+    plan, part, tensor, splits = _planned(("step", _key(q), _key(k_pages), _key(v_pages), _key(table), _key(lengths), scale, window, softcap, _key(slopes), slopes is not None and slopes.requires_grad,
                      (k_pages.data_ptr() | v_pages.data_ptr()) % 16), lambda: _step_plan(q, k_pages, v_pages, table, lengths, scale, window, softcap, slopes))
     q, table, lengths = _flat(q), _flat(table), _flat(lengths)
     slopes = slopes if slopes is None else _flat(slopes)
@@ -202,5 +222,12 @@ def paged_attention_int4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
     a.q, a.k, a.v, a.out = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
     a.table, a.lengths, a.slopes, a.err = table.data_ptr(), lengths.data_ptr(), K._ptr(slopes), K.error_word(q.device)
     with on_device(q):
-        K._check(K.lib().lmoe_int4_step_any(ctypes.byref(a), _TYPES[q.dtype], K._st()), "int4_step_any")
+        if not tensor:
+            K._check(K.lib().lmoe_int4_step_any(ctypes.byref(a), _TYPES[q.dtype], K._st()), "int4_step_any")
+            return out
+        if part:
+            work = torch.empty(part + 2 * (part // q.shape[2]), dtype=torch.float32, device=q.device)
+            a.part = work.data_ptr()
+            a.ml = a.part + 4 * part
+        K._check(K.lib().lmoe_int4_step(ctypes.byref(a), int(q.dtype == torch.float16), K._st()), "int4_step", 1 if splits <= MAX_CLUSTER else 2)
     return out
