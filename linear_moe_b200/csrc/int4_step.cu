@@ -28,21 +28,61 @@ namespace lmoe {
 namespace int4 {
 namespace cg = cooperative_groups;
 
-constexpr int WARPS = 4, STAGES = 4, MAX_CLUSTER = 8, HEADS = 8;
+#ifndef XCTAS
+#define XCTAS 4
+#endif
+constexpr int CTAS = XCTAS, WARPS = 4, STAGES = 4, MAX_CLUSTER = 8, HEADS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 __device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ float lower(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float upper(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack2(float2 x) { return pack2(x.x, x.y); }
 // What rounding two numbers to bf16 took away, rounded itself
-__device__ __forceinline__ uint32_t rest(float x, float y, uint32_t rounded) { return pack2(x - lower(rounded), y - upper(rounded)); }
+__device__ __forceinline__ uint32_t rest(float2 x, uint32_t rounded) { return pack2(__ffma2_rn(make_float2(lower(rounded), upper(rounded)), make_float2(-1.f, -1.f), x)); }
+// Shared memory by its 32-bit addresses, with the constant part in the instruction
+template <int AT> __device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t x; asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(x) : "r"(a), "n"(AT)); return x; }
+template <int AT> __device__ __forceinline__ uint32_t lds16(uint32_t a) { uint32_t x; asm volatile("ld.shared.u16 %0, [%1+%2];" : "=r"(x) : "r"(a), "n"(AT)); return x; }
+template <int AT> __device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 x; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2+%3];" : "=r"(x.x), "=r"(x.y) : "r"(a), "n"(AT)); return x; }
+// An 8 x 8 matrix of 32-bit numbers, whose row g lies in the lanes 4 g + t, two numbers each: turned
+__device__ __forceinline__ void turn(float2 x, uint32_t& a, uint32_t& b) {
+    const uint32_t x0 = __float_as_uint(x.x), x1 = __float_as_uint(x.y);
+    uint32_t lo = __byte_perm(x0, x1, 0x5410), hi = __byte_perm(x0, x1, 0x7632);
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(lo));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(hi));
+    a = __byte_perm(lo, hi, 0x5410);
+    b = __byte_perm(lo, hi, 0x7632);
+}
+// A row's N sizes, behind its N lows
+template <int N, int AT> __device__ __forceinline__ void sizes(uint32_t row, float (&s)[N]) {
+    if constexpr (N == 4) {
+        const uint2 x = lds64<AT + 8>(row);
+        s[0] = lower(x.x), s[1] = upper(x.x), s[2] = lower(x.y), s[3] = upper(x.y);
+    } else if constexpr (N == 3) {
+        const uint32_t x = lds32<AT + 4>(row), y = lds32<AT + 8>(row);
+        s[0] = upper(x), s[1] = lower(y), s[2] = upper(y);
+    } else if constexpr (N == 2) {
+        const uint32_t x = lds32<AT + 4>(row);
+        s[0] = lower(x), s[1] = upper(x);
+    } else s[0] = upper(lds32<AT>(row));
+}
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Codes i and i + 4 of eight, as 128 + code
-__device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Codes i and i + 4 of eight, as 128 + code: one shift and one mask, whose constants stay in registers (as immediates they take a move each)
+struct Mask { uint32_t keep, set; };
+__device__ __forceinline__ Mask mask() { Mask m; asm volatile("mov.b32 %0, 0x000f000f;\nmov.b32 %1, 0x43004300;" : "=r"(m.keep), "=r"(m.set)); return m; }
+__device__ __forceinline__ uint32_t codes(uint32_t w, int i, const Mask& m) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(m.keep), "r"(m.set));
+    return x;
+}
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(tc::s32(dst)), "l"(src), "r"(bytes), "r"(tc::s32(bar)) : "memory");
 }
@@ -52,7 +92,7 @@ template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) {
 
 // N: groups of a head.  The pointers are read behind pdl_wait by plain loads: the kernel may start while the one before it runs.
 template <typename T, int N>
-__global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepArgs a) {
     constexpr bool TWO = sizeof(T) == 2 && !std::is_same<T, bf16>::value;      // queries in two parts
     constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF_STAGE = CODES + SCALES, STAGE = 2 * HALF_STAGE;      // bytes
     extern __shared__ __align__(128) unsigned char smem[];
@@ -89,13 +129,17 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
 
     unsigned char* ring = smem + w * STAGES * STAGE;
     const int n_mine = beg + w < end ? (end - beg - w + WARPS - 1) / WARPS : 0;              // groups beg + w, beg + w + WARPS, ...
-    int pages_ahead = 0, bad = 0;                                      // a lane's page number; a bit per stage whose page is none
+    int page_ahead = 0, row_ahead = 0, bad = 0;                        // of the group that is a lane's; a bit per stage whose page is none
     const long long bytes = page_bytes(a.page, D);
     auto issue = [&](int j) {
         if (j >= n_mine) return;
         const int gi = beg + w + j * WARPS, st = j % STAGES;
-        if ((j & 31) == 0) pages_ahead = j + lane < n_mine ? a.table[b * a.table_ld + (gi + lane * WARPS) * GROUP / a.page] : 0;
-        const int page = __shfl_sync(0xffffffffu, pages_ahead, j & 31), row = gi * GROUP % a.page;
+        if ((j & 31) == 0) {
+            const int key = (gi + lane * WARPS) * GROUP, at = key / a.page;
+            page_ahead = j + lane < n_mine ? a.table[b * a.table_ld + at] : 0;
+            row_ahead = key - at * a.page;
+        }
+        const int page = __shfl_sync(0xffffffffu, page_ahead, j & 31), row = __shfl_sync(0xffffffffu, row_ahead, j & 31);
         const bool there = page >= 0 && page < a.pages;
         bad = there ? bad & ~(1 << st) : bad | 1 << st;
         if (!there) {
@@ -125,7 +169,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             qa[c][i] = pack2(q[i], q[i + 4]);
-            if constexpr (TWO) qb[c][i] = rest(q[i], q[i + 4], qa[c][i]);
+            if constexpr (TWO) qb[c][i] = rest(make_float2(q[i], q[i + 4]), qa[c][i]);
             sum += q[i] + q[i + 4];
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -149,6 +193,10 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
+    // What a lane reads of a stage: of keys, rows g g + 8's words t and sizes; of values, rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9's half-words g and sizes
+    const Mask mk = mask();
+    const uint32_t at_k = g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = g * (D / 8), at_ks = at_s + 4 * t, at_v2 = 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
+    auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };
     bool alive = true;
     int j = 0;
     for (; j < n_mine; ++j) {
@@ -157,7 +205,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
         issue(j + STAGES - 1);                                         // into the stage that was read last
         alive = fatc::mbar_wait_warp(&full[w][st], j / STAGES & 1, &abort_flag, a.err, 0x44000 | st);
         if (!alive) break;
-        unsigned char *K = ring + st * STAGE, *V = K + HALF_STAGE, *KS = K + CODES, *VS = V + CODES;
+        unsigned char *K = ring + st * STAGE, *VS = K + HALF_STAGE + CODES;
         const bool edge = hidden || key0 < sh.lo || key0 + GROUP > sh.len;
         if (edge) {                                                    // hidden rows get scales of zero
             for (int i = lane; i < GROUP * N; i += 32) {
@@ -167,29 +215,38 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // ahead of the next copy into this stage
             __syncwarp();
         }
-        uint32_t v[4];                                                 // scores: keys 8 (e >> 1) + 2 t + (e & 1)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            const int row = 8 * n + g;
-            uint32_t sc = 2 * t < 2 * N ? reinterpret_cast<const uint32_t*>(KS + row * (D / 8))[t] : 0u;
-            mma(x, sums[0], sums[2], sums[1], 0u, sc, sc);
-            float x0 = x[0] + x[2], x1 = x[1] + x[3];
-            const uint16_t* s0 = reinterpret_cast<const uint16_t*>(KS + (8 * n + 2 * t) * (D / 8)) + N;
+        // (where a group of 32 numbers lies depends on the row modulo 8 alone, in rows of a power of two of bytes: an exclusive or of the address)
+        const uint32_t base_k = tc::s32(K), base_v = base_k + HALF_STAGE;
+        // Scores of rows g and g + 8, heads 2 t and 2 t + 1.  (The other way round, heads as the 16 rows: twice the products, and the rows that no head has have to be put beside every operand.)
+        float2 s0, s1;
+        {
+            const uint32_t c0 = 2 * t < 2 * N ? lds32<CODES>(base_k + at_ks) : 0u, c1 = 2 * t < 2 * N ? lds32<CODES + D>(base_k + at_ks) : 0u;
+            float x[4];
+            mma_first(x, c0, c1, c0, c1, sums[0], sums[1]);
+            mma(x, c0, c1, 0u, 0u, sums[2], 0u);
+            s0 = make_float2(x[0], x[1]), s1 = make_float2(x[2], x[3]);
+            float k0[N], k1[N];
+            sizes<N, CODES>(base_k + at_s, k0);
+            sizes<N, CODES + D>(base_k + at_s, k1);
 #pragma unroll
             for (int c = 0; c < N; ++c) {
-                const uint32_t y = reinterpret_cast<const uint32_t*>(K + row * (D / 2) + place(N, row, c) * 16)[t];
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                mma(d, qa[c][0], TWO ? qb[TWO ? c : 0][0] : 0u, qa[c][1], TWO ? qb[TWO ? c : 0][1] : 0u, codes(y, 0), codes(y, 1));
-                mma(d, qa[c][2], TWO ? qb[TWO ? c : 0][2] : 0u, qa[c][3], TWO ? qb[TWO ? c : 0][3] : 0u, codes(y, 2), codes(y, 3));
-                if constexpr (TWO) d[0] += d[2], d[1] += d[3];
-                x0 += __uint_as_float((uint32_t)s0[c] << 16) * d[0];
-                x1 += __uint_as_float((uint32_t)s0[2 * N + c] << 16) * d[1];
+                const uint32_t from = chunk(base_k + at_k, c), y = lds32<0>(from), z = lds32<4 * D>(from);
+                float d[4];
+                mma_first(d, codes(y, 0, mk), codes(z, 0, mk), codes(y, 1, mk), codes(z, 1, mk), qa[c][0], qa[c][1]);
+                mma(d, codes(y, 2, mk), codes(z, 2, mk), codes(y, 3, mk), codes(z, 3, mk), qa[c][2], qa[c][3]);
+                if constexpr (TWO) {
+                    mma(d, codes(y, 0, mk), codes(z, 0, mk), codes(y, 1, mk), codes(z, 1, mk), qb[TWO ? c : 0][0], qb[TWO ? c : 0][1]);
+                    mma(d, codes(y, 2, mk), codes(z, 2, mk), codes(y, 3, mk), codes(z, 3, mk), qb[TWO ? c : 0][2], qb[TWO ? c : 0][3]);
+                }
+                s0 = __ffma2_rn(make_float2(k0[c], k0[c]), make_float2(d[0], d[1]), s0);
+                s1 = __ffma2_rn(make_float2(k1[c], k1[c]), make_float2(d[2], d[3]), s1);
             }
-            v[2 * n] = __float_as_uint(x0);
-            v[2 * n + 1] = __float_as_uint(x1);
         }
-        if (a.cap > 0.f) fatc::tanh_each(v, pre);
+        // turned, by halves of their bits: head g, keys 8 (e >> 1) + 2 t + (e & 1)
+        uint32_t v[4];
+        turn(s0, v[0], v[1]);
+        turn(s1, v[2], v[3]);
+        if (a.cap > 0.f) fatc::tanh_of(v, pre);
         float x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -218,31 +275,29 @@ __global__ void __launch_bounds__(WARPS * 32, 4) int4_step_kernel(const StepArgs
         l += (x[0] + x[1]) + (x[2] + x[3]);
         // the weights' sums of lows and sizes
         {
-            const uint32_t p0 = pack2(x[0], x[1]), p1 = pack2(x[2], x[3]);
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(VS) + g;
+            const float2 w0 = make_float2(x[0], x[1]), w1 = make_float2(x[2], x[3]);
+            const uint32_t p0 = pack2(w0), p1 = pack2(w1);
             uint32_t b0 = 0, b1 = 0;
             if (g < 2 * N) {
-                b0 = s[2 * t * 2 * N] | (uint32_t)s[(2 * t + 1) * 2 * N] << 16;
-                b1 = s[(2 * t + 8) * 2 * N] | (uint32_t)s[(2 * t + 9) * 2 * N] << 16;
+                b0 = lds16<CODES>(base_v + at_vs) | lds16<CODES + D / 8>(base_v + at_vs) << 16;
+                b1 = lds16<CODES + D>(base_v + at_vs) | lds16<CODES + 9 * (D / 8)>(base_v + at_vs) << 16;
             }
-            mma(e, p0, rest(x[0], x[1], p0), p1, rest(x[2], x[3], p1), b0, b1);
+            mma(e, p0, rest(w0, p0), p1, rest(w1, p1), b0, b1);
         }
+        float vs[4][N];
+        sizes<N, CODES>(base_v + at_v2, vs[0]);
+        sizes<N, CODES + D / 8>(base_v + at_v2, vs[1]);
+        sizes<N, CODES + D>(base_v + at_v2, vs[2]);
+        sizes<N, CODES + 9 * (D / 8)>(base_v + at_v2, vs[3]);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = x[i] * __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(VS + (8 * (i >> 1) + 2 * t + (i & 1)) * (D / 8))[N + c] << 16);
-            const uint32_t h0_ = pack2(y[0], y[1]), h1_ = pack2(y[2], y[3]), r0 = rest(y[0], y[1], h0_), r1 = rest(y[2], y[3], h1_);
-            uint32_t z[4];                                             // four codes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 8 * (i >> 1) + 2 * t + (i & 1);
-                z[i] = reinterpret_cast<const uint16_t*>(V + row * (D / 2) + place(N, row, c) * 16)[g];
-            }
-            const uint32_t z0 = z[0] | z[1] << 16, z1 = z[2] | z[3] << 16;
+            const float2 y0 = __fmul2_rn(make_float2(x[0], x[1]), make_float2(vs[0][c], vs[1][c])), y1 = __fmul2_rn(make_float2(x[2], x[3]), make_float2(vs[2][c], vs[3][c]));
+            const uint32_t h0_ = pack2(y0), h1_ = pack2(y1), r0 = rest(y0, h0_), r1 = rest(y1, h1_);
+            // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
+            const uint32_t from = chunk(base_v + at_v, c), z0 = lds16<0>(from) | lds16<D / 2>(from) << 16, z1 = lds16<4 * D>(from) | lds16<9 * (D / 2)>(from) << 16;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t a0 = codes(z0, 2 * u), a1 = codes(z0, 2 * u + 1), a2 = codes(z1, 2 * u), a3 = codes(z1, 2 * u + 1);
+                const uint32_t a0 = codes(z0, 2 * u, mk), a1 = codes(z0, 2 * u + 1, mk), a2 = codes(z1, 2 * u, mk), a3 = codes(z1, 2 * u + 1, mk);
                 mma(o[2 * c + u], a0, a1, a2, a3, h0_, h1_);
                 mma(o[2 * c + u], a0, a1, a2, a3, r0, r1);
             }
