@@ -29,9 +29,9 @@ namespace int4 {
 namespace cg = cooperative_groups;
 
 #ifndef XCTAS
-#define XCTAS 4
+#define XCTAS 3
 #endif
-constexpr int CTAS = XCTAS, WARPS = 4, STAGES = 4, MAX_CLUSTER = 8, HEADS = 8;
+constexpr int CTAS = XCTAS, WARPS = 4, STAGES = 3, MAX_CLUSTER = 8, HEADS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 __device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
@@ -94,7 +94,7 @@ template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) {
 template <typename T, int N>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepArgs a) {
     constexpr bool TWO = sizeof(T) == 2 && !std::is_same<T, bf16>::value;      // queries in two parts
-    constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF_STAGE = CODES + SCALES, STAGE = 2 * HALF_STAGE;      // bytes
+    constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF = CODES + SCALES, PART = 2 * HALF, STAGE = 2 * PART;      // bytes: keys or values of a group, a group, two
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
     __shared__ float part_m[WARPS][HEADS], part_l[WARPS][HEADS], cta_m[HEADS], cta_l[HEADS];
@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         lens[threadIdx.x] = mine;
         __syncthreads();
         int rank = 0;
-        for (int i = 0; i < a.B; ++i) rank += lens[i] > mine || (lens[i] == mine && i < threadIdx.x);
+        if (w * 32 < a.B)
+            for (int i = 0; i < a.B; ++i) rank += lens[i] > mine || (lens[i] == mine && i < threadIdx.x);
         if (threadIdx.x < a.B && rank == blockIdx.z) chosen = threadIdx.x;
         __syncthreads();
         b = chosen;
@@ -128,30 +129,39 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     if (beg >= end && a.splits > MAX_CLUSTER) return;                  // (a cluster's CTAs all stay, and one of them writes zeros where there is nothing to see)
 
     unsigned char* ring = smem + w * STAGES * STAGE;
-    const int n_mine = beg + w < end ? (end - beg - w + WARPS - 1) / WARPS : 0;              // groups beg + w, beg + w + WARPS, ...
-    int page_ahead = 0, row_ahead = 0, bad = 0;                        // of the group that is a lane's; a bit per stage whose page is none
-    const long long bytes = page_bytes(a.page, D);
+    // Pairs of groups: beg + 2 w, beg + 2 (w + WARPS), ...; the last one may have no second group
+    const int n_mine = beg + 2 * w < end ? (end - beg - 2 * w + 2 * WARPS - 1) / (2 * WARPS) : 0;
+    long long page_ahead = 0;                                          // where the page and head lie of the group that is a lane's, 16 pairs at a time; -1: not there
+    int row_ahead = 0;
+    uint32_t have = 0;                                                 // two bits per stage: the groups that are there
+    // a lane's copy: codes or scales, of keys or of values, of the first or the second group
+    const unsigned char* from = (lane & 2 ? a.v : a.k) + (lane & 1 ? (long long)a.page * (D / 2) : 0);
+    const int row_bytes = lane & 1 ? D / 8 : D / 2;
+    unsigned char* to = ring + (lane >> 2) * PART + (lane >> 1 & 1) * HALF + (lane & 1) * CODES;
     auto issue = [&](int j) {
         if (j >= n_mine) return;
-        const int gi = beg + w + j * WARPS, st = j % STAGES;
-        if ((j & 31) == 0) {
-            const int key = (gi + lane * WARPS) * GROUP, at = key / a.page;
-            page_ahead = j + lane < n_mine ? a.table[b * a.table_ld + at] : 0;
-            row_ahead = key - at * a.page;
+        const int st = j % STAGES;
+        if ((j & 15) == 0) {
+            const int gi = beg + 2 * (w + (j + (lane >> 1)) * WARPS) + (lane & 1);
+            page_ahead = -1;
+            if (gi < end) {
+                const int at = gi * GROUP / a.page, page = a.table[b * a.table_ld + at];
+                row_ahead = gi * GROUP - at * a.page;
+                if (page >= 0 && page < a.pages) page_ahead = ((long long)page * a.G + hk) * page_bytes(a.page, D);
+                else atomicCAS(a.err, 0, 0x43000);
+            }
         }
-        const int page = __shfl_sync(0xffffffffu, page_ahead, j & 31), row = __shfl_sync(0xffffffffu, row_ahead, j & 31);
-        const bool there = page >= 0 && page < a.pages;
-        bad = there ? bad & ~(1 << st) : bad | 1 << st;
-        if (!there) {
-            if (lane == 0) atomicCAS(a.err, 0, 0x43000), tc::mbar_arrive(&full[w][st]);
-            return;
+        const int src = 2 * (j & 15) + (lane >> 2 & 1);
+        const long long page = __shfl_sync(0xffffffffu, page_ahead, src);
+        const int row = __shfl_sync(0xffffffffu, row_ahead, src);
+        const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0) & 0x11u;      // bits 0 and 4
+        have = (have & ~(3u << (2 * st))) | ((groups | groups >> 3) & 3u) << (2 * st);
+        if (lane == 0) {
+            if (groups) tc::mbar_expect_tx(&full[w][st], groups == 0x11u ? STAGE : PART);
+            else tc::mbar_arrive(&full[w][st]);
         }
-        if (lane == 0) tc::mbar_expect_tx(&full[w][st], STAGE);
         __syncwarp();
-        if (lane < 4) {                                                // codes and scales of keys, and of values
-            const unsigned char* from = (lane < 2 ? a.k : a.v) + ((long long)page * a.G + hk) * bytes + (lane & 1 ? a.page * (D / 2) + row * (D / 8) : row * (D / 2));
-            bulk_load(ring + st * STAGE + (lane >> 1) * HALF_STAGE + (lane & 1) * CODES, from, lane & 1 ? SCALES : CODES, &full[w][st]);
-        }
+        if (lane < 8 && page >= 0) bulk_load(to + st * STAGE, from + page + row * row_bytes, lane & 1 ? SCALES : CODES, &full[w][st]);
     };
 #pragma unroll
     for (int j = 0; j < STAGES - 1; ++j) issue(j);
@@ -164,7 +174,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     for (int c = 0; c < N; ++c) {
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = there ? val(((const T*)a.q)[b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t + i]) : 0.f;
+        for (int i = 0; i < 8; ++i) q[i] = 0.f;
+        const T* row = (const T*)a.q + b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t;
+        if (there && a.q_rows) load8(row, q);
+        else if (there)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = val(row[i]);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -200,37 +215,38 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     bool alive = true;
     int j = 0;
     for (; j < n_mine; ++j) {
-        const int st = j % STAGES, key0 = (beg + w + j * WARPS) * GROUP;
-        const bool hidden = bad >> st & 1;
+        const int st = j % STAGES, key0 = (beg + 2 * (w + j * WARPS)) * GROUP;
+        const uint32_t groups = have >> (2 * st) & 3u;
         issue(j + STAGES - 1);                                         // into the stage that was read last
         alive = fatc::mbar_wait_warp(&full[w][st], j / STAGES & 1, &abort_flag, a.err, 0x44000 | st);
         if (!alive) break;
-        unsigned char *K = ring + st * STAGE, *VS = K + HALF_STAGE + CODES;
-        const bool edge = hidden || key0 < sh.lo || key0 + GROUP > sh.len;
+        unsigned char* stage = ring + st * STAGE;
+        const bool edge = groups != 3u || key0 < sh.lo || key0 + 2 * GROUP > sh.len;
+        auto seen = [&](int key) -> bool { return (groups >> ((key - key0) / GROUP) & 1u) && key >= sh.lo && key < sh.len; };
         if (edge) {                                                    // hidden rows get scales of zero
-            for (int i = lane; i < GROUP * N; i += 32) {
-                const int key = key0 + i / N;
-                if (hidden || key < sh.lo || key >= sh.len) reinterpret_cast<uint32_t*>(VS)[i] = 0;
-            }
+            for (int i = lane; i < 2 * GROUP * N; i += 32)
+                if (!seen(key0 + i / N)) reinterpret_cast<uint32_t*>(stage + i / (GROUP * N) * PART + HALF + CODES)[i % (GROUP * N)] = 0;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // ahead of the next copy into this stage
             __syncwarp();
         }
         // (where a group of 32 numbers lies depends on the row modulo 8 alone, in rows of a power of two of bytes: an exclusive or of the address)
-        const uint32_t base_k = tc::s32(K), base_v = base_k + HALF_STAGE;
-        // Scores of rows g and g + 8, heads 2 t and 2 t + 1.  (The other way round, heads as the 16 rows: twice the products, and the rows that no head has have to be put beside every operand.)
-        float2 s0, s1;
-        {
-            const uint32_t c0 = 2 * t < 2 * N ? lds32<CODES>(base_k + at_ks) : 0u, c1 = 2 * t < 2 * N ? lds32<CODES + D>(base_k + at_ks) : 0u;
+        const uint32_t base = tc::s32(stage);
+        uint32_t v[8];                                                 // scores: head g, keys 8 (e >> 1) + 2 t + (e & 1)
+        // Scores of rows g and g + 8 of a group, heads 2 t and 2 t + 1.  (The other way round, heads as the 16 rows: twice the products, and the rows that no head has have to be put beside every operand.)
+        auto scores = [&](auto which) {
+            constexpr int AT = decltype(which)::value * PART, E = decltype(which)::value * 4;
+            float2 s0, s1;
+            const uint32_t c0 = 2 * t < 2 * N ? lds32<AT + CODES>(base + at_ks) : 0u, c1 = 2 * t < 2 * N ? lds32<AT + CODES + D>(base + at_ks) : 0u;
             float x[4];
             mma_first(x, c0, c1, c0, c1, sums[0], sums[1]);
             mma(x, c0, c1, 0u, 0u, sums[2], 0u);
             s0 = make_float2(x[0], x[1]), s1 = make_float2(x[2], x[3]);
             float k0[N], k1[N];
-            sizes<N, CODES>(base_k + at_s, k0);
-            sizes<N, CODES + D>(base_k + at_s, k1);
+            sizes<N, AT + CODES>(base + at_s, k0);
+            sizes<N, AT + CODES + D>(base + at_s, k1);
 #pragma unroll
             for (int c = 0; c < N; ++c) {
-                const uint32_t from = chunk(base_k + at_k, c), y = lds32<0>(from), z = lds32<4 * D>(from);
+                const uint32_t row = chunk(base + at_k, c), y = lds32<AT>(row), z = lds32<AT + 4 * D>(row);
                 float d[4];
                 mma_first(d, codes(y, 0, mk), codes(z, 0, mk), codes(y, 1, mk), codes(z, 1, mk), qa[c][0], qa[c][1]);
                 mma(d, codes(y, 2, mk), codes(z, 2, mk), codes(y, 3, mk), codes(z, 3, mk), qa[c][2], qa[c][3]);
@@ -241,21 +257,25 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
                 s0 = __ffma2_rn(make_float2(k0[c], k0[c]), make_float2(d[0], d[1]), s0);
                 s1 = __ffma2_rn(make_float2(k1[c], k1[c]), make_float2(d[2], d[3]), s1);
             }
-        }
-        // turned, by halves of their bits: head g, keys 8 (e >> 1) + 2 t + (e & 1)
-        uint32_t v[4];
-        turn(s0, v[0], v[1]);
-        turn(s1, v[2], v[3]);
+            turn(s0, v[E], v[E + 1]);                                  // by halves of their bits
+            turn(s1, v[E + 2], v[E + 3]);
+        };
+        scores(std::integral_constant<int, 0>());
+        scores(std::integral_constant<int, 1>());
         if (a.cap > 0.f) fatc::tanh_of(v, pre);
-        float x[4];
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 8 * (i >> 1) + 2 * t + (i & 1);
-            x[i] = __uint_as_float(v[i]) * unit;
-            if (a.slopes != nullptr) x[i] -= slope * (float)(sh.len - 1 - key);
-            if (edge && (hidden || key < sh.lo || key >= sh.len)) x[i] = -INFINITY;
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[i]) * unit;
+        if (a.slopes != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] -= slope * (float)(sh.len - 1 - (key0 + 8 * (i >> 1) + 2 * t + (i & 1)));
         }
-        const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!seen(key0 + 8 * (i >> 1) + 2 * t + (i & 1))) x[i] = -INFINITY;
+        }
+        const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any_sync(0xffffffffu, most > m + LAG)) {                 // the first visible keys too
             float mx = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -269,39 +289,43 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
             for (int i = 0; i < 2 * N; ++i) o[i][0] *= c0, o[i][1] *= c1, o[i][2] *= c0, o[i][3] *= c1;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float low = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - base);
-        l += (x[0] + x[1]) + (x[2] + x[3]);
-        // the weights' sums of lows and sizes
-        {
-            const float2 w0 = make_float2(x[0], x[1]), w1 = make_float2(x[2], x[3]);
-            const uint32_t p0 = pack2(w0), p1 = pack2(w1);
-            uint32_t b0 = 0, b1 = 0;
-            if (g < 2 * N) {
-                b0 = lds16<CODES>(base_v + at_vs) | lds16<CODES + D / 8>(base_v + at_vs) << 16;
-                b1 = lds16<CODES + D>(base_v + at_vs) | lds16<CODES + 9 * (D / 8)>(base_v + at_vs) << 16;
+        for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - low);
+        l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        auto values = [&](auto which) {
+            constexpr int AT = decltype(which)::value * PART + HALF, S = AT + CODES, E = decltype(which)::value * 4;
+            const float2 w0 = make_float2(x[E], x[E + 1]), w1 = make_float2(x[E + 2], x[E + 3]);
+            {                                                          // the weights' sums of lows and sizes
+                const uint32_t p0 = pack2(w0), p1 = pack2(w1);
+                uint32_t b0 = 0, b1 = 0;
+                if (g < 2 * N) {
+                    b0 = lds16<S>(base + at_vs) | lds16<S + D / 8>(base + at_vs) << 16;
+                    b1 = lds16<S + D>(base + at_vs) | lds16<S + 9 * (D / 8)>(base + at_vs) << 16;
+                }
+                mma(e, p0, rest(w0, p0), p1, rest(w1, p1), b0, b1);
             }
-            mma(e, p0, rest(w0, p0), p1, rest(w1, p1), b0, b1);
-        }
-        float vs[4][N];
-        sizes<N, CODES>(base_v + at_v2, vs[0]);
-        sizes<N, CODES + D / 8>(base_v + at_v2, vs[1]);
-        sizes<N, CODES + D>(base_v + at_v2, vs[2]);
-        sizes<N, CODES + 9 * (D / 8)>(base_v + at_v2, vs[3]);
+            float vs[4][N];
+            sizes<N, S>(base + at_v2, vs[0]);
+            sizes<N, S + D / 8>(base + at_v2, vs[1]);
+            sizes<N, S + D>(base + at_v2, vs[2]);
+            sizes<N, S + 9 * (D / 8)>(base + at_v2, vs[3]);
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-            const float2 y0 = __fmul2_rn(make_float2(x[0], x[1]), make_float2(vs[0][c], vs[1][c])), y1 = __fmul2_rn(make_float2(x[2], x[3]), make_float2(vs[2][c], vs[3][c]));
-            const uint32_t h0_ = pack2(y0), h1_ = pack2(y1), r0 = rest(y0, h0_), r1 = rest(y1, h1_);
-            // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
-            const uint32_t from = chunk(base_v + at_v, c), z0 = lds16<0>(from) | lds16<D / 2>(from) << 16, z1 = lds16<4 * D>(from) | lds16<9 * (D / 2)>(from) << 16;
+            for (int c = 0; c < N; ++c) {
+                const float2 y0 = __fmul2_rn(w0, make_float2(vs[0][c], vs[1][c])), y1 = __fmul2_rn(w1, make_float2(vs[2][c], vs[3][c]));
+                const uint32_t p0 = pack2(y0), p1 = pack2(y1), r0 = rest(y0, p0), r1 = rest(y1, p1);
+                // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
+                const uint32_t row = chunk(base + at_v, c), z0 = lds16<AT>(row) | lds16<AT + D / 2>(row) << 16, z1 = lds16<AT + 4 * D>(row) | lds16<AT + 9 * (D / 2)>(row) << 16;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t a0 = codes(z0, 2 * u, mk), a1 = codes(z0, 2 * u + 1, mk), a2 = codes(z1, 2 * u, mk), a3 = codes(z1, 2 * u + 1, mk);
-                mma(o[2 * c + u], a0, a1, a2, a3, h0_, h1_);
-                mma(o[2 * c + u], a0, a1, a2, a3, r0, r1);
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t a0 = codes(z0, 2 * u, mk), a1 = codes(z0, 2 * u + 1, mk), a2 = codes(z1, 2 * u, mk), a3 = codes(z1, 2 * u + 1, mk);
+                    mma(o[2 * c + u], a0, a1, a2, a3, p0, p1);
+                    mma(o[2 * c + u], a0, a1, a2, a3, r0, r1);
+                }
             }
-        }
+        };
+        values(std::integral_constant<int, 0>());
+        values(std::integral_constant<int, 1>());
         __syncwarp();                                                  // the stage is read; the next issue() fills it
     }
     if (!alive)                                                        // after a wait that ran out: copies in flight, again within a limit
@@ -431,7 +455,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) 
 
 template <typename T, int N>
 static int launch(const StepArgs& a, cudaStream_t st) {
-    constexpr int D = 32 * N, ring = WARPS * STAGES * 2 * GROUP * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
+    constexpr int D = 32 * N, ring = WARPS * STAGES * 4 * GROUP * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
     int rc = (int)cudaFuncSetAttribute(int4_step_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc) return rc;
     const int tiles = (a.H / a.G + HEADS - 1) / HEADS;

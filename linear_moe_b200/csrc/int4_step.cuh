@@ -14,12 +14,13 @@ struct StepArgs {
     const int *table, *lengths;           // [B, table_n], [B]
     long long q_b, q_h, table_ld;
     int B, H, G, D, page, pages, table_n, window, splits;
+    int q_rows;                           // queries on 16-byte boundaries
     int sorted;                           // more CTAs than fit at once: the longest requests come first
     float scale, cap;                     // cap 0: none
     int* err;
 };
 
-constexpr int GROUP = 16, MIN_GROUPS = 16;              // keys of a group; groups that a CTA has at least when a request is split
+constexpr int GROUP = 16, MIN_GROUPS = 8;               // keys of a group; groups that a CTA has at least when a request is split
 
 // The groups of 16 keys that a request's CTAs share: CTA s has [first + s per, first + (s + 1) per) of [first, last).
 struct Share { int len, lo, first, last, per; };

@@ -31,7 +31,7 @@ class _Rows(ctypes.Structure):
 
 class _Step(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "part", "ml", "slopes", "table", "lengths")] + [(n, ctypes.c_longlong) for n in ("q_b", "q_h", "table_ld")] +
-                [(n, ctypes.c_int) for n in ("B", "H", "G", "D", "page", "pages", "table_n", "window", "splits", "sorted")] +
+                [(n, ctypes.c_int) for n in ("B", "H", "G", "D", "page", "pages", "table_n", "window", "splits", "q_rows", "sorted")] +
                 [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("err", ctypes.c_void_p)])
 
 
@@ -166,13 +166,13 @@ def read_rows_int4(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Te
 
 
 # ---- attention of one token -------------------------------------------------------------------------------------------------------
-HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 16                  # csrc/int4_step.cu, .cuh
+HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 8                  # csrc/int4_step.cu, .cuh
 
 
 def splits_of(B: int, G: int, heads: int, D: int, keys: int) -> Tuple[int, int]:
-    """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first): parts for one wave, of 256 keys at least."""
+    """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first): parts for one wave, of 128 keys at least."""
     from . import cuda as K
-    work, slots = max(1, B * G * -(-heads // HEADS)), 4 * K.num_sms()
+    work, slots = max(1, B * G * -(-heads // HEADS)), 3 * K.num_sms()
     n = slots // work if 2 * work <= slots else 2 if work < 4 * slots else 1
     n = min(n, -(-keys // (GROUP * MIN_GROUPS)))
     n = MAX_CLUSTER if MAX_CLUSTER < n < 16 else max(n, 1)
@@ -219,6 +219,7 @@ def paged_attention_int4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
         return out
     a = _Step.from_buffer_copy(plan)
     a.q_b, a.q_h, a.table_ld = q.stride(0), q.stride(1), table.stride(0)
+    a.q_rows = int(q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0)
     a.q, a.k, a.v, a.out = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
     a.table, a.lengths, a.slopes, a.err = table.data_ptr(), lengths.data_ptr(), K._ptr(slopes), K.error_word(q.device)
     with on_device(q):
