@@ -2,12 +2,14 @@
 //   x_j = cap tanh(scale q k_j / cap) - slope_h (n - 1 - j),   o = sum_j softmax_j(x_j) v_j   over the keys  max(0, n - window) <= j < n
 //
 // Bound by reading the visible rows once, 5/8 byte a number.  That is less than a third of what bf16 rows take, so a key has to be worked through in a third of the time, and what is spent on it is the
-// conversion of codes; they go to the tensor cores as they are, two at a time by one mask: 128 + code is a bf16 number whose lowest bits are the code.  With t = 128 + code
-//   q k_j = sum_c size_jc (q t_j)_c + sum_c (low_jc - 128 size_jc) Q_c        c: groups of 32, Q_c the query's sum over the group
-//   o = sum_j (p_j size_jc) t_j + sum_j p_j (low_jc - 128 size_jc)
-// The first sums are products of 16-bit numbers with one result per group of a row (keys: 8 at a time, the heads are the 16 rows of an m16n8k16 product; values: 16 numbers of a group at a time, the heads are
-// its 8 columns).  The second ones are one small product each, whose other operand is the row's lows and sizes as they lie in the cache.  Q in three bf16 parts, p and p size in two, fp16 queries in two (rows 8 to
-// 15 of the products, which no head has).
+// conversion of codes; they go to the tensor cores as they are, two at a time by one mask: a code in the lowest bits of an fp16 number is code 2^-24, the next one above it 16 code 2^-24 (both exact: numbers below
+// 2^-13 are 2^-24 apart).  So
+//   q k_j = sum_c size_jc (q code_j)_c + sum_c low_jc Q_c        c: groups of 32, Q_c the query's sum over the group
+//   o = sum_j (p_j size_jc) code_j + sum_j p_j low_jc
+// The first sums are products of fp16 numbers with one result per group of a row (keys: 16 rows at a time, the heads are the 8 columns of an m16n8k16 product; values: 16 numbers of a group at a time).  The
+// second ones are one small product each of bf16 numbers, whose other operand is the row's lows as they lie in the cache; Q in three parts, p in two.
+// Queries go in scaled by a power of two per head, which fp16 holds exactly but for what is below 2^-35 of the head's largest number.  p size is rounded to 11 bits, for fp16 outputs to 22 (a second product); a power of
+// two per warp keeps it at 2^15 at most, where p is 1 and size the largest one seen at 2^7 (fp16 tells 2^-24 apart there).
 //
 // A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys; a warp takes every fourth group of 16 keys and has a ring of its own, which bulk copies fill (a lane per copy), so no warp waits
 // for another one until the end.  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
@@ -28,10 +30,13 @@ namespace lmoe {
 namespace int4 {
 namespace cg = cooperative_groups;
 
-#ifndef XCTAS
-#define XCTAS 3
+#ifndef XST
+#define XST 2
 #endif
-constexpr int CTAS = XCTAS, WARPS = 4, STAGES = 3, MAX_CLUSTER = 8, HEADS = 8;
+#ifndef XCTAS
+#define XCTAS 4
+#endif
+constexpr int CTAS = XCTAS, WARPS = 4, STAGES = XST, MAX_CLUSTER = 8, HEADS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 __device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
@@ -53,36 +58,52 @@ __device__ __forceinline__ void turn(float2 x, uint32_t& a, uint32_t& b) {
     a = __byte_perm(lo, hi, 0x5410);
     b = __byte_perm(lo, hi, 0x7632);
 }
-// A row's N sizes, behind its N lows
-template <int N, int AT> __device__ __forceinline__ void sizes(uint32_t row, float (&s)[N]) {
+// A row's N sizes, behind its N lows; with `most`: the largest ones of two columns so far, as bits
+template <int N, int AT> __device__ __forceinline__ void sizes(uint32_t row, float (&s)[N], uint32_t* most = nullptr) {
     if constexpr (N == 4) {
         const uint2 x = lds64<AT + 8>(row);
+        if (most) *most = __vimax3_u16x2(*most, x.x, x.y);
         s[0] = lower(x.x), s[1] = upper(x.x), s[2] = lower(x.y), s[3] = upper(x.y);
     } else if constexpr (N == 3) {
         const uint32_t x = lds32<AT + 4>(row), y = lds32<AT + 8>(row);
+        if (most) *most = __vimax3_u16x2(*most, x & 0xffff0000u, y);
         s[0] = upper(x), s[1] = lower(y), s[2] = upper(y);
     } else if constexpr (N == 2) {
         const uint32_t x = lds32<AT + 4>(row);
+        if (most) *most = __vmaxu2(*most, x);
         s[0] = lower(x), s[1] = upper(x);
-    } else s[0] = upper(lds32<AT>(row));
+    } else {
+        const uint32_t x = lds32<AT>(row);
+        if (most) *most = __vmaxu2(*most, x & 0xffff0000u);
+        s[0] = upper(x);
+    }
 }
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// Codes i and i + 4 of eight, as 128 + code: one shift and one mask, whose constants stay in registers (as immediates they take a move each)
-struct Mask { uint32_t keep, set; };
-__device__ __forceinline__ Mask mask() { Mask m; asm volatile("mov.b32 %0, 0x000f000f;\nmov.b32 %1, 0x43004300;" : "=r"(m.keep), "=r"(m.set)); return m; }
-__device__ __forceinline__ uint32_t codes(uint32_t w, int i, const Mask& m) {
-    uint32_t x;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * i)), "r"(m.keep), "r"(m.set));
-    return x;
+// Codes 0 and 4 of eight as fp16 numbers, in units of 2^-24; codes 1 and 5, in units of 2^-20 (2 and 6, 3 and 7: of w >> 8)
+__device__ __forceinline__ uint32_t even(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t odd(uint32_t w) { return w & 0x00f000f0u; }
+__device__ __forceinline__ uint32_t pack16(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t rest16(float2 x, uint32_t rounded) {
+    const float2 r = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&rounded)), make_float2(-1.f, -1.f), x);
+    return pack16(r.x, r.y);
 }
+__device__ __forceinline__ float two_to(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }      // -126 <= n <= 127
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" :: "r"(tc::s32(dst)), "l"(src), "r"(bytes), "r"(tc::s32(bar)) : "memory");
 }
@@ -93,7 +114,7 @@ template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) {
 // N: groups of a head.  The pointers are read behind pdl_wait by plain loads: the kernel may start while the one before it runs.
 template <typename T, int N>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepArgs a) {
-    constexpr bool TWO = sizeof(T) == 2 && !std::is_same<T, bf16>::value;      // queries in two parts
+    constexpr bool TWO = !std::is_same<T, bf16>::value;                // p size in two parts
     constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF = CODES + SCALES, PART = 2 * HALF, STAGE = 2 * PART;      // bytes: keys or values of a group, a group, two
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
@@ -166,50 +187,63 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
     for (int j = 0; j < STAGES - 1; ++j) issue(j);
 
-    // Queries: a lane's numbers 8 t .. 8 t + 7 of every group, in the order of `codes`; row g the head, row g + 8 what its rounding took away
-    uint32_t qa[N][4], qb[TWO ? N : 1][4], sums[3] = {0, 0, 0};
+    // Queries: a lane's numbers 8 t .. 8 t + 7 of every group of head g, in the order of the codes, scaled by a power of two; beside the rows' lows their sums, in three parts
+    uint32_t qa[N][4], sums[3] = {0, 0, 0};
     const bool there = g < nh;
     const float slope = there && a.slopes != nullptr ? a.slopes[h0 + g] * LOG2E : 0.f;
+    float unit_q;                                                      // of the scores
+    {
+        float q[N][8], most = 0.f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-        float q[8];
+        for (int c = 0; c < N; ++c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = 0.f;
-        const T* row = (const T*)a.q + b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t;
-        if (there && a.q_rows) load8(row, q);
-        else if (there)
+            for (int i = 0; i < 8; ++i) q[c][i] = 0.f;
+            const T* row = (const T*)a.q + b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t;
+            if (there && a.q_rows) load8(row, q[c]);
+            else if (there)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = val(row[i]);
-        float sum = 0.f;
+                for (int i = 0; i < 8; ++i) q[c][i] = val(row[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            qa[c][i] = pack2(q[i], q[i + 4]);
-            if constexpr (TWO) qb[c][i] = rest(make_float2(q[i], q[i + 4]), qa[c][i]);
-            sum += q[i] + q[i + 4];
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(q[c][i]));
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        // beside a row's lows (numbers c) and sizes (N + c), in three parts
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int top = most > 0.f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 116) : 0;      // up to 2^15, the odd codes' numbers up to 2^11
+        const float scale = two_to(14 - top);
+        unit_q = two_to(10 + top);
+        const float back = two_to(-10 - top);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = c + i * N;
-            if (at / 2 != t) continue;
-            float x = i ? -128.f * sum : sum;
+        for (int c = 0; c < N; ++c) {
+            float sum = 0.f;
 #pragma unroll
-            for (int y = 0; y < 3; ++y) {
-                const uint32_t part = pack2(x, 0.f);
-                sums[y] |= part << (at & 1 ? 16 : 0);
-                x -= lower(part);
+            for (int i = 0; i < 4; ++i) {
+                qa[c][i] = pack16(q[c][i] * (i & 1 ? scale * 0.0625f : scale), q[c][i + 4] * (i & 1 ? scale * 0.0625f : scale));
+                sum += q[c][i] * back + q[c][i + 4] * back;
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (c / 2 == t) {
+#pragma unroll
+                for (int y = 0; y < 3; ++y) {
+                    const uint32_t part = pack2(sum, 0.f);
+                    sums[y] |= part << (c & 1 ? 16 : 0);
+                    sum -= lower(part);
+                }
             }
         }
     }
-    const float pre = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap = a.cap * LOG2E, unit = a.cap > 0.f ? cap : pre;
-    float m = -INFINITY, l = 0.f, o[2 * N][4], e[4] = {0.f, 0.f, 0.f, 0.f};      // o: numbers 4 g + 2 u, 4 g + 2 u + 1 of group c, heads 2 t, 2 t + 1;  e: head g, numbers 2 t, 2 t + 1 of the scales
+    const float pre = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * unit_q, unit = a.cap > 0.f ? a.cap * LOG2E : pre;      // (scores of head g)
+    // Weights are 2^(score - m + shift), with which p size is at most 2^(LAG + 7) where no size is above 2^(7 - shift).  Beyond 2^20 and below 2^-20 the sizes are scaled by 2^wide as well: the sums of weights
+    // and of weights times lows have to stay within fp32.
+    float m = -INFINITY, l = 0.f, shift = 7.f;
+    int wide = 0;
+    uint32_t bound = 0;                                                // the power of two that no size so far is above, as the upper bits of a bf16 number, twice
+    // o: numbers 4 g + 2 u, 4 g + 2 u + 1 (times 16) of group c, heads 2 t, 2 t + 1;  e: head g, numbers 2 t, 2 t + 1 of the scales
+    float o[2 * N][4], e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     // What a lane reads of a stage: of keys, rows g g + 8's words t and sizes; of values, rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9's half-words g and sizes
-    const Mask mk = mask();
     const uint32_t at_k = g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = g * (D / 8), at_ks = at_s + 4 * t, at_v2 = 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
     auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };
     bool alive = true;
@@ -236,7 +270,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         auto scores = [&](auto which) {
             constexpr int AT = decltype(which)::value * PART, E = decltype(which)::value * 4;
             float2 s0, s1;
-            const uint32_t c0 = 2 * t < 2 * N ? lds32<AT + CODES>(base + at_ks) : 0u, c1 = 2 * t < 2 * N ? lds32<AT + CODES + D>(base + at_ks) : 0u;
+            const uint32_t c0 = 2 * t < N ? lds32<AT + CODES>(base + at_ks) : 0u, c1 = 2 * t < N ? lds32<AT + CODES + D>(base + at_ks) : 0u;
             float x[4];
             mma_first(x, c0, c1, c0, c1, sums[0], sums[1]);
             mma(x, c0, c1, 0u, 0u, sums[2], 0u);
@@ -248,12 +282,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             for (int c = 0; c < N; ++c) {
                 const uint32_t row = chunk(base + at_k, c), y = lds32<AT>(row), z = lds32<AT + 4 * D>(row);
                 float d[4];
-                mma_first(d, codes(y, 0, mk), codes(z, 0, mk), codes(y, 1, mk), codes(z, 1, mk), qa[c][0], qa[c][1]);
-                mma(d, codes(y, 2, mk), codes(z, 2, mk), codes(y, 3, mk), codes(z, 3, mk), qa[c][2], qa[c][3]);
-                if constexpr (TWO) {
-                    mma(d, codes(y, 0, mk), codes(z, 0, mk), codes(y, 1, mk), codes(z, 1, mk), qb[TWO ? c : 0][0], qb[TWO ? c : 0][1]);
-                    mma(d, codes(y, 2, mk), codes(z, 2, mk), codes(y, 3, mk), codes(z, 3, mk), qb[TWO ? c : 0][2], qb[TWO ? c : 0][3]);
-                }
+                mma16_first(d, even(y), even(z), odd(y), odd(z), qa[c][0], qa[c][1]);
+                mma16(d, even(y >> 8), even(z >> 8), odd(y >> 8), odd(z >> 8), qa[c][2], qa[c][3]);
                 s0 = __ffma2_rn(make_float2(k0[c], k0[c]), make_float2(d[0], d[1]), s0);
                 s1 = __ffma2_rn(make_float2(k1[c], k1[c]), make_float2(d[2], d[3]), s1);
             }
@@ -275,52 +305,71 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             for (int i = 0; i < 8; ++i)
                 if (!seen(key0 + 8 * (i >> 1) + 2 * t + (i & 1))) x[i] = -INFINITY;
         }
+        float vs[8][N];                                                // sizes of the values of keys 8 (e >> 1) + 2 t + (e & 1)
+        uint32_t largest = 0;
+        sizes<N, HALF + CODES>(base + at_v2, vs[0], &largest);
+        sizes<N, HALF + CODES + D / 8>(base + at_v2, vs[1], &largest);
+        sizes<N, HALF + CODES + D>(base + at_v2, vs[2], &largest);
+        sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2, vs[3], &largest);
+        sizes<N, PART + HALF + CODES>(base + at_v2, vs[4], &largest);
+        sizes<N, PART + HALF + CODES + D / 8>(base + at_v2, vs[5], &largest);
+        sizes<N, PART + HALF + CODES + D>(base + at_v2, vs[6], &largest);
+        sizes<N, PART + HALF + CODES + 9 * (D / 8)>(base + at_v2, vs[7], &largest);
         const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__any_sync(0xffffffffu, most > m + LAG)) {                 // the first visible keys too
+        if (__any_sync(0xffffffffu, most > m + LAG || __vmaxu2(largest, bound) != bound)) {      // the first visible keys too
             float mx = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             mx = fmaxf(mx, m);
-            const float corr = m == -INFINITY ? 1.f : ex2(m - mx);     // nothing has been summed up in front of the first one
-            m = mx;
+            const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(largest & 0xffffu, largest >> 16), bound >> 16));
+            const int power = top == 0 ? 0 : (int)((top + 0x7fu) >> 7) - 127, kept = min(max(power, -20), 20);      // no size is above 2^power
+            bound = min(top + 0x7fu, 0x7f80u) & 0xff80u;
+            bound |= bound << 16;
+            const float shift_now = 7.f - (float)kept;
+            const float corr = m == -INFINITY ? 1.f : ex2(m - mx + (shift_now - shift));      // nothing has been summed up in front of the first one
+            const float corr_o = corr * two_to(max(-126, kept - power - wide));
+            m = mx, shift = shift_now, wide = kept - power;
             l *= corr;
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] *= corr;
-            const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);      // of heads 2 t, 2 t + 1
+            const float c0 = __shfl_sync(0xffffffffu, corr_o, 8 * t), c1 = __shfl_sync(0xffffffffu, corr_o, 8 * t + 4);      // of heads 2 t, 2 t + 1
 #pragma unroll
             for (int i = 0; i < 2 * N; ++i) o[i][0] *= c0, o[i][1] *= c1, o[i][2] *= c0, o[i][3] *= c1;
         }
-        const float low = m == -INFINITY ? 0.f : m;
+        if (wide != 0) {
+            const float f = two_to(wide);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < N; ++c) vs[i][c] *= f;
+        }
+        const float low = (m == -INFINITY ? 0.f : m) - shift;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - low);
         l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         auto values = [&](auto which) {
             constexpr int AT = decltype(which)::value * PART + HALF, S = AT + CODES, E = decltype(which)::value * 4;
             const float2 w0 = make_float2(x[E], x[E + 1]), w1 = make_float2(x[E + 2], x[E + 3]);
-            {                                                          // the weights' sums of lows and sizes
+            {                                                          // the weights' sums of lows
                 const uint32_t p0 = pack2(w0), p1 = pack2(w1);
                 uint32_t b0 = 0, b1 = 0;
-                if (g < 2 * N) {
+                if (g < N) {
                     b0 = lds16<S>(base + at_vs) | lds16<S + D / 8>(base + at_vs) << 16;
                     b1 = lds16<S + D>(base + at_vs) | lds16<S + 9 * (D / 8)>(base + at_vs) << 16;
                 }
                 mma(e, p0, rest(w0, p0), p1, rest(w1, p1), b0, b1);
             }
-            float vs[4][N];
-            sizes<N, S>(base + at_v2, vs[0]);
-            sizes<N, S + D / 8>(base + at_v2, vs[1]);
-            sizes<N, S + D>(base + at_v2, vs[2]);
-            sizes<N, S + 9 * (D / 8)>(base + at_v2, vs[3]);
 #pragma unroll
             for (int c = 0; c < N; ++c) {
-                const float2 y0 = __fmul2_rn(w0, make_float2(vs[0][c], vs[1][c])), y1 = __fmul2_rn(w1, make_float2(vs[2][c], vs[3][c]));
-                const uint32_t p0 = pack2(y0), p1 = pack2(y1), r0 = rest(y0, p0), r1 = rest(y1, p1);
+                const float2 y0 = __fmul2_rn(w0, make_float2(vs[E][c], vs[E + 1][c])), y1 = __fmul2_rn(w1, make_float2(vs[E + 2][c], vs[E + 3][c]));
+                const uint32_t p0 = pack16(y0.x, y0.y), p1 = pack16(y1.x, y1.y);
                 // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
                 const uint32_t row = chunk(base + at_v, c), z0 = lds16<AT>(row) | lds16<AT + D / 2>(row) << 16, z1 = lds16<AT + 4 * D>(row) | lds16<AT + 9 * (D / 2)>(row) << 16;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t a0 = codes(z0, 2 * u, mk), a1 = codes(z0, 2 * u + 1, mk), a2 = codes(z1, 2 * u, mk), a3 = codes(z1, 2 * u + 1, mk);
-                    mma(o[2 * c + u], a0, a1, a2, a3, p0, p1);
-                    mma(o[2 * c + u], a0, a1, a2, a3, r0, r1);
+                mma16(o[2 * c], even(z0), odd(z0), even(z1), odd(z1), p0, p1);
+                mma16(o[2 * c + 1], even(z0 >> 8), odd(z0 >> 8), even(z1 >> 8), odd(z1 >> 8), p0, p1);
+                if constexpr (TWO) {
+                    const uint32_t r0 = rest16(y0, p0), r1 = rest16(y1, p1);
+                    mma16(o[2 * c], even(z0), odd(z0), even(z1), odd(z1), r0, r1);
+                    mma16(o[2 * c + 1], even(z0 >> 8), odd(z0 >> 8), even(z1 >> 8), odd(z1 >> 8), r0, r1);
                 }
             }
         };
@@ -334,7 +383,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     // the warps' parts meet in shared memory
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0) part_m[w][g] = m, part_l[w][g] = l;
+    if (t == 0) part_m[w][g] = m, part_l[w][g] = l * ex2(-shift);
     __syncthreads();
     constexpr int LD = D + 4;
     float *O = reinterpret_cast<float*>(smem), *E = O + WARPS * HEADS * LD;      // [WARPS][HEADS][LD], [WARPS][HEADS][8], over the rings
@@ -344,12 +393,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         for (int y = 1; y < WARPS; ++y) top = fmaxf(top, part_m[y][head]);
         return part_m[w][head] == -INFINITY ? 0.f : ex2(part_m[w][head] - top);
     };
-    const float f0 = factor(2 * t), f1 = factor(2 * t + 1), fg = factor(g);
+    // (the weights' shift is in l, o and e alike and is taken out here; codes are in units of 2^-24, the odd ones of 2^-20)
+    const float unshift = ex2(-shift), unscale = unshift * two_to(min(24 - wide, 127)), f0 = factor(2 * t) * unscale, f1 = factor(2 * t + 1) * unscale, fg = factor(g) * unshift;
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) {
         const int d = i / 2 * 32 + 4 * g + 2 * (i & 1);
-        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t) * LD + d) = make_float2(f0 * o[i][0], f0 * o[i][2]);
-        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t + 1) * LD + d) = make_float2(f1 * o[i][1], f1 * o[i][3]);
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t) * LD + d) = make_float2(f0 * o[i][0], f0 * 0.0625f * o[i][2]);
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t + 1) * LD + d) = make_float2(f1 * o[i][1], f1 * 0.0625f * o[i][3]);
     }
     *reinterpret_cast<float2*>(E + (w * HEADS + g) * 8 + 2 * t) = make_float2(fg * (e[0] + e[2]), fg * (e[1] + e[3]));
     if (threadIdx.x < HEADS) {
@@ -371,7 +421,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         for (int x = 0; x < WARPS; ++x) {
             const float4 z = load4(O + (x * HEADS + r) * LD + d);
             y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-            rest_ += E[(x * HEADS + r) * 8 + c] - 128.f * E[(x * HEADS + r) * 8 + N + c];
+            rest_ += E[(x * HEADS + r) * 8 + c];
         }
         y.x += rest_; y.y += rest_; y.z += rest_; y.w += rest_;
         const long long bh = (long long)b * a.H + h0 + r;

@@ -2,9 +2,11 @@
 
 Bounds.  What is stored is defined step by step in 32 bits, so pools are equal byte for byte; a number comes back within half a size, and the size is at most (range + 2^-7 |low|) / 15 (1 + 2^-7): ``low`` and ``size``
 are each rounded away from the group by one bf16 step, 2^-7 of them at most.
-Attention: u = finfo(type).eps / 2, one rounding of the output.  On the tensor cores a weight times a value's size goes in as two bf16 numbers, 2^-16 of it; codes go in with 128 on top, so a score's sum of products, which
-the tensor cores round to 2^-23 of its largest part per step of 16, is off by D / 16 2^-23 of scale sum |q| (143 size + |low|) for bf16 queries and as much again for fp16 ones, which go in as two numbers; tanh by 1e-6 of the
-score.  In 32 bits throughout: N + 8 roundings of scale sum |q| |k|, and a chain of additions as long as a warp's keys.  A weight is off by twice what its score is, and 2^-20 for the exponentials.  fp16 numbers below 2^-14
+Attention: u = finfo(type).eps / 2, one rounding of the output.  On the tensor cores codes go in as they are and queries exactly (but for 2^-39 of the head's largest number), so a score's sum of products, which the
+tensor cores round to 2^-23 of its largest part per step of 16, is off by D / 16 2^-23 of scale sum |q| (15 size + |low|), and as much again for the sum over the groups; tanh by 1e-6 of the score.  A weight times a
+value's size is rounded to 2^-12 of it for bf16 outputs and to 2^-22 for fp16 ones, of 15 sizes at most; it goes in as fp16 numbers, whose smallest is 2^-32 of the largest size that a warp has met (rounded up to a
+power of two, and weights may be counted from a maximum 2^8 below the largest score: half of 2^-31 times 15 a key).  In 32 bits throughout: N + 8 roundings of scale sum |q| |k|, and a chain of additions as long as a
+warp's keys.  A weight is off by twice what its score is, and 2^-20 for the exponentials.  fp16 numbers below 2^-14
 are rounded by up to 2^-25."""
 import pytest
 import torch
@@ -65,7 +67,7 @@ def formula(s, window=None, cap=None, slopes=None, scale=None, tensor=True):
         if tensor:
             codes, scales = R._parts(s["k"], D)
             sc = scales[at, :, keys % page].contiguous().view(BF).double().unflatten(-1, (2, -1)).abs()
-            reach = (143 * sc[:, :, 1] + sc[:, :, 0]).repeat_interleave(32, -1).repeat_interleave(H // G, 1)
+            reach = (15 * sc[:, :, 1] + sc[:, :, 0]).repeat_interleave(32, -1).repeat_interleave(H // G, 1)
             off = 2 * (D / 16) * 2 ** -23 * scale * torch.einsum("hd,jhd->hj", q[b].abs(), reach)
         else:
             off = (D / 32 + 8) * 2 ** -24 * scale * torch.einsum("hd,jhd->hj", q[b].abs(), k.abs()) + 4 * 2 ** -24 * x.abs()
@@ -77,12 +79,14 @@ def formula(s, window=None, cap=None, slopes=None, scale=None, tensor=True):
             x, off = x - far, off + 4 * 2 ** -24 * (far + x.abs())
         p = torch.softmax(x, -1)
         # a weight far below the largest one may be off by more than its share: its score's error counts by the weight
-        rel = (p * off).sum(-1, keepdim=True) + off + 2 ** -20 + (2 ** -16 if tensor else (n / 8 + 64) * 2 ** -24)
+        rel = (p * off).sum(-1, keepdim=True) + off + 2 ** -20 + (2.0 ** (-13 if s["q"].dtype == BF else -22) if tensor else (n / 8 + 64) * 2 ** -24)      # doubled below
         out[b] = torch.einsum("hj,jhd->hd", p, v)
         if tensor:                                           # lows and codes are added up by themselves
             sv = R._parts(s["v"], D)[1][at, :, keys % page].contiguous().view(BF).double().unflatten(-1, (2, -1)).abs()
             v = (sv[:, :, 0] + 15 * sv[:, :, 1]).repeat_interleave(32, -1).repeat_interleave(H // G, 1)
         room[b] = 2 * torch.einsum("hj,jhd->hd", p * rel, v.abs())
+        if tensor:
+            room[b] += len(keys) * 15 * 2.0 ** -32 * sv[:, :, 1].max()
     return out, room
 
 
