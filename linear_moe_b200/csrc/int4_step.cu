@@ -31,12 +31,12 @@ namespace int4 {
 namespace cg = cooperative_groups;
 
 #ifndef XST
-#define XST 2
+#define XST 3
 #endif
 #ifndef XCTAS
-#define XCTAS 4
+#define XCTAS 3
 #endif
-constexpr int CTAS = XCTAS, WARPS = 4, STAGES = XST, MAX_CLUSTER = 8, HEADS = 8;
+constexpr int CTAS = XCTAS, WARPS = 4, STAGES = XST, MAX_CLUSTER = 8, HEADS = 8, ROWS = 64;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 __device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
@@ -115,9 +115,10 @@ template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) {
 template <typename T, int N>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepArgs a) {
     constexpr bool TWO = !std::is_same<T, bf16>::value;                // p size in two parts
-    constexpr int D = 32 * N, CODES = GROUP * D / 2, SCALES = GROUP * D / 8, HALF = CODES + SCALES, PART = 2 * HALF, STAGE = 2 * PART;      // bytes: keys or values of a group, a group, two
+    constexpr int D = 32 * N, CODES = ROWS * D / 2, HALF = CODES + ROWS * D / 8, PART = 2 * HALF, STAGE = 2 * PART;      // bytes: keys' or values' codes of 64 rows, with their scales, both, twice
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ __align__(8) uint64_t full[WARPS][STAGES];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+    __shared__ uint32_t there_of[STAGES];                              // a bit per copy's lane: the groups that are there
     __shared__ float part_m[WARPS][HEADS], part_l[WARPS][HEADS], cta_m[HEADS], cta_l[HEADS];
     __shared__ int abort_flag, drain_flag, chosen, lens[WARPS * 32];
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -125,9 +126,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     int b = blockIdx.z;
     const int hk = blockIdx.y / tiles, tile = blockIdx.y % tiles, split = blockIdx.x;
     const int h0 = hk * qpg + tile * HEADS, nh = min(HEADS, hk * qpg + qpg - h0);
-    if (threadIdx.x == 0) abort_flag = drain_flag = 0;
-    if (lane == 0) {
-        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[w][s], 1);
+    if (threadIdx.x == 0) {
+        abort_flag = drain_flag = 0;
+        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -149,43 +150,41 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0 && a.lengths[b] != sh.len) atomicCAS(a.err, 0, 0x42000);
     if (beg >= end && a.splits > MAX_CLUSTER) return;                  // (a cluster's CTAs all stay, and one of them writes zeros where there is nothing to see)
 
-    unsigned char* ring = smem + w * STAGES * STAGE;
-    // Pairs of groups: beg + 2 w, beg + 2 (w + WARPS), ...; the last one may have no second group
-    const int n_mine = beg + 2 * w < end ? (end - beg - 2 * w + 2 * WARPS - 1) / (2 * WARPS) : 0;
-    long long page_ahead = 0;                                          // where the page and head lie of the group that is a lane's, 16 pairs at a time; -1: not there
-    int row_ahead = 0;
-    uint32_t have = 0;                                                 // two bits per stage: the groups that are there
-    // a lane's copy: codes or scales, of keys or of values, of the first or the second group
+    // Stages of eight groups, of which a warp reads two; the warps take turns in filling them.
+    const int n_stages = beg < end ? (end - beg + 7) / 8 : 0;
+    const bool blocks = a.page % ROWS == 0;                            // 64 rows lie together: a copy each for their codes and their scales, otherwise for a group's
+    // a lane's copy: codes or scales, of keys or of values, of group lane / 4
     const unsigned char* from = (lane & 2 ? a.v : a.k) + (lane & 1 ? (long long)a.page * (D / 2) : 0);
-    const int row_bytes = lane & 1 ? D / 8 : D / 2;
-    unsigned char* to = ring + (lane >> 2) * PART + (lane >> 1 & 1) * HALF + (lane & 1) * CODES;
-    auto issue = [&](int j) {
-        if (j >= n_mine) return;
-        const int st = j % STAGES;
-        if ((j & 15) == 0) {
-            const int gi = beg + 2 * (w + (j + (lane >> 1)) * WARPS) + (lane & 1);
-            page_ahead = -1;
-            if (gi < end) {
-                const int at = gi * GROUP / a.page, page = a.table[b * a.table_ld + at];
-                row_ahead = gi * GROUP - at * a.page;
-                if (page >= 0 && page < a.pages) page_ahead = ((long long)page * a.G + hk) * page_bytes(a.page, D);
-                else atomicCAS(a.err, 0, 0x43000);
-            }
+    const int row_bytes = lane & 1 ? D / 8 : D / 2, copy_bytes = (blocks ? ROWS : GROUP) * row_bytes;
+    unsigned char* to = smem + (lane >> 4) * PART + (lane >> 1 & 1) * HALF + (lane & 1) * CODES + (lane >> 2 & 3) * GROUP * row_bytes;
+    int filled = w - WARPS;                                            // the last stage that this warp has filled
+    long long page_at = -1;                                            // for the next one: where the page and head lie of this lane's group (-1: not there), and its row
+    int row_at = 0;
+    auto look_up = [&]() {
+        const int gi = beg + 8 * (filled + WARPS) + (lane >> 2);
+        page_at = -1;
+        if (gi < end && (!blocks || (lane & 12) == 0)) {
+            const int at = gi * GROUP / a.page, page = a.table[b * a.table_ld + at];
+            row_at = gi * GROUP - at * a.page;
+            if (page >= 0 && page < a.pages) page_at = ((long long)page * a.G + hk) * page_bytes(a.page, D);
+            else atomicCAS(a.err, 0, 0x43000);
         }
-        const int src = 2 * (j & 15) + (lane >> 2 & 1);
-        const long long page = __shfl_sync(0xffffffffu, page_ahead, src);
-        const int row = __shfl_sync(0xffffffffu, row_ahead, src);
-        const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0) & 0x11u;      // bits 0 and 4
-        have = (have & ~(3u << (2 * st))) | ((groups | groups >> 3) & 3u) << (2 * st);
+    };
+    auto fill = [&]() {
+        filled += WARPS;
+        const int st = filled % STAGES;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, page_at >= 0);
         if (lane == 0) {
-            if (groups) tc::mbar_expect_tx(&full[w][st], groups == 0x11u ? STAGE : PART);
-            else tc::mbar_arrive(&full[w][st]);
+            there_of[st] = blocks ? (lanes & 1u ? 0xffffu : 0u) | (lanes >> 16 & 1u ? 0xffff0000u : 0u) : lanes;
+            if (lanes) tc::mbar_expect_tx(&full[st], __popc(lanes) / 4 * (blocks ? ROWS : GROUP) * (D + D / 4));
+            else tc::mbar_arrive(&full[st]);
         }
         __syncwarp();
-        if (lane < 8 && page >= 0) bulk_load(to + st * STAGE, from + page + row * row_bytes, lane & 1 ? SCALES : CODES, &full[w][st]);
+        if (page_at >= 0) bulk_load(to + st * STAGE, from + page_at + row_at * row_bytes, copy_bytes, &full[st]);
+        look_up();
     };
-#pragma unroll
-    for (int j = 0; j < STAGES - 1; ++j) issue(j);
+    look_up();
+    if (filled + WARPS < min(STAGES - 1, n_stages)) fill();
 
     // Queries: a lane's numbers 8 t .. 8 t + 7 of every group of head g, in the order of the codes, scaled by a power of two; beside the rows' lows their sums, in three parts
     uint32_t qa[N][4], sums[3] = {0, 0, 0};
@@ -244,40 +243,45 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     for (int i = 0; i < 2 * N; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     // What a lane reads of a stage: of keys, rows g g + 8's words t and sizes; of values, rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9's half-words g and sizes
-    const uint32_t at_k = g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = g * (D / 8), at_ks = at_s + 4 * t, at_v2 = 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
+    const uint32_t part = (w >> 1) * PART, codes_at = part + (w & 1) * 2 * GROUP * (D / 2), scales_at = part + (w & 1) * 2 * GROUP * (D / 8);
+    const uint32_t at_k = codes_at + g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = codes_at + 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = scales_at + g * (D / 8), at_ks = at_s + 4 * t, at_v2 = scales_at + 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
     auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };
     bool alive = true;
     int j = 0;
-    for (; j < n_mine; ++j) {
-        const int st = j % STAGES, key0 = (beg + 2 * (w + j * WARPS)) * GROUP;
-        const uint32_t groups = have >> (2 * st) & 3u;
-        issue(j + STAGES - 1);                                         // into the stage that was read last
-        alive = fatc::mbar_wait_warp(&full[w][st], j / STAGES & 1, &abort_flag, a.err, 0x44000 | st);
+    for (; j < n_stages; ++j) {
+        const int st = j % STAGES, key0 = (beg + 8 * j + 2 * w) * GROUP;
+        if (filled + WARPS == j + STAGES - 1 && j + STAGES - 1 < n_stages) {      // this warp's turn, into the stage that was read last
+            if (j > 0) alive = fatc::mbar_wait_warp(&empty[(j - 1) % STAGES], (j - 1) / STAGES & 1, &abort_flag, a.err, 0x44020);
+            if (!alive) break;
+            fill();
+        }
+        alive = fatc::mbar_wait_warp(&full[st], j / STAGES & 1, &abort_flag, a.err, 0x44000 | st);
         if (!alive) break;
-        unsigned char* stage = ring + st * STAGE;
+        const uint32_t here = there_of[st] >> (8 * w), groups = (here & 1u) | (here >> 3 & 2u);
         const bool edge = groups != 3u || key0 < sh.lo || key0 + 2 * GROUP > sh.len;
         auto seen = [&](int key) -> bool { return (groups >> ((key - key0) / GROUP) & 1u) && key >= sh.lo && key < sh.len; };
         if (edge) {                                                    // hidden rows get scales of zero
+            uint32_t* scales = reinterpret_cast<uint32_t*>(smem + st * STAGE + (w >> 1) * PART + HALF + CODES + (w & 1) * 2 * GROUP * (D / 8));
             for (int i = lane; i < 2 * GROUP * N; i += 32)
-                if (!seen(key0 + i / N)) reinterpret_cast<uint32_t*>(stage + i / (GROUP * N) * PART + HALF + CODES)[i % (GROUP * N)] = 0;
+                if (!seen(key0 + i / N)) scales[i] = 0;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // ahead of the next copy into this stage
             __syncwarp();
         }
         // (where a group of 32 numbers lies depends on the row modulo 8 alone, in rows of a power of two of bytes: an exclusive or of the address)
-        const uint32_t base = tc::s32(stage);
+        const uint32_t base = tc::s32(smem) + st * STAGE;
         uint32_t v[8];                                                 // scores: head g, keys 8 (e >> 1) + 2 t + (e & 1)
         // Scores of rows g and g + 8 of a group, heads 2 t and 2 t + 1.  (The other way round, heads as the 16 rows: twice the products, and the rows that no head has have to be put beside every operand.)
         auto scores = [&](auto which) {
-            constexpr int AT = decltype(which)::value * PART, E = decltype(which)::value * 4;
+            constexpr int AT = decltype(which)::value * GROUP * (D / 2), S = CODES + decltype(which)::value * GROUP * (D / 8), E = decltype(which)::value * 4;
             float2 s0, s1;
-            const uint32_t c0 = 2 * t < N ? lds32<AT + CODES>(base + at_ks) : 0u, c1 = 2 * t < N ? lds32<AT + CODES + D>(base + at_ks) : 0u;
+            const uint32_t c0 = 2 * t < N ? lds32<S>(base + at_ks) : 0u, c1 = 2 * t < N ? lds32<S + D>(base + at_ks) : 0u;
             float x[4];
             mma_first(x, c0, c1, c0, c1, sums[0], sums[1]);
             mma(x, c0, c1, 0u, 0u, sums[2], 0u);
             s0 = make_float2(x[0], x[1]), s1 = make_float2(x[2], x[3]);
             float k0[N], k1[N];
-            sizes<N, AT + CODES>(base + at_s, k0);
-            sizes<N, AT + CODES + D>(base + at_s, k1);
+            sizes<N, S>(base + at_s, k0);
+            sizes<N, S + D>(base + at_s, k1);
 #pragma unroll
             for (int c = 0; c < N; ++c) {
                 const uint32_t row = chunk(base + at_k, c), y = lds32<AT>(row), z = lds32<AT + 4 * D>(row);
@@ -311,10 +315,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         sizes<N, HALF + CODES + D / 8>(base + at_v2, vs[1], &largest);
         sizes<N, HALF + CODES + D>(base + at_v2, vs[2], &largest);
         sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2, vs[3], &largest);
-        sizes<N, PART + HALF + CODES>(base + at_v2, vs[4], &largest);
-        sizes<N, PART + HALF + CODES + D / 8>(base + at_v2, vs[5], &largest);
-        sizes<N, PART + HALF + CODES + D>(base + at_v2, vs[6], &largest);
-        sizes<N, PART + HALF + CODES + 9 * (D / 8)>(base + at_v2, vs[7], &largest);
+        sizes<N, HALF + CODES + 2 * D>(base + at_v2, vs[4], &largest);
+        sizes<N, HALF + CODES + 2 * D + D / 8>(base + at_v2, vs[5], &largest);
+        sizes<N, HALF + CODES + 2 * D + D>(base + at_v2, vs[6], &largest);
+        sizes<N, HALF + CODES + 2 * D + 9 * (D / 8)>(base + at_v2, vs[7], &largest);
         const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any_sync(0xffffffffu, most > m + LAG || __vmaxu2(largest, bound) != bound)) {      // the first visible keys too
             float mx = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - low);
         l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         auto values = [&](auto which) {
-            constexpr int AT = decltype(which)::value * PART + HALF, S = AT + CODES, E = decltype(which)::value * 4;
+            constexpr int AT = HALF + decltype(which)::value * GROUP * (D / 2), S = HALF + CODES + decltype(which)::value * GROUP * (D / 8), E = decltype(which)::value * 4;
             const float2 w0 = make_float2(x[E], x[E + 1]), w1 = make_float2(x[E + 2], x[E + 3]);
             {                                                          // the weights' sums of lows
                 const uint32_t p0 = pack2(w0), p1 = pack2(w1);
@@ -375,10 +379,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         };
         values(std::integral_constant<int, 0>());
         values(std::integral_constant<int, 1>());
-        __syncwarp();                                                  // the stage is read; the next issue() fills it
+        __syncwarp();                                                  // the stage is read
+        if (lane == 0) tc::mbar_arrive(&empty[st]);
     }
-    if (!alive)                                                        // after a wait that ran out: copies in flight, again within a limit
-        for (int i = j; i < min(j + STAGES, n_mine); ++i) fatc::mbar_wait_suspend(&full[w][i % STAGES], i / STAGES & 1, &drain_flag, a.err, 0x44010);
+    if (!alive && filled >= j) fatc::mbar_wait_suspend(&full[filled % STAGES], filled / STAGES & 1, &drain_flag, a.err, 0x44010);      // after a wait that ran out: copies in flight, again within a limit
 
     // the warps' parts meet in shared memory
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) 
 
 template <typename T, int N>
 static int launch(const StepArgs& a, cudaStream_t st) {
-    constexpr int D = 32 * N, ring = WARPS * STAGES * 4 * GROUP * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
+    constexpr int D = 32 * N, ring = STAGES * 4 * ROWS * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
     int rc = (int)cudaFuncSetAttribute(int4_step_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc) return rc;
     const int tiles = (a.H / a.G + HEADS - 1) / HEADS;

@@ -22,15 +22,16 @@ struct StepArgs {
 
 constexpr int GROUP = 16, MIN_GROUPS = 8;               // keys of a group; groups that a CTA has at least when a request is split
 
-// The groups of 16 keys that a request's CTAs share: CTA s has [first + s per, first + (s + 1) per) of [first, last).
+// The groups of 16 keys that a request's CTAs share: CTA s has [first + s per, first + (s + 1) per) of [first, last), from 64-key boundaries on.
 struct Share { int len, lo, first, last, per; };
 __device__ __forceinline__ Share share_of(const StepArgs& a, int b) {
     Share s;
     s.len = min(max(a.lengths[b], 0), a.table_n * a.page);
     s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
-    s.first = s.lo / GROUP;
+    s.first = s.lo / (4 * GROUP) * 4;
     s.last = (s.len + GROUP - 1) / GROUP;
-    s.per = a.splits == 1 ? s.last - s.first : max(MIN_GROUPS, (s.last - s.first + a.splits - 1) / a.splits);
+    s.per = max(MIN_GROUPS, ((s.last - s.first + a.splits - 1) / a.splits + 3) & ~3);
+    if (a.splits == 1) s.per = max(s.last - s.first, 0);
     return s;
 }
 
