@@ -31,10 +31,10 @@ namespace int4 {
 namespace cg = cooperative_groups;
 
 #ifndef XST
-#define XST 3
+#define XST 2
 #endif
 #ifndef XCTAS
-#define XCTAS 3
+#define XCTAS 4
 #endif
 constexpr int CTAS = XCTAS, WARPS = 4, STAGES = XST, MAX_CLUSTER = 8, HEADS = 8, ROWS = 64;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
@@ -58,25 +58,26 @@ __device__ __forceinline__ void turn(float2 x, uint32_t& a, uint32_t& b) {
     a = __byte_perm(lo, hi, 0x5410);
     b = __byte_perm(lo, hi, 0x7632);
 }
-// A row's N sizes, behind its N lows; with `most`: the largest ones of two columns so far, as bits
-template <int N, int AT> __device__ __forceinline__ void sizes(uint32_t row, float (&s)[N], uint32_t* most = nullptr) {
+// A row's N sizes, behind its N lows: as they lie (two to a word, what is not a size set to zero), and one of them
+template <int N> struct Sizes { uint32_t w[N == 4 || N == 3 ? 2 : 1]; };
+template <int N, int AT> __device__ __forceinline__ Sizes<N> sizes(uint32_t row) {
+    Sizes<N> s;
     if constexpr (N == 4) {
         const uint2 x = lds64<AT + 8>(row);
-        if (most) *most = __vimax3_u16x2(*most, x.x, x.y);
-        s[0] = lower(x.x), s[1] = upper(x.x), s[2] = lower(x.y), s[3] = upper(x.y);
+        s.w[0] = x.x, s.w[1] = x.y;
     } else if constexpr (N == 3) {
-        const uint32_t x = lds32<AT + 4>(row), y = lds32<AT + 8>(row);
-        if (most) *most = __vimax3_u16x2(*most, x & 0xffff0000u, y);
-        s[0] = upper(x), s[1] = lower(y), s[2] = upper(y);
-    } else if constexpr (N == 2) {
-        const uint32_t x = lds32<AT + 4>(row);
-        if (most) *most = __vmaxu2(*most, x);
-        s[0] = lower(x), s[1] = upper(x);
-    } else {
-        const uint32_t x = lds32<AT>(row);
-        if (most) *most = __vmaxu2(*most, x & 0xffff0000u);
-        s[0] = upper(x);
-    }
+        s.w[0] = lds32<AT + 4>(row) & 0xffff0000u, s.w[1] = lds32<AT + 8>(row);
+    } else if constexpr (N == 2) s.w[0] = lds32<AT + 4>(row);
+    else s.w[0] = lds32<AT>(row) & 0xffff0000u;
+    return s;
+}
+template <int N> __device__ __forceinline__ float size_of(const Sizes<N>& s, int c) {
+    const int i = N % 2 + c;
+    return i % 2 ? upper(s.w[i / 2]) : lower(s.w[i / 2]);
+}
+template <int N> __device__ __forceinline__ uint32_t larger(uint32_t most, const Sizes<N>& s) {      // of the even and of the odd ones, as bits
+    if constexpr (N >= 3) return __vimax3_u16x2(most, s.w[0], s.w[1]);
+    else return __vmaxu2(most, s.w[0]);
 }
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -279,17 +280,16 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             mma_first(x, c0, c1, c0, c1, sums[0], sums[1]);
             mma(x, c0, c1, 0u, 0u, sums[2], 0u);
             s0 = make_float2(x[0], x[1]), s1 = make_float2(x[2], x[3]);
-            float k0[N], k1[N];
-            sizes<N, S>(base + at_s, k0);
-            sizes<N, S + D>(base + at_s, k1);
+            const Sizes<N> k0 = sizes<N, S>(base + at_s), k1 = sizes<N, S + D>(base + at_s);
 #pragma unroll
             for (int c = 0; c < N; ++c) {
                 const uint32_t row = chunk(base + at_k, c), y = lds32<AT>(row), z = lds32<AT + 4 * D>(row);
                 float d[4];
                 mma16_first(d, even(y), even(z), odd(y), odd(z), qa[c][0], qa[c][1]);
                 mma16(d, even(y >> 8), even(z >> 8), odd(y >> 8), odd(z >> 8), qa[c][2], qa[c][3]);
-                s0 = __ffma2_rn(make_float2(k0[c], k0[c]), make_float2(d[0], d[1]), s0);
-                s1 = __ffma2_rn(make_float2(k1[c], k1[c]), make_float2(d[2], d[3]), s1);
+                const float f0 = size_of(k0, c), f1 = size_of(k1, c);
+                s0 = __ffma2_rn(make_float2(f0, f0), make_float2(d[0], d[1]), s0);
+                s1 = __ffma2_rn(make_float2(f1, f1), make_float2(d[2], d[3]), s1);
             }
             turn(s0, v[E], v[E + 1]);                                  // by halves of their bits
             turn(s1, v[E + 2], v[E + 3]);
@@ -309,16 +309,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             for (int i = 0; i < 8; ++i)
                 if (!seen(key0 + 8 * (i >> 1) + 2 * t + (i & 1))) x[i] = -INFINITY;
         }
-        float vs[8][N];                                                // sizes of the values of keys 8 (e >> 1) + 2 t + (e & 1)
+        // sizes of the values of keys 8 (e >> 1) + 2 t + (e & 1)
+        const Sizes<N> vs[8] = {sizes<N, HALF + CODES>(base + at_v2), sizes<N, HALF + CODES + D / 8>(base + at_v2), sizes<N, HALF + CODES + D>(base + at_v2), sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2),
+                                sizes<N, HALF + CODES + 2 * D>(base + at_v2), sizes<N, HALF + CODES + 17 * (D / 8)>(base + at_v2), sizes<N, HALF + CODES + 3 * D>(base + at_v2),
+                                sizes<N, HALF + CODES + 25 * (D / 8)>(base + at_v2)};
         uint32_t largest = 0;
-        sizes<N, HALF + CODES>(base + at_v2, vs[0], &largest);
-        sizes<N, HALF + CODES + D / 8>(base + at_v2, vs[1], &largest);
-        sizes<N, HALF + CODES + D>(base + at_v2, vs[2], &largest);
-        sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2, vs[3], &largest);
-        sizes<N, HALF + CODES + 2 * D>(base + at_v2, vs[4], &largest);
-        sizes<N, HALF + CODES + 2 * D + D / 8>(base + at_v2, vs[5], &largest);
-        sizes<N, HALF + CODES + 2 * D + D>(base + at_v2, vs[6], &largest);
-        sizes<N, HALF + CODES + 2 * D + 9 * (D / 8)>(base + at_v2, vs[7], &largest);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = larger(largest, vs[i]);
         const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any_sync(0xffffffffu, most > m + LAG || __vmaxu2(largest, bound) != bound)) {      // the first visible keys too
             float mx = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -339,13 +336,6 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
             for (int i = 0; i < 2 * N; ++i) o[i][0] *= c0, o[i][1] *= c1, o[i][2] *= c0, o[i][3] *= c1;
         }
-        if (wide != 0) {
-            const float f = two_to(wide);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int c = 0; c < N; ++c) vs[i][c] *= f;
-        }
         const float low = (m == -INFINITY ? 0.f : m) - shift;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - low);
@@ -353,6 +343,11 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         auto values = [&](auto which) {
             constexpr int AT = HALF + decltype(which)::value * GROUP * (D / 2), S = HALF + CODES + decltype(which)::value * GROUP * (D / 8), E = decltype(which)::value * 4;
             const float2 w0 = make_float2(x[E], x[E + 1]), w1 = make_float2(x[E + 2], x[E + 3]);
+            float2 u0 = w0, u1 = w1;
+            if (wide != 0) {
+                const float f = two_to(wide);
+                u0.x *= f, u0.y *= f, u1.x *= f, u1.y *= f;
+            }
             {                                                          // the weights' sums of lows
                 const uint32_t p0 = pack2(w0), p1 = pack2(w1);
                 uint32_t b0 = 0, b1 = 0;
@@ -364,7 +359,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             }
 #pragma unroll
             for (int c = 0; c < N; ++c) {
-                const float2 y0 = __fmul2_rn(w0, make_float2(vs[E][c], vs[E + 1][c])), y1 = __fmul2_rn(w1, make_float2(vs[E + 2][c], vs[E + 3][c]));
+                const float2 y0 = __fmul2_rn(u0, make_float2(size_of(vs[E], c), size_of(vs[E + 1], c))), y1 = __fmul2_rn(u1, make_float2(size_of(vs[E + 2], c), size_of(vs[E + 3], c)));
                 const uint32_t p0 = pack16(y0.x, y0.y), p1 = pack16(y1.x, y1.y);
                 // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
                 const uint32_t row = chunk(base + at_v, c), z0 = lds16<AT>(row) | lds16<AT + D / 2>(row) << 16, z1 = lds16<AT + 4 * D>(row) | lds16<AT + 9 * (D / 2)>(row) << 16;

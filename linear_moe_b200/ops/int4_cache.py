@@ -172,7 +172,7 @@ HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 8                  # csrc/int4_step.cu, .
 def splits_of(B: int, G: int, heads: int, D: int, keys: int) -> Tuple[int, int]:
     """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first): parts for one wave, of 128 keys at least."""
     from . import cuda as K
-    work, slots = max(1, B * G * -(-heads // HEADS)), 3 * K.num_sms()
+    work, slots = max(1, B * G * -(-heads // HEADS)), 4 * K.num_sms()
     n = slots // work if 2 * work <= slots else 2 if work < 4 * slots else 1
     n = min(n, -(-keys // (GROUP * MIN_GROUPS)))
     n = MAX_CLUSTER if MAX_CLUSTER < n < 16 else max(n, 1)
