@@ -19,9 +19,10 @@ struct Args {
     const void* at;                                   // [rows], the tables' row of every token; null: token t of a sequence has row t
     const void *dq, *dk, *dv;                         // backward; null: zeros
     void *dx, *dwq, *dwk;
-    float* part;                                      // [parts, 2, D]
+    float* part;                                      // of the weights' gradients: [parts, 2, D]; heads of vectors [parts, D], those of queries and then those of keys
     long long x_b, x_t, rows;
     int T, G, r, D, R, tokens, interleaved, at_wide, w_type, parts;
+    int vectors, parts_q, parts_k;                    // heads of vectors: blocks of queries and of keys (the rest are values'); backward: one part each
     float eps;
     int* err;
 };
@@ -153,15 +154,209 @@ __global__ void __launch_bounds__(WARPS * 32) heads_any_bwd_kernel(const Args a)
         }
 }
 
+// Heads of vectors: 16 bytes of a thread, twice.  A head is up to 32 threads', and what turns together one thread's: numbers from E j and from R / 2 + E j on (behind R: E neighbours twice), or, where
+// neighbours turn, from E j and from D / 2 + E j on.  A block works on queries, keys or values alone, so that a thread keeps its numbers' weights, and their gradients, in registers.
+constexpr int VT = 256;
+template <typename T> struct Chunk { static constexpr int E = 16 / sizeof(T); float x[2 * E]; };
+template <typename T> __device__ __forceinline__ void load_chunk(const T* p, float* x) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::E; ++i) x[i] = val(reinterpret_cast<const T*>(&raw)[i]);
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const float* x) {
+    __align__(16) T y[Chunk<T>::E];
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::E; ++i) y[i] = num<T>(x[i]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(y);
+}
+template <int TPH> __device__ __forceinline__ float head_sum(float v) {
+#pragma unroll
+    for (int o = TPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+struct Place { int kind, block, blocks, at[2]; bool in, turns[2]; };      // kind: 0 queries, 1 keys, 2 values; first numbers of a thread's vectors
+template <typename T, int TPH> __device__ __forceinline__ Place place_of(const Args& a) {
+    constexpr int E = Chunk<T>::E;
+    Place p;
+    const int b = blockIdx.x, j = threadIdx.x % TPH;
+    p.kind = b < a.parts_q ? 0 : b < a.parts_q + a.parts_k ? 1 : 2;
+    p.block = p.kind == 0 ? b : p.kind == 1 ? b - a.parts_q : b - a.parts_q - a.parts_k;
+    p.blocks = p.kind == 0 ? a.parts_q : p.kind == 1 ? a.parts_k : gridDim.x - a.parts_q - a.parts_k;
+    p.in = j < a.D / (2 * E);
+    if (a.interleaved) p.at[0] = E * j, p.at[1] = a.D / 2 + E * j;
+    else if (E * j < a.R / 2) p.at[0] = E * j, p.at[1] = a.R / 2 + E * j;
+    else p.at[0] = 2 * E * j, p.at[1] = p.at[0] + E;
+    p.turns[0] = p.at[0] < a.R, p.turns[1] = p.at[1] < a.R;
+    return p;
+}
+// Cosines and sines of a thread's numbers: pairs of neighbours have E / 2 each per vector, halves E for both
+template <int E> __device__ __forceinline__ void load_table(const float* p, float* x) {
+#pragma unroll
+    for (int i = 0; i < E; i += (E % 4 ? 2 : 4))
+        if constexpr (E % 4 == 0) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(p + i);
+        else *reinterpret_cast<float2*>(x + i) = *reinterpret_cast<const float2*>(p + i);
+}
+// (a, b) -> (a cos - b sin, a sin + b cos), with the sine's sign
+template <typename T, bool INTER> __device__ __forceinline__ void turn(const Args& a, const Place& p, long long pos, float sign, float* x) {
+    constexpr int E = Chunk<T>::E;
+    const int half = a.R / 2;
+    const float *cos = a.cos + pos * half, *sin = a.sin + pos * half;
+    float c[E], s[E];
+    if constexpr (!INTER) {
+        if (!p.turns[0]) return;
+        load_table<E>(cos + p.at[0], c);
+        load_table<E>(sin + p.at[0], s);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float u = x[i], v = x[E + i], sn = sign * s[i];
+            x[i] = u * c[i] - v * sn, x[E + i] = u * sn + v * c[i];
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!p.turns[h]) continue;
+            load_table<E / 2>(cos + p.at[h] / 2, c);
+            load_table<E / 2>(sin + p.at[h] / 2, s);
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                const float u = x[h * E + 2 * i], v = x[h * E + 2 * i + 1], sn = sign * s[i];
+                x[h * E + 2 * i] = u * c[i] - v * sn, x[h * E + 2 * i + 1] = u * sn + v * c[i];
+            }
+        }
+    }
+}
+// Head `it` of a kind: its token's row, and where it lies in the projection
+struct Head { long long row, from; };
+__device__ __forceinline__ Head head_of(const Args& a, int kind, unsigned it, long long ld_b, long long ld_t) {
+    const unsigned n = kind == 0 ? a.G * a.r : a.G, row = it / n, h = it - row * n, g = kind == 0 ? h / a.r : h;
+    const unsigned b = ld_b == ld_t * a.T ? 0u : row / a.T;
+    Head y;
+    y.row = row;
+    y.from = b * ld_b + (long long)(row - b * a.T) * ld_t + (long long)(kind == 0 ? h + 2 * g : g * (a.r + 2) + a.r + kind - 1) * a.D;
+    return y;
+}
+
+template <typename T, int TPH, bool INTER>
+__global__ void __launch_bounds__(VT) heads_vec_kernel(const Args a) {
+    constexpr int E = Chunk<T>::E, HEADS = VT / TPH;
+    const Place p = place_of<T, TPH>(a);
+    const void* wp = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr;
+    float w[2 * E];
+    if (wp != nullptr && p.in)
+#pragma unroll
+        for (int i = 0; i < 2 * E; ++i) w[i] = weight(wp, a.w_type, p.at[i / E] + i % E);
+    T* out = (T*)(p.kind == 0 ? a.q : p.kind == 1 ? a.k : a.v);
+    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1);
+    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += p.blocks * HEADS) {
+        const unsigned it = it0 + threadIdx.x / TPH;
+        const bool there = p.in && it < items;
+        float x[2 * E];
+#pragma unroll
+        for (int i = 0; i < 2 * E; ++i) x[i] = 0.f;
+        Head h;
+        if (there) {
+            h = head_of(a, p.kind, it, a.x_b, a.x_t);
+            load_chunk((const T*)a.x + h.from + p.at[0], x);
+            load_chunk((const T*)a.x + h.from + p.at[1], x + E);
+        }
+        if (wp != nullptr) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * E; ++i) sum += x[i] * x[i];
+            const float inv = 1.f / sqrtf(head_sum<TPH>(sum) / a.D + a.eps);
+#pragma unroll
+            for (int i = 0; i < 2 * E; ++i) x[i] = x[i] * inv * w[i];
+        }
+        if (!there) continue;
+        if (a.R > 0 && p.kind < 2) turn<T, INTER>(a, p, row_of(a, h.row), 1.f, x);
+        store_chunk(out + (long long)it * a.D + p.at[0], x);
+        store_chunk(out + (long long)it * a.D + p.at[1], x + E);
+    }
+}
+
+template <typename T, int TPH, bool INTER>
+__global__ void __launch_bounds__(VT) heads_vec_bwd_kernel(const Args a) {
+    constexpr int E = Chunk<T>::E, HEADS = VT / TPH;
+    __shared__ float red[HEADS][TPH * 2 * E];
+    const Place p = place_of<T, TPH>(a);
+    pdl_trigger();
+    const void* wp = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr;
+    float w[2 * E], dw[2 * E];
+#pragma unroll
+    for (int i = 0; i < 2 * E; ++i) {
+        dw[i] = 0.f;
+        w[i] = wp != nullptr && p.in ? weight(wp, a.w_type, p.at[i / E] + i % E) : 0.f;
+    }
+    const T* from = (const T*)(p.kind == 0 ? a.dq : p.kind == 1 ? a.dk : a.dv);
+    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1);
+    const long long ld = (long long)a.G * (a.r + 2) * a.D;
+    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += p.blocks * HEADS) {
+        const unsigned it = it0 + threadIdx.x / TPH;
+        const bool there = p.in && it < items;
+        float x[2 * E], dy[2 * E];
+#pragma unroll
+        for (int i = 0; i < 2 * E; ++i) x[i] = dy[i] = 0.f;
+        Head h, to;
+        if (there) {
+            to = head_of(a, p.kind, it, ld * a.T, ld);
+            if (from != nullptr) {
+                load_chunk(from + (long long)it * a.D + p.at[0], dy);
+                load_chunk(from + (long long)it * a.D + p.at[1], dy + E);
+            }
+            if (wp != nullptr) {
+                h = head_of(a, p.kind, it, a.x_b, a.x_t);
+                load_chunk((const T*)a.x + h.from + p.at[0], x);
+                load_chunk((const T*)a.x + h.from + p.at[1], x + E);
+            }
+            if (a.R > 0 && p.kind < 2 && from != nullptr) turn<T, INTER>(a, p, row_of(a, to.row), -1.f, dy);
+        }
+        if (wp != nullptr) {
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * E; ++i) sum += x[i] * x[i];
+            const float rms = sqrtf(head_sum<TPH>(sum) / a.D + a.eps), inv = it < items ? 1.f / rms : 0.f;      // (threads without a head add nothing)
+#pragma unroll
+            for (int i = 0; i < 2 * E; ++i) {
+                x[i] *= inv;
+                dw[i] += dy[i] * x[i];
+                dy[i] *= w[i];
+                dot += dy[i] * x[i];
+            }
+            dot = head_sum<TPH>(dot) / a.D;
+#pragma unroll
+            for (int i = 0; i < 2 * E; ++i) dy[i] = (dy[i] - x[i] * dot) * inv;
+        }
+        if (!there) continue;
+        store_chunk((T*)a.dx + to.from + p.at[0], dy);
+        store_chunk((T*)a.dx + to.from + p.at[1], dy + E);
+    }
+    if (a.part == nullptr || wp == nullptr) return;
+    if (p.in)
+#pragma unroll
+        for (int i = 0; i < 2 * E; ++i) red[threadIdx.x / TPH][p.at[i / E] + i % E] = dw[i];
+    __syncthreads();
+    float* out = a.part + (long long)(p.kind == 0 ? p.block : a.parts_q + p.block) * a.D;
+    for (int d = threadIdx.x; d < a.D; d += VT) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int y = 0; y < HEADS; ++y) s += red[y][d];
+        out[d] = s;
+    }
+}
+
 // Weights' gradients out of the blocks' parts, in the order of the blocks: a block for 32 numbers of one weight, its warps take the parts in turn.
 constexpr int SUM_WARPS = 16;
-__global__ void __launch_bounds__(SUM_WARPS * 32) heads_sum_kernel(const Args a) {
+__global__ void __launch_bounds__(SUM_WARPS * 32) heads_sum_kernel(Args a) {
     __shared__ float red[SUM_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane, n = blockIdx.y;
     pdl_wait();
+    const int count = a.vectors ? (n == 0 ? a.parts_q : a.parts_k) : a.parts;
+    const float* part = a.part + (long long)(a.vectors ? n * a.parts_q : n) * a.D + d;
+    const long long ld = a.vectors ? a.D : 2 * a.D;
     float s = 0.f;
-    if (d < a.D)
-        for (int p = warp; p < a.parts; p += SUM_WARPS) s += a.part[((long long)p * 2 + n) * a.D + d];
+    if (d < a.D && (n == 0 ? a.dwq : a.dwk) != nullptr)
+#pragma unroll 8
+        for (int p = warp; p < count; p += SUM_WARPS) s += part[p * ld];
     red[warp][lane] = s;
     __syncthreads();
     if (warp > 0 || d >= a.D) return;
@@ -175,6 +370,19 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) heads_sum_kernel(const Args a)
     else ((__half*)out)[d] = num<__half>(s);
 }
 
+static int sum_up(const Args& a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((a.D + 31) / 32, 2);
+    cfg.blockDim = dim3(SUM_WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, heads_sum_kernel, a);
+    return (int)cudaGetLastError();
+}
 template <typename T, int PER>
 static int run_any(const Args& a, bool back, cudaStream_t st) {
     const long long blocks = (a.rows * a.G * (a.r + 2) + WARPS - 1) / WARPS;
@@ -185,11 +393,27 @@ static int run_any(const Args& a, bool back, cudaStream_t st) {
     heads_any_bwd_kernel<T, PER><<<a.parts, WARPS * 32, 0, st>>>(a);
     const int rc = (int)cudaGetLastError();
     if (rc || a.part == nullptr) return rc;
-    heads_sum_kernel<<<dim3((a.D + 31) / 32, 2), SUM_WARPS * 32, 0, st>>>(a);
-    return (int)cudaGetLastError();
+    return sum_up(a, st);
 }
+template <typename T, int TPH, bool INTER>
+static int run_vec(const Args& a, bool back, cudaStream_t st) {
+    if (back) heads_vec_bwd_kernel<T, TPH, INTER><<<a.parts, VT, 0, st>>>(a);
+    else heads_vec_kernel<T, TPH, INTER><<<a.parts, VT, 0, st>>>(a);
+    const int rc = (int)cudaGetLastError();
+    return rc || !back || a.part == nullptr ? rc : sum_up(a, st);
+}
+template <typename T, int TPH>
+static int run_vec(const Args& a, bool back, cudaStream_t st) { return a.interleaved ? run_vec<T, TPH, true>(a, back, st) : run_vec<T, TPH, false>(a, back, st); }
 template <typename T>
 static int by_width(const Args& a, bool back, cudaStream_t st) {
+    if (a.vectors) {
+        const int threads = a.D / (2 * Chunk<T>::E);
+        if (threads > 32 || a.D % (2 * Chunk<T>::E) || a.R % (2 * Chunk<T>::E) || a.rows * a.G * a.r > 0x7fffffffll || a.parts_q < 1 || a.parts_k < 1 || a.parts <= a.parts_q + a.parts_k) return -1;
+        if (threads <= 4) return run_vec<T, 4>(a, back, st);
+        if (threads <= 8) return run_vec<T, 8>(a, back, st);
+        if (threads <= 16) return run_vec<T, 16>(a, back, st);
+        return run_vec<T, 32>(a, back, st);
+    }
     if (a.D <= 128) return run_any<T, 4>(a, back, st);
     if (a.D <= 256) return run_any<T, 8>(a, back, st);
     return run_any<T, 32>(a, back, st);

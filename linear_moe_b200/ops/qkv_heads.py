@@ -21,7 +21,7 @@ from .scored_attn import on_device
 class _Args(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "wq", "wk", "q", "k", "v", "cos", "sin", "at", "dq", "dk", "dv", "dx", "dwq", "dwk", "part")] +
                 [(n, ctypes.c_longlong) for n in ("x_b", "x_t", "rows")] +
-                [(n, ctypes.c_int) for n in ("T", "G", "r", "D", "R", "tokens", "interleaved", "at_wide", "w_type", "parts")] +
+                [(n, ctypes.c_int) for n in ("T", "G", "r", "D", "R", "tokens", "interleaved", "at_wide", "w_type", "parts", "vectors", "parts_q", "parts_k")] +
                 [("eps", ctypes.c_float), ("err", ctypes.c_void_p)])
 
 
@@ -86,23 +86,52 @@ def _dense_heads(t: torch.Tensor) -> bool:
     return t[0, 0].is_contiguous() if t.numel() else True
 
 
+def _blocks(a: _Args, size: int, back: bool):
+    """Blocks of the vectors' kernels: of queries, keys and values by their number, up to what the GPU holds at once."""
+    from . import cuda as K
+    threads = 4
+    while threads * 2 * (16 // size) < a.D:
+        threads *= 2
+    keys = -(-a.rows * a.G * threads // 256)
+    most = (4 if back else 6) * K.num_sms()
+    share = max(1, min(keys, most // (a.r + 2)))
+    a.parts_k, a.parts_q = share, max(1, min(-(-a.rows * a.G * a.r * threads // 256), most - 2 * share))
+    a.parts = a.parts_q + 2 * share
+
+
+def _vectors(a: _Args, size: int) -> bool:
+    """Do heads of this size go through the kernels that read 16 bytes at a time?  Then what does not lie on 16-byte boundaries is copied: the result is the same wherever a tensor lies."""
+    e = 16 // size
+    return a.D % (2 * e) == 0 and a.D <= 64 * e and a.R % (2 * e) == 0 and a.rows * a.G * a.r < 1 << 31
+
+
+def _aligned(t: Optional[torch.Tensor], strides=()) -> bool:
+    return t is None or not t.data_ptr() % 16 and all(s * t.element_size() % 16 == 0 for s in strides)
+
+
+def _forward(qkv, wq, wk, plan, cos, sin, at):
+    from . import cuda as K
+    B, T, G, S, D = qkv.shape
+    dev, dt = qkv.device, qkv.dtype
+    q, k, v = (torch.empty((B, T, n, D), dtype=dt, device=dev) for n in (G * (S - 2), G, G))
+    a = _Args.from_buffer_copy(plan)
+    a.x, a.wq, a.wk, a.q, a.k, a.v = qkv.data_ptr(), K._ptr(wq), K._ptr(wk), q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.cos, a.sin, a.at, a.err = K._ptr(cos), K._ptr(sin), K._ptr(at), K.error_word(dev)
+    with on_device(qkv):
+        if _vectors(a, dt.itemsize):
+            a.vectors = 1
+            _blocks(a, dt.itemsize, False)
+        K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), _TYPES[dt], 0, K._st()), "qkv_heads")
+    return q, k, v
+
+
 class _QkvHeads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, plan, cos, sin, at):
-        from . import cuda as K
-        B, T, G, S, D = qkv.shape
-        dev, dt = qkv.device, qkv.dtype
-        q = torch.empty((B, T, G * (S - 2), D), dtype=dt, device=dev)
-        k, v = torch.empty((B, T, G, D), dtype=dt, device=dev), torch.empty((B, T, G, D), dtype=dt, device=dev)
-        a = _Args.from_buffer_copy(plan)
-        a.x, a.wq, a.wk, a.q, a.k, a.v = qkv.data_ptr(), K._ptr(wq), K._ptr(wk), q.data_ptr(), k.data_ptr(), v.data_ptr()
-        a.cos, a.sin, a.at, a.err = K._ptr(cos), K._ptr(sin), K._ptr(at), K.error_word(dev)
-        with on_device(qkv):
-            K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), _TYPES[dt], 0, K._st()), "qkv_heads")
         ctx.save_for_backward(qkv, wq, wk, cos, sin, at)
         ctx.plan = plan
         ctx.set_materialize_grads(False)
-        return q, k, v
+        return _forward(qkv, wq, wk, plan, cos, sin, at)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -114,13 +143,21 @@ class _QkvHeads(torch.autograd.Function):
         grads = [None if g is None else g.contiguous() for g in (dq, dk, dv)]
         dx = torch.empty(qkv.shape, dtype=qkv.dtype, device=dev)
         dws = [torch.empty_like(w) if w is not None and need else None for w, need in zip((wq, wk), ctx.needs_input_grad[1:3])]
-        items = a.rows * a.G * (a.r + 2)
-        a.parts = max(1, min(-(-items // 8), 8 * K.num_sms()))
-        work = torch.empty(a.parts * 2 * D, dtype=torch.float32, device=dev) if any(w is not None for w in dws) else None
         a.x, a.wq, a.wk, a.cos, a.sin, a.at, a.err = qkv.data_ptr(), K._ptr(wq), K._ptr(wk), K._ptr(cos), K._ptr(sin), K._ptr(at), K.error_word(dev)
         a.dq, a.dk, a.dv = (K._ptr(g) for g in grads)
-        a.dx, a.dwq, a.dwk, a.part = dx.data_ptr(), K._ptr(dws[0]), K._ptr(dws[1]), K._ptr(work)
+        a.dx, a.dwq, a.dwk = dx.data_ptr(), K._ptr(dws[0]), K._ptr(dws[1])
         with on_device(qkv):
+            if _vectors(a, qkv.dtype.itemsize):
+                grads = [g if _aligned(g) else g.clone() for g in grads]
+                a.dq, a.dk, a.dv = (K._ptr(g) for g in grads)
+                a.vectors = 1
+                _blocks(a, qkv.dtype.itemsize, True)
+                parts = a.parts_q + a.parts_k
+            else:
+                a.parts = max(1, min(-(-a.rows * a.G * (a.r + 2) // 8), 8 * K.num_sms()))
+                parts = 2 * a.parts
+            work = torch.empty(parts * D, dtype=torch.float32, device=dev) if dws[0] is not None or dws[1] is not None else None
+            a.part = K._ptr(work)
             K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), _TYPES[qkv.dtype], 1, K._st()), "qkv_heads backward", 1 if work is None else 2)
         return (dx, *dws, None, None, None, None)
 
@@ -144,4 +181,10 @@ def qkv_heads(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weig
     B, T, G, S, D = qkv.shape
     if B * T * G == 0:
         return qkv[..., : S - 2, :].reshape(B, T, G * (S - 2), D), qkv[..., S - 2, :], qkv[..., S - 1, :]
+    if not _aligned(qkv, qkv.stride()[:2]) or not _aligned(cos) or not _aligned(sin):
+        if _vectors(_Args.from_buffer_copy(plan), qkv.element_size()):
+            qkv = qkv if _aligned(qkv, qkv.stride()[:2]) else qkv.clone(memory_format=torch.contiguous_format)
+            return qkv_heads(qkv, q_weight, k_weight, eps, *(t if _aligned(t) else t.clone() for t in (cos, sin)), positions=positions, interleaved=interleaved)
+    if not torch.is_grad_enabled() or not (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
+        return _forward(qkv, q_weight, k_weight, plan, cos, sin, positions)
     return _QkvHeads.apply(qkv, q_weight, k_weight, plan, cos, sin, positions)
