@@ -22,6 +22,7 @@ struct Args {
     float* part;                                      // of the weights' gradients: [parts, 2, D]; heads of vectors [parts, D], those of queries and then those of keys
     long long x_b, x_t, rows;
     int T, G, r, D, R, tokens, interleaved, at_wide, w_type, parts;
+    unsigned div[4][2];                               // heads of vectors: divisors G r, G, r and T (`over`)
     int vectors, parts_q, parts_k;                    // heads of vectors: blocks of queries and of keys (the rest are values'); backward: one part each
     float eps;
     int* err;
@@ -157,18 +158,27 @@ __global__ void __launch_bounds__(WARPS * 32) heads_any_bwd_kernel(const Args a)
 // Heads of vectors: 16 bytes of a thread, twice.  A head is up to 32 threads', and what turns together one thread's: numbers from E j and from R / 2 + E j on (behind R: E neighbours twice), or, where
 // neighbours turn, from E j and from D / 2 + E j on.  A block works on queries, keys or values alone, so that a thread keeps its numbers' weights, and their gradients, in registers.
 constexpr int VT = 256;
-template <typename T> struct Chunk { static constexpr int E = 16 / sizeof(T); float x[2 * E]; };
-template <typename T> __device__ __forceinline__ void load_chunk(const T* p, float* x) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-    for (int i = 0; i < Chunk<T>::E; ++i) x[i] = val(reinterpret_cast<const T*>(&raw)[i]);
+template <typename T> struct Chunk { static constexpr int E = 16 / sizeof(T); };      // numbers of a vector
+template <typename T> __device__ __forceinline__ float2 pair_of(const uint4& raw, int i);      // numbers 2 i, 2 i + 1
+template <> __device__ __forceinline__ float2 pair_of<float>(const uint4& raw, int i) { return reinterpret_cast<const float2*>(&raw)[i]; }
+template <> __device__ __forceinline__ float2 pair_of<bf16>(const uint4& raw, int i) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&raw)[i];
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <typename T> __device__ __forceinline__ void store_chunk(T* p, const float* x) {
+template <> __device__ __forceinline__ float2 pair_of<__half>(const uint4& raw, int i) { return __half22float2(reinterpret_cast<const __half2*>(&raw)[i]); }
+template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float2* x) {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::E / 2; ++i) x[i] = pair_of<T>(raw, i);
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const float2* x) {
     __align__(16) T y[Chunk<T>::E];
 #pragma unroll
-    for (int i = 0; i < Chunk<T>::E; ++i) y[i] = num<T>(x[i]);
+    for (int i = 0; i < Chunk<T>::E / 2; ++i) y[2 * i] = num<T>(x[i].x), y[2 * i + 1] = num<T>(x[i].y);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(y);
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// n / d for n < 2^31 by a product (Granlund and Montgomery, "Division by invariant integers using multiplication"): d's multiplier and shift come from the host
+__device__ __forceinline__ unsigned over(unsigned n, const unsigned (&d)[2]) { return (__umulhi(n, d[0]) + n) >> d[1]; }
 template <int TPH> __device__ __forceinline__ float head_sum(float v) {
 #pragma unroll
     for (int o = TPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -189,151 +199,168 @@ template <typename T, int TPH> __device__ __forceinline__ Place place_of(const A
     p.turns[0] = p.at[0] < a.R, p.turns[1] = p.at[1] < a.R;
     return p;
 }
-// Cosines and sines of a thread's numbers: pairs of neighbours have E / 2 each per vector, halves E for both
-template <int E> __device__ __forceinline__ void load_table(const float* p, float* x) {
+// Cosines or sines, N in a row
+template <int N> __device__ __forceinline__ void load_table(const float* p, float2* x) {
 #pragma unroll
-    for (int i = 0; i < E; i += (E % 4 ? 2 : 4))
-        if constexpr (E % 4 == 0) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(p + i);
-        else *reinterpret_cast<float2*>(x + i) = *reinterpret_cast<const float2*>(p + i);
+    for (int i = 0; i < N; i += 4)
+        if constexpr (N % 4 == 0) {
+            const float4 y = __ldg(reinterpret_cast<const float4*>(p + i));
+            x[i / 2] = make_float2(y.x, y.y), x[i / 2 + 1] = make_float2(y.z, y.w);
+        } else x[i / 2] = __ldg(reinterpret_cast<const float2*>(p + i));
 }
 // (a, b) -> (a cos - b sin, a sin + b cos), with the sine's sign
-template <typename T, bool INTER> __device__ __forceinline__ void turn(const Args& a, const Place& p, long long pos, float sign, float* x) {
+template <typename T, bool INTER> __device__ __forceinline__ void turn(const Args& a, const Place& p, long long pos, float sign, float2* x) {
     constexpr int E = Chunk<T>::E;
     const int half = a.R / 2;
     const float *cos = a.cos + pos * half, *sin = a.sin + pos * half;
-    float c[E], s[E];
     if constexpr (!INTER) {
         if (!p.turns[0]) return;
+        float2 c[E / 2], s[E / 2];
         load_table<E>(cos + p.at[0], c);
         load_table<E>(sin + p.at[0], s);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float u = x[i], v = x[E + i], sn = sign * s[i];
-            x[i] = u * c[i] - v * sn, x[E + i] = u * sn + v * c[i];
+        for (int i = 0; i < E / 2; ++i) {
+            const float2 u = x[i], v = x[E / 2 + i], sn = __fmul2_rn(s[i], both(sign));
+            x[i] = __ffma2_rn(v, make_float2(-sn.x, -sn.y), __fmul2_rn(u, c[i]));
+            x[E / 2 + i] = __ffma2_rn(u, sn, __fmul2_rn(v, c[i]));
         }
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (!p.turns[h]) continue;
+            float2 c[E / 4], s[E / 4];
             load_table<E / 2>(cos + p.at[h] / 2, c);
             load_table<E / 2>(sin + p.at[h] / 2, s);
 #pragma unroll
             for (int i = 0; i < E / 2; ++i) {
-                const float u = x[h * E + 2 * i], v = x[h * E + 2 * i + 1], sn = sign * s[i];
-                x[h * E + 2 * i] = u * c[i] - v * sn, x[h * E + 2 * i + 1] = u * sn + v * c[i];
+                float2& y = x[h * (E / 2) + i];
+                const float cs = i & 1 ? c[i / 2].y : c[i / 2].x, sn = sign * (i & 1 ? s[i / 2].y : s[i / 2].x);
+                y = make_float2(y.x * cs - y.y * sn, y.x * sn + y.y * cs);
             }
         }
     }
 }
-// Head `it` of a kind: its token's row, and where it lies in the projection
-struct Head { long long row, from; };
+// Head `it` of a kind: its token, its row in the tables if it is its place, and where it lies in the projection
+struct Head { unsigned row, t; long long from; };
 __device__ __forceinline__ Head head_of(const Args& a, int kind, unsigned it, long long ld_b, long long ld_t) {
-    const unsigned n = kind == 0 ? a.G * a.r : a.G, row = it / n, h = it - row * n, g = kind == 0 ? h / a.r : h;
-    const unsigned b = ld_b == ld_t * a.T ? 0u : row / a.T;
     Head y;
-    y.row = row;
-    y.from = b * ld_b + (long long)(row - b * a.T) * ld_t + (long long)(kind == 0 ? h + 2 * g : g * (a.r + 2) + a.r + kind - 1) * a.D;
+    y.row = over(it, a.div[kind == 0 ? 0 : 1]);
+    const unsigned h = it - y.row * (kind == 0 ? a.G * a.r : a.G), b = over(y.row, a.div[3]);
+    y.t = y.row - b * a.T;
+    y.from = b * ld_b + y.t * ld_t + (long long)(kind == 0 ? h + 2 * over(h, a.div[2]) : h * (a.r + 2) + a.r + kind - 1) * a.D;
     return y;
 }
+__device__ __forceinline__ uint4 load16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
 template <typename T, int TPH, bool INTER>
-__global__ void __launch_bounds__(VT) heads_vec_kernel(const Args a) {
+__global__ void __launch_bounds__(VT, 4) heads_vec_kernel(const Args a) {
     constexpr int E = Chunk<T>::E, HEADS = VT / TPH;
     const Place p = place_of<T, TPH>(a);
     const void* wp = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr;
-    float w[2 * E];
+    float2 w[E];
     if (wp != nullptr && p.in)
 #pragma unroll
-        for (int i = 0; i < 2 * E; ++i) w[i] = weight(wp, a.w_type, p.at[i / E] + i % E);
-    T* out = (T*)(p.kind == 0 ? a.q : p.kind == 1 ? a.k : a.v);
-    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1);
-    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += p.blocks * HEADS) {
-        const unsigned it = it0 + threadIdx.x / TPH;
-        const bool there = p.in && it < items;
-        float x[2 * E];
-#pragma unroll
-        for (int i = 0; i < 2 * E; ++i) x[i] = 0.f;
-        Head h;
-        if (there) {
-            h = head_of(a, p.kind, it, a.x_b, a.x_t);
-            load_chunk((const T*)a.x + h.from + p.at[0], x);
-            load_chunk((const T*)a.x + h.from + p.at[1], x + E);
+        for (int i = 0; i < E; ++i) {
+            const int d = p.at[2 * i / E] + 2 * i % E;
+            w[i] = make_float2(weight(wp, a.w_type, d), weight(wp, a.w_type, d + 1));
         }
+    T* out = (T*)(p.kind == 0 ? a.q : p.kind == 1 ? a.k : a.v);
+    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1), step = p.blocks * HEADS;
+    unsigned it = p.block * HEADS + threadIdx.x / TPH;
+    // the next head's numbers are on their way while this one's are worked on
+    Head next;
+    uint4 raw[2] = {};
+    auto fetch = [&](unsigned i) {
+        if (!p.in || i >= items) return;
+        next = head_of(a, p.kind, i, a.x_b, a.x_t);
+        const T* x = (const T*)a.x + next.from;
+        raw[0] = load16(x + p.at[0]), raw[1] = load16(x + p.at[1]);
+    };
+    fetch(it);
+    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += step, it += step) {
+        const bool there = p.in && it < items;
+        const Head h = next;
+        float2 x[E];
+        unpack<T>(raw[0], x), unpack<T>(raw[1], x + E / 2);
+        fetch(it + step);
         if (wp != nullptr) {
-            float sum = 0.f;
+            float2 sum = both(0.f);
 #pragma unroll
-            for (int i = 0; i < 2 * E; ++i) sum += x[i] * x[i];
-            const float inv = 1.f / sqrtf(head_sum<TPH>(sum) / a.D + a.eps);
+            for (int i = 0; i < E; ++i) sum = __ffma2_rn(x[i], x[i], sum);
+            const float inv = 1.f / sqrtf(head_sum<TPH>(p.in ? sum.x + sum.y : 0.f) / a.D + a.eps);
 #pragma unroll
-            for (int i = 0; i < 2 * E; ++i) x[i] = x[i] * inv * w[i];
+            for (int i = 0; i < E; ++i) x[i] = __fmul2_rn(__fmul2_rn(x[i], both(inv)), w[i]);
         }
         if (!there) continue;
-        if (a.R > 0 && p.kind < 2) turn<T, INTER>(a, p, row_of(a, h.row), 1.f, x);
+        if (a.R > 0 && p.kind < 2) turn<T, INTER>(a, p, a.at == nullptr ? h.t : row_of(a, h.row), 1.f, x);
         store_chunk(out + (long long)it * a.D + p.at[0], x);
-        store_chunk(out + (long long)it * a.D + p.at[1], x + E);
+        store_chunk(out + (long long)it * a.D + p.at[1], x + E / 2);
     }
 }
 
 template <typename T, int TPH, bool INTER>
-__global__ void __launch_bounds__(VT) heads_vec_bwd_kernel(const Args a) {
+__global__ void __launch_bounds__(VT, 2) heads_vec_bwd_kernel(const Args a) {
     constexpr int E = Chunk<T>::E, HEADS = VT / TPH;
     __shared__ float red[HEADS][TPH * 2 * E];
     const Place p = place_of<T, TPH>(a);
     pdl_trigger();
     const void* wp = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr;
-    float w[2 * E], dw[2 * E];
+    float2 w[E], dw[E];
 #pragma unroll
-    for (int i = 0; i < 2 * E; ++i) {
-        dw[i] = 0.f;
-        w[i] = wp != nullptr && p.in ? weight(wp, a.w_type, p.at[i / E] + i % E) : 0.f;
+    for (int i = 0; i < E; ++i) {
+        const int d = p.at[2 * i / E] + 2 * i % E;
+        dw[i] = both(0.f);
+        w[i] = wp != nullptr && p.in ? make_float2(weight(wp, a.w_type, d), weight(wp, a.w_type, d + 1)) : both(0.f);
     }
     const T* from = (const T*)(p.kind == 0 ? a.dq : p.kind == 1 ? a.dk : a.dv);
-    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1);
+    const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1), step = p.blocks * HEADS;
     const long long ld = (long long)a.G * (a.r + 2) * a.D;
-    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += p.blocks * HEADS) {
-        const unsigned it = it0 + threadIdx.x / TPH;
-        const bool there = p.in && it < items;
-        float x[2 * E], dy[2 * E];
-#pragma unroll
-        for (int i = 0; i < 2 * E; ++i) x[i] = dy[i] = 0.f;
-        Head h, to;
-        if (there) {
-            to = head_of(a, p.kind, it, ld * a.T, ld);
-            if (from != nullptr) {
-                load_chunk(from + (long long)it * a.D + p.at[0], dy);
-                load_chunk(from + (long long)it * a.D + p.at[1], dy + E);
-            }
-            if (wp != nullptr) {
-                h = head_of(a, p.kind, it, a.x_b, a.x_t);
-                load_chunk((const T*)a.x + h.from + p.at[0], x);
-                load_chunk((const T*)a.x + h.from + p.at[1], x + E);
-            }
-            if (a.R > 0 && p.kind < 2 && from != nullptr) turn<T, INTER>(a, p, row_of(a, to.row), -1.f, dy);
-        }
+    const bool same = a.x_t == ld && a.x_b == ld * a.T;                // the projection and its gradient lie alike
+    unsigned it = p.block * HEADS + threadIdx.x / TPH;
+    Head next;
+    uint4 raw_x[2] = {}, raw_d[2] = {};
+    auto fetch = [&](unsigned i) {
+        if (!p.in || i >= items) return;
+        next = head_of(a, p.kind, i, ld * a.T, ld);
+        if (from != nullptr) raw_d[0] = load16(from + (long long)i * a.D + p.at[0]), raw_d[1] = load16(from + (long long)i * a.D + p.at[1]);
         if (wp != nullptr) {
-            float sum = 0.f, dot = 0.f;
+            const T* x = (const T*)a.x + (same ? next.from : head_of(a, p.kind, i, a.x_b, a.x_t).from);
+            raw_x[0] = load16(x + p.at[0]), raw_x[1] = load16(x + p.at[1]);
+        }
+    };
+    fetch(it);
+    for (unsigned it0 = p.block * HEADS; it0 < items; it0 += step, it += step) {
+        const bool there = p.in && it < items;
+        const Head h = next;
+        float2 x[E], dy[E];
+        unpack<T>(raw_x[0], x), unpack<T>(raw_x[1], x + E / 2);
+        unpack<T>(raw_d[0], dy), unpack<T>(raw_d[1], dy + E / 2);
+        fetch(it + step);
+        if (there && a.R > 0 && p.kind < 2 && from != nullptr) turn<T, INTER>(a, p, a.at == nullptr ? h.t : row_of(a, h.row), -1.f, dy);
+        if (wp != nullptr) {
+            float2 sum = both(0.f), dot = both(0.f);
 #pragma unroll
-            for (int i = 0; i < 2 * E; ++i) sum += x[i] * x[i];
-            const float rms = sqrtf(head_sum<TPH>(sum) / a.D + a.eps), inv = it < items ? 1.f / rms : 0.f;      // (threads without a head add nothing)
+            for (int i = 0; i < E; ++i) sum = __ffma2_rn(x[i], x[i], sum);
+            const float rms = sqrtf(head_sum<TPH>(p.in ? sum.x + sum.y : 0.f) / a.D + a.eps), inv = there ? 1.f / rms : 0.f;      // (threads without a head add nothing)
 #pragma unroll
-            for (int i = 0; i < 2 * E; ++i) {
-                x[i] *= inv;
-                dw[i] += dy[i] * x[i];
-                dy[i] *= w[i];
-                dot += dy[i] * x[i];
+            for (int i = 0; i < E; ++i) {
+                x[i] = __fmul2_rn(x[i], both(inv));
+                dw[i] = __ffma2_rn(dy[i], x[i], dw[i]);
+                dy[i] = __fmul2_rn(dy[i], w[i]);
+                dot = __ffma2_rn(dy[i], x[i], dot);
             }
-            dot = head_sum<TPH>(dot) / a.D;
+            const float mean = head_sum<TPH>(there ? dot.x + dot.y : 0.f) / a.D;
 #pragma unroll
-            for (int i = 0; i < 2 * E; ++i) dy[i] = (dy[i] - x[i] * dot) * inv;
+            for (int i = 0; i < E; ++i) dy[i] = __fmul2_rn(__ffma2_rn(x[i], both(-mean), dy[i]), both(inv));
         }
         if (!there) continue;
-        store_chunk((T*)a.dx + to.from + p.at[0], dy);
-        store_chunk((T*)a.dx + to.from + p.at[1], dy + E);
+        store_chunk((T*)a.dx + h.from + p.at[0], dy);
+        store_chunk((T*)a.dx + h.from + p.at[1], dy + E / 2);
     }
     if (a.part == nullptr || wp == nullptr) return;
     if (p.in)
 #pragma unroll
-        for (int i = 0; i < 2 * E; ++i) red[threadIdx.x / TPH][p.at[i / E] + i % E] = dw[i];
+        for (int i = 0; i < E; ++i) *reinterpret_cast<float2*>(&red[threadIdx.x / TPH][p.at[2 * i / E] + 2 * i % E]) = dw[i];
     __syncthreads();
     float* out = a.part + (long long)(p.kind == 0 ? p.block : a.parts_q + p.block) * a.D;
     for (int d = threadIdx.x; d < a.D; d += VT) {

@@ -21,7 +21,7 @@ from .scored_attn import on_device
 class _Args(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "wq", "wk", "q", "k", "v", "cos", "sin", "at", "dq", "dk", "dv", "dx", "dwq", "dwk", "part")] +
                 [(n, ctypes.c_longlong) for n in ("x_b", "x_t", "rows")] +
-                [(n, ctypes.c_int) for n in ("T", "G", "r", "D", "R", "tokens", "interleaved", "at_wide", "w_type", "parts", "vectors", "parts_q", "parts_k")] +
+                [(n, ctypes.c_int) for n in ("T", "G", "r", "D", "R", "tokens", "interleaved", "at_wide", "w_type", "parts")] + [("div", ctypes.c_uint * 8)] + [(n, ctypes.c_int) for n in ("vectors", "parts_q", "parts_k")] +
                 [("eps", ctypes.c_float), ("err", ctypes.c_void_p)])
 
 
@@ -78,7 +78,15 @@ def _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved) -> byt
     w = q_weight if q_weight is not None else k_weight
     a = _Args(x_b=qkv.stride(0), x_t=qkv.stride(1), rows=B * T, T=T, G=G, r=S - 2, D=D, R=0 if cos is None else 2 * cos.shape[1], tokens=0 if cos is None else cos.shape[0],
               interleaved=int(interleaved), at_wide=int(positions is not None and positions.dtype == torch.int64), w_type=0 if w is None else _TYPES[w.dtype], parts=0, eps=eps)
+    for i, d in enumerate((a.G * a.r, a.G, a.r, a.T)):
+        a.div[2 * i:2 * i + 2] = _divisor(max(d, 1))
     return bytes(a)
+
+
+def _divisor(d: int):
+    """Multiplier and shift of a division by d (``over`` in csrc/qkv_heads.cu): floor(2^32 (2^s - d) / d) + 1 with s = ceil(log2 d)."""
+    s = (d - 1).bit_length()
+    return (((1 << s) - d << 32) // d + 1) & 0xffffffff, s
 
 
 def _dense_heads(t: torch.Tensor) -> bool:
@@ -93,7 +101,7 @@ def _blocks(a: _Args, size: int, back: bool):
     while threads * 2 * (16 // size) < a.D:
         threads *= 2
     keys = -(-a.rows * a.G * threads // 256)
-    most = (4 if back else 6) * K.num_sms()
+    most = (2 if back else 4) * K.num_sms()
     share = max(1, min(keys, most // (a.r + 2)))
     a.parts_k, a.parts_q = share, max(1, min(-(-a.rows * a.G * a.r * threads // 256), most - 2 * share))
     a.parts = a.parts_q + 2 * share

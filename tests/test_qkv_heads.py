@@ -294,3 +294,16 @@ def test_nothing_and_positions_outside_on_the_gpu():
             s["at"][0, 1] = near
             assert all(torch.equal(x, y) for x, y in zip(got, ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"], positions=s["at"])))
     assert math.isfinite(float(got[0].float().sum()))
+
+
+def test_divisions():
+    """n / d as the kernel does it: a product's upper half, a sum that stays below 2^32, a shift."""
+    from linear_moe_b200.ops.qkv_heads import _divisor
+    gen = torch.Generator().manual_seed(0)
+    for d in [1, 2, 3, 5, 7, 8, 31, 32, 33, 48, 1000, 4097, 16384, 65535, (1 << 20) + 1, (1 << 30) - 1, 1 << 30, (1 << 31) - 1] + torch.randint(1, 1 << 31, (200,), generator=gen).tolist():
+        m, s = _divisor(d)
+        assert m < 1 << 32
+        top = (1 << 31) - 1
+        for n in {0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, top, top // d * d, max(top // d * d - 1, 0)} | set(torch.randint(0, top, (20,), generator=gen).tolist()):
+            if n <= top:
+                assert ((m * n >> 32) + n) >> s == n // d, (n, d)
