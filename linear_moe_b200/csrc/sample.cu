@@ -37,6 +37,10 @@ typedef unsigned long long u64;
 __device__ __forceinline__ float val(float x) { return x; }
 __device__ __forceinline__ float val(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float val(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T num(float x);
+template <> __device__ __forceinline__ float num<float>(float x) { return x; }
+template <> __device__ __forceinline__ bf16 num<bf16>(float x) { return __float2bfloat16(x); }
+template <> __device__ __forceinline__ __half num<__half>(float x) { return __float2half(x); }
 // NaN counts as minus infinity, zeros are equal
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x == 0.f ? 0.f : x; }
 // Whole numbers in the order of the floating-point ones
@@ -70,13 +74,14 @@ struct Shared {
     double powers[32];
     uint32_t count[WARPS];
     u64 mass[WARPS];
-    u64 total;                                         // of this CTA, read by the others
-    uint32_t ties, top;
-    int found;
+    uint32_t top;                                      // this CTA's, read by the others
+    u64 above[WARPS];                                  // per warp: weight of the tokens above the edge, and how many lie on it
+    uint32_t on_edge[WARPS];
+    int found, chosen;
     uint32_t at_count;
     u64 at_mass;
-    int owner;
-    u64 rest;
+    uint32_t tied;                                     // of the chosen warp: tokens on the edge, and weight, ahead of it
+    u64 ahead, whole, goal;
 };
 
 __device__ __forceinline__ u64 up_to(u64 v) {          // inclusive over the lanes
@@ -112,16 +117,33 @@ template <typename N> __device__ __forceinline__ N before(N v, N* warps, N& all)
     return ahead + in - v;
 }
 
+// Four neighbouring logits; `n`: how many there are.  Those behind the last one are minus infinity, and weigh nothing.
+template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&x)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(p);
+        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+    } else {
+        const uint2 raw = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = val(reinterpret_cast<const T*>(&raw)[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = clean(x[i]);
+}
+template <typename T> __device__ __forceinline__ void some_of(const T* p, int left, float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = i < left ? clean(val(p[i])) : -INFINITY;
+}
+
 template <typename T, bool HELD>                       // HELD: the part of a row lies in shared memory
 __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     extern __shared__ __align__(16) unsigned char held[];
     __shared__ Shared sm;
     cg::cluster_group cl = cg::this_cluster();
-    const int b = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const int b = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = rank * a.len, n = max(0, min(a.len, a.V - first));
     const T* row = (const T*)a.logits + b * a.ld + first;
     T* mine = reinterpret_cast<T*>(held);
-    const T* x = HELD ? mine : row;
     if (tid < 32) sm.powers[tid] = POWERS[tid];
     for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[0])[i] = 0;
 
@@ -133,17 +155,33 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     const bool by_mass = top_p < 1.f && k > 1, cut = by_mass || k < a.V;
 
     // the part, and the largest logit
+    constexpr int E = 16 / sizeof(T);
+    const bool wide = reinterpret_cast<uintptr_t>(row) % 16 == 0;
+    const int padded = (n + 127) & ~127;               // (a.len is a multiple of 128)
     float top = -INFINITY;
-    for (int i = tid; i < n; i += THREADS) {
+    if (wide) {
+#pragma unroll 4
+        for (int i = tid * E; i + E <= n; i += THREADS * E) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
+            if constexpr (HELD) *reinterpret_cast<uint4*>(mine + i) = raw;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, clean(val(reinterpret_cast<const T*>(&raw)[e])));
+        }
+    }
+#pragma unroll 4
+    for (int i = (wide ? n / E * E : 0) + tid; i < n; i += THREADS) {
         const T raw = row[i];
         if constexpr (HELD) mine[i] = raw;
         top = fmaxf(top, clean(val(raw)));
     }
+    if constexpr (HELD)
+        for (int i = n + tid; i < padded; i += THREADS) mine[i] = num<T>(-INFINITY);
     top = warp_max(top);
-    if (lane == 0) sm.count[tid >> 5] = key_of(top);
+    if (lane == 0) sm.count[warp] = key_of(top);
     __syncthreads();
     if (tid == 0) {
         uint32_t y = 0;
+#pragma unroll
         for (int w = 0; w < WARPS; ++w) y = max(y, sm.count[w]);
         sm.top = y;
     }
@@ -153,53 +191,68 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     Scale s;
     s.max = __uint_as_float(top_key >> 31 ? top_key & 0x7fffffffu : ~top_key);
     s.c = greedy ? 1.0 : 1.4426950408889634 / (double)temperature;
+    auto four = [&](int i, float (&x)[4]) {            // logits i .. i + 3 of the part
+        if constexpr (HELD) four_of(mine + i, x);
+        else if (wide && i + 4 <= n) four_of(row + i, x);
+        else some_of(row + i, n - i, x);
+    };
 
-    // the bin that the cut lies in, then the logit: tokens with keys above `edge` are kept, and `ties` of those equal to it
-    uint32_t edge = 0, ties = 0xffffffffu;
+    // The logit that the cut lies at: tokens with keys above `edge` are kept, and `ties` of those equal to it.  First its bin (16 of them for a factor of two in weight), then its key among those of the bin.
+    uint32_t edge = 0, ties = 0;
     int turn = 0;
     if (cut && k == 1) edge = top_key, ties = 1;
     else if (cut) {
         const float slope = (float)fmin(s.c * PER_OCTAVE, 1e30);
-        uint32_t lo = 0, hi = 0;                       // keys of the bin; level 0: not yet known
-        int shift = 0;
-        uint32_t ahead = 0;                            // tokens, and weight, above the bin
+        auto bin_of = [&](float v) -> int { return min((int)((s.max - v) * slope), BINS - 1); };      // (infinite logits: of infinity alone, in bin 0)
+        uint32_t lo = key_of(-INFINITY), hi = top_key; // around the keys of the bin
+        int shift = 0, chosen = 0;
+        uint32_t ahead = 0;                            // tokens, and weight, above the edge
         u64 ahead_mass = 0, limit = ~0ull;             // a token is kept if less than the limit comes before it
         for (int level = 0;; ++level, turn ^= 1) {
             Bins& h = sm.bins[turn];
-            for (int i = tid; i < n; i += THREADS) {
-                const float v = clean(val(x[i]));
-                const uint32_t key = key_of(v);
-                if (level > 0 && (key < lo || key > hi)) continue;
-                const u64 w = weight(v, s, sm.powers);
-                if (w == 0) continue;                  // never drawn
-                const int bin = level == 0 ? min((int)((s.max - v) * slope), BINS - 1) : (int)((hi - key) >> shift);
-                atomicAdd(&h.count[bin], 1u);
-                if (by_mass)
+            for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+                float x[4];
+                four(i, x);
 #pragma unroll
-                    for (int j = 0; j < 3; ++j) {
-                        const uint32_t y = (uint32_t)(w >> (15 * j)) & 0x7fffu;
-                        if (y) atomicAdd(&h.part[j][bin], y);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float v = x[e];
+                    const uint32_t key = key_of(v);
+                    if (level > 0 && (key < lo || key > hi || bin_of(v) != chosen)) continue;
+                    const u64 w = weight(v, s, sm.powers);
+                    if (w == 0) continue;              // never drawn
+                    const int bin = level == 0 ? bin_of(v) : (int)((hi - key) >> shift);
+                    atomicAdd(&h.count[bin], 1u);
+                    if (by_mass)
+#pragma unroll
+                        for (int j = 0; j < 3; ++j) {
+                            const uint32_t y = (uint32_t)(w >> (15 * j)) & 0x7fffu;
+                            if (y) atomicAdd(&h.part[j][bin], y);
+                        }
+                }
             }
             cl.sync();
             for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[turn ^ 1])[i] = 0;
             uint32_t count[2] = {0, 0};
             u64 mass[2] = {0, 0};
+            if (2 * tid < BINS)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int bin = 2 * tid + j;
-                if (bin < BINS)
-                    for (int r = 0; r < a.parts; ++r) {
-                        const Bins* o = cl.map_shared_rank(&h, r);
-                        count[j] += o->count[bin];
-                        if (by_mass) mass[j] += (u64)o->part[0][bin] + ((u64)o->part[1][bin] << 15) + ((u64)o->part[2][bin] << 30);
+                for (int r = 0; r < MAX_PARTS; ++r) {
+                    if (r >= a.parts) break;
+                    const Bins* o = cl.map_shared_rank(&h, r);
+                    const uint2 c = *reinterpret_cast<const uint2*>(&o->count[2 * tid]);
+                    count[0] += c.x, count[1] += c.y;
+                    if (by_mass) {
+                        const uint2 p0 = *reinterpret_cast<const uint2*>(&o->part[0][2 * tid]), p1 = *reinterpret_cast<const uint2*>(&o->part[1][2 * tid]),
+                                    p2 = *reinterpret_cast<const uint2*>(&o->part[2][2 * tid]);
+                        mass[0] += (u64)p0.x + ((u64)p1.x << 15) + ((u64)p2.x << 30);
+                        mass[1] += (u64)p0.y + ((u64)p1.y << 15) + ((u64)p2.y << 30);
                     }
-            }
+                }
             uint32_t all;
-            u64 all_mass;
+            u64 all_mass = 0, m0 = ahead_mass;
             if (tid == 0) sm.found = -1;
             const uint32_t c0 = ahead + before(count[0] + count[1], sm.count, all);
-            const u64 m0 = ahead_mass + before(mass[0] + mass[1], sm.mass, all_mass);
+            if (by_mass) m0 += before(mass[0] + mass[1], sm.mass, all_mass);
             if (level == 0 && by_mass) limit = top_p > 0.f ? max(1ull, (u64)ceil((double)top_p * (double)all_mass)) : 1ull;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -215,41 +268,22 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             }
             __syncthreads();
             if (bin < 0) break;                        // nothing above minus infinity
+            if (level == 0 && !by_mass && all <= (uint32_t)k) break;      // no more tokens than k
             ahead = sm.at_count;
             ahead_mass = sm.at_mass;
             if (level == 0) {
-                if (!by_mass && all <= (uint32_t)k) break;     // no more tokens than k
-                // Keys that are certainly around the bin's (roundings are within 2^-22 of the logits), then its ends by bisection: bins fall as keys rise.
-                hi = top_key, lo = key_of(-INFINITY);
-                if (slope > 1e-20f && slope < 1e20f) {
-                    const float up = s.max - (float)bin / slope, down = bin == BINS - 1 ? -INFINITY : s.max - (float)(bin + 1) / slope;
-                    const float slack = 1e-6f * (fabsf(s.max) + fabsf(up) + (down == -INFINITY ? 0.f : fabsf(down)));
-                    hi = min(hi, key_of(clean(up + slack) == -INFINITY ? INFINITY : up + slack));
-                    lo = max(lo, key_of(clean(down - slack)));
+                chosen = bin;
+                // The bin's logits, and some beside them: roundings are within 2^-22 of the numbers that go in.  (An endless or vanishing temperature: all logits.)
+                if (slope > 1e-20f && slope < 1e20f && fabsf(s.max) < 1e30f) {
+                    const float up = s.max - (float)bin / slope, down = s.max - (float)(bin + 1) / slope, slack = 1e-6f * (fabsf(s.max) + fabsf(up) + fabsf(down));
+                    hi = min(hi, key_of(clean(up + slack)));
+                    if (bin < BINS - 1) lo = max(lo, key_of(clean(down - slack)));
                 }
-                auto bin_of = [&](uint32_t key) -> int {
-                    const float v = __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
-                    return min((int)((s.max - v) * slope), BINS - 1);
-                };
-                uint32_t l = lo, h2 = hi;              // the largest key of this bin
-                while (l < h2) {
-                    const uint32_t mid = l + (h2 - l + 1) / 2;
-                    if (bin_of(mid) >= bin) l = mid;
-                    else h2 = mid - 1;
-                }
-                hi = l;
-                l = lo, h2 = hi;                       // the smallest one
-                while (l < h2) {
-                    const uint32_t mid = l + (h2 - l) / 2;
-                    if (bin_of(mid) <= bin) h2 = mid;
-                    else l = mid + 1;
-                }
-                lo = l;
             } else {
                 hi -= (uint32_t)bin << shift;
                 lo = max(lo, hi - ((1u << shift) - 1));
             }
-            if (lo == hi) {
+            if (level > 0 && lo == hi) {
                 edge = lo;
                 const u64 w = weight(__uint_as_float(edge >> 31 ? edge & 0x7fffffffu : ~edge), s, sm.powers);
                 ties = (uint32_t)k - ahead;
@@ -259,61 +293,97 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             shift = max(0, 32 - __clz(hi - lo) - SUB_BITS);
         }
     }
-    __syncthreads();
 
-    // a thread's share of the part, in order: an odd number of words, so that neighbours read from different banks
-    constexpr int WORD = sizeof(T) == 4 ? 1 : 2;
-    int share = (n + THREADS - 1) / THREADS;
-    share = ((share + WORD - 1) / WORD | 1) * WORD;
-    const int from = min(n, tid * share), to = min(n, from + share);
-    // ties that lie before this thread's
-    uint32_t tied = 0;
-    if (cut && ties != 0xffffffffu) {
-        uint32_t own = 0, all;
-        for (int i = from; i < to; ++i) own += key_of(clean(val(x[i]))) == edge;
-        tied = before(own, sm.count, all);
-        if (tid == 0) sm.ties = all;
-        cl.sync();
-        for (int r = 0; r < rank; ++r) tied += *cl.map_shared_rank(&sm.ties, r);
-    }
+    // Kept weight: a warp takes a segment of the part, in order.  Tokens on the edge weigh the same, so their number is enough.
     const u64 least = min_p > 0.f ? (u64)ceil((double)min_p * (double)(1ull << BITS)) : 0ull;
-    // the kept weight of token i, whose predecessors among the ties are `t`
-    auto kept = [&](int i, uint32_t& t) -> u64 {
-        const float v = clean(val(x[i]));
-        if (cut) {
-            const uint32_t key = key_of(v);
-            if (key < edge || (key == edge && t++ >= ties)) return 0;
-        }
+    auto kept = [&](float v, uint32_t key) -> u64 {    // of a token above the edge
+        if (key <= edge) return 0;
         const u64 w = weight(v, s, sm.powers);
         return w >= least || v == s.max ? w : 0;       // the largest ones stay whatever min_p
     };
-    u64 sum = 0, all;
-    uint32_t t = tied;
-    for (int i = from; i < to; ++i) sum += kept(i, t);
-    u64 ahead = before(sum, sm.mass, all);
-    if (tid == 0) sm.total = all, sm.owner = -1;
-    cl.sync();
-    u64 whole = 0, parts_ahead = 0;
-    for (int r = 0; r < a.parts; ++r) {
-        const u64 y = *cl.map_shared_rank(&sm.total, r);
-        if (r < rank) parts_ahead += y;
-        whole += y;
+    const float edge_value = __uint_as_float(edge >> 31 ? edge & 0x7fffffffu : ~edge);
+    u64 edge_weight = 0;
+    if (edge != 0) {
+        edge_weight = weight(edge_value, s, sm.powers);
+        if (edge_weight < least && edge_value != s.max) edge_weight = 0;
     }
-    ahead += parts_ahead;
+    const int seg = (padded / 128 + WARPS - 1) / WARPS * 128, from = min(padded, warp * seg), to = min(padded, from + seg);
+    u64 sum = 0;
+    uint32_t on = 0;
+    for (int i = from + 4 * lane; i < to; i += 128) {
+        float x[4];
+        four(i, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t key = key_of(x[e]);
+            sum += kept(x[e], key);
+            on += edge != 0 && key == edge;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        on += __shfl_xor_sync(0xffffffffu, on, o);
+    }
+    if (lane == 0) sm.above[warp] = sum, sm.on_edge[warp] = on;
+    if (tid == 0) sm.chosen = -1;
+    cl.sync();
+    // the segments of all CTAs, in order: a thread each
+    const bool one = tid < a.parts * WARPS;
+    const u64 above = one ? *cl.map_shared_rank(&sm.above[tid % WARPS], tid / WARPS) : 0;
+    const uint32_t edges = one ? *cl.map_shared_rank(&sm.on_edge[tid % WARPS], tid / WARPS) : 0;
+    uint32_t all_edges;
+    u64 whole;
+    const uint32_t tied = before(edges, sm.count, all_edges);
+    const u64 weight_here = above + edge_weight * (tied >= ties ? 0u : min(edges, ties - tied));
+    const u64 ahead = before(weight_here, sm.mass, whole);
     const double u = (double)a.draw[b];
     u64 goal = u > 0.0 ? (u64)(u * (double)whole) : 0ull;      // the token up to which the weights exceed it
     if (whole > 0 && goal >= whole) goal = whole - 1;
-    if (sum > 0 && ahead <= goal && goal < ahead + sum) {
-        u64 upto = ahead;
-        t = tied;
-        for (int i = from; i < to; ++i) {
-            const u64 w = kept(i, t);
-            upto += w;
-            if (upto > goal) {
-                a.token[b] = first + i;
-                a.logp[b] = (float)log((double)w / (double)whole);
-                break;
+    if (one && tid / WARPS == rank && ahead <= goal && goal < ahead + weight_here) {
+        sm.chosen = tid % WARPS;
+        sm.tied = tied;
+        sm.ahead = ahead;
+    }
+    __syncthreads();
+    if (warp == sm.chosen) {
+        u64 sofar = sm.ahead;
+        uint32_t rank_on = sm.tied;
+        for (int i0 = from; i0 < to; i0 += 128) {
+            const int i = i0 + 4 * lane;
+            float x[4];
+            four(i, x);
+            u64 w[4], own = 0;
+            uint32_t mark = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t key = key_of(x[e]);
+                w[e] = kept(x[e], key);
+                mark += edge != 0 && key == edge;
             }
+            const uint32_t marks = up_to(mark);
+            uint32_t mine_on = rank_on + marks - mark;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (edge != 0 && key_of(x[e]) == edge && mine_on++ < ties) w[e] = edge_weight;
+                own += w[e];
+            }
+            const u64 upto = up_to(own);
+            rank_on += __shfl_sync(0xffffffffu, marks, 31);
+            const bool hit = sofar + upto - own <= goal && goal < sofar + upto;
+            if (hit) {
+                u64 y = sofar + upto - own;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (y <= goal && goal < y + w[e]) {
+                        a.token[b] = first + i + e;
+                        a.logp[b] = (float)log((double)w[e] / (double)whole);
+                    }
+                    y += w[e];
+                }
+            }
+            if (__any_sync(0xffffffffu, hit)) break;
+            sofar += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     if (whole == 0 && rank == 0 && tid == 0) a.token[b] = 0, a.logp[b] = -INFINITY;       // a row of nothing but minus infinity
@@ -323,7 +393,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
 template <typename T>
 static int launch(const Args& a, cudaStream_t st) {
     const long long bytes = (long long)a.len * sizeof(T);
-    const bool held = bytes <= 160 * 1024;
+    const bool held = bytes <= 192 * 1024;
     auto kernel = held ? sample_kernel<T, true> : sample_kernel<T, false>;
     if (held) {
         const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
@@ -351,6 +421,6 @@ static int launch(const Args& a, cudaStream_t st) {
 LMOE_API int lmoe_sample(const lmoe::sample::Args* ap, int type, cudaStream_t st) {
     using namespace lmoe::sample;
     const Args& a = *ap;
-    if (a.B <= 0 || a.B > 65535 || a.V <= 0 || a.V > 1 << 19 || a.parts < 1 || a.parts > MAX_PARTS || a.len <= 0 || a.len > 1 << 16 || (long long)a.parts * a.len < a.V) return -1;
+    if (a.B <= 0 || a.B > 65535 || a.V <= 0 || a.V > 1 << 19 || a.parts < 1 || a.parts > MAX_PARTS || a.len <= 0 || a.len > 1 << 16 || a.len % 128 != 0 || (long long)a.parts * a.len < a.V) return -1;
     return type == 0 ? launch<float>(a, st) : type == 1 ? launch<lmoe::bf16>(a, st) : launch<__half>(a, st);
 }

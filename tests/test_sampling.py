@@ -210,4 +210,4 @@ def test_refusals():
 @pytest.mark.parametrize("B,V", [(1, 1), (1, 4096), (1, 1 << 19), (128, 128256), (1000, 77), (7, 65537), (64, 65536)])
 def test_shares(B, V):
     parts, length = S._shares(B, V, 148)
-    assert parts in (1, 2, 4, 8) and parts * length >= V and length <= S.PART and length % 8 == 0
+    assert parts in (1, 2, 4, 8) and parts * length >= V and length <= S.PART and length % 128 == 0
