@@ -43,8 +43,14 @@ template <> __device__ __forceinline__ bf16 num<bf16>(float x) { return __float2
 template <> __device__ __forceinline__ __half num<__half>(float x) { return __float2half(x); }
 // NaN counts as minus infinity, zeros are equal
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x == 0.f ? 0.f : x; }
-// Whole numbers in the order of the floating-point ones
-__device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return b >> 31 ? ~b : b | 0x80000000u; }
+// Whole numbers in the order of the floating-point ones, without the bits that 16-bit types never have
+template <typename T> struct Spare { static constexpr int BITS = sizeof(T) == 4 ? 0 : sizeof(T) == 2 && alignof(T) == 2 ? 13 : 0; };
+template <> struct Spare<bf16> { static constexpr int BITS = 16; };
+template <typename T> __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return (b >> 31 ? ~b : b | 0x80000000u) >> Spare<T>::BITS; }
+template <typename T> __device__ __forceinline__ float value_of(uint32_t key) {
+    key <<= Spare<T>::BITS;
+    return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~(key | ((1u << Spare<T>::BITS) - 1)));
+}
 
 // 2^(i / 32)
 __constant__ double POWERS[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
@@ -52,25 +58,28 @@ __constant__ double POWERS[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1
     1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
     1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
-struct Scale { float max; double c; };                 // log2(e) / temperature
-// 2^44 exp((x - max) / temperature), rounded
+struct Scale { float top; double max, c; };            // the largest logit, log2(e) / temperature
+// 2^44 exp((x - max) / temperature), rounded.  (No branches, so that several go on side by side: with them a pass over 16000 logits took 28000 cycles.)
 __device__ __forceinline__ u64 weight(float x, const Scale& s, const double* powers) {
-    if (x == s.max) return x == -INFINITY ? 0 : 1ull << BITS;
-    if (x == -INFINITY || s.max == INFINITY) return 0;
-    const double y = ((double)x - (double)s.max) * s.c;
-    if (!(y > -46.0)) return 0;
+    double y = ((double)x - s.max) * s.c;
+    y = x == -INFINITY ? -64.0 : x == s.top ? 0.0 : fmax(y, -64.0);      // (infinities, whose differences and products may be NaN)
     const double magic = 6755399441055744.0;           // 1.5 2^52: what is added to it is rounded to a whole number in its lower bits
-    const double shifted = y * 32.0 + magic;
+    const double shifted = fma(y, 32.0, magic);
     const int n = (int)__double_as_longlong(shifted);
-    const double f = (y - (shifted - magic) * 0.03125) * 0.6931471805599453;      // up to ln 2 / 64
-    const double e = 1.0 + f * (1.0 + f * (0.5 + f * (1.0 / 6 + f * (1.0 / 24 + f * (1.0 / 120)))));
-    const double scaled = powers[n & 31] * e * __longlong_as_double((long long)(1023 + BITS + (n >> 5)) << 52);
-    return (u64)(__double_as_longlong(scaled + 6755399441055744.0) - 0x4338000000000000ll);
+    const double f = fma(shifted - magic, -0.03125, y) * 0.6931471805599453;      // up to ln 2 / 64
+    const double e = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
+    const double power = __longlong_as_double(__double_as_longlong(powers[n & 31]) + ((long long)(BITS + (n >> 5)) << 52));
+    return (u64)(__double_as_longlong(fma(power, e, magic)) - 0x4338000000000000ll);
 }
 
 struct Bins { uint32_t count[BINS], part[3][BINS]; };  // weights in three parts of 15 bits, whose sums over a CTA's logits 32 bits hold
+__device__ __forceinline__ u64 mass_of(const Bins& h, int bin) { return (u64)h.part[0][bin] + ((u64)h.part[1][bin] << 15) + ((u64)h.part[2][bin] << 30); }
+constexpr int COARSE = BINS / 32;
+static_assert(COARSE <= 32, "a lane for 32 bins");
 struct Shared {
     Bins bins[2];
+    u64 coarse_mass[COARSE], all_mass[MAX_PARTS][32];  // of 32 bins together, read by the others; what they have
+    uint32_t coarse_count[COARSE], all_count[MAX_PARTS][32];
     double powers[32];
     uint32_t count[WARPS];
     u64 mass[WARPS];
@@ -78,8 +87,8 @@ struct Shared {
     u64 above[WARPS];                                  // per warp: weight of the tokens above the edge, and how many lie on it
     uint32_t on_edge[WARPS];
     int found, chosen;
-    uint32_t at_count;
-    u64 at_mass;
+    uint32_t at_count, total_count;
+    u64 at_mass, total_mass;
     uint32_t tied;                                     // of the chosen warp: tokens on the edge, and weight, ahead of it
     u64 ahead, whole, goal;
 };
@@ -177,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     if constexpr (HELD)
         for (int i = n + tid; i < padded; i += THREADS) mine[i] = num<T>(-INFINITY);
     top = warp_max(top);
-    if (lane == 0) sm.count[warp] = key_of(top);
+    if (lane == 0) sm.count[warp] = key_of<T>(top);
     __syncthreads();
     if (tid == 0) {
         uint32_t y = 0;
@@ -189,7 +198,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     uint32_t top_key = 0;
     for (int r = 0; r < a.parts; ++r) top_key = max(top_key, *cl.map_shared_rank(&sm.top, r));
     Scale s;
-    s.max = __uint_as_float(top_key >> 31 ? top_key & 0x7fffffffu : ~top_key);
+    s.top = value_of<T>(top_key);
+    s.max = s.top;
     s.c = greedy ? 1.0 : 1.4426950408889634 / (double)temperature;
     auto four = [&](int i, float (&x)[4]) {            // logits i .. i + 3 of the part
         if constexpr (HELD) four_of(mine + i, x);
@@ -203,81 +213,101 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     if (cut && k == 1) edge = top_key, ties = 1;
     else if (cut) {
         const float slope = (float)fmin(s.c * PER_OCTAVE, 1e30);
-        auto bin_of = [&](float v) -> int { return min((int)((s.max - v) * slope), BINS - 1); };      // (infinite logits: of infinity alone, in bin 0)
-        uint32_t lo = key_of(-INFINITY), hi = top_key; // around the keys of the bin
+        auto bin_of = [&](float v) -> int { return min((int)((s.top - v) * slope), BINS - 1); };      // (infinite logits: of infinity alone, in bin 0)
+        uint32_t lo = key_of<T>(-INFINITY), hi = top_key; // around the keys of the bin
         int shift = 0, chosen = 0;
         uint32_t ahead = 0;                            // tokens, and weight, above the edge
         u64 ahead_mass = 0, limit = ~0ull;             // a token is kept if less than the limit comes before it
         for (int level = 0;; ++level, turn ^= 1) {
             Bins& h = sm.bins[turn];
+            uint32_t all = 0;
             for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
                 float x[4];
                 four(i, x);
+                uint32_t key[4];
+                bool in[4], any = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float v = x[e];
-                    const uint32_t key = key_of(v);
-                    if (level > 0 && (key < lo || key > hi || bin_of(v) != chosen)) continue;
-                    const u64 w = weight(v, s, sm.powers);
-                    if (w == 0) continue;              // never drawn
-                    const int bin = level == 0 ? bin_of(v) : (int)((hi - key) >> shift);
+                    key[e] = key_of<T>(x[e]);
+                    in[e] = level == 0 || (key[e] >= lo && key[e] <= hi && bin_of(x[e]) == chosen);
+                    any |= in[e];
+                }
+                if (!any) continue;
+                u64 w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = weight(x[e], s, sm.powers);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (!in[e] || w[e] == 0) continue; // (of no weight: never drawn)
+                    const int bin = level == 0 ? bin_of(x[e]) : (int)((hi - key[e]) >> shift);
                     atomicAdd(&h.count[bin], 1u);
                     if (by_mass)
 #pragma unroll
                         for (int j = 0; j < 3; ++j) {
-                            const uint32_t y = (uint32_t)(w >> (15 * j)) & 0x7fffu;
+                            const uint32_t y = (uint32_t)(w[e] >> (15 * j)) & 0x7fffu;
                             if (y) atomicAdd(&h.part[j][bin], y);
                         }
                 }
             }
+            __syncthreads();
+            // The CTAs' bins: sums of 32 neighbours first, which tell the 32 that have to be read.  (All bins of all CTAs: 98 KB a CTA through the cluster's network, 12000 cycles.)
+            for (int c = warp; c < COARSE; c += WARPS) {
+                uint32_t count = h.count[32 * c + lane];
+                u64 mass = mass_of(h, 32 * c + lane);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    count += __shfl_xor_sync(0xffffffffu, count, o);
+                    mass += __shfl_xor_sync(0xffffffffu, mass, o);
+                }
+                if (lane == 0) sm.coarse_count[c] = count, sm.coarse_mass[c] = mass;
+            }
             cl.sync();
             for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[turn ^ 1])[i] = 0;
-            uint32_t count[2] = {0, 0};
-            u64 mass[2] = {0, 0};
-            if (2 * tid < BINS)
+            uint32_t from_count = ahead;
+            u64 from_mass = ahead_mass;
+            int bin = 0;
 #pragma unroll
-                for (int r = 0; r < MAX_PARTS; ++r) {
-                    if (r >= a.parts) break;
-                    const Bins* o = cl.map_shared_rank(&h, r);
-                    const uint2 c = *reinterpret_cast<const uint2*>(&o->count[2 * tid]);
-                    count[0] += c.x, count[1] += c.y;
-                    if (by_mass) {
-                        const uint2 p0 = *reinterpret_cast<const uint2*>(&o->part[0][2 * tid]), p1 = *reinterpret_cast<const uint2*>(&o->part[1][2 * tid]),
-                                    p2 = *reinterpret_cast<const uint2*>(&o->part[2][2 * tid]);
-                        mass[0] += (u64)p0.x + ((u64)p1.x << 15) + ((u64)p2.x << 30);
-                        mass[1] += (u64)p0.y + ((u64)p1.y << 15) + ((u64)p2.y << 30);
-                    }
+            for (int step = 0; step < 2; ++step) {     // the 32 bins, then the bin
+                if (warp < a.parts) {
+                    const Shared* o = cl.map_shared_rank(&sm, warp);
+                    const bool there = step == 1 || lane < COARSE;
+                    sm.all_count[warp][lane] = !there ? 0 : step ? o->bins[turn].count[bin + lane] : o->coarse_count[lane];
+                    sm.all_mass[warp][lane] = !there || !by_mass ? 0 : step ? mass_of(o->bins[turn], bin + lane) : o->coarse_mass[lane];
                 }
-            uint32_t all;
-            u64 all_mass = 0, m0 = ahead_mass;
-            if (tid == 0) sm.found = -1;
-            const uint32_t c0 = ahead + before(count[0] + count[1], sm.count, all);
-            if (by_mass) m0 += before(mass[0] + mass[1], sm.mass, all_mass);
-            if (level == 0 && by_mass) limit = top_p > 0.f ? max(1ull, (u64)ceil((double)top_p * (double)all_mass)) : 1ull;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t c = c0 + (j ? count[0] : 0);
-                const u64 m = m0 + (j ? mass[0] : 0);
-                if (count[j] > 0 && c < (uint32_t)k && m < limit) atomicMax(&sm.found, 2 * tid + j);
+                __syncthreads();
+                if (warp == 0) {
+                    uint32_t count = 0;
+                    u64 mass = 0;
+                    for (int r = 0; r < a.parts; ++r) count += sm.all_count[r][lane], mass += sm.all_mass[r][lane];
+                    const uint32_t c1 = up_to(count);
+                    const u64 m1 = up_to(mass), whole = __shfl_sync(0xffffffffu, m1, 31);
+                    if (level == 0 && step == 0 && by_mass) limit = top_p > 0.f ? max(1ull, (u64)ceil((double)top_p * (double)whole)) : 1ull;
+                    const uint32_t c = from_count + c1 - count;
+                    const u64 m = from_mass + m1 - mass;
+                    const uint32_t good = __ballot_sync(0xffffffffu, count > 0 && c < (uint32_t)k && m < limit);
+                    const int last = 31 - __clz(good);
+                    if (lane == max(last, 0)) sm.found = last, sm.at_count = c, sm.at_mass = m;
+                    if (lane == 31) sm.total_count = c1, sm.total_mass = limit;
+                }
+                __syncthreads();
+                if (sm.found < 0) { bin = -1; break; }
+                bin = step ? bin + sm.found : 32 * sm.found;
+                from_count = sm.at_count, from_mass = sm.at_mass;
+                if (step == 0) all = sm.total_count;
+                limit = sm.total_mass;
+                __syncthreads();
             }
-            __syncthreads();
-            const int bin = sm.found;
-            if (bin >= 0 && bin / 2 == tid) {
-                sm.at_count = c0 + (bin & 1 ? count[0] : 0);
-                sm.at_mass = m0 + (bin & 1 ? mass[0] : 0);
-            }
-            __syncthreads();
             if (bin < 0) break;                        // nothing above minus infinity
             if (level == 0 && !by_mass && all <= (uint32_t)k) break;      // no more tokens than k
-            ahead = sm.at_count;
-            ahead_mass = sm.at_mass;
+            ahead = from_count;
+            ahead_mass = from_mass;
             if (level == 0) {
                 chosen = bin;
                 // The bin's logits, and some beside them: roundings are within 2^-22 of the numbers that go in.  (An endless or vanishing temperature: all logits.)
-                if (slope > 1e-20f && slope < 1e20f && fabsf(s.max) < 1e30f) {
-                    const float up = s.max - (float)bin / slope, down = s.max - (float)(bin + 1) / slope, slack = 1e-6f * (fabsf(s.max) + fabsf(up) + fabsf(down));
-                    hi = min(hi, key_of(clean(up + slack)));
-                    if (bin < BINS - 1) lo = max(lo, key_of(clean(down - slack)));
+                if (slope > 1e-20f && slope < 1e20f && fabsf(s.top) < 1e30f) {
+                    const float up = s.top - (float)bin / slope, down = s.top - (float)(bin + 1) / slope, slack = 1e-6f * (fabsf(s.top) + fabsf(up) + fabsf(down));
+                    hi = min(hi, key_of<T>(clean(up + slack)));
+                    if (bin < BINS - 1) lo = max(lo, key_of<T>(clean(down - slack)));
                 }
             } else {
                 hi -= (uint32_t)bin << shift;
@@ -285,7 +315,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             }
             if (level > 0 && lo == hi) {
                 edge = lo;
-                const u64 w = weight(__uint_as_float(edge >> 31 ? edge & 0x7fffffffu : ~edge), s, sm.powers);
+                const u64 w = weight(value_of<T>(edge), s, sm.powers);
                 ties = (uint32_t)k - ahead;
                 if (by_mass) ties = (uint32_t)min((u64)ties, (limit - ahead_mass + w - 1) / w);
                 break;
@@ -299,13 +329,13 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     auto kept = [&](float v, uint32_t key) -> u64 {    // of a token above the edge
         if (key <= edge) return 0;
         const u64 w = weight(v, s, sm.powers);
-        return w >= least || v == s.max ? w : 0;       // the largest ones stay whatever min_p
+        return w >= least || v == s.top ? w : 0;       // the largest ones stay whatever min_p
     };
-    const float edge_value = __uint_as_float(edge >> 31 ? edge & 0x7fffffffu : ~edge);
+    const float edge_value = value_of<T>(edge);
     u64 edge_weight = 0;
     if (edge != 0) {
         edge_weight = weight(edge_value, s, sm.powers);
-        if (edge_weight < least && edge_value != s.max) edge_weight = 0;
+        if (edge_weight < least && edge_value != s.top) edge_weight = 0;
     }
     const int seg = (padded / 128 + WARPS - 1) / WARPS * 128, from = min(padded, warp * seg), to = min(padded, from + seg);
     u64 sum = 0;
@@ -315,7 +345,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
         four(i, x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t key = key_of(x[e]);
+            const uint32_t key = key_of<T>(x[e]);
             sum += kept(x[e], key);
             on += edge != 0 && key == edge;
         }
@@ -357,7 +387,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             uint32_t mark = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t key = key_of(x[e]);
+                const uint32_t key = key_of<T>(x[e]);
                 w[e] = kept(x[e], key);
                 mark += edge != 0 && key == edge;
             }
@@ -365,7 +395,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             uint32_t mine_on = rank_on + marks - mark;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (edge != 0 && key_of(x[e]) == edge && mine_on++ < ties) w[e] = edge_weight;
+                if (edge != 0 && key_of<T>(x[e]) == edge && mine_on++ < ties) w[e] = edge_weight;
                 own += w[e];
             }
             const u64 upto = up_to(own);
