@@ -10,6 +10,7 @@
 // by their numbers.  Last, the kept weights are summed up per thread, and a scan finds the thread, and the token, that the random number falls to.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -34,22 +35,34 @@ constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 768, PER_OCTAVE = 16, 
 constexpr int BITS = 44;                               // of a weight of one: 2^19 of them stay below 2^63
 typedef unsigned long long u64;
 
-__device__ __forceinline__ float val(float x) { return x; }
-__device__ __forceinline__ float val(bf16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float val(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T num(float x);
-template <> __device__ __forceinline__ float num<float>(float x) { return x; }
-template <> __device__ __forceinline__ bf16 num<bf16>(float x) { return __float2bfloat16(x); }
-template <> __device__ __forceinline__ __half num<__half>(float x) { return __float2half(x); }
-// NaN counts as minus infinity, zeros are equal
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x == 0.f ? 0.f : x; }
-// Whole numbers in the order of the floating-point ones, without the bits that 16-bit types never have
-template <typename T> struct Spare { static constexpr int BITS = sizeof(T) == 4 ? 0 : sizeof(T) == 2 && alignof(T) == 2 ? 13 : 0; };
-template <> struct Spare<bf16> { static constexpr int BITS = 16; };
-template <typename T> __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return (b >> 31 ? ~b : b | 0x80000000u) >> Spare<T>::BITS; }
+// Logits go as whole numbers of their own width, in the logits' order: NaN is minus infinity, zeros are equal.
+template <typename T> struct Key { typedef uint16_t N; static constexpr uint32_t SIGN = 0x8000u, ONES = 0xffffu; };
+template <> struct Key<float> { typedef uint32_t N; static constexpr uint32_t SIGN = 0x80000000u, ONES = 0xffffffffu; };
+template <typename T> __device__ __forceinline__ uint32_t infinity();
+template <> __device__ __forceinline__ uint32_t infinity<float>() { return 0x7f800000u; }
+template <> __device__ __forceinline__ uint32_t infinity<bf16>() { return 0x7f80u; }
+template <> __device__ __forceinline__ uint32_t infinity<__half>() { return 0x7c00u; }
+template <typename T> __device__ __forceinline__ uint32_t lowest() { return Key<T>::ONES ^ (Key<T>::SIGN | infinity<T>()); }      // minus infinity's
+template <typename T> __device__ __forceinline__ uint32_t key_of_bits(uint32_t b) {
+    const uint32_t size = b & ~Key<T>::SIGN, key = size == 0 ? Key<T>::SIGN : b & Key<T>::SIGN ? b ^ Key<T>::ONES : b | Key<T>::SIGN;
+    return size > infinity<T>() ? lowest<T>() : key;
+}
 template <typename T> __device__ __forceinline__ float value_of(uint32_t key) {
-    key <<= Spare<T>::BITS;
-    return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~(key | ((1u << Spare<T>::BITS) - 1)));
+    const uint32_t b = key & Key<T>::SIGN ? key ^ Key<T>::SIGN : key ^ Key<T>::ONES;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(b);
+    else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(b << 16);
+    else return __half2float(__ushort_as_half((unsigned short)b));
+}
+// The key at or below a number in 32 bits, and at or above it
+template <typename T> __device__ __forceinline__ uint32_t key_down(float x) {
+    if constexpr (sizeof(T) == 4) return key_of_bits<T>(__float_as_uint(x));
+    else if constexpr (std::is_same<T, bf16>::value) return key_of_bits<T>(__bfloat16_as_ushort(__float2bfloat16_rd(x)));
+    else return key_of_bits<T>(__half_as_ushort(__float2half_rd(x)));
+}
+template <typename T> __device__ __forceinline__ uint32_t key_up(float x) {
+    if constexpr (sizeof(T) == 4) return key_of_bits<T>(__float_as_uint(x));
+    else if constexpr (std::is_same<T, bf16>::value) return key_of_bits<T>(__bfloat16_as_ushort(__float2bfloat16_ru(x)));
+    else return key_of_bits<T>(__half_as_ushort(__float2half_ru(x)));
 }
 
 // 2^(i / 32)
@@ -58,18 +71,23 @@ __constant__ double POWERS[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1
     1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
     1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
-struct Scale { float top; double max, c; };            // the largest logit, log2(e) / temperature
-// 2^44 exp((x - max) / temperature), rounded.  (No branches, so that several go on side by side: with them a pass over 16000 logits took 28000 cycles.)
-__device__ __forceinline__ u64 weight(float x, const Scale& s, const double* powers) {
-    double y = ((double)x - s.max) * s.c;
-    y = x == -INFINITY ? -64.0 : x == s.top ? 0.0 : fmax(y, -64.0);      // (infinities, whose differences and products may be NaN)
+struct Scale { uint32_t top; double max, c; };         // the largest logit, log2(e) / temperature
+// 2^44 exp((x - max) / temperature), rounded, and its bin.  (No branches, so that several go on side by side: with them a pass over 16000 logits took 28000 cycles.)
+template <typename T> __device__ __forceinline__ u64 weight(uint32_t key, const Scale& s, const double* powers, int& bin) {
+    double y = ((double)value_of<T>(key) - s.max) * s.c;
+    y = key == lowest<T>() ? -64.0 : key == s.top ? 0.0 : fmax(y, -64.0);      // (infinities, whose differences and products may be NaN)
     const double magic = 6755399441055744.0;           // 1.5 2^52: what is added to it is rounded to a whole number in its lower bits
     const double shifted = fma(y, 32.0, magic);
     const int n = (int)__double_as_longlong(shifted);
     const double f = fma(shifted - magic, -0.03125, y) * 0.6931471805599453;      // up to ln 2 / 64
     const double e = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
     const double power = __longlong_as_double(__double_as_longlong(powers[n & 31]) + ((long long)(BITS + (n >> 5)) << 52));
+    bin = min(-n >> 1, BINS - 1);
     return (u64)(__double_as_longlong(fma(power, e, magic)) - 0x4338000000000000ll);
+}
+template <typename T> __device__ __forceinline__ u64 weight(uint32_t key, const Scale& s, const double* powers) {
+    int bin;
+    return weight<T>(key, s, powers, bin);
 }
 
 struct Bins { uint32_t count[BINS], part[3][BINS]; };  // weights in three parts of 15 bits, whose sums over a CTA's logits 32 bits hold
@@ -126,22 +144,11 @@ template <typename N> __device__ __forceinline__ N before(N v, N* warps, N& all)
     return ahead + in - v;
 }
 
-// Four neighbouring logits; `n`: how many there are.  Those behind the last one are minus infinity, and weigh nothing.
-template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&x)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(p);
-        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-    } else {
-        const uint2 raw = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = val(reinterpret_cast<const T*>(&raw)[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = clean(x[i]);
-}
-template <typename T> __device__ __forceinline__ void some_of(const T* p, int left, float (&x)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = i < left ? clean(val(p[i])) : -INFINITY;
+// Keys of four neighbours in shared memory, or out of the logits (aligned, or some of them)
+__device__ __forceinline__ void four_keys(const uint32_t* p, uint32_t (&k)[4]) { const uint4 y = *reinterpret_cast<const uint4*>(p); k[0] = y.x, k[1] = y.y, k[2] = y.z, k[3] = y.w; }
+__device__ __forceinline__ void four_keys(const uint16_t* p, uint32_t (&k)[4]) {
+    const uint2 y = *reinterpret_cast<const uint2*>(p);
+    k[0] = y.x & 0xffffu, k[1] = y.x >> 16, k[2] = y.y & 0xffffu, k[3] = y.y >> 16;
 }
 
 template <typename T, bool HELD>                       // HELD: the part of a row lies in shared memory
@@ -151,8 +158,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     cg::cluster_group cl = cg::this_cluster();
     const int b = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = rank * a.len, n = max(0, min(a.len, a.V - first));
-    const T* row = (const T*)a.logits + b * a.ld + first;
-    T* mine = reinterpret_cast<T*>(held);
+    typedef typename Key<T>::N N;
+    const N* row = (const N*)a.logits + b * a.ld + first;
+    N* mine = reinterpret_cast<N*>(held);
     if (tid < 32) sm.powers[tid] = POWERS[tid];
     for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[0])[i] = 0;
 
@@ -167,26 +175,31 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     constexpr int E = 16 / sizeof(T);
     const bool wide = reinterpret_cast<uintptr_t>(row) % 16 == 0;
     const int padded = (n + 127) & ~127;               // (a.len is a multiple of 128)
-    float top = -INFINITY;
+    uint32_t top = 0;
     if (wide) {
 #pragma unroll 4
         for (int i = tid * E; i + E <= n; i += THREADS * E) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
-            if constexpr (HELD) *reinterpret_cast<uint4*>(mine + i) = raw;
+            uint4 raw = *reinterpret_cast<const uint4*>(row + i);
+            N* keys = reinterpret_cast<N*>(&raw);
 #pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, clean(val(reinterpret_cast<const T*>(&raw)[e])));
+            for (int e = 0; e < E; ++e) {
+                const uint32_t key = key_of_bits<T>(keys[e]);
+                keys[e] = (N)key;
+                top = max(top, key);
+            }
+            if constexpr (HELD) *reinterpret_cast<uint4*>(mine + i) = raw;
         }
     }
 #pragma unroll 4
     for (int i = (wide ? n / E * E : 0) + tid; i < n; i += THREADS) {
-        const T raw = row[i];
-        if constexpr (HELD) mine[i] = raw;
-        top = fmaxf(top, clean(val(raw)));
+        const uint32_t key = key_of_bits<T>(row[i]);
+        if constexpr (HELD) mine[i] = (N)key;
+        top = max(top, key);
     }
     if constexpr (HELD)
-        for (int i = n + tid; i < padded; i += THREADS) mine[i] = num<T>(-INFINITY);
-    top = warp_max(top);
-    if (lane == 0) sm.count[warp] = key_of<T>(top);
+        for (int i = n + tid; i < padded; i += THREADS) mine[i] = (N)lowest<T>();
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) sm.count[warp] = top;
     __syncthreads();
     if (tid == 0) {
         uint32_t y = 0;
@@ -197,14 +210,17 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     cl.sync();
     uint32_t top_key = 0;
     for (int r = 0; r < a.parts; ++r) top_key = max(top_key, *cl.map_shared_rank(&sm.top, r));
+    top_key = max(top_key, lowest<T>());               // (a CTA without logits has none)
     Scale s;
-    s.top = value_of<T>(top_key);
-    s.max = s.top;
+    s.top = top_key;
+    s.max = value_of<T>(top_key);
     s.c = greedy ? 1.0 : 1.4426950408889634 / (double)temperature;
-    auto four = [&](int i, float (&x)[4]) {            // logits i .. i + 3 of the part
-        if constexpr (HELD) four_of(mine + i, x);
-        else if (wide && i + 4 <= n) four_of(row + i, x);
-        else some_of(row + i, n - i, x);
+    auto four = [&](int i, uint32_t (&k)[4]) {         // logits i .. i + 3 of the part; behind the last one minus infinity, which weighs nothing
+        if constexpr (HELD) four_keys(mine + i, k);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = i + e < n ? key_of_bits<T>(row[i + e]) : lowest<T>();
+        }
     };
 
     // The logit that the cut lies at: tokens with keys above `edge` are kept, and `ties` of those equal to it.  First its bin (16 of them for a factor of two in weight), then its key among those of the bin.
@@ -212,9 +228,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     int turn = 0;
     if (cut && k == 1) edge = top_key, ties = 1;
     else if (cut) {
-        const float slope = (float)fmin(s.c * PER_OCTAVE, 1e30);
-        auto bin_of = [&](float v) -> int { return min((int)((s.top - v) * slope), BINS - 1); };      // (infinite logits: of infinity alone, in bin 0)
-        uint32_t lo = key_of<T>(-INFINITY), hi = top_key; // around the keys of the bin
+        uint32_t lo = lowest<T>(), hi = top_key;       // around the keys of the bin
         int shift = 0, chosen = 0;
         uint32_t ahead = 0;                            // tokens, and weight, above the edge
         u64 ahead_mass = 0, limit = ~0ull;             // a token is kept if less than the limit comes before it
@@ -222,24 +236,20 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             Bins& h = sm.bins[turn];
             uint32_t all = 0;
             for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
-                float x[4];
-                four(i, x);
                 uint32_t key[4];
-                bool in[4], any = false;
+                four(i, key);
+                bool any = level == 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    key[e] = key_of<T>(x[e]);
-                    in[e] = level == 0 || (key[e] >= lo && key[e] <= hi && bin_of(x[e]) == chosen);
-                    any |= in[e];
-                }
+                for (int e = 0; e < 4; ++e) any |= key[e] - lo <= hi - lo;
                 if (!any) continue;
                 u64 w[4];
+                int of[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = weight(x[e], s, sm.powers);
+                for (int e = 0; e < 4; ++e) w[e] = weight<T>(key[e], s, sm.powers, of[e]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (!in[e] || w[e] == 0) continue; // (of no weight: never drawn)
-                    const int bin = level == 0 ? bin_of(x[e]) : (int)((hi - key[e]) >> shift);
+                    if (w[e] == 0 || (level > 0 && (of[e] != chosen || key[e] - lo > hi - lo))) continue;      // (of no weight: never drawn)
+                    const int bin = level == 0 ? of[e] : (int)((hi - key[e]) >> shift);
                     atomicAdd(&h.count[bin], 1u);
                     if (by_mass)
 #pragma unroll
@@ -303,11 +313,12 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             ahead_mass = from_mass;
             if (level == 0) {
                 chosen = bin;
-                // The bin's logits, and some beside them: roundings are within 2^-22 of the numbers that go in.  (An endless or vanishing temperature: all logits.)
-                if (slope > 1e-20f && slope < 1e20f && fabsf(s.top) < 1e30f) {
-                    const float up = s.top - (float)bin / slope, down = s.top - (float)(bin + 1) / slope, slack = 1e-6f * (fabsf(s.top) + fabsf(up) + fabsf(down));
-                    hi = min(hi, key_of<T>(clean(up + slack)));
-                    if (bin < BINS - 1) lo = max(lo, key_of<T>(clean(down - slack)));
+                // The bin's logits, and some beside them: 16 y lies between -bin - 3/4 and -bin + 1/4, up to the roundings of 32 bits.  (An endless or vanishing temperature: all logits.)
+                const float slope = (float)fmin(s.c * PER_OCTAVE, 1e30), top_value = (float)s.max;
+                if (slope > 1e-20f && slope < 1e20f && fabsf(top_value) < 1e30f) {
+                    const float up = top_value - ((float)bin - 0.25f) / slope, down = top_value - ((float)bin + 0.75f) / slope, slack = 1e-6f * (fabsf(top_value) + fabsf(up) + fabsf(down));
+                    hi = min(hi, key_up<T>(up + slack));
+                    if (bin < BINS - 1) lo = max(lo, key_down<T>(down - slack));
                 }
             } else {
                 hi -= (uint32_t)bin << shift;
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
             }
             if (level > 0 && lo == hi) {
                 edge = lo;
-                const u64 w = weight(value_of<T>(edge), s, sm.powers);
+                const u64 w = weight<T>(edge, s, sm.powers);
                 ties = (uint32_t)k - ahead;
                 if (by_mass) ties = (uint32_t)min((u64)ties, (limit - ahead_mass + w - 1) / w);
                 break;
@@ -326,29 +337,29 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
 
     // Kept weight: a warp takes a segment of the part, in order.  Tokens on the edge weigh the same, so their number is enough.
     const u64 least = min_p > 0.f ? (u64)ceil((double)min_p * (double)(1ull << BITS)) : 0ull;
-    auto kept = [&](float v, uint32_t key) -> u64 {    // of a token above the edge
-        if (key <= edge) return 0;
-        const u64 w = weight(v, s, sm.powers);
-        return w >= least || v == s.top ? w : 0;       // the largest ones stay whatever min_p
+    auto kept = [&](uint32_t key) -> u64 {             // of a token above the edge
+        const u64 w = weight<T>(key, s, sm.powers);
+        return key > edge && (w >= least || key == top_key) ? w : 0;      // the largest ones stay whatever min_p
     };
-    const float edge_value = value_of<T>(edge);
     u64 edge_weight = 0;
     if (edge != 0) {
-        edge_weight = weight(edge_value, s, sm.powers);
-        if (edge_weight < least && edge_value != s.top) edge_weight = 0;
+        edge_weight = weight<T>(edge, s, sm.powers);
+        if (edge_weight < least && edge != top_key) edge_weight = 0;
     }
     const int seg = (padded / 128 + WARPS - 1) / WARPS * 128, from = min(padded, warp * seg), to = min(padded, from + seg);
     u64 sum = 0;
     uint32_t on = 0;
     for (int i = from + 4 * lane; i < to; i += 128) {
-        float x[4];
-        four(i, x);
+        uint32_t key[4];
+        four(i, key);
+        bool any = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t key = key_of<T>(x[e]);
-            sum += kept(x[e], key);
-            on += edge != 0 && key == edge;
-        }
+        for (int e = 0; e < 4; ++e) any |= key[e] > edge, on += key[e] == edge;      // (an edge of 0 is no key)
+        if (!any) continue;
+        u64 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = kept(key[e]);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -381,21 +392,20 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
         uint32_t rank_on = sm.tied;
         for (int i0 = from; i0 < to; i0 += 128) {
             const int i = i0 + 4 * lane;
-            float x[4];
-            four(i, x);
+            uint32_t key[4];
+            four(i, key);
             u64 w[4], own = 0;
             uint32_t mark = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t key = key_of<T>(x[e]);
-                w[e] = kept(x[e], key);
-                mark += edge != 0 && key == edge;
+                w[e] = kept(key[e]);
+                mark += key[e] == edge;
             }
             const uint32_t marks = up_to(mark);
             uint32_t mine_on = rank_on + marks - mark;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (edge != 0 && key_of<T>(x[e]) == edge && mine_on++ < ties) w[e] = edge_weight;
+                if (key[e] == edge && mine_on++ < ties) w[e] = edge_weight;
                 own += w[e];
             }
             const u64 upto = up_to(own);

@@ -73,7 +73,7 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
 def _shares(B: int, V: int, slots: int) -> Tuple[int, int]:
     """(CTAs of a row, logits of each)."""
     parts = 1
-    while parts < 8 and (parts * PART < V or (2 * B * parts <= 4 * slots and parts * 2048 < V)):
+    while parts < 8 and parts * 2048 < V:
         parts *= 2
     return parts, -(-V // (parts * 128)) * 128
 
