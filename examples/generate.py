@@ -52,18 +52,21 @@ if __name__ == "__main__":
             load_checkpoint(tc.load, [model], None, None, mesh, load_rng=False)
     if args.paged_kv_cache and not (model.packed_rows or PagedCache.supported(model)):
         raise SystemExit("--paged-kv-cache is for models of softmax and linear layers (no latent attention, no context parallelism)")
+    if args.kv_cache_bits != 16 and (model.packed_rows or not args.paged_kv_cache):
+        raise SystemExit("--kv-cache-bits goes with --paged-kv-cache, for models of softmax and linear layers")
     port = int(os.environ.get("LMOE_SERVE_PORT", "0"))
     if port:
         # HTTP endpoint (PUT /api, the request fields of Megatron's text-generation server): rank 0 serves, the other
         # ranks of a parallel replica join every generation call
         from linear_moe_b200.infer.server import build_app, serve_followers
         graph, paged = getattr(args, "cuda_graph_decode", False), getattr(args, "paged_kv_cache", False)
+        how = dict(cache_bits=args.kv_cache_bits, fused_sampling=args.fused_sampling)
         if mesh.rank == 0:
             import uvicorn
-            uvicorn.run(build_app(model.eval(), tok, cuda_graph=graph, paged=paged), host=os.environ.get("LMOE_SERVE_HOST", "127.0.0.1"),
+            uvicorn.run(build_app(model.eval(), tok, cuda_graph=graph, paged=paged, **how), host=os.environ.get("LMOE_SERVE_HOST", "127.0.0.1"),
                         port=port, log_level="warning")
         else:
-            serve_followers(model.eval(), tok, cuda_graph=graph, paged=paged)
+            serve_followers(model.eval(), tok, cuda_graph=graph, paged=paged, **how)
         sys.exit(0)
     outs = GPTPredictor(model, tok, args).predict()
     if mesh.rank == 0:

@@ -83,6 +83,8 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--use-mcore-models", action="store_true")
     _flag(g, "--use-flash-attn", action="store_true")
     _flag(g, "--no-rope-fusion", action="store_true")
+    _flag(g, "--fused-qkv-heads", action="store_true",
+          help="softmax layers split their projection, norm queries and keys and rotate them in one pass, forward and backward (rounded once instead of after each step)")
     _flag(g, "--no-bias-swiglu-fusion", action="store_true")
     _flag(g, "--no-masked-softmax-fusion", action="store_true")
     _flag(g, "--no-create-attention-mask-in-dataloader", action="store_true")
@@ -256,6 +258,8 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--paged-kv-cache", action="store_true",
           help="generation keeps the softmax layers' keys and values in pages: nothing is concatenated, --cuda-graph-decode captures these layers too, and beam search "
                "runs one token a step")
+    _flag(g, "--kv-cache-bits", type=int, default=16, choices=[4, 16],
+          help="with --paged-kv-cache: 4 keeps keys and values in 4 bits a number, with a low and a size for every 32 (heads of a multiple of 32 numbers, up to 256)")
     _flag(g, "--cuda-graph-decode", action="store_true",
           help="generation: replay one-token steps from a CUDA graph (models with fixed-size caches)")
     _flag(g, "--cpu-offloading", action="store_true")
@@ -352,6 +356,9 @@ def build_parser() -> argparse.ArgumentParser:
     _flag(g, "--top-p", type=float, default=0.0)
     _flag(g, "--top-k", type=int, default=0)
     _flag(g, "--temperature", type=float, default=1.0)
+    _flag(g, "--min-p", type=float, default=0.0, help="keep tokens of at least this share of the most probable one's probability (samples as --fused-sampling does)")
+    _flag(g, "--fused-sampling", action="store_true",
+          help="draw tokens by one random number each in one kernel; --top-k and --top-p may then be given together")
     _flag(g, "--out-seq-length", type=int, default=1024)
     _flag(g, "--generation-length", type=int, default=None)
     _flag(g, "--repetition-penalty", "--repetition_penalty", type=float, default=1.0, dest="repetition_penalty")
@@ -433,7 +440,7 @@ def configs_from_args(args: argparse.Namespace) -> Tuple[ModelConfig, ParallelCo
         add_qkv_bias=args.add_qkv_bias and not args.disable_bias_attn_fc,
         tie_embeddings=not args.untie_embeddings_and_output_weights,
         init_method_std=args.init_method_std, hidden_dropout=args.hidden_dropout,
-        attention_dropout=args.attention_dropout, qk_layernorm=args.qk_layernorm,
+        attention_dropout=args.attention_dropout, qk_layernorm=args.qk_layernorm, fused_qkv_heads=args.fused_qkv_heads,
         sliding_window=args.sliding_window, attn_logit_softcapping=args.attn_logit_softcapping, position_embedding_type=pos,
         rotary_base=args.rotary_base, rotary_percent=args.rotary_percent,
         rotary_interleaved=args.rotary_interleaved, rotary_scaling_factor=args.rotary_scaling_factor,
@@ -591,7 +598,7 @@ def flags_without_effect(parser: argparse.ArgumentParser, args: argparse.Namespa
 
 # what --use-checkpoint-args does NOT take from the checkpoint: how the model is run, not what it is
 _RUNTIME_FIELDS = frozenset("""params_dtype recompute_granularity recompute_method recompute_num_layers moe_layer_recompute
-cpu_offloading cpu_offloading_num_layers cross_entropy_chunk test_mode fp8 la_mode hidden_dropout attention_dropout
+cpu_offloading cpu_offloading_num_layers cross_entropy_chunk test_mode fp8 la_mode hidden_dropout attention_dropout fused_qkv_heads
 moe_token_dispatcher_type""".split())
 
 

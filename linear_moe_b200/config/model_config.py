@@ -59,6 +59,7 @@ class ModelConfig:
     hidden_dropout: float = 0.0
     attention_dropout: float = 0.0
     qk_layernorm: bool = False
+    fused_qkv_heads: bool = False                 # softmax layers: norms, rotation and split of the projection in one pass, rounded once
     sliding_window: Optional[int] = None
     attn_logit_softcapping: Optional[float] = None    # softmax layers: scores become cap * tanh(scores / cap)
     # ---- positional -----------------------------------------------------

@@ -63,6 +63,12 @@ def sample(logits: torch.Tensor, top_k: int = 0, top_p: float = 0.0, temperature
     return out
 
 
+def sample_fused(logits: torch.Tensor, top_k: int = 0, top_p: float = 0.0, temperature: float = 1.0, vocab_size: Optional[int] = None, generator=None, min_p: float = 0.0) -> torch.Tensor:
+    """A token per row ``[B, V]`` by one random number each (``ops.sample_tokens``): temperature, then what ``top_k``, ``top_p`` (0: all) and ``min_p`` leave, all of the same softmax."""
+    draw = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+    return ops.sample_tokens(logits[:, :vocab_size] if vocab_size else logits, draw, temperature, top_k, top_p if top_p > 0.0 else 1.0, min_p)[0]
+
+
 def apply_repetition_penalty(logits: torch.Tensor, tokens: torch.Tensor, penalty: float) -> torch.Tensor:
     if penalty == 1.0:
         return logits
@@ -181,19 +187,29 @@ def generate_tokens(model, tokens: torch.Tensor, lengths: torch.Tensor, *, eod: 
                     top_p: float = 0.0, temperature: float = 1.0, repetition_penalty: float = 1.0,
                     return_log_probs: bool = False, use_eod_for_early_termination: bool = True,
                     stop_on_double_eol: bool = False, stop_on_eol: bool = False, generator=None,
-                    cuda_graph: bool = False, paged: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+                    cuda_graph: bool = False, paged: bool = False, cache_bits: int = 16, min_p: float = 0.0,
+                    fused_sampling: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """Fill ``tokens [B, L]`` from the shortest prompt length to L.  Returns (tokens, generated lengths, log-probs).
     ``cuda_graph``: replay the one-token steps from a CUDA graph (``GraphedDecodeStep``) when the model allows it; the
     prefill and the first two one-token steps run eagerly (they also serve as the warm-up before the capture).
-    ``paged``: softmax layers keep their keys and values in pages (``PagedCache``) instead of concatenating them for every token, and their steps are captured too."""
+    ``paged``: softmax layers keep their keys and values in pages (``PagedCache``) instead of concatenating them for every token, and their steps are captured too;
+    ``cache_bits`` 4: in 4 bits a number.  ``fused_sampling``, or a ``min_p`` above 0: tokens are drawn by ``sample_fused``."""
     model.eval()
+    if cache_bits != 16 and (not paged or getattr(model, "packed_rows", False)):
+        raise ValueError(f"a cache of {cache_bits} bits a number is a paged one of softmax layers (not of the layer-list designs)")
+    if not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"min_p of {min_p}")
+
+    def draw(lg):
+        if fused_sampling or min_p > 0.0:
+            return sample_fused(lg, top_k, top_p, temperature, model.cfg.vocab_size, generator, min_p)
+        return sample(lg, top_k, top_p, temperature, model.cfg.vocab_size, generator)
     if getattr(model, "packed_rows", False):
         return _generate_packed(model, tokens, lengths, eod if use_eod_for_early_termination else None,
-                                lambda lg: sample(lg, top_k, top_p, temperature, model.cfg.vocab_size, generator),
-                                repetition_penalty, return_log_probs, cuda_graph)
+                                draw, repetition_penalty, return_log_probs, cuda_graph)
     B, L = tokens.shape
     min_len = int(lengths.min())
-    caches = PagedCache(model, B, L) if paged else model.new_cache()
+    caches = PagedCache(model, B, L, bits=cache_bits) if paged else model.new_cache()
     done = torch.zeros(B, dtype=torch.bool, device=tokens.device)
     gen_len = torch.full((B,), L, dtype=torch.long, device=tokens.device)
     logps = torch.zeros(B, L - 1, dtype=torch.float32, device=tokens.device) if return_log_probs else None
@@ -217,7 +233,7 @@ def generate_tokens(model, tokens: torch.Tensor, lengths: torch.Tensor, *, eod: 
         if logits is not None:                                # last pipeline stage (or no pipeline): sample here
             last = logits[:, -1].float()
             last = apply_repetition_penalty(last, tokens[:, :ctx], repetition_penalty)
-            new = sample(last, top_k, top_p, temperature, model.cfg.vocab_size, generator)
+            new = draw(last)
         # every stage gets the sampled tokens, so token buffers and termination flags stay identical on all of them
         new = PF.broadcast_from_last_stage(model, new, (B,), torch.long, tokens.device)
         started = lengths <= ctx
@@ -338,10 +354,12 @@ def _states_by_row(model, prompt: torch.Tensor) -> bool:
 
 @torch.no_grad()
 def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int, eod: int, length_penalty: float = 1.0,
-                num_return: int = 1, paged: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+                num_return: int = 1, paged: bool = False, cache_bits: int = 16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Beam search for one prompt ``[1, P]`` (``beam_search_and_return_on_first_stage``).  The whole beam is re-scored from its tokens each step; with
-    ``paged`` a step runs the new token of every beam alone, on caches whose states and pages follow the beams (``PagedCache.reorder``)."""
+    ``paged`` a step runs the new token of every beam alone, on caches whose states and pages follow the beams (``PagedCache.reorder``), with ``cache_bits`` 4 in 4 bits a number."""
     model.eval()
+    if cache_bits != 16 and not paged:
+        raise ValueError(f"a cache of {cache_bits} bits a number is a paged one")
     device = prompt.device
     P = prompt.shape[1]
     caches = None
@@ -350,7 +368,7 @@ def beam_search(model, prompt: torch.Tensor, beam_size: int, max_new_tokens: int
             raise ValueError("a paged beam search is for models of softmax and linear layers on one pipeline stage, without a mixture of memories")
         if beam_size > 1 and not _states_by_row(model, prompt):
             raise ValueError("a layer of this model keeps states that do not follow a beam")
-        caches = PagedCache(model, beam_size, P + max_new_tokens, live=1)
+        caches = PagedCache(model, beam_size, P + max_new_tokens, live=1, bits=cache_bits)
     beams = prompt.repeat(beam_size, 1)
     scores = torch.zeros(beam_size, device=device)
     scores[1:] = -1e9                                   # all beams start identical: keep one alive
@@ -396,7 +414,7 @@ def generate_and_post_process(model, tokenizer, prompts: Sequence[str], tokens_t
                               return_output_log_probs: bool = False, top_k_sampling: int = 0, top_p_sampling: float = 0.0,
                               temperature: float = 1.0, add_BOS: bool = False, use_eod_token_for_early_termination: bool = True,
                               repetition_penalty: float = 1.0, random_seed: int = -1, device=None,
-                              cuda_graph: bool = False, paged: bool = False):
+                              cuda_graph: bool = False, paged: bool = False, cache_bits: int = 16, min_p: float = 0.0, fused_sampling: bool = False):
     """Strings in, strings out (api.py:25-111): returns (texts, token lists, log-probs or None)."""
     device = device or next(model.parameters()).device
     gen = None
@@ -410,7 +428,7 @@ def generate_and_post_process(model, tokenizer, prompts: Sequence[str], tokens_t
                                           top_p=top_p_sampling, temperature=temperature,
                                           repetition_penalty=repetition_penalty, return_log_probs=return_output_log_probs,
                                           use_eod_for_early_termination=use_eod_token_for_early_termination, generator=gen,
-                                          cuda_graph=cuda_graph, paged=paged)
+                                          cuda_graph=cuda_graph, paged=paged, cache_bits=cache_bits, min_p=min_p, fused_sampling=fused_sampling)
     out_tokens = [tokens[i, : int(gen_len[i])].tolist() for i in range(tokens.shape[0])]
     texts = [tokenizer.decode(t) for t in out_tokens]
     return texts, out_tokens, lp
@@ -440,7 +458,8 @@ class GPTPredictor:
                                                     top_k_sampling=a.top_k, top_p_sampling=a.top_p,
                                                     temperature=a.temperature, repetition_penalty=a.repetition_penalty,
                                                     cuda_graph=getattr(a, "cuda_graph_decode", False),
-                                                    paged=getattr(a, "paged_kv_cache", False))
+                                                    paged=getattr(a, "paged_kv_cache", False), cache_bits=getattr(a, "kv_cache_bits", 16),
+                                                    min_p=getattr(a, "min_p", 0.0), fused_sampling=getattr(a, "fused_sampling", False))
             outs.append(texts[0])
         if a.text_generate_output_file and getattr(getattr(self.model, "mesh", None), "rank", 0) == 0:
             with open(a.text_generate_output_file, "a", encoding="utf-8") as f:

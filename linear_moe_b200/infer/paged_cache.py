@@ -1,7 +1,7 @@
 """Decoding caches of a model whose softmax layers keep their keys and values in pages.
 
 A :class:`PagedCache` is the list of per-layer dicts that ``CausalLM.forward`` takes.  The linear layers' dicts are filled by the layers themselves, as ever.  A softmax layer's holds its two
-pools ``k_pages`` / ``v_pages`` ``[pages, PAGE, heads, dim]`` and, the same tensors in every layer, the requests' page ``table [rows, n]``, their ``lengths [rows]`` (the tokens of the running call
+pools ``k_pages`` / ``v_pages`` ``[pages, PAGE, heads, dim]`` (of 4 bits a number: ``[pages, heads, bytes]``, ``ops/int4_cache.py``) and, the same tensors in every layer, the requests' page ``table [rows, n]``, their ``lengths [rows]`` (the tokens of the running call
 counted) and the rotary tables.  Nothing moves or grows while requests are decoded, so one-token steps can be captured in a CUDA graph; the dense cache is concatenated anew for every token.
 
 All rows are at the same position, as in ``generate_tokens``.  :meth:`advance` comes before the forward pass of every call.  :meth:`reorder` makes row i go on from row ``parents[i]`` (beam search):
@@ -18,10 +18,14 @@ from .kv_cache import PAGE
 
 
 class PagedCache(list):
-    def __init__(self, model, rows: int, tokens: int, live: Optional[int] = None):
-        """Room for ``rows`` requests of up to ``tokens`` tokens; ``live``: rows of the first calls (default: all; :meth:`reorder` sets their number)."""
+    def __init__(self, model, rows: int, tokens: int, live: Optional[int] = None, bits: int = 16):
+        """Room for ``rows`` requests of up to ``tokens`` tokens; ``live``: rows of the first calls (default: all; :meth:`reorder` sets their number).  ``bits``: 4 keeps
+        keys and values in 4 bits a number (``ops.int4_pages``), 16 in the layers' own type."""
         if not self.supported(model):
             raise ValueError("a paged cache is for softmax layers on one context-parallel rank (no latent attention, no layer-list designs)")
+        if bits not in (4, 16) or (bits == 4 and any(model.decoder.layers[i]._mixer().D % 32 or model.decoder.layers[i]._mixer().D > 256
+                                                     for i, s in enumerate(model.specs) if s.mixer == "attn")):
+            raise ValueError(f"pages of {bits} bits a number: 16, or 4 for heads of a multiple of 32 numbers, up to 256")
         super().__init__({} for _ in model.specs)
         dev = next(model.parameters()).device
         cfg = model.cfg
@@ -40,7 +44,7 @@ class PagedCache(list):
             if att.rope is not None and rope is None:
                 rope = R.rope_freqs(width * PAGE, int(att.D * cfg.rotary_percent), cfg.rotary_base, 0, dev, cfg.rotary_seq_len_interpolation_factor)
             for name in ("k_pages", "v_pages"):
-                self[i][name] = torch.zeros(len(self.free), PAGE, att.Gl, att.D, dtype=att.linear_qkv.weight.dtype, device=dev)
+                self[i][name] = ops.int4_pages(len(self.free), att.Gl, att.D, PAGE, dev) if bits == 4 else torch.zeros(len(self.free), PAGE, att.Gl, att.D, dtype=att.linear_qkv.weight.dtype, device=dev)
             if rope is not None:
                 self[i]["cos"], self[i]["sin"] = rope
         self._bind()

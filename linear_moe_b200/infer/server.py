@@ -2,7 +2,7 @@
 
 The reference reaches generation through ``generation/api.py::generate_and_post_process`` from batch scripts
 (gpt_predictor.py:27-104); Megatron-LM pairs the same call with a small REST server (``PUT /api``:
-``{"prompts": [...], "tokens_to_generate": n, "top_k": .., "top_p": .., "temperature": .., "logprobs": bool, ...}``).
+``{"prompts": [...], "tokens_to_generate": n, "top_k": .., "top_p": .., "temperature": .., "min_p": .., "logprobs": bool, ...}``).
 This module is that endpoint on FastAPI.  Requests are served one at a time under a lock: a request is one batched
 ``generate_and_post_process`` call, whose decode steps replay a CUDA graph when ``cuda_graph`` is set, so there is
 nothing to gain from interleaving two of them on one model replica.
@@ -45,6 +45,9 @@ def _validate(req: dict) -> Optional[str]:
         return "cannot set both top_k and top_p"
     if not isinstance(t, (int, float)) or not 0.0 < t <= 100.0:
         return "temperature must be a positive number (at most 100)"
+    m = req.get("min_p", 0.0)
+    if not isinstance(m, (int, float)) or not 0.0 <= m <= 1.0:
+        return "min_p must be a number in [0, 1]"
     b = req.get("beam_width")
     if b is not None:
         if not isinstance(b, int) or b < 1:
@@ -57,20 +60,22 @@ def _validate(req: dict) -> Optional[str]:
     return None
 
 
-def run_request(model, tokenizer, req: dict, cuda_graph: bool = False, paged: bool = False) -> dict:
+def run_request(model, tokenizer, req: dict, cuda_graph: bool = False, paged: bool = False, cache_bits: int = 16, fused_sampling: bool = False) -> dict:
     """One validated request -> response body (the collective part: every rank of a parallel model calls this)."""
     if req.get("beam_width"):
         device = next(model.parameters()).device
         ids = torch.tensor([tokenizer.tokenize(req["prompts"][0])], dtype=torch.long, device=device)
         toks, scores = beam_search(model, ids, req["beam_width"], req.get("tokens_to_generate", 64), tokenizer.eod,
-                                   length_penalty=req.get("length_penalty", 1.0), num_return=req.get("beam_width"), paged=paged and can_page_beams(model))
+                                   length_penalty=req.get("length_penalty", 1.0), num_return=req.get("beam_width"), paged=paged and can_page_beams(model),
+                                   cache_bits=cache_bits if paged and can_page_beams(model) else 16)
         return {"text": [tokenizer.decode(t) for t in toks.tolist()], "tokens": toks.tolist(), "score": scores.tolist()}
     texts, tokens, lp = generate_and_post_process(
         model, tokenizer, req["prompts"], tokens_to_generate=req.get("tokens_to_generate", 64),
         return_output_log_probs=bool(req.get("logprobs", False)), top_k_sampling=req.get("top_k", 0),
         top_p_sampling=req.get("top_p", 0.0), temperature=req.get("temperature", 1.0), add_BOS=bool(req.get("add_BOS", False)),
         use_eod_token_for_early_termination=bool(req.get("use_eod_token_for_early_termination", True)),
-        repetition_penalty=req.get("repetition_penalty", 1.0), random_seed=req.get("random_seed", -1), cuda_graph=cuda_graph, paged=paged)
+        repetition_penalty=req.get("repetition_penalty", 1.0), random_seed=req.get("random_seed", -1), cuda_graph=cuda_graph, paged=paged,
+        cache_bits=cache_bits, min_p=req.get("min_p", 0.0), fused_sampling=fused_sampling)
     out = {"text": texts, "tokens": tokens}
     if lp is not None:
         out["logprobs"] = [row[: max(len(t) - 1, 0)] for row, t in zip(lp.tolist(), tokens)]
@@ -84,7 +89,7 @@ def _broadcast_request(req: Optional[dict], group) -> Optional[dict]:
     return box[0]
 
 
-def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False, paged: bool = False):
+def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False, paged: bool = False, cache_bits: int = 16, fused_sampling: bool = False):
     """Ranks other than 0 of a tensor- / pipeline-parallel replica: wait for rank 0's requests and join each generation
     call; a broadcast ``None`` ends the loop."""
     while True:
@@ -92,10 +97,10 @@ def serve_followers(model, tokenizer, group=None, cuda_graph: bool = False, page
         if req is None:
             return
         with torch.no_grad():
-            run_request(model, tokenizer, req, cuda_graph, paged)
+            run_request(model, tokenizer, req, cuda_graph, paged, cache_bits, fused_sampling)
 
 
-def build_app(model, tokenizer, cuda_graph: bool = False, group=None, paged: bool = False):
+def build_app(model, tokenizer, cuda_graph: bool = False, group=None, paged: bool = False, cache_bits: int = 16, fused_sampling: bool = False):
     from fastapi import FastAPI, Request
     from fastapi.responses import JSONResponse
     import torch.distributed as dist
@@ -125,7 +130,7 @@ def build_app(model, tokenizer, cuda_graph: bool = False, group=None, paged: boo
         with lock, torch.no_grad():
             if parallel:
                 _broadcast_request(req, group)
-            return run_request(model, tokenizer, req, cuda_graph, paged)
+            return run_request(model, tokenizer, req, cuda_graph, paged, cache_bits, fused_sampling)
 
     @app.get("/health")
     async def health():

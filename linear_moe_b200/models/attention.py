@@ -119,6 +119,14 @@ class SelfAttention(nn.Module):
         cfg = self.cfg
         kp, vp, table, lengths = cache["k_pages"], cache["v_pages"], cache["table"], cache["lengths"]
         T = q.shape[1]
+        if kp.dtype == torch.uint8:                        # 4 bits a number
+            ops.store_rows_int4(k, v, kp, vp, table, lengths)
+            if T == 1:
+                return ops.paged_attention_int4(q[:, 0], kp, vp, table, lengths, None, cfg.sliding_window, **self._scores(q.device))[:, None]
+            if position_offset:                            # a portion sees its own rows as they are, those in front of it as the pages hold them
+                old = ops.read_rows_int4(kp, vp, table, lengths, position_offset, self.D, k.dtype)
+                k, v = (torch.cat(t, dim=1) for t in zip(old, (k, v)))
+            return ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, position_offset, cfg.sliding_window, **self._scores(q.device))
         if T == 1:
             return ops.paged_attention(q[:, 0], kp, vp, table, lengths, None, cfg.sliding_window, k_new=k[:, 0], v_new=v[:, 0], **self._scores(q.device))[:, None]
         page = kp.shape[1]
@@ -136,29 +144,52 @@ class SelfAttention(nn.Module):
         qkv = self.linear_qkv(x)
         B, T = qkv.shape[:2]
         qkv = qkv.reshape(B, T, self.Gl, self.qpg + 2, self.D)
-        q = qkv[:, :, :, : self.qpg].reshape(B, T, self.Gl * self.qpg, self.D)
-        k, v = qkv[:, :, :, self.qpg], qkv[:, :, :, self.qpg + 1]
-        if cfg.qk_layernorm:
-            q = ops.rms_norm(q.contiguous(), self.q_layernorm.weight, cfg.norm_eps)
-            k = ops.rms_norm(k.contiguous(), self.k_layernorm.weight, cfg.norm_eps)
         cp = self.mesh["cp"]
         past = cache["k"].shape[1] if (cache is not None and "k" in cache) else 0
         # position_offset is the absolute position of this call's first token (the cache length when decoding)
         pos0 = position_offset + (cp.rank * T if not cp.is_trivial else 0)
         paged = cache is not None and "table" in cache
+        if self.rope is not None and rotary is not None and rotary[0].shape[0] != B * T:
+            raise ValueError(f"{rotary[0].shape[0]} positions for {B} x {T} tokens")
+        if cfg.fused_qkv_heads:
+            q, k, v = self._heads(qkv, cache if paged else None, pos0, rotary)
+            return self._attend(q, k, v, cache, position_offset, key_first)
+        q = qkv[:, :, :, : self.qpg].reshape(B, T, self.Gl * self.qpg, self.D)
+        k, v = qkv[:, :, :, self.qpg], qkv[:, :, :, self.qpg + 1]
+        if cfg.qk_layernorm:
+            q = ops.rms_norm(q.contiguous(), self.q_layernorm.weight, cfg.norm_eps)
+            k = ops.rms_norm(k.contiguous(), self.k_layernorm.weight, cfg.norm_eps)
         if self.rope is not None and paged and T == 1:     # the positions are on the device: a captured step goes on from them
             at = cache["lengths"][:, None].long() - 1
             q = ops.apply_rope_at(q.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
             k = ops.apply_rope_at(k.contiguous(), cache["cos"], cache["sin"], at, cfg.rotary_interleaved)
         elif self.rope is not None and rotary is not None:
-            if rotary[0].shape[0] != B * T:
-                raise ValueError(f"{rotary[0].shape[0]} positions for {B} x {T} tokens")
             q, k = (ops.apply_rope(t.reshape(1, B * T, *t.shape[2:]), *rotary, cfg.rotary_interleaved).view(t.shape) for t in (q, k))
         elif self.rope is not None:
             cos, sin = self.rope.get(T, pos0, x.device)
             q = ops.apply_rope(q.contiguous(), cos, sin, cfg.rotary_interleaved)
             k = ops.apply_rope(k.contiguous(), cos, sin, cfg.rotary_interleaved)
-        if paged:
+        return self._attend(q, k, v, cache, position_offset, key_first)
+
+    def _heads(self, qkv, pages: Optional[dict], first: int, rotary):
+        """Queries, keys and values out of the projection in one pass."""
+        cfg = self.cfg
+        B, T = qkv.shape[:2]
+        weights = (self.q_layernorm.weight, self.k_layernorm.weight) if cfg.qk_layernorm else (None, None)
+        cos = sin = at = None
+        if self.rope is not None and pages is not None and T == 1:      # the positions are on the device: a captured step goes on from them
+            cos, sin, at = pages["cos"], pages["sin"], (pages["lengths"] - 1)[:, None]
+        elif self.rope is not None and rotary is not None:              # a row of the tables for every token
+            cos, sin = rotary
+            at = torch.arange(B * T, device=qkv.device).view(B, T)
+        elif self.rope is not None:
+            cos, sin = self.rope.get(T, first, qkv.device)
+        return ops.qkv_heads(qkv, *weights, cfg.norm_eps, cos, sin, positions=at, interleaved=cfg.rotary_interleaved)
+
+    def _attend(self, q, k, v, cache: Optional[dict], position_offset: int, key_first):
+        cfg, cp = self.cfg, self.mesh["cp"]
+        B, T = q.shape[:2]
+        if cache is not None and "table" in cache:
             o = self._from_pages(q, k, v, cache, position_offset)
             return self.linear_proj(o.reshape(B, T, -1))
         k, v, q_off = _kv_cache_update(cache, k, v)
@@ -167,7 +198,7 @@ class SelfAttention(nn.Module):
             v = C.all_gather(v.contiguous(), cp, dim=1)
             q_off = cp.rank * T
         o = ops.softmax_attention(q.contiguous(), k.contiguous(), v.contiguous(), None, True, q_off, cfg.sliding_window, key_first=key_first,
-                                  **self._scores(x.device))
+                                  **self._scores(q.device))
         return self.linear_proj(o.reshape(B, T, -1))
 
     @torch.no_grad()
