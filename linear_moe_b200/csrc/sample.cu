@@ -96,8 +96,9 @@ constexpr int COARSE = BINS / 32;
 static_assert(COARSE <= 32, "a lane for 32 bins");
 struct Shared {
     Bins bins[2];
-    u64 coarse_mass[COARSE], all_mass[MAX_PARTS][32];  // of 32 bins together, read by the others; what they have
-    uint32_t coarse_count[COARSE], all_count[MAX_PARTS][32];
+    // of 32 bins together, read by the others, who may still be at it when this CTA has gone on to its next level: two sets in turn, as of the bins
+    u64 coarse_mass[2][COARSE], all_mass[MAX_PARTS][32];
+    uint32_t coarse_count[2][COARSE], all_count[MAX_PARTS][32];
     double powers[32];
     uint32_t count[WARPS];
     u64 mass[WARPS];
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
                     count += __shfl_xor_sync(0xffffffffu, count, o);
                     mass += __shfl_xor_sync(0xffffffffu, mass, o);
                 }
-                if (lane == 0) sm.coarse_count[c] = count, sm.coarse_mass[c] = mass;
+                if (lane == 0) sm.coarse_count[turn][c] = count, sm.coarse_mass[turn][c] = mass;
             }
             cl.sync();
             for (int i = tid; i < (int)(sizeof(Bins) / 4); i += THREADS) reinterpret_cast<uint32_t*>(&sm.bins[turn ^ 1])[i] = 0;
@@ -281,8 +282,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
                 if (warp < a.parts) {
                     const Shared* o = cl.map_shared_rank(&sm, warp);
                     const bool there = step == 1 || lane < COARSE;
-                    sm.all_count[warp][lane] = !there ? 0 : step ? o->bins[turn].count[bin + lane] : o->coarse_count[lane];
-                    sm.all_mass[warp][lane] = !there || !by_mass ? 0 : step ? mass_of(o->bins[turn], bin + lane) : o->coarse_mass[lane];
+                    sm.all_count[warp][lane] = !there ? 0 : step ? o->bins[turn].count[bin + lane] : o->coarse_count[turn][lane];
+                    sm.all_mass[warp][lane] = !there || !by_mass ? 0 : step ? mass_of(o->bins[turn], bin + lane) : o->coarse_mass[turn][lane];
                 }
                 __syncthreads();
                 if (warp == 0) {
