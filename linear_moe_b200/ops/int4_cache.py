@@ -97,8 +97,8 @@ def _store_plan(k_new, v_new, k_pages, v_pages, table, lengths):
         raise ValueError("rows are [B, T, heads, D], keys and values alike, in fp32, bf16 or fp16, where the pools lie")
     B, T, G, D = k_new.shape
     page = _check_pools(k_pages, v_pages, table, lengths, B, G, D)
-    if T >= 1 << 30 or B * T * G * D // 8 >= (1 << 31) * 128:
-        raise ValueError(f"{B} x {T} rows are more than the kernel counts")
+    if T >= 1 << 30 or G > 32767:
+        raise ValueError(f"{T} rows of {G} heads are more than the kernel counts")
     a = _rows_args(table, page, k_pages.shape[0], G, D, T)
     rows = True                                             # strides of the rows as they are: 16-byte steps
     for i, t in enumerate((k_new, v_new)):
@@ -138,8 +138,8 @@ def _read_plan(k_pages, v_pages, table, lengths, n, dim, dtype):
     if table.dim() != 2:
         raise ValueError("the table is int32 [B, pages]")
     page = _check_pools(k_pages, v_pages, table, lengths, table.shape[0], None, dim)
-    if n >= 1 << 30 or table.shape[0] * n * k_pages.shape[1] * dim // 8 >= (1 << 31) * 128:
-        raise ValueError(f"{table.shape[0]} x {n} rows are more than the kernel counts")
+    if n >= 1 << 30 or k_pages.shape[1] > 32767:
+        raise ValueError(f"{n} rows of {k_pages.shape[1]} heads are more than the kernel counts")
     return bytes(_rows_args(table, page, k_pages.shape[0], k_pages.shape[1], dim, n))
 
 
