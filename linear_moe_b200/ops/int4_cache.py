@@ -26,7 +26,7 @@ UNIT, GROUP, WIDEST = R.UNIT, 16, 256
 
 class _Rows(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p * 2), ("pool", ctypes.c_void_p * 2), ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("x_b", ctypes.c_longlong * 2), ("x_t", ctypes.c_longlong * 2),
-                ("x_g", ctypes.c_longlong * 2), ("table_ld", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in ("B", "T", "G", "D", "page", "pages", "table_n")] + [("err", ctypes.c_void_p)]
+                ("x_g", ctypes.c_longlong * 2), ("table_ld", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in ("B", "T", "G", "D", "page", "pages", "table_n", "page_bits")] + [("err", ctypes.c_void_p)]
 
 
 class _Step(ctypes.Structure):
@@ -88,7 +88,7 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_args(table, page, pages, G, D, T) -> _Rows:
-    return _Rows(table_ld=table.stride(0), B=table.shape[0], T=T, G=G, D=D, page=page, pages=pages, table_n=table.shape[1])
+    return _Rows(table_ld=table.stride(0), B=table.shape[0], T=T, G=G, D=D, page=page, pages=pages, table_n=table.shape[1], page_bits=page.bit_length() - 1 if page & (page - 1) == 0 else -1)
 
 
 # ---- rows into the cache ----------------------------------------------------------------------------------------------------------

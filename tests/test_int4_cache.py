@@ -120,6 +120,12 @@ def groups():
         x[17] = float(bad)
         g.append(x)
     g += [torch.randn(32, generator=gen) * 10.0 ** i for i in range(-6, 7)]
+    for i in range(20):                                     # quotients at and next to the borders between two codes
+        size = 2.0 ** (i - 10)
+        x = torch.randint(0, 30, (32,), generator=gen).float() / 2 * size
+        x[3], x[20] = 0.0, 14.96875 * size              # a size that is a power of two
+        x[i] = x[i].nextafter(torch.tensor(100.0 if i % 2 else -100.0)) if float(x[i]) > 0 else x[i]
+        g.append(x - (i % 3) * 4 * size)
     return torch.stack(g)
 
 
