@@ -172,7 +172,7 @@ static int by_width(const RowArgs& a, bool read, cudaStream_t st) {
 LMOE_API int lmoe_int4_rows(const lmoe::int4::RowArgs* ap, int type, int read, cudaStream_t st) {
     using namespace lmoe::int4;
     const RowArgs& a = *ap;
-    if (a.B <= 0 || a.B > 65535 || a.T <= 0 || a.G <= 0 || a.G > 32767 || a.D <= 0 || a.D > 256 || a.D % UNIT != 0 || a.page <= 0 || a.page % 16 != 0 || a.pages < 0 || a.table_n < 0 ||
-        (long long)a.table_n * a.page > 0x7fffffff - 16) return -1;
+    if (a.B <= 0 || a.B > 65535 || a.T <= 0 || a.G <= 0 || a.G > 32767 || a.D <= 0 || a.D > 256 || a.D % UNIT != 0 || a.page <= 0 || a.page > 65536 || a.page % 16 != 0 || a.pages < 0 || a.table_n < 0 ||
+        (long long)a.table_n * a.page > 0x7fffffff - 4096) return -1;
     return type == 0 ? by_width<float>(a, read, st) : type == 1 ? by_width<lmoe::bf16>(a, read, st) : by_width<__half>(a, read, st);
 }

@@ -11,8 +11,13 @@
 // Queries go in scaled by a power of two per head, which fp16 holds exactly but for what is below 2^-35 of the head's largest number.  p size is rounded to 11 bits, for fp16 outputs to 22 (a second product); a power of
 // two per warp keeps it at 2^15 at most, where p is 1 and size the largest one seen at 2^7 (fp16 tells 2^-24 apart there).
 //
-// A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys; a warp takes every fourth group of 16 keys and has a ring of its own, which bulk copies fill (a lane per copy), so no warp waits
-// for another one until the end.  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
+// A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys, 128 at a time: a stage of a ring of two, of which a warp reads 32 keys.  The warps take turns in filling the stages by bulk
+// copies, a lane per copy (64 rows of a page lie together: eight copies a stage; pages of other sizes: 32).  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
+//
+// 64 requests of up to 8192 keys, 32 over 8 heads of 128, capped (390 MB, 59 us at the copy rate): 107 us.  Issue slots are what it runs out of: 390 instructions for 16 keys, half of them on the ALU pipe, with 16 warps
+// per SM.  What took it there: heads as the rows of the score products, codes as 128 + code in bf16 and their sums taken out again 185; keys as the rows, addresses of 32 bits 152; two groups of 16 keys at a time 137; codes
+// as small fp16 numbers 129; rings of the CTA instead of the warps' own (fewer, larger copies) 121; four CTAs per SM with two stages instead of three with three 113.  Two of up to 100001 keys, 16 over 2 heads of 64: 24 us.
+// (Keys and values in five places of their own, more of them on their way: 123, for a second wait in every stage.)
 // Rows of a group that are hidden (behind the last key, in front of the window, on a page that is none) are masked, and their values' scales set to zero in the ring, so that nothing stale meets a weight of zero.
 // A NaN score raises no maximum, so what has seen nothing is told by its sum of zero, not by its maximum: a head that sees NaN gives NaN.
 //
@@ -30,13 +35,7 @@ namespace lmoe {
 namespace int4 {
 namespace cg = cooperative_groups;
 
-#ifndef XST
-#define XST 2
-#endif
-#ifndef XCTAS
-#define XCTAS 4
-#endif
-constexpr int CTAS = XCTAS, WARPS = 4, STAGES = XST, MAX_CLUSTER = 8, HEADS = 8, ROWS = 64;
+constexpr int CTAS = 4, WARPS = 4, STAGES = 2, MAX_CLUSTER = 8, HEADS = 8, ROWS = 64;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 __device__ __forceinline__ uint32_t pack2(float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-    // What a lane reads of a stage: of keys, rows g g + 8's words t and sizes; of values, rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9's half-words g and sizes
+    // What a lane reads of a stage: of keys, the words t and the sizes of rows g and g + 8; of values, the half-words g and the sizes of rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9
     const uint32_t part = (w >> 1) * PART, codes_at = part + (w & 1) * 2 * GROUP * (D / 2), scales_at = part + (w & 1) * 2 * GROUP * (D / 8);
     const uint32_t at_k = codes_at + g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = codes_at + 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = scales_at + g * (D / 8), at_ks = at_s + 4 * t, at_v2 = scales_at + 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
     auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };

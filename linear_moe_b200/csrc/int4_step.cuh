@@ -36,8 +36,8 @@ __device__ __forceinline__ Share share_of(const StepArgs& a, int b) {
 }
 
 inline bool fits(const StepArgs& a) {
-    return a.B > 0 && a.B <= 65535 && a.G > 0 && a.H > 0 && a.H % a.G == 0 && a.D > 0 && a.D <= 256 && a.D % UNIT == 0 && a.page > 0 && a.page % GROUP == 0 && a.pages >= 0 && a.table_n >= 0 &&
-           (long long)a.table_n * a.page <= 0x7fffffff - GROUP && a.splits >= 1;
+    return a.B > 0 && a.B <= 65535 && a.G > 0 && a.H > 0 && a.H % a.G == 0 && a.D > 0 && a.D <= 256 && a.D % UNIT == 0 && a.page > 0 && a.page <= 65536 && a.page % GROUP == 0 && a.pages >= 0 && a.table_n >= 0 &&
+           (long long)a.table_n * a.page <= 0x7fffffff - 4096 && a.splits >= 1;
 }
 
 }  // namespace int4

@@ -8,6 +8,10 @@
 // A row is one cluster's: each CTA reads its part of the logits once and keeps it in shared memory where that holds it.  Then, if anything is cut off: a histogram over the weights' logarithms (16 bins
 // for a factor of two) with the number and the weight of each bin's tokens tells the bin in which the cut lies; histograms over the numbers inside of it tell the logit, and the equal ones are counted
 // by their numbers.  Last, the kept weights are summed up per thread, and a scan finds the thread, and the token, that the random number falls to.
+//
+// One row of 32000 logits 16 us, 17 rows of 50257 with settings of their own 24, 128 rows of 128256 in fp32 with top-p 165 (the logits alone take 10 at the copy rate): what it spends its time on is some 60 instructions
+// around each exponential, once for the histogram and once for what is kept, and the cluster's barriers (about 1 us each, five or six of them).  The first form, a CTA per 65536 logits with branches around its
+// exponentials, took 68, 96 and 273.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>

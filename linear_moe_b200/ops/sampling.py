@@ -70,8 +70,9 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
     return token, torch.where(whole[:, 0] > 0, share[:, 0].log(), float("-inf")).float()
 
 
-def _shares(B: int, V: int, slots: int) -> Tuple[int, int]:
-    """(CTAs of a row, logits of each)."""
+def _shares(V: int) -> Tuple[int, int]:
+    """(CTAs of a row, logits of each): as many as a cluster has, of 2048 logits at least (one row of 32000: 43 us in one part, 31 in two, 23 in four, 18 in eight; 128 rows of 128256 in fp32, top-p: 197 in two,
+    201 in four, 162 in eight; in bf16 with the 50 largest 133, 107, 125)."""
     parts = 1
     while parts < 8 and parts * 2048 < V:
         parts *= 2
@@ -86,10 +87,9 @@ _PLANS: Dict[tuple, bytes] = {}
 
 
 def _plan(logits, draw, temperature, top_k, top_p, min_p) -> bytes:
-    from . import cuda as K
     _check(logits, draw, temperature, top_k, top_p, min_p)
     B, V = logits.shape
-    parts, length = _shares(B, V, K.num_sms())
+    parts, length = _shares(V)
     def number(x):
         return 0 if torch.is_tensor(x) else x
     return bytes(_Args(ld=logits.stride(0), B=B, V=V, parts=parts, len=length, k=min(int(number(top_k)), MOST), t=number(temperature), p=min(float(number(top_p)), 2.0), least=number(min_p)))

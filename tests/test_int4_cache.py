@@ -441,3 +441,16 @@ def test_pages_copied_with_the_others():
     want = attend(s)
     s["table"][0, :2] = torch.tensor(free, dtype=torch.int32)
     assert torch.equal(attend(s), want)
+
+
+def test_sizes_that_the_kernels_do_not_count():
+    """Refused by shape alone: long tables and pages, many heads."""
+    lengths = torch.zeros(1, dtype=torch.int32)
+    pool = ops.int4_pages(1, 1, 32)
+    with pytest.raises(ValueError, match="longer tables"):
+        ops.read_rows_int4(pool, pool, torch.zeros(1, dtype=torch.int32).expand(1, (1 << 31) // 64), lengths, 1, 32, F)
+    with pytest.raises(ValueError):
+        ops.int4_pages(1, 1, 32, 65552)
+    wide = torch.zeros(0, 32768, 320, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="heads are more"):
+        ops.read_rows_int4(wide, wide, torch.zeros(1, 0, dtype=torch.int32), lengths, 1, 32, F)
