@@ -3,8 +3,8 @@
 // so that every number of the group lies between low and low + 15 size and comes back within size / 2.  Each step is one IEEE operation in 32 bits (compiled without approximate functions), so the codes
 // are the same wherever they are computed.  A group with a number that is not finite, or whose range 32 bits do not hold, comes back as NaN.
 //
-// Bound by memory: a thread takes eight numbers of four rows, four threads a group, a block the rows of one head of a request, so that codes and scales are written and read in whole sectors and four loads
-// are on their way at once.
+// Bound by memory, if few instructions are spent on a number: a thread takes half a group of each of four rows, a block the rows of one head of a request, so that codes and scales are written and read in whole
+// sectors and four loads are on their way at once.
 #include "int4_cache.cuh"
 
 namespace lmoe {
@@ -20,7 +20,7 @@ struct RowArgs {
 };
 __device__ __forceinline__ int over_page(const RowArgs& a, int key) { return a.page_bits >= 0 ? key >> a.page_bits : key / a.page; }
 
-constexpr int ROWS = 4, READ_ROWS = 4;   // of a thread
+constexpr int ROWS = 4;                  // of a thread
 // The page of a request's key; -1: none (reported)
 __device__ __forceinline__ int page_of(const RowArgs& a, int b, int key) {
     const int p = a.table[b * a.table_ld + over_page(a, key)];
@@ -32,120 +32,114 @@ __device__ __forceinline__ int page_of(const RowArgs& a, int b, int key) {
 // N: groups of a head.  Block (x, y, z): rows of head y / 2, keys or values, of request z.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) int4_store_kernel(const RowArgs a) {
-    constexpr int UNITS = 4 * N, D = 32 * N;
+    constexpr int UNITS = 2 * N, D = 32 * N;
     const int z = blockIdx.y & 1, g = blockIdx.y >> 1, b = blockIdx.z, step = blockDim.x / UNITS, u = threadIdx.x % UNITS, first = blockIdx.x * step * ROWS + threadIdx.x / UNITS;
-    if (threadIdx.x >= step * UNITS) return;         // (a group's four threads stay or go together)
-    const unsigned group = 0xfu << (threadIdx.x & 28);
+    if (threadIdx.x >= step * UNITS) return;         // (a group's two threads stay or go together)
+    const unsigned group = 3u << (threadIdx.x & 30);
     const int n = a.lengths[b];
     if (n < 0 || n > a.table_n * a.page) {
         if (u == 0) atomicCAS(a.err, 0, 0x42000);
         return;
     }
-    float x[ROWS][8];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const int t = first + i * step;
-        if (t < a.T && n - a.T + t >= 0) load8((const T*)a.x[z] + b * a.x_b[z] + t * a.x_t[z] + g * a.x_g[z] + u * 8, x[i]);
-    }
+    const int c = u / 2;
+    const T* from = (const T*)a.x[z] + b * a.x_b[z] + g * a.x_g[z] + u * 16;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int t = first + i * step, key = n - a.T + t;
         if (t >= a.T || key < 0) continue;           // (in front of the request's first row)
+        float x[16];
+        load_row<16>(from + t * a.x_t[z], x);
         const int page = page_of(a, b, key), row = key - over_page(a, key) * a.page;
         if (page < 0) continue;
-        float least = x[i][0], most = x[i][0];
-        bool finite = true;
+        float least = x[0], most = x[0], sum = x[0] * 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            least = fminf(least, x[i][j]);
-            most = fmaxf(most, x[i][j]);
-            finite = finite && fabsf(x[i][j]) <= 3.402823466e38f;
+        for (int j = 1; j < 16; ++j) {
+            least = fminf(least, x[j]);
+            most = fmaxf(most, x[j]);
+            sum = fmaf(x[j], 0.f, sum);              // NaN of infinities and NaN, which least and most pass over
         }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            least = fminf(least, __shfl_xor_sync(group, least, o));
-            most = fmaxf(most, __shfl_xor_sync(group, most, o));
-        }
+        least = fminf(least, __shfl_xor_sync(group, least, 1));
+        most = fmaxf(most, __shfl_xor_sync(group, most, 1));
+        sum += __shfl_xor_sync(group, sum, 1);
         const uint32_t lb = least == 0.f ? 0u : __float_as_uint(least);      // of zeros the positive one
         float low = __uint_as_float((lb >> 31 ? lb + 0xffffu : lb) & 0xffff0000u);
         float size = __uint_as_float((__float_as_uint(__fmul_rn(__fsub_rn(most, low), 1.f / 15.f)) + 0xffffu) & 0xffff0000u);
-        finite = __all_sync(group, finite) && fabsf(low) <= 3.402823466e38f && size <= 3.402823466e38f;
-        if (!finite) low = __uint_as_float(0x7fc00000u), size = 0.f;
+        if (!(sum == 0.f && fabsf(low) <= 3.402823466e38f && size <= 3.402823466e38f)) low = __uint_as_float(0x7fc00000u), size = 0.f;
         // The quotient by a product with the reciprocal is off by less than 4 2^-20 (of 16 at most): where it is that near to a border between two codes, and for sizes whose reciprocal may overflow,
-        // it is divided out.  (Eight divisions for every thread: 27 us instead of 17 for 4 x 1531 rows of 8 heads of 96.)
-        uint32_t code = 0;
+        // it is divided out.
+        uint32_t code[2] = {0, 0};
         if (size > 0.f) {
             const float inverse = __fdiv_rn(1.f, size), magic = 12582912.f;      // 1.5 2^23: what is added to it is rounded to a whole number, which its lowest bits are
-            bool near = !(size > 1e-30f);
+            float far = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float q = fminf(__fmul_rn(__fsub_rn(x[i][j], low), inverse), 15.25f), r = __fadd_rn(q, magic);
-                near |= !(fabsf(__fsub_rn(q, __fsub_rn(r, magic))) < 0.49998f);
-                code |= (__float_as_uint(r) & 15u) << (4 * j);
+            for (int j = 0; j < 16; ++j) {
+                const float q = fminf(__fmul_rn(__fsub_rn(x[j], low), inverse), 15.25f), r = __fadd_rn(q, magic);
+                far = fmaxf(far, fabsf(__fsub_rn(q, __fsub_rn(r, magic))));
+                code[j / 8] |= (__float_as_uint(r) & 15u) << (4 * (j % 8));
             }
-            if (near) {
-                code = 0;
+            if (!(far < 0.49998f && size > 1e-30f)) {
+                code[0] = code[1] = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) code |= (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(x[i][j], low), size)), 15.f) << (4 * j);
+                for (int j = 0; j < 16; ++j) code[j / 8] |= (uint32_t)fminf(rintf(__fdiv_rn(__fsub_rn(x[j], low), size)), 15.f) << (4 * (j % 8));
             }
         }
-        const int c = u / 4;
         unsigned char* at = a.pool[z] + ((long long)page * a.G + g) * page_bytes(a.page, D);
-        reinterpret_cast<uint32_t*>(at + row * (D / 2) + place(N, row, c) * 16)[u % 4] = code;
-        if (u % 4 == 0) {
-            uint16_t* s = reinterpret_cast<uint16_t*>(at + a.page * (D / 2) + row * (D / 8));
-            s[c] = __float_as_uint(low) >> 16;
-            s[N + c] = __float_as_uint(size) >> 16;
-        }
+        *reinterpret_cast<uint2*>(at + row * (D / 2) + place(N, row, c) * 16 + (u & 1) * 8) = make_uint2(code[0], code[1]);
+        reinterpret_cast<uint16_t*>(at + a.page * (D / 2) + row * (D / 8))[u & 1 ? N + c : c] = __float_as_uint(u & 1 ? size : low) >> 16;
     }
 }
 
 // Rows behind a request's last one are zeros.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) int4_read_kernel(const RowArgs a) {
-    constexpr int UNITS = 4 * N, D = 32 * N;
-    const int z = blockIdx.y & 1, g = blockIdx.y >> 1, b = blockIdx.z, step = blockDim.x / UNITS, u = threadIdx.x % UNITS, first = blockIdx.x * step * READ_ROWS + threadIdx.x / UNITS;
+    constexpr int UNITS = 2 * N, D = 32 * N;
+    const int z = blockIdx.y & 1, g = blockIdx.y >> 1, b = blockIdx.z, step = blockDim.x / UNITS, u = threadIdx.x % UNITS, first = blockIdx.x * step * ROWS + threadIdx.x / UNITS;
     if (threadIdx.x >= step * UNITS) return;
-    const int n = a.lengths[b], c = u / 4;
-    int pages[READ_ROWS];                            // (asked for ahead of the length)
+    const int n = a.lengths[b], c = u / 2;
+    int pages[ROWS];                                 // (asked for ahead of the length)
 #pragma unroll
-    for (int i = 0; i < READ_ROWS; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
         const int at = over_page(a, first + i * step);
         pages[i] = at < a.table_n ? a.table[b * a.table_ld + at] : -1;
     }
-    if ((n < 0 || n > a.table_n * a.page) && u == 0) atomicCAS(a.err, 0, 0x42000);
-    uint32_t code[READ_ROWS];
-    float low[READ_ROWS], size[READ_ROWS];
+    const int last = min(n, a.table_n * a.page);
+    if (n != max(last, 0) && u == 0) atomicCAS(a.err, 0, 0x42000);
+    uint2 code[ROWS];
+    float low[ROWS], size[ROWS];
 #pragma unroll
-    for (int i = 0; i < READ_ROWS; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
         const int t = first + i * step;
-        code[i] = 0, low[i] = size[i] = 0.f;
-        if (t >= min(n, a.table_n * a.page) || t >= a.T) continue;
+        code[i] = make_uint2(0, 0), low[i] = size[i] = 0.f;
+        if (t >= last || t >= a.T) continue;
         const int page = pages[i], row = t - over_page(a, t) * a.page;
         if (page < 0 || page >= a.pages) {
             atomicCAS(a.err, 0, 0x43000);
             continue;
         }
         const unsigned char* at = a.pool[z] + ((long long)page * a.G + g) * page_bytes(a.page, D);
-        code[i] = reinterpret_cast<const uint32_t*>(at + row * (D / 2) + place(N, row, c) * 16)[u % 4];
+        code[i] = *reinterpret_cast<const uint2*>(at + row * (D / 2) + place(N, row, c) * 16 + (u & 1) * 8);
         const uint16_t* s = reinterpret_cast<const uint16_t*>(at + a.page * (D / 2) + row * (D / 8));
         low[i] = __uint_as_float((uint32_t)s[c] << 16), size[i] = __uint_as_float((uint32_t)s[N + c] << 16);
     }
+    T* to = (T*)a.x[z] + ((long long)b * a.T * a.G + g) * D + u * 16;
 #pragma unroll
-    for (int i = 0; i < READ_ROWS; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
         const int t = first + i * step;
         if (t >= a.T) continue;
-        float x[8];
+        float x[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = low[i] + size[i] * (__uint_as_float((code[i] >> (4 * j) & 15u) | 0x4b000000u) - 8388608.f);      // (2^23 + code: no conversion)
-        store8((T*)a.x[z] + (((long long)b * a.T + t) * a.G + g) * D + u * 8, x);
+        for (int j = 0; j < 16; ++j) {               // (2^23 + code: no conversion)
+            const uint32_t w = j < 8 ? code[i].x : code[i].y;
+            x[j] = low[i] + size[i] * (__uint_as_float((w >> (4 * (j % 8)) & 15u) | 0x4b000000u) - 8388608.f);
+        }
+        store_row<16>(to + (long long)t * a.G * D, x);
     }
 }
 
 template <typename T, int N>
 static int run(const RowArgs& a, bool read, cudaStream_t st) {
     // blocks of few threads where there are few rows
-    const int units = 4 * N, want = (a.T < 64 ? (a.T * units + 31) / 32 * 32 : 256), threads = want < 32 ? 32 : want < 256 ? want : 256, rows = threads / units * (read ? READ_ROWS : ROWS);
+    const int units = 2 * N, want = (a.T < 64 ? (a.T * units + 31) / 32 * 32 : 256), threads = want < 32 ? 32 : want < 256 ? want : 256, rows = threads / units * ROWS;
     const dim3 grid((unsigned)((a.T + rows - 1) / rows), 2 * a.G, a.B);
     if (read) int4_read_kernel<T, N><<<grid, threads, 0, st>>>(a);
     else int4_store_kernel<T, N><<<grid, threads, 0, st>>>(a);

@@ -24,22 +24,24 @@ template <> __device__ __forceinline__ float num<float>(float x) { return x; }
 template <> __device__ __forceinline__ bf16 num<bf16>(float x) { return __float2bfloat16(x); }
 template <> __device__ __forceinline__ __half num<__half>(float x) { return __float2half(x); }
 
-// Eight consecutive numbers, 16-byte aligned
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    constexpr int N = sizeof(T) / 2;
-    uint4 raw[N];
+// K consecutive numbers (a multiple of eight), 16-byte aligned
+template <int K, typename T> __device__ __forceinline__ void load_row(const T* p, float (&x)[K]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < K * (int)sizeof(T) / 16; ++i) {
+        const uint4 raw = reinterpret_cast<const uint4*>(p)[i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = val(reinterpret_cast<const T*>(raw)[i]);
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[i * (16 / (int)sizeof(T)) + j] = val(reinterpret_cast<const T*>(&raw)[j]);
+    }
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-    constexpr int N = sizeof(T) / 2;
-    __align__(16) T y[8];
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) { load_row<8>(p, x); }
+template <int K, typename T> __device__ __forceinline__ void store_row(T* p, const float (&x)[K]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = num<T>(x[i]);
+    for (int i = 0; i < K * (int)sizeof(T) / 16; ++i) {
+        __align__(16) T y[16 / sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(y)[i];
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) y[j] = num<T>(x[i * (16 / (int)sizeof(T)) + j]);
+        reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(y);
+    }
 }
 
 }  // namespace int4
