@@ -68,11 +68,16 @@ def _key(t: Optional[torch.Tensor]):
     return t if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-_CHECKED: Dict[tuple, bytes] = {}
+class _Plan:
+    """What follows from shapes, strides and types alone: the arguments without their addresses, forward and backward."""
+    __slots__ = ("forward", "backward", "type", "vectors", "rows", "parts", "shapes")
 
 
-def _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved) -> bytes:
-    """The arguments without their addresses: what follows from shapes, strides and types alone."""
+_PLANS: Dict[tuple, _Plan] = {}
+
+
+def _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved) -> _Plan:
+    from . import cuda as K
     _check(qkv, q_weight, k_weight, eps, cos, sin, positions)
     B, T, G, S, D = qkv.shape
     w = q_weight if q_weight is not None else k_weight
@@ -80,7 +85,34 @@ def _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved) -> byt
               interleaved=int(interleaved), at_wide=int(positions is not None and positions.dtype == torch.int64), w_type=0 if w is None else _TYPES[w.dtype], parts=0, eps=eps)
     for i, d in enumerate((a.G * a.r, a.G, a.r, a.T)):
         a.div[2 * i:2 * i + 2] = _divisor(max(d, 1))
-    return bytes(a)
+    p, size = _Plan(), qkv.element_size()
+    p.type, p.shapes = _TYPES[qkv.dtype], ((B, T, G * (S - 2), D), (B, T, G, D))
+    # Heads that divide into 16 bytes a thread; what does not lie on 16-byte boundaries is copied for them, so that the result is the same wherever a tensor lies.
+    e = 16 // size
+    p.vectors = a.D % (2 * e) == 0 and a.D <= 64 * e and a.R % (2 * e) == 0 and a.rows * a.G * a.r < 1 << 31
+    p.rows = not p.vectors or all(s * size % 16 == 0 for s in qkv.stride()[:2])
+    a.vectors = int(p.vectors)
+    if p.vectors:
+        _blocks(a, size, 4 * K.num_sms())
+    p.forward = bytes(a)
+    if p.vectors:
+        _blocks(a, size, 2 * K.num_sms())
+        p.parts = a.parts_q + a.parts_k
+    else:
+        a.parts = max(1, min(-(-a.rows * a.G * S // 8), 8 * K.num_sms()))
+        p.parts = 2 * a.parts
+    p.backward = bytes(a)
+    return p
+
+
+def _blocks(a: _Args, size: int, most: int):
+    """Blocks of the vectors' kernels: of queries, keys and values by their number, up to what the GPU holds at once (four per SM forward, two backward)."""
+    threads = 4
+    while threads * 2 * (16 // size) < a.D:
+        threads *= 2
+    share = max(1, min(-(-a.rows * a.G * threads // 256), most // (a.r + 2)))
+    a.parts_k, a.parts_q = share, max(1, min(-(-a.rows * a.G * a.r * threads // 256), most - 2 * share))
+    a.parts = a.parts_q + 2 * share
 
 
 def _divisor(d: int):
@@ -94,43 +126,28 @@ def _dense_heads(t: torch.Tensor) -> bool:
     return t[0, 0].is_contiguous() if t.numel() else True
 
 
-def _blocks(a: _Args, size: int, back: bool):
-    """Blocks of the vectors' kernels: of queries, keys and values by their number, up to what the GPU holds at once."""
-    from . import cuda as K
-    threads = 4
-    while threads * 2 * (16 // size) < a.D:
-        threads *= 2
-    keys = -(-a.rows * a.G * threads // 256)
-    most = (2 if back else 4) * K.num_sms()
-    share = max(1, min(keys, most // (a.r + 2)))
-    a.parts_k, a.parts_q = share, max(1, min(-(-a.rows * a.G * a.r * threads // 256), most - 2 * share))
-    a.parts = a.parts_q + 2 * share
-
-
-def _vectors(a: _Args, size: int) -> bool:
-    """Do heads of this size go through the kernels that read 16 bytes at a time?  Then what does not lie on 16-byte boundaries is copied: the result is the same wherever a tensor lies."""
-    e = 16 // size
-    return a.D % (2 * e) == 0 and a.D <= 64 * e and a.R % (2 * e) == 0 and a.rows * a.G * a.r < 1 << 31
-
-
-def _aligned(t: Optional[torch.Tensor], strides=()) -> bool:
-    return t is None or not t.data_ptr() % 16 and all(s * t.element_size() % 16 == 0 for s in strides)
-
-
 def _forward(qkv, wq, wk, plan, cos, sin, at):
     from . import cuda as K
-    B, T, G, S, D = qkv.shape
     dev, dt = qkv.device, qkv.dtype
-    q, k, v = (torch.empty((B, T, n, D), dtype=dt, device=dev) for n in (G * (S - 2), G, G))
-    a = _Args.from_buffer_copy(plan)
-    a.x, a.wq, a.wk, a.q, a.k, a.v = qkv.data_ptr(), K._ptr(wq), K._ptr(wk), q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.cos, a.sin, a.at, a.err = K._ptr(cos), K._ptr(sin), K._ptr(at), K.error_word(dev)
+    heads, keys = plan.shapes
+    q, k, v = torch.empty(heads, dtype=dt, device=dev), torch.empty(keys, dtype=dt, device=dev), torch.empty(keys, dtype=dt, device=dev)
+    a = _Args.from_buffer_copy(plan.forward)
+    a.x, a.q, a.k, a.v, a.err = qkv.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), K.error_word(dev)
+    _inputs(a, wq, wk, cos, sin, at)
     with on_device(qkv):
-        if _vectors(a, dt.itemsize):
-            a.vectors = 1
-            _blocks(a, dt.itemsize, False)
-        K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), _TYPES[dt], 0, K._st()), "qkv_heads")
+        K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), plan.type, 0, K._st()), "qkv_heads")
     return q, k, v
+
+
+def _inputs(a: _Args, wq, wk, cos, sin, at):
+    if wq is not None:
+        a.wq = wq.data_ptr()
+    if wk is not None:
+        a.wk = wk.data_ptr()
+    if cos is not None:
+        a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+        if at is not None:
+            a.at = at.data_ptr()
 
 
 class _QkvHeads(torch.autograd.Function):
@@ -146,27 +163,20 @@ class _QkvHeads(torch.autograd.Function):
     def backward(ctx, dq, dk, dv):
         from . import cuda as K
         qkv, wq, wk, cos, sin, at = ctx.saved_tensors
-        dev, D = qkv.device, qkv.shape[4]
-        a = _Args.from_buffer_copy(ctx.plan)
-        grads = [None if g is None else g.contiguous() for g in (dq, dk, dv)]
+        dev, plan = qkv.device, ctx.plan
+        a = _Args.from_buffer_copy(plan.backward)
+        grads = [g if g is None or (g.is_contiguous() and not (plan.vectors and g.data_ptr() % 16)) else g.clone(memory_format=torch.contiguous_format) for g in (dq, dk, dv)]
+        a.dq, a.dk, a.dv = (K._ptr(g) for g in grads)
         dx = torch.empty(qkv.shape, dtype=qkv.dtype, device=dev)
         dws = [torch.empty_like(w) if w is not None and need else None for w, need in zip((wq, wk), ctx.needs_input_grad[1:3])]
-        a.x, a.wq, a.wk, a.cos, a.sin, a.at, a.err = qkv.data_ptr(), K._ptr(wq), K._ptr(wk), K._ptr(cos), K._ptr(sin), K._ptr(at), K.error_word(dev)
-        a.dq, a.dk, a.dv = (K._ptr(g) for g in grads)
-        a.dx, a.dwq, a.dwk = dx.data_ptr(), K._ptr(dws[0]), K._ptr(dws[1])
+        a.x, a.dx, a.dwq, a.dwk, a.err = qkv.data_ptr(), dx.data_ptr(), K._ptr(dws[0]), K._ptr(dws[1]), K.error_word(dev)
+        _inputs(a, wq, wk, cos, sin, at)
+        work = None
+        if dws[0] is not None or dws[1] is not None:
+            work = torch.empty(plan.parts * a.D, dtype=torch.float32, device=dev)
+            a.part = work.data_ptr()
         with on_device(qkv):
-            if _vectors(a, qkv.dtype.itemsize):
-                grads = [g if _aligned(g) else g.clone() for g in grads]
-                a.dq, a.dk, a.dv = (K._ptr(g) for g in grads)
-                a.vectors = 1
-                _blocks(a, qkv.dtype.itemsize, True)
-                parts = a.parts_q + a.parts_k
-            else:
-                a.parts = max(1, min(-(-a.rows * a.G * (a.r + 2) // 8), 8 * K.num_sms()))
-                parts = 2 * a.parts
-            work = torch.empty(parts * D, dtype=torch.float32, device=dev) if dws[0] is not None or dws[1] is not None else None
-            a.part = K._ptr(work)
-            K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), _TYPES[qkv.dtype], 1, K._st()), "qkv_heads backward", 1 if work is None else 2)
+            K._check(K.lib().lmoe_qkv_heads(ctypes.byref(a), plan.type, 1, K._st()), "qkv_heads backward", 1 if work is None else 2)
         return (dx, *dws, None, None, None, None)
 
 
@@ -176,23 +186,24 @@ def qkv_heads(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weig
     if not qkv.is_cuda:
         _check(qkv, q_weight, k_weight, eps, cos, sin, positions)
         return R.qkv_heads(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved)
+    # the host's share of a short call is as long as the kernels: checks, strides and the launch's shape are worked out once per layout
     key = (_key(qkv), _key(q_weight), _key(k_weight), eps, _key(cos), _key(sin), _key(positions), interleaved, cos is not None and (cos.requires_grad or sin.requires_grad))
-    plan = _CHECKED.get(key)
+    plan = _PLANS.get(key)
     if plan is None:
-        if len(_CHECKED) >= 4096:
-            _CHECKED.clear()
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
         if not all(t is None or t.is_contiguous() for t in (q_weight, k_weight, cos, sin, positions)) or not _dense_heads(qkv):
             _check(qkv, q_weight, k_weight, eps, cos, sin, positions)
             flat = lambda t: t if t is None else t.contiguous()      # noqa: E731
             return qkv_heads(qkv if _dense_heads(qkv) else qkv.contiguous(), flat(q_weight), flat(k_weight), eps, flat(cos), flat(sin), positions=flat(positions), interleaved=interleaved)
-        plan = _CHECKED[key] = _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved)
-    B, T, G, S, D = qkv.shape
-    if B * T * G == 0:
+        plan = _PLANS[key] = _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved)
+    if qkv.numel() == 0:
+        B, T, G, S, D = qkv.shape
         return qkv[..., : S - 2, :].reshape(B, T, G * (S - 2), D), qkv[..., S - 2, :], qkv[..., S - 1, :]
-    if not _aligned(qkv, qkv.stride()[:2]) or not _aligned(cos) or not _aligned(sin):
-        if _vectors(_Args.from_buffer_copy(plan), qkv.element_size()):
-            qkv = qkv if _aligned(qkv, qkv.stride()[:2]) else qkv.clone(memory_format=torch.contiguous_format)
-            return qkv_heads(qkv, q_weight, k_weight, eps, *(t if _aligned(t) else t.clone() for t in (cos, sin)), positions=positions, interleaved=interleaved)
+    if plan.vectors and (not plan.rows or (qkv.data_ptr() | (0 if cos is None else cos.data_ptr() | sin.data_ptr())) % 16):
+        qkv = qkv if plan.rows and not qkv.data_ptr() % 16 else qkv.clone(memory_format=torch.contiguous_format)
+        cos, sin = (t if t is None or not t.data_ptr() % 16 else t.clone() for t in (cos, sin))
+        return qkv_heads(qkv, q_weight, k_weight, eps, cos, sin, positions=positions, interleaved=interleaved)
     if not torch.is_grad_enabled() or not (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
         return _forward(qkv, q_weight, k_weight, plan, cos, sin, positions)
     return _QkvHeads.apply(qkv, q_weight, k_weight, plan, cos, sin, positions)

@@ -80,19 +80,29 @@ def _shares(V: int) -> Tuple[int, int]:
 
 
 def _key(x):
-    return (x.shape, x.stride(), x.dtype, x.device) if torch.is_tensor(x) else x
+    return (x.shape, x.stride(), x.dtype, x.device) if isinstance(x, torch.Tensor) else x
 
 
-_PLANS: Dict[tuple, bytes] = {}
+class _Plan:
+    """What follows from shapes, strides, types and the numbers among the settings: the arguments without their addresses."""
+    __slots__ = ("args", "type", "flat", "tensors")
 
 
-def _plan(logits, draw, temperature, top_k, top_p, min_p) -> bytes:
+_PLANS: Dict[tuple, _Plan] = {}
+
+
+def _plan(logits, draw, temperature, top_k, top_p, min_p) -> _Plan:
     _check(logits, draw, temperature, top_k, top_p, min_p)
     B, V = logits.shape
     parts, length = _shares(V)
-    def number(x):
-        return 0 if torch.is_tensor(x) else x
-    return bytes(_Args(ld=logits.stride(0), B=B, V=V, parts=parts, len=length, k=min(int(number(top_k)), MOST), t=number(temperature), p=min(float(number(top_p)), 2.0), least=number(min_p)))
+    settings = (temperature, top_k, top_p, min_p)
+    t, k, share, least = (0 if isinstance(x, torch.Tensor) else x for x in settings)
+    p = _Plan()
+    p.args = bytes(_Args(ld=logits.stride(0), B=B, V=V, parts=parts, len=length, k=min(int(k), MOST), t=t, p=min(float(share), 2.0), least=least))
+    p.type = _TYPES[logits.dtype]
+    p.flat = all(not isinstance(x, torch.Tensor) or x.stride(-1) == 1 or x.shape[-1] <= 1 for x in (logits, draw, *settings))
+    p.tensors = [(name, i) for i, (name, x) in enumerate(zip(("temperature", "top_k", "top_p", "min_p"), settings)) if isinstance(x, torch.Tensor)]
+    return p
 
 
 def sample_tokens(logits: torch.Tensor, draw: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0, top_p: Setting = 1.0, min_p: Setting = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -109,16 +119,17 @@ def sample_tokens(logits: torch.Tensor, draw: torch.Tensor, temperature: Setting
         if len(_PLANS) >= 4096:
             _PLANS.clear()
         plan = _PLANS[key] = _plan(logits, draw, temperature, top_k, top_p, min_p)
-    B, V = logits.shape
-    flat = [t if not torch.is_tensor(t) or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous() for t in (logits, draw, temperature, top_k, top_p, min_p)]
-    if flat[0] is not logits:
-        return sample_tokens(*flat)
-    token, logp = torch.empty(B, dtype=torch.int64, device=logits.device), torch.empty(B, dtype=torch.float32, device=logits.device)
+    settings = (temperature, top_k, top_p, min_p)
+    if not plan.flat:
+        return sample_tokens(*(t.contiguous() if isinstance(t, torch.Tensor) and t.stride(-1) != 1 else t for t in (logits, draw, *settings)))
+    B, dev = logits.shape[0], logits.device
+    token, logp = torch.empty(B, dtype=torch.int64, device=dev), torch.empty(B, dtype=torch.float32, device=dev)
     if B == 0:
         return token, logp
-    a = _Args.from_buffer_copy(plan)
-    a.logits, a.draw, a.token, a.logp = logits.data_ptr(), flat[1].data_ptr(), token.data_ptr(), logp.data_ptr()
-    a.temperature, a.top_k, a.top_p, a.min_p = (t.data_ptr() if torch.is_tensor(t) else 0 for t in flat[2:])
+    a = _Args.from_buffer_copy(plan.args)
+    a.logits, a.draw, a.token, a.logp = logits.data_ptr(), draw.data_ptr(), token.data_ptr(), logp.data_ptr()
+    for name, i in plan.tensors:
+        setattr(a, name, settings[i].data_ptr())
     with on_device(logits):
-        K._check(K.lib().lmoe_sample(ctypes.byref(a), _TYPES[logits.dtype], K._st()), "sample")
+        K._check(K.lib().lmoe_sample(ctypes.byref(a), plan.type, K._st()), "sample")
     return token, logp
