@@ -16,7 +16,7 @@
 //
 // 64 requests of up to 8192 keys, 32 over 8 heads of 128, capped (390 MB, 59 us at the copy rate): 107 us.  Issue slots are what it runs out of: 390 instructions for 16 keys, half of them on the ALU pipe, with 16 warps
 // per SM.  What took it there: heads as the rows of the score products, codes as 128 + code in bf16 and their sums taken out again 185; keys as the rows, addresses of 32 bits 152; two groups of 16 keys at a time 137; codes
-// as small fp16 numbers 129; rings of the CTA instead of the warps' own (fewer, larger copies) 121; four CTAs per SM with two stages instead of three with three 113.  Two of up to 100001 keys, 16 over 2 heads of 64: 24 us.
+// as small fp16 numbers 129; rings of the CTA instead of the warps' own (fewer, larger copies) 121; four CTAs per SM with two stages instead of three with three 113.  Two of up to 100001 keys, 16 over 2 heads of 64: 23 us.
 // (Keys and values in five places of their own, more of them on their way: 123, for a second wait in every stage.)
 // Rows of a group that are hidden (behind the last key, in front of the window, on a page that is none) are masked, and their values' scales set to zero in the ring, so that nothing stale meets a weight of zero.
 // A NaN score raises no maximum, so what has seen nothing is told by its sum of zero, not by its maximum: a head that sees NaN gives NaN.
@@ -459,36 +459,46 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     cl.sync();                                                         // the other CTAs have read this one's part
 }
 
-// The parts of a request's CTAs: a block per (request, query head), a warp per part, a lane per four numbers.
-constexpr int JOIN_WARPS = 8;
-template <typename T>
+// The parts of a request's CTAs: a block per (request, query head), a lane per four numbers of a part, as many parts a warp as it has lanes for.  (A part a warp, eight warps: 148 parts of 64 numbers 24.8 us with
+// the kernel ahead of it, now 22.8, replayed.)
+constexpr int JOIN_WARPS = 16;
+template <typename T, int N>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) {
-    __shared__ float4 O[JOIN_WARPS][32];
+    constexpr int D = 32 * N, LANES = N == 3 ? 32 : D / 4, SUB = 32 / LANES;
+    __shared__ float4 O[JOIN_WARPS][LANES];
     __shared__ float L[JOIN_WARPS];
     pdl_wait();
-    const int bh = blockIdx.x, b = bh / a.H, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int bh = blockIdx.x, b = bh / a.H, w = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LANES * 4;
     const Share sh = share_of(a, b);
     const int n = (sh.last - sh.first + sh.per - 1) / sh.per;
     const float* ml = a.ml + (long long)bh * a.splits * 2;
-    const float* part = a.part + (long long)bh * a.splits * a.D + lane * 4;
-    const bool mine = lane * 4 < a.D;
+    const float* part = a.part + (long long)bh * a.splits * D + d;
+    const bool mine = d < D;
     float top = -INFINITY;                                             // of all parts, first: then no part waits for the one before it
     for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[2 * s]);
     top = warp_max(top);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = w; s < n; s += JOIN_WARPS) {
+    for (int s = w * SUB + lane / LANES; s < n; s += JOIN_WARPS * SUB) {
         const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
-        const float4 y = mine ? load4(part + (long long)s * a.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 y = mine ? load4(part + (long long)s * D) : make_float4(0.f, 0.f, 0.f, 0.f);
         const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
         l += x.y * f;
         o.x += y.x * f; o.y += y.y * f; o.z += y.z * f; o.w += y.w * f;
     }
-    O[w][lane] = o;
+#pragma unroll
+    for (int x = LANES; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, x);
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, x);
+        o.y += __shfl_xor_sync(0xffffffffu, o.y, x);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, x);
+        o.w += __shfl_xor_sync(0xffffffffu, o.w, x);
+    }
+    if (lane < LANES) O[w][lane] = o;
     if (lane == 0) L[w] = l;
     __syncthreads();
-    if (w > 0) return;
+    if (w > 0 || lane >= LANES) return;
     float sum = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) 
         o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
     const float inv = inverse(sum);
-    if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * a.D + lane * 4) = make_uint2(out2<T>(o.x * inv, o.y * inv), out2<T>(o.z * inv, o.w * inv));
+    if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * D + d) = make_uint2(out2<T>(o.x * inv, o.y * inv), out2<T>(o.z * inv, o.w * inv));
 }
 
 template <typename T, int N>
@@ -523,7 +533,7 @@ static int launch(const StepArgs& a, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, int4_step_kernel<T, N>, a);
     rc = (int)cudaGetLastError();
     if (rc || a.splits <= MAX_CLUSTER) return rc;
-    return launch_early(int4_join_kernel<T>, (int64_t)a.B * a.H, JOIN_WARPS * 32, st, a);
+    return launch_early(int4_join_kernel<T, N>, (int64_t)a.B * a.H, JOIN_WARPS * 32, st, a);
 }
 template <typename T>
 static int by_width(const StepArgs& a, cudaStream_t st) {

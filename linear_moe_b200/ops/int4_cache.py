@@ -172,8 +172,8 @@ HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 8                  # csrc/int4_step.cu, .
 def splits_of(B: int, G: int, heads: int, D: int, keys: int) -> Tuple[int, int]:
     """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first).
 
-    One wave: as many parts as give every slot of the GPU a CTA, of 128 keys at least (300 keys in three parts 8.5 us, in one 10.5, replayed).  Two of up to 100001 keys, 2 heads of 64: 69 us in 16 parts, 41 in 32, 29 in
-    148.  Requests that fill more than half of the slots by themselves, but not four waves, go in two parts each, the longest ones first (64 of up to 8192 keys, 8 heads of 128: 131 us, in one part each 156, in four 139; in
+    One wave: as many parts as give every slot of the GPU a CTA, of 128 keys at least (300 keys in three parts 8.5 us, in one 10.5, replayed).  Two of up to 100001 keys, 2 heads of 64: 69 us in 16 parts, 41 in 32, 25 in
+    111, 23 in 148.  Requests that fill more than half of the slots by themselves, but not four waves, go in two parts each, the longest ones first (64 of up to 8192 keys, 8 heads of 128: 131 us, in one part each 156, in four 139; in
     two unsorted 137)."""
     from . import cuda as K
     work, slots = max(1, B * G * -(-heads // HEADS)), 4 * K.num_sms()
