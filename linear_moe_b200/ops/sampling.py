@@ -7,7 +7,7 @@ if ``w_i >= min_p``; the first one always is.  The token drawn is the first one,
 a function of the logits: sums are exact in units of 2^-44 of the largest weight (weights below half of that are never drawn), so it does not depend on how a row is shared out.
 
 NaN logits count as minus infinity; tokens at plus infinity share the whole weight.  A row of nothing but minus infinity gives token 0 and a log-probability of minus infinity.  A temperature that is not
-above zero takes the largest logit; ``top_k`` below 1 and ``top_p`` of 1 or more cut nothing off."""
+above zero takes the largest logit; ``top_k`` below 1 and ``top_p`` of 1 or more cut nothing off, nor do a ``top_p`` and a ``min_p`` of NaN in a tensor."""
 from __future__ import annotations
 
 import ctypes
@@ -49,6 +49,7 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
     def setting(x):
         return (x if torch.is_tensor(x) else torch.full((B,), float(x), dtype=torch.float32, device=dev))[:, None].double()
     t, k, p, least = (setting(x) for x in (temperature, top_k, top_p, min_p))
+    p = torch.nan_to_num(p, nan=1.0)
     x = torch.nan_to_num(logits.double(), nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
     x, order = torch.sort(x, dim=-1, descending=True, stable=True)
     top = x[:, :1]

@@ -2,7 +2,7 @@
 
 Bounds.  What is stored is defined step by step in 32 bits, so pools are equal byte for byte; a number comes back within half a size, and the size is at most (range + 2^-7 |low|) / 15 (1 + 2^-7): ``low`` and ``size``
 are each rounded away from the group by one bf16 step, 2^-7 of them at most.
-Attention: u = finfo(type).eps / 2, one rounding of the output.  On the tensor cores codes go in as they are and queries exactly (but for 2^-39 of the head's largest number), so a score's sum of products, which the
+Attention: u = finfo(type).eps / 2, one rounding of the output.  On the tensor cores codes go in as they are and queries exactly (but for 2^-36 of the head's largest number), so a score's sum of products, which the
 tensor cores round to 2^-23 of its largest part per step of 16, is off by D / 16 2^-23 of scale sum |q| (15 size + |low|), and as much again for the sum over the groups; tanh by 1e-6 of the score.  A weight times a
 value's size is rounded to 2^-12 of it for bf16 outputs and to 2^-22 for fp16 ones, of 15 sizes at most; it goes in as fp16 numbers, whose smallest is 2^-32 of the largest size that a warp has met (rounded up to a
 power of two, and weights may be counted from a maximum 2^8 below the largest score: half of 2^-31 times 15 a key).  In 32 bits throughout: N + 8 roundings of scale sum |q| |k|, and a chain of additions as long as a

@@ -307,3 +307,38 @@ def test_divisions():
         for n in {0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, top, top // d * d, max(top // d * d - 1, 0)} | set(torch.randint(0, top, (20,), generator=gen).tolist()):
             if n <= top:
                 assert ((m * n >> 32) + n) >> s == n // d, (n, d)
+
+
+@gpu
+def test_captured_training():
+    """Forward and backward in one graph: replayed on other numbers they give what the eager pass gives."""
+    s = make(2, 33, 2, 3, 64, dtype=torch.bfloat16, device="cuda")
+    leaves = [s[k].requires_grad_() for k in ("qkv", "wq", "wk")]
+
+    def step():
+        outs = ops.qkv_heads(*leaves, 1e-6, s["cos"], s["sin"])
+        return (*outs, *torch.autograd.grad(outs, leaves, s["grads"]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(2):
+        other = make(2, 33, 2, 3, 64, dtype=torch.bfloat16, device="cuda", seed=i + 1)
+        with torch.no_grad():
+            for leaf, k in zip(leaves, ("qkv", "wq", "wk")):
+                leaf.copy_(other[k])
+            for g, o in zip(s["grads"], other["grads"]):
+                g.copy_(o)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_error_texts():
+    assert "a position outside the tables" in gemm.error_text(0x41000)
+    for code, text in ((0x42000, "a length outside the page table"), (0x43000, "a page number outside the pool"), (0x44021, "a bounded wait expired")):
+        assert "4 bits a number: " + text in gemm.error_text(code)

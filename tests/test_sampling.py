@@ -211,3 +211,28 @@ def test_refusals():
 def test_shares(V):
     parts, length = S._shares(V)
     assert parts in (1, 2, 4, 8) and parts * length >= V and length <= S.PART and length % 128 == 0
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_settings_outside_their_ranges(device):
+    """Tensors are not looked at on the host: NaN cuts nothing off (a temperature of NaN takes the largest), numbers beyond the ends are the ends."""
+    x, u = rows(6, 300, device=device)
+    nan = float("nan")
+    one = lambda v, dtype=torch.float32: torch.full((6,), v, dtype=dtype, device=device)            # noqa: E731
+    plain, best = ops.sample_tokens(x, u), ops.sample_tokens(x, u, 0.0)
+    for kw, want in ((dict(top_p=one(nan)), plain), (dict(min_p=one(nan)), plain), (dict(min_p=one(-1.0)), plain), (dict(top_p=one(7.0)), plain), (dict(top_k=one(-3, torch.int32)), plain),
+                     (dict(top_k=one((1 << 31) - 1, torch.int32)), plain), (dict(temperature=one(nan)), best), (dict(temperature=one(-1.0)), best), (dict(top_p=one(-0.5)), best), (dict(min_p=one(3.0)), best)):
+        got = ops.sample_tokens(x, u, **kw)
+        assert torch.equal(got[0], want[0]) and torch.allclose(got[1], want[1], atol=1e-6), kw
+
+
+@gpu
+def test_many_rows_again_and_again():
+    """The CTAs of a row go through the levels of a search at their own pace; the answer is the same every time."""
+    for dtype, kw in ((torch.float32, dict(top_p=0.95)), (torch.float32, dict(top_k=500, temperature=1.4)), (torch.bfloat16, dict(top_p=0.7, top_k=3000, temperature=2.0))):
+        x, u = rows(160, 40000, dtype, device="cuda", seed=3)
+        want = ops.sample_tokens(x, u, **kw)
+        got = [ops.sample_tokens(x, u, **kw) for _ in range(150)]
+        assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+        eager = S._eager(x, u, kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), 0.0)
+        assert torch.equal(want[0], eager[0])
