@@ -8,8 +8,10 @@
 //   o = sum_j (p_j size_jc) code_j + sum_j p_j low_jc
 // The first sums are products of fp16 numbers with one result per group of a row (keys: 16 rows at a time, the heads are the 8 columns of an m16n8k16 product; values: 16 numbers of a group at a time).  The
 // second ones are one small product each of bf16 numbers, whose other operand is the row's lows as they lie in the cache; Q in three parts, p in two.
-// Queries go in scaled by a power of two per head, which fp16 holds exactly but for what is below 2^-35 of the head's largest number.  p size is rounded to 11 bits, for fp16 outputs to 22 (a second product); a power of
-// two per warp keeps it at 2^15 at most, where p is 1 and size the largest one seen at 2^7 (fp16 tells 2^-24 apart there).
+// Queries go in scaled by a power of two per head, which fp16 holds exactly but for what is below 2^-35 of the head's largest number.  p size goes in as two fp16 numbers, what it is rounded to and the rest of it, together
+// 22 bits: where a key head has up to four query heads the columns 4 to 7 of the products, which would be empty, take the heads 0 to 3 once more with the rests, otherwise there are second products.  (The
+// rounded one alone, 11 bits, put one bf16 output in seven on the wrong neighbour of the 64-bit value; 64 requests of up to 8192 keys, replayed: 113 us without the rests, 117 with them.)  A power of two per warp keeps p size at 2^15 at most, where p is 1 and size the largest one seen at 2^7
+// (fp16 tells 2^-24 apart there).
 //
 // A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys, 128 at a time: a stage of a ring of two, of which a warp reads 32 keys.  The warps take turns in filling the stages by bulk
 // copies, a lane per copy (64 rows of a page lie together: eight copies a stage; pages of other sizes: 32).  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
@@ -99,8 +101,9 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ uint32_t even(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t odd(uint32_t w) { return w & 0x00f000f0u; }
 __device__ __forceinline__ uint32_t pack16(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
-__device__ __forceinline__ uint32_t rest16(float2 x, uint32_t rounded) {
-    const float2 r = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&rounded)), make_float2(-1.f, -1.f), x);
+// What rounding two numbers to fp16 took away, rounded itself (by -1), or the numbers rounded (by 0)
+__device__ __forceinline__ uint32_t rest16(float2 x, uint32_t rounded, float by) {
+    const float2 r = __ffma2_rn(__half22float2(*reinterpret_cast<const __half2*>(&rounded)), make_float2(by, by), x);
     return pack16(r.x, r.y);
 }
 __device__ __forceinline__ float two_to(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }      // -126 <= n <= 127
@@ -111,17 +114,17 @@ template <typename T> __device__ __forceinline__ uint32_t out2(float x, float y)
 template <> __device__ __forceinline__ uint32_t out2<bf16>(float x, float y) { return pack2(x, y); }
 template <> __device__ __forceinline__ uint32_t out2<__half>(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
 
-// N: groups of a head.  The pointers are read behind pdl_wait by plain loads: the kernel may start while the one before it runs.
-template <typename T, int N>
+// N: groups of a head.  TWICE: up to four query heads, columns 4 to 7 are those of 0 to 3 (the same scores, weights and sums; a product's column depends on nothing but its own operands).
+// The pointers are read behind pdl_wait by plain loads: the kernel may start while the one before it runs.
+template <typename T, int N, bool TWICE>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepArgs a) {
-    constexpr bool TWO = !std::is_same<T, bf16>::value;                // p size in two parts
     constexpr int D = 32 * N, CODES = ROWS * D / 2, HALF = CODES + ROWS * D / 8, PART = 2 * HALF, STAGE = 2 * PART;      // bytes: keys' or values' codes of 64 rows, with their scales, both, twice
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
     __shared__ uint32_t there_of[STAGES];                              // a bit per copy's lane: the groups that are there
     __shared__ float part_m[WARPS][HEADS], part_l[WARPS][HEADS], cta_m[HEADS], cta_l[HEADS];
     __shared__ int abort_flag, drain_flag, chosen, lens[WARPS * 32];
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, gh = TWICE ? g & 3 : g;      // gh: the head of column g
     const int qpg = a.H / a.G, tiles = (qpg + HEADS - 1) / HEADS;
     int b = blockIdx.z;
     const int hk = blockIdx.y / tiles, tile = blockIdx.y % tiles, split = blockIdx.x;
@@ -188,8 +191,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 
     // Queries: a lane's numbers 8 t .. 8 t + 7 of every group of head g, in the order of the codes, scaled by a power of two; beside the rows' lows their sums, in three parts
     uint32_t qa[N][4], sums[3] = {0, 0, 0};
-    const bool there = g < nh;
-    const float slope = there && a.slopes != nullptr ? a.slopes[h0 + g] * LOG2E : 0.f;
+    const bool there = gh < nh;
+    const float slope = there && a.slopes != nullptr ? a.slopes[h0 + gh] * LOG2E : 0.f;
     float unit_q;                                                      // of the scores
     {
         float q[N][8], most = 0.f;
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         for (int c = 0; c < N; ++c) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[c][i] = 0.f;
-            const T* row = (const T*)a.q + b * a.q_b + (h0 + g) * a.q_h + c * 32 + 8 * t;
+            const T* row = (const T*)a.q + b * a.q_b + (h0 + gh) * a.q_h + c * 32 + 8 * t;
             if (there && a.q_rows) load8(row, q[c]);
             else if (there)
 #pragma unroll
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     const uint32_t part = (w >> 1) * PART, codes_at = part + (w & 1) * 2 * GROUP * (D / 2), scales_at = part + (w & 1) * 2 * GROUP * (D / 8);
     const uint32_t at_k = codes_at + g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = codes_at + 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = scales_at + g * (D / 8), at_ks = at_s + 4 * t, at_v2 = scales_at + 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
     auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };
+    const float rests = TWICE && g < 4 ? 0.f : -1.f;
     bool alive = true;
     int j = 0;
     for (; j < n_stages; ++j) {
@@ -359,13 +363,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
             for (int c = 0; c < N; ++c) {
                 const float2 y0 = __fmul2_rn(u0, make_float2(size_of(vs[E], c), size_of(vs[E + 1], c))), y1 = __fmul2_rn(u1, make_float2(size_of(vs[E + 2], c), size_of(vs[E + 3], c)));
-                const uint32_t p0 = pack16(y0.x, y0.y), p1 = pack16(y1.x, y1.y);
+                uint32_t p0 = pack16(y0.x, y0.y), p1 = pack16(y1.x, y1.y);
+                const uint32_t r0 = rest16(y0, p0, rests), r1 = rest16(y1, p1, rests);
+                if constexpr (TWICE) p0 = r0, p1 = r1;
                 // four codes of keys 2 t and 2 t + 1, and of 2 t + 8 and 2 t + 9
                 const uint32_t row = chunk(base + at_v, c), z0 = lds16<AT>(row) | lds16<AT + D / 2>(row) << 16, z1 = lds16<AT + 4 * D>(row) | lds16<AT + 9 * (D / 2)>(row) << 16;
                 mma16(o[2 * c], even(z0), odd(z0), even(z1), odd(z1), p0, p1);
                 mma16(o[2 * c + 1], even(z0 >> 8), odd(z0 >> 8), even(z1 >> 8), odd(z1 >> 8), p0, p1);
-                if constexpr (TWO) {
-                    const uint32_t r0 = rest16(y0, p0), r1 = rest16(y1, p1);
+                if constexpr (!TWICE) {
                     mma16(o[2 * c], even(z0), odd(z0), even(z1), odd(z1), r0, r1);
                     mma16(o[2 * c + 1], even(z0 >> 8), odd(z0 >> 8), even(z1 >> 8), odd(z1 >> 8), r0, r1);
                 }
@@ -419,6 +424,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         for (int x = 0; x < WARPS; ++x) {
             const float4 z = load4(O + (x * HEADS + r) * LD + d);
             y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            if constexpr (TWICE) {
+                const float4 u = load4(O + (x * HEADS + r + 4) * LD + d);
+                y.x += u.x; y.y += u.y; y.z += u.z; y.w += u.w;
+            }
             rest_ += E[(x * HEADS + r) * 8 + c];
         }
         y.x += rest_; y.y += rest_; y.z += rest_; y.w += rest_;
@@ -511,10 +520,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) 
     if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * D + d) = make_uint2(out2<T>(o.x * inv, o.y * inv), out2<T>(o.z * inv, o.w * inv));
 }
 
-template <typename T, int N>
+template <typename T, int N, bool TWICE>
 static int launch(const StepArgs& a, cudaStream_t st) {
     constexpr int D = 32 * N, ring = STAGES * 4 * ROWS * (D / 2 + D / 8), ends = WARPS * HEADS * (D + 4 + 8) * 4, smem = ring > ends ? ring : ends;
-    int rc = (int)cudaFuncSetAttribute(int4_step_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    int rc = (int)cudaFuncSetAttribute(int4_step_kernel<T, N, TWICE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc) return rc;
     const int tiles = (a.H / a.G + HEADS - 1) / HEADS;
     cudaLaunchConfig_t cfg = {};
@@ -530,11 +539,13 @@ static int launch(const StepArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.splits > 1 && a.splits <= MAX_CLUSTER ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, int4_step_kernel<T, N>, a);
+    cudaLaunchKernelEx(&cfg, int4_step_kernel<T, N, TWICE>, a);
     rc = (int)cudaGetLastError();
     if (rc || a.splits <= MAX_CLUSTER) return rc;
     return launch_early(int4_join_kernel<T, N>, (int64_t)a.B * a.H, JOIN_WARPS * 32, st, a);
 }
+template <typename T, int N>
+static int launch(const StepArgs& a, cudaStream_t st) { return a.H / a.G <= 4 ? launch<T, N, true>(a, st) : launch<T, N, false>(a, st); }
 template <typename T>
 static int by_width(const StepArgs& a, cudaStream_t st) {
     switch (a.D / 32) {

@@ -454,3 +454,21 @@ def test_sizes_that_the_kernels_do_not_count():
     wide = torch.zeros(0, 32768, 320, dtype=torch.uint8)
     with pytest.raises(ValueError, match="heads are more"):
         ops.read_rows_int4(wide, wide, torch.zeros(1, 0, dtype=torch.int32), lengths, 1, 32, F)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("H,G,D", [(2, 2, 128), (4, 2, 32), (9, 3, 96), (16, 4, 128), (8, 2, 64), (10, 2, 64), (16, 2, 128), (12, 1, 96), (20, 1, 128)])
+def test_weights_times_sizes_of_22_bits(H, G, D, dtype):
+    """The output is the 64-bit value rounded once, to the neighbour that 22 bits of a weight times its value's size leave open.  With queries as small as here scores are off by less than 2^-24, so what is left
+    of a weight's room is 2^-20 for its exponential and 2^-22; rounding is monotone, so the output lies between the rounded ends of that room (a number goes to 32 bits on its way to 16: 2^-24 more)."""
+    for lens in ([1, 2, 3, 5, 9, 17, 33, 70], [1500, 4], [20000]):
+        s = make(lens, H, G, D, dtype=dtype, size=1e-3)
+        for kw in (dict(), dict(window=6)):
+            got = attend(s, **kw)
+            want, room = formula(dict(s, q=s["q"].float()), tensor=True, **kw)
+            room = room + 2.0 ** -24 * want.abs()
+            low, high = (want - room).to(dtype), (want + room).to(dtype)
+            wrong = (got < low) | (got > high)
+            assert not wrong.any(), (lens, kw, int(wrong.sum()), wrong.numel())
+    gemm.check_error()
