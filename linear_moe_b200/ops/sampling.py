@@ -59,8 +59,8 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
     w = torch.where(x == float("-inf"), 0.0, (y.exp() * unit).round()).to(torch.int64)      # (minus infinity over an endless temperature is NaN)
     upto = w.cumsum(-1)
     before, whole = upto - w, upto[:, -1:]
-    limit = torch.where(p >= 1, float(1 << 62), (p * whole.double()).ceil().clamp_min(1)).to(torch.int64)
-    keep = (torch.arange(V, device=dev) < torch.where(greedy, 1, torch.where(k >= 1, k, V))) & (before < limit)
+    limit = (p.clamp_max(1) * whole.double()).ceil().clamp_min(1).to(torch.int64)
+    keep = (torch.arange(V, device=dev) < torch.where(greedy, 1, torch.where(k >= 1, k, V))) & ((before < limit) | (p >= 1))
     keep &= (w >= (torch.nan_to_num(least, nan=0.0).clamp(0, 1) * unit).ceil().to(torch.int64)) | (x == top)
     kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0))
     upto = kept.cumsum(-1)

@@ -236,3 +236,12 @@ def test_many_rows_again_and_again():
         assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
         eager = S._eager(x, u, kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), 0.0)
         assert torch.equal(want[0], eager[0])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_nothing_is_cut_off_of_long_flat_rows(device):
+    """The whole of 300001 equal weights is above 2^62 units of 2^-44."""
+    x = torch.zeros(4, 300001, device=device)
+    u = torch.tensor([0.1, 0.87, 0.95, 0.999], device=device)
+    for kw in (dict(), dict(min_p=0.5), dict(top_k=290000), dict(top_p=torch.full((4,), 1.0, device=device))):
+        check(x, u, **kw)
