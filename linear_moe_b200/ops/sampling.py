@@ -4,7 +4,8 @@
 
 Tokens are put in the order of falling logits, equal ones by their number.  A token is kept while fewer than ``top_k`` come before it, while the weight of those before it is below ``top_p`` of the whole, and
 if ``w_i >= min_p``; the first one always is.  The token drawn is the first one, in the order of the vocabulary, up to which the kept weights exceed ``draw`` times their sum.  Given the random numbers, the result is
-a function of the logits: sums are exact in units of 2^-44 of the largest weight (weights below half of that are never drawn), so it does not depend on how a row is shared out.
+a function of the logits: sums are exact in units of 2^-44 of the largest weight (weights below half of that are never drawn), so it does not depend on how a row is shared out.  (More than 2^19 logits, which the
+eager form takes on CUDA too: in units of 2^-43, one bit less for every doubling, so that the sums stay within 2^63.)
 
 NaN logits count as minus infinity; tokens at plus infinity share the whole weight.  A row of nothing but minus infinity gives token 0 and a log-probability of minus infinity.  A temperature that is not
 above zero takes the largest logit; ``top_k`` below 1 and ``top_p`` of 1 or more cut nothing off, nor do a ``top_p`` and a ``min_p`` of NaN in a tensor."""
@@ -55,20 +56,27 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
     top = x[:, :1]
     greedy = ~(t > 0)
     y = torch.where(x == top, 0.0, (x - top) / torch.where(greedy, 1.0, t))
-    unit = 2.0 ** 44
+    unit = 2.0 ** min(44, 63 - (V - 1).bit_length())                                        # V of them: 2^63 at most
     w = torch.where(x == float("-inf"), 0.0, (y.exp() * unit).round()).to(torch.int64)      # (minus infinity over an endless temperature is NaN)
-    upto = w.cumsum(-1)
-    before, whole = upto - w, upto[:, -1:]
-    limit = (p.clamp_max(1) * whole.double()).ceil().clamp_min(1).to(torch.int64)
+    before, whole, _ = _sums(w)
+    limit = (torch.where(p >= 1, 0.0, p) * whole).ceil().clamp_min(1).to(torch.int64)
     keep = (torch.arange(V, device=dev) < torch.where(greedy, 1, torch.where(k >= 1, k, V))) & ((before < limit) | (p >= 1))
     keep &= (w >= (torch.nan_to_num(least, nan=0.0).clamp(0, 1) * unit).ceil().to(torch.int64)) | (x == top)
     kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0))
-    upto = kept.cumsum(-1)
-    whole = upto[:, -1:]
-    goal = torch.minimum((torch.nan_to_num(draw, nan=0.0).clamp_min(0)[:, None].double() * whole.double()).to(torch.int64), (whole - 1).clamp_min(0))
-    token = torch.where(whole[:, 0] > 0, (upto <= goal).sum(-1), 0)
-    share = kept.gather(1, token[:, None]).double() / whole.double()
-    return token, torch.where(whole[:, 0] > 0, share[:, 0].log(), float("-inf")).float()
+    before, whole, last = _sums(kept)
+    u = torch.nan_to_num(draw, nan=0.0).clamp_min(0)[:, None].double()
+    goal = torch.where(u < 1, torch.minimum((u * whole).to(torch.int64), last), last)
+    some = last[:, 0] >= 0
+    token = torch.where(some, (before <= goal).sum(-1) - 1, 0)                               # the last one that the goal reaches
+    share = kept.gather(1, token[:, None]).double() / whole
+    return token, torch.where(some, share[:, 0].log(), float("-inf")).float()
+
+
+def _sums(w):
+    """What comes before every weight, the whole as a 64-bit number, and the whole less one: 2^63 itself 63 bits do not hold."""
+    before = torch.nn.functional.pad(w[:, :-1].cumsum(-1), (1, 0))
+    last = before[:, -1:] + (w[:, -1:] - 1)
+    return before, (last.clamp_max((1 << 63) - 2) + 1).double(), last
 
 
 def _shares(V: int) -> Tuple[int, int]:

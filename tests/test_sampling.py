@@ -245,3 +245,27 @@ def test_nothing_is_cut_off_of_long_flat_rows(device):
     u = torch.tensor([0.1, 0.87, 0.95, 0.999], device=device)
     for kw in (dict(), dict(min_p=0.5), dict(top_k=290000), dict(top_p=torch.full((4,), 1.0, device=device))):
         check(x, u, **kw)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("V", [(1 << 19) - 1, 1 << 19, (1 << 19) + 1, 1 << 20, 1100000, 1 << 21])
+def test_sums_of_long_rows(V, device):
+    """Equal weights, whose sum is 2^63 units at 2^19 and 2^20 logits, and weights that a high temperature makes nearly so; draws half a token off the borders (of equal weights)."""
+    flat = torch.zeros(5, V, device=device)
+    u = ((torch.tensor([0.0, 0.3, 0.5, 0.9, 1.0], dtype=torch.float64) * (V - 1)).floor() + 0.5) / V
+    u = u.float().clamp_max(1 - 2.0 ** -24).to(device)
+    u[1] = 0.300048828125                                # a draw of few bits: the product is exact
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=V // 3), dict(top_k=V - 1, top_p=0.999), dict(min_p=0.5)):
+        check(flat, u, **kw)
+    x, u = rows(2, V, device=device, seed=V % 1000)
+    for kw in (dict(temperature=30.0), dict(temperature=5.0), dict(temperature=30.0, top_p=0.8, top_k=V // 2), dict(temperature=INF)):
+        check(x, u, **kw)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_draws_far_outside(device):
+    """A draw times the sum may leave 63 bits: from one on it is the last kept token."""
+    x = torch.tensor([[-4.0, 1.0, 0.5, -INF, -2.0]], device=device).repeat(5, 1)
+    u = torch.tensor([1e6, 3e38, INF, -3e38, -INF], device=device)
+    assert ops.sample_tokens(x, u)[0].tolist() == [4, 4, 4, 0, 0]
+    assert ops.sample_tokens(x, u, top_k=2)[0].tolist() == [2, 2, 2, 1, 1]
