@@ -57,7 +57,7 @@ def _eager(logits, draw, temperature, top_k, top_p, min_p):
     greedy = ~(t > 0)
     y = torch.where(x == top, 0.0, (x - top) / torch.where(greedy, 1.0, t))
     unit = 2.0 ** min(44, 63 - (V - 1).bit_length())                                        # V of them: 2^63 at most
-    w = torch.where(x == float("-inf"), 0.0, (y.exp() * unit).round()).to(torch.int64)      # (minus infinity over an endless temperature is NaN)
+    w = torch.where((x == float("-inf")) | y.isnan(), 0.0, (y.exp() * unit).round()).to(torch.int64)               # (NaN: minus infinity over an endless temperature)
     before, whole, _ = _sums(w)
     limit = (torch.where(p >= 1, 0.0, p) * whole).ceil().clamp_min(1).to(torch.int64)
     keep = (torch.arange(V, device=dev) < torch.where(greedy, 1, torch.where(k >= 1, k, V))) & ((before < limit) | (p >= 1))

@@ -269,3 +269,15 @@ def test_draws_far_outside(device):
     u = torch.tensor([1e6, 3e38, INF, -3e38, -INF], device=device)
     assert ops.sample_tokens(x, u)[0].tolist() == [4, 4, 4, 0, 0]
     assert ops.sample_tokens(x, u, top_k=2)[0].tolist() == [2, 2, 2, 1, 1]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_plus_infinity_and_an_endless_temperature(device):
+    """Tokens at plus infinity share the whole weight whatever the temperature, and what top_p leaves of them is counted by weight."""
+    u = torch.tensor([0.1, 0.3, 0.6, 0.9], device=device)
+    for other in (2.0, -INF):
+        x = torch.tensor([[1.0, INF, other, INF, -INF, INF, INF, float("nan")]], device=device).repeat(4, 1)
+        for t in (INF, 1e30, 1.0, 0.001):
+            for top_p, want in ((1.0, [1, 3, 5, 6]), (0.9, [1, 3, 5, 6]), (0.7, [1, 1, 3, 5]), (0.4, [1, 1, 3, 3])):
+                token, logp = ops.sample_tokens(x, u, t, 0, top_p)
+                assert token.tolist() == want and torch.allclose(logp.exp(), torch.full((4,), 1 / len(set(want)), device=device)), (other, t, top_p)
