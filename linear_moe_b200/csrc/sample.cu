@@ -435,13 +435,15 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
     cl.sync();                                         // the others have read this one's sums
 }
 
+constexpr int MOST_HELD = 192 * 1024;                       // bytes of a part in shared memory, at most
+static_assert(sizeof(Shared) + MOST_HELD <= 227 * 1024, "a CTA's shared memory");
 template <typename T>
 static int launch(const Args& a, cudaStream_t st) {
     const long long bytes = (long long)a.len * sizeof(T);
-    const bool held = bytes <= 192 * 1024;
+    const bool held = bytes <= MOST_HELD;
     auto kernel = held ? sample_kernel<T, true> : sample_kernel<T, false>;
-    if (held) {
-        const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (held) {                                        // (the same for every call: it belongs to the kernel, and another thread may be between this and its launch)
+        const int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_HELD);
         if (rc) return rc;
     }
     cudaLaunchConfig_t cfg = {};

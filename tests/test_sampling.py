@@ -281,3 +281,28 @@ def test_plus_infinity_and_an_endless_temperature(device):
             for top_p, want in ((1.0, [1, 3, 5, 6]), (0.9, [1, 3, 5, 6]), (0.7, [1, 1, 3, 5]), (0.4, [1, 1, 3, 3])):
                 token, logp = ops.sample_tokens(x, u, t, 0, top_p)
                 assert token.tolist() == want and torch.allclose(logp.exp(), torch.full((4,), 1 / len(set(want)), device=device)), (other, t, top_p)
+
+
+@gpu
+def test_rows_of_different_lengths_from_two_threads():
+    """What a launch may have of shared memory belongs to the kernel, not to the call: a call of short rows must not take it from one of long rows in another thread."""
+    import threading
+    errors = []
+
+    def work(V):
+        try:
+            x, u = rows(1, V, device="cuda", seed=V)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                torch.cuda.synchronize()
+                want = ops.sample_tokens(x, u, top_p=0.9)
+                for _ in range(40):
+                    got = [ops.sample_tokens(x, u, top_p=0.9) for _ in range(50)]
+                    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+        except BaseException as e:      # noqa: B036
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(V,)) for V in (300001, 1000, 131072, 2000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
