@@ -1106,12 +1106,17 @@ def _lsm_combine(rev, states, gdecay, gconst, seed, final_out, BH, H, G, cpg, T,
 _LASP_CTX = None          # set by parallel.fused_comm.lasp2_scalar while a sequence-parallel call is running
 
 
+def _unwatched() -> bool:
+    """Do neither forward-mode AD nor a functional transform nor tracing look on?  Their tensors need not require a gradient, and what a call outside an autograd function makes of them loses its tangents."""
+    return not (torch.autograd.forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
+                or torch._C._get_tracing_state() is not None)
+
+
 def _plain_call() -> bool:
     """Is this call outside everything that looks into an autograd function (gradients, forward-mode AD, functional transforms,
     tracing)?  Then its forward pass is called directly: a prompt of 777 tokens, 8 heads of 64, whose kernels take 13 us, took
     70 us with the function's bookkeeping, argument structs filled field by field and three host calls, and takes 40 without."""
-    return not (torch.is_grad_enabled() or torch.autograd.forward_ad._current_level >= 0
-                or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._get_tracing_state() is not None)
+    return not torch.is_grad_enabled() and _unwatched()
 
 
 def _scalar_forward(q, k, v, g, scale, init):

@@ -4,7 +4,8 @@
 
 A token's row of the projection holds, group by group, the r query heads that share a key head, the key and the value: ``[B, T, G, r + 2, D]``.  The cosines and sines come from tables in fp32
 ``[tokens, R / 2]``, whose row is a token's place in its sequence or what ``positions [B, T]`` says (on the device, so captured steps go on).  Everything between the projection and the results is
-computed in 32 bits and rounded once.  The backward pass gives the projection's gradient in one tensor and those of the norms' weights, summed in an order that the sizes alone decide.
+computed in 32 bits and rounded once.  The backward pass gives the projection's gradient in one tensor and those of the norms' weights, summed in an order that the sizes alone decide.  (On CUDA
+there are no second derivatives and no forward mode: both raise.)
 
 A position outside the tables raises on the CPU; on CUDA it sets the kernels' error word (``ops.gemm.check_error``) and the nearest row is taken."""
 from __future__ import annotations
@@ -204,6 +205,7 @@ def qkv_heads(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weig
         qkv = qkv if plan.rows and not qkv.data_ptr() % 16 else qkv.clone(memory_format=torch.contiguous_format)
         cos, sin = (t if t is None or not t.data_ptr() % 16 else t.clone() for t in (cos, sin))
         return qkv_heads(qkv, q_weight, k_weight, eps, cos, sin, positions=positions, interleaved=interleaved)
-    if not torch.is_grad_enabled() or not (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
+    from . import cuda as K
+    if K._unwatched() and (not torch.is_grad_enabled() or not (qkv.requires_grad or (q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad))):
         return _forward(qkv, q_weight, k_weight, plan, cos, sin, positions)
     return _QkvHeads.apply(qkv, q_weight, k_weight, plan, cos, sin, positions)

@@ -342,3 +342,21 @@ def test_error_texts():
     assert "a position outside the tables" in gemm.error_text(0x41000)
     for code, text in ((0x42000, "a length outside the page table"), (0x43000, "a page number outside the pool"), (0x44021, "a bounded wait expired")):
         assert "4 bits a number: " + text in gemm.error_text(code)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", ["qkv", "wq"])
+def test_forward_mode(which, grad, device):
+    """Tangents come through (the eager form) or are refused: they are not dropped."""
+    import torch.autograd.forward_ad as fw
+    s = make(1, 5, 2, 2, 64, device=device)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        plain = ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])            # a level alone changes nothing
+        assert all(fw.unpack_dual(t).tangent is None for t in plain)
+        s[which] = fw.make_dual(s[which], torch.ones_like(s[which]))
+        if device == "cuda":
+            with pytest.raises(RuntimeError):
+                ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])
+        else:
+            assert fw.unpack_dual(ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])[0]).tangent is not None
