@@ -199,8 +199,7 @@ def qkv_heads(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weig
             return qkv_heads(qkv if _dense_heads(qkv) else qkv.contiguous(), flat(q_weight), flat(k_weight), eps, flat(cos), flat(sin), positions=flat(positions), interleaved=interleaved)
         plan = _PLANS[key] = _plan(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved)
     if qkv.numel() == 0:
-        B, T, G, S, D = qkv.shape
-        return qkv[..., : S - 2, :].reshape(B, T, G * (S - 2), D), qkv[..., S - 2, :], qkv[..., S - 1, :]
+        return R.qkv_heads(qkv, q_weight, k_weight, eps, cos, sin, positions, interleaved)
     if plan.vectors and (not plan.rows or (qkv.data_ptr() | (0 if cos is None else cos.data_ptr() | sin.data_ptr())) % 16):
         qkv = qkv if plan.rows and not qkv.data_ptr() % 16 else qkv.clone(memory_format=torch.contiguous_format)
         cos, sin = (t if t is None or not t.data_ptr() % 16 else t.clone() for t in (cos, sin))

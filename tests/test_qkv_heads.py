@@ -360,3 +360,14 @@ def test_forward_mode(which, grad, device):
                 ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])
         else:
             assert fw.unpack_dual(ops.qkv_heads(s["qkv"], s["wq"], s["wk"], 1e-6, s["cos"], s["sin"])[0]).tangent is not None
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("B,T", [(0, 3), (2, 0)])
+def test_gradients_of_nothing(B, T, device):
+    """No tokens: the weights' gradients are zeros."""
+    s = make(B, T, 2, 2, 64, device=device, at=7)
+    leaves = [s[k].requires_grad_() for k in ("qkv", "wq", "wk")]
+    outs = ops.qkv_heads(*leaves, 1e-6, s["cos"], s["sin"], positions=s["at"])
+    grads = torch.autograd.grad(outs, leaves, s["grads"])
+    assert [g.shape for g in grads] == [t.shape for t in leaves] and not grads[1].any() and not grads[2].any()
