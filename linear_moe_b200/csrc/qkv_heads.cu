@@ -307,7 +307,8 @@ __global__ void __launch_bounds__(VT, 2) heads_vec_bwd_kernel(const Args a) {
     __shared__ float red[HEADS][TPH * 2 * E];
     const Place p = place_of<T, TPH>(a);
     pdl_trigger();
-    const void* wp = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr;
+    const T* from = (const T*)(p.kind == 0 ? a.dq : p.kind == 1 ? a.dk : a.dv);
+    const void *weights = p.kind == 0 ? a.wq : p.kind == 1 ? a.wk : nullptr, *wp = from != nullptr ? weights : nullptr;      // (what nothing asks of is not looked at: zero whatever lies there)
     float2 w[E], dw[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -315,7 +316,6 @@ __global__ void __launch_bounds__(VT, 2) heads_vec_bwd_kernel(const Args a) {
         dw[i] = both(0.f);
         w[i] = wp != nullptr && p.in ? make_float2(weight(wp, a.w_type, d), weight(wp, a.w_type, d + 1)) : both(0.f);
     }
-    const T* from = (const T*)(p.kind == 0 ? a.dq : p.kind == 1 ? a.dk : a.dv);
     const unsigned items = (unsigned)(a.rows * a.G) * (p.kind == 0 ? a.r : 1), step = p.blocks * HEADS;
     const long long ld = (long long)a.G * (a.r + 2) * a.D;
     const bool same = a.x_t == ld && a.x_b == ld * a.T;                // the projection and its gradient lie alike
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(VT, 2) heads_vec_bwd_kernel(const Args a) {
         store_chunk((T*)a.dx + h.from + p.at[0], dy);
         store_chunk((T*)a.dx + h.from + p.at[1], dy + E / 2);
     }
-    if (a.part == nullptr || wp == nullptr) return;
+    if (a.part == nullptr || weights == nullptr) return;
     if (p.in)
 #pragma unroll
         for (int i = 0; i < E; ++i) *reinterpret_cast<float2*>(&red[threadIdx.x / TPH][p.at[2 * i / E] + 2 * i % E]) = dw[i];

@@ -371,3 +371,15 @@ def test_gradients_of_nothing(B, T, device):
     outs = ops.qkv_heads(*leaves, 1e-6, s["cos"], s["sin"], positions=s["at"])
     grads = torch.autograd.grad(outs, leaves, s["grads"])
     assert [g.shape for g in grads] == [t.shape for t in leaves] and not grads[1].any() and not grads[2].any()
+
+@gpu
+@pytest.mark.parametrize("D", [64, 6])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 0.0])
+def test_outputs_that_nothing_uses_bring_no_nan(bad, D):
+    """What nothing asks of has a gradient of zero, whatever lies there: NaN, infinities, and zeros without an epsilon, whose norm has no slope."""
+    s = make(2, 17, 2, 2, D, dtype=torch.bfloat16, device="cuda")
+    s["qkv"][0, 3, 1, 2] = bad                                # a key
+    leaves = [s[k].requires_grad_() for k in ("qkv", "wq", "wk")]
+    q, _, v = ops.qkv_heads(*leaves, 0.0, s["cos"], s["sin"])
+    dx, dwq, dwk = torch.autograd.grad((q, v), leaves, (s["grads"][0], s["grads"][2]))
+    assert dx.isfinite().all() and dwq.isfinite().all() and not dwk.any() and not dx[:, :, :, 2].any()
