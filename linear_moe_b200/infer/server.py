@@ -24,8 +24,8 @@ MAX_PROMPTS = 128
 MAX_TOKENS = 4096
 
 
-def _validate(req: dict) -> Optional[str]:
-    """Megatron's server-side checks, as one message or None."""
+def _validate(req: dict, fused_sampling: bool = False) -> Optional[str]:
+    """Megatron's server-side checks, as one message or None.  Tokens that are drawn by one random number each (``fused_sampling``, or a ``min_p``) take ``top_k`` and ``top_p`` together."""
     prompts = req.get("prompts")
     if not isinstance(prompts, list) or not prompts or not all(isinstance(p, str) for p in prompts):
         return "prompts must be a non-empty list of strings"
@@ -41,13 +41,13 @@ def _validate(req: dict) -> Optional[str]:
         return "top_k must be an integer in [0, 1000]"
     if not isinstance(p, (int, float)) or not 0.0 <= p <= 1.0:
         return "top_p must be a number in [0, 1]"
-    if k > 0 and p > 0.0:
-        return "cannot set both top_k and top_p"
-    if not isinstance(t, (int, float)) or not 0.0 < t <= 100.0:
-        return "temperature must be a positive number (at most 100)"
     m = req.get("min_p", 0.0)
     if not isinstance(m, (int, float)) or not 0.0 <= m <= 1.0:
         return "min_p must be a number in [0, 1]"
+    if k > 0 and p > 0.0 and not (fused_sampling or m > 0.0):
+        return "cannot set both top_k and top_p (without fused sampling or a min_p)"
+    if not isinstance(t, (int, float)) or not 0.0 < t <= 100.0:
+        return "temperature must be a positive number (at most 100)"
     b = req.get("beam_width")
     if b is not None:
         if not isinstance(b, int) or b < 1:
@@ -124,7 +124,7 @@ def build_app(model, tokenizer, cuda_graph: bool = False, group=None, paged: boo
             return JSONResponse({"message": "the request body must be JSON"}, status_code=400)
         if not isinstance(req, dict):
             return JSONResponse({"message": "the request body must be a JSON object"}, status_code=400)
-        err = _validate(req)
+        err = _validate(req, fused_sampling)
         if err is not None:
             return JSONResponse({"message": err}, status_code=400)
         with lock, torch.no_grad():

@@ -205,3 +205,23 @@ def test_train_then_sample():
                                    generator=torch.Generator("cuda").manual_seed(1))
     assert out.shape == (3, P + n) and torch.isfinite(lp).all() and int(out.max()) < 512
     gemm.check_error()
+
+
+def test_requests_with_top_k_and_top_p():
+    """Together where the tokens are drawn by one random number each: a server started with fused sampling, or a request with a min_p."""
+    from fastapi.testclient import TestClient
+    from linear_moe_b200.data.tokenizer import NullTokenizer
+    from linear_moe_b200.infer.server import build_app
+    m, tok = model(), NullTokenizer(64)
+    body = {"prompts": ["1 2 3 4"], "tokens_to_generate": 6, "top_k": 8, "top_p": 0.8, "temperature": 2.0, "random_seed": 3}
+    for fused in (False, True):
+        with TestClient(build_app(m, tok, fused_sampling=fused)) as c:
+            for extra in (dict(), dict(min_p=0.0), dict(min_p=0.05)):
+                got = c.put("/api", json={**body, **extra})
+                if not fused and not extra.get("min_p"):
+                    assert got.status_code == 400 and "top_k and top_p" in got.json()["message"]
+                    continue
+                with torch.no_grad():
+                    want = G.generate_and_post_process(m, tok, body["prompts"], 6, top_k_sampling=8, top_p_sampling=0.8, temperature=2.0, random_seed=3, fused_sampling=fused, **extra)
+                assert got.status_code == 200 and got.json()["tokens"] == want[1]
+            assert c.put("/api", json={**body, "min_p": "x"}).status_code == 400
