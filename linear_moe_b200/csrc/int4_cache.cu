@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) int4_store_kernel(const RowArgs a) {
         sum += __shfl_xor_sync(group, sum, 1);
         const uint32_t lb = least == 0.f ? 0u : __float_as_uint(least);      // of zeros the positive one
         float low = __uint_as_float((lb >> 31 ? lb + 0xffffu : lb) & 0xffff0000u);
-        float size = __uint_as_float((__float_as_uint(__fmul_rn(__fsub_rn(most, low), 1.f / 15.f)) + 0xffffu) & 0xffff0000u);
+        float size = __uint_as_float((__float_as_uint(fabsf(__fmul_rn(__fsub_rn(most, low), 1.f / 15.f))) + 0xffffu) & 0xffff0000u);      // (not -0: sizes are compared by their bits)
         if (!(sum == 0.f && fabsf(low) <= 3.402823466e38f && size <= 3.402823466e38f)) low = __uint_as_float(0x7fc00000u), size = 0.f;
         // The quotient by a product with the reciprocal is off by less than 4 2^-20 (of 16 at most): where it is that near to a border between two codes, and for sizes whose reciprocal may overflow,
         // it is divided out.

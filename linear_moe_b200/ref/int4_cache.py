@@ -21,7 +21,7 @@ def encode(x: torch.Tensor):
     least = g.amin(-1)
     bits = torch.where(least == 0, 0.0, least).view(torch.int32)                          # of zeros the positive one
     low = (torch.where(bits < 0, bits + 0xffff, bits) & -65536).view(torch.float32)
-    size = ((((g.amax(-1) - low) * FIFTEENTH).view(torch.int32) + 0xffff) & -65536).view(torch.float32)
+    size = ((((g.amax(-1) - low) * FIFTEENTH).abs().view(torch.int32) + 0xffff) & -65536).view(torch.float32)      # (never -0)
     finite = finite & low.isfinite() & size.isfinite()
     code = torch.round((g - low[..., None]) / torch.where(size > 0, size, 1.0)[..., None]).clamp(0, 15)
     code = torch.where((finite & (size > 0))[..., None], code, 0.0)

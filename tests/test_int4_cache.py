@@ -472,3 +472,31 @@ def test_weights_times_sizes_of_22_bits(H, G, D, dtype):
             wrong = (got < low) | (got > high)
             assert not wrong.any(), (lens, kw, int(wrong.sum()), wrong.numel())
     gemm.check_error()
+
+
+def test_sizes_are_not_negative():
+    """Of zeros either sign has a size of +0: as bits the other one is larger than every size."""
+    x = torch.cat([-torch.zeros(1, 32), torch.zeros(1, 32), torch.tensor([[-0.0, 0.0] * 16]), torch.full((1, 32), -2.0)])
+    code, low, size = R.encode(x)
+    assert (size.view(torch.int16) >= 0).all() and not size.any() and not code.any() and low.flatten().tolist() == [0.0, 0.0, 0.0, -2.0]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HALF, F])
+@pytest.mark.parametrize("H,G,D", [(4, 2, 64), (16, 2, 128), (3, 1, 96), (1, 1, 32)])
+def test_values_of_negative_zeros(H, G, D, dtype):
+    """A key whose value is nothing but -0.0 leaves the others as they are."""
+    def values(gen, n, G, D):
+        x = torch.randn(n, G, D, generator=gen)
+        x[n // 2] = -0.0
+        x[n // 3, :, :32] = -0.0
+        return x
+    s = make([40, 9, 1, 700], H, G, D, dtype=dtype, values=values)
+    pools = [torch.full_like(s[k], 255) for k in "kv"]                # (the rows once more, by the kernel)
+    rows = ops.read_rows_int4(s["k"], s["v"], s["table"], s["lengths"], 700, D, F)
+    back = [torch.cat([torch.zeros(700 - n, G, D, device="cuda"), r[i, :n]]) for r in rows for i, n in enumerate([40, 9, 1, 700])]
+    back = [torch.where(r == 0, -0.0, r) for r in back]
+    ops.store_rows_int4(torch.stack(back[:4]), torch.stack(back[4:]), *pools, s["table"], s["lengths"])
+    for k, v in ((s["k"], s["v"]), pools):
+        check(dict(s, k=k, v=v))
+        check(dict(s, k=k, v=v), window=20)
