@@ -80,6 +80,13 @@ template <int N> __device__ __forceinline__ uint32_t larger(uint32_t most, const
     if constexpr (N >= 3) return __vimax3_u16x2(most, s.w[0], s.w[1]);
     else return __vmaxu2(most, s.w[0]);
 }
+// Two bf16 numbers times a power of two.  (No .ftz: sizes below 2^-126 are numbers too.)
+__device__ __forceinline__ uint32_t scaled(uint32_t w, float f) {
+    float x, y;
+    asm("mul.rn.f32 %0, %1, %2;" : "=f"(x) : "f"(lower(w)), "f"(f));
+    asm("mul.rn.f32 %0, %1, %2;" : "=f"(y) : "f"(upper(w)), "f"(f));
+    return __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xffff0000u);
+}
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }      // zero: nothing seen
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -235,8 +242,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         }
     }
     const float pre = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * unit_q, unit = a.cap > 0.f ? a.cap * LOG2E : pre;      // (scores of head g)
-    // Weights are 2^(score - m + shift), with which p size is at most 2^(LAG + 7) where no size is above 2^(7 - shift).  Beyond 2^20 and below 2^-20 the sizes are scaled by 2^wide as well: the sums of weights
-    // and of weights times lows have to stay within fp32.
+    // Weights are 2^(score - m + shift), with which p size is at most 2^(LAG + 7) where no size is above 2^(7 - shift).  Beyond 2^40 and below 2^-20 the sizes are scaled by 2^wide as well (before the
+    // weights, which alone would leave fp32): the sums of weights and of weights times lows have to stay within it.
     float m = -INFINITY, l = 0.f, shift = 7.f;
     int wide = 0;
     uint32_t bound = 0;                                                // the power of two that no size so far is above, as the upper bits of a bf16 number, twice
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
                 if (!seen(key0 + 8 * (i >> 1) + 2 * t + (i & 1))) x[i] = -INFINITY;
         }
         // sizes of the values of keys 8 (e >> 1) + 2 t + (e & 1)
-        const Sizes<N> vs[8] = {sizes<N, HALF + CODES>(base + at_v2), sizes<N, HALF + CODES + D / 8>(base + at_v2), sizes<N, HALF + CODES + D>(base + at_v2), sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2),
+        Sizes<N> vs[8] = {sizes<N, HALF + CODES>(base + at_v2), sizes<N, HALF + CODES + D / 8>(base + at_v2), sizes<N, HALF + CODES + D>(base + at_v2), sizes<N, HALF + CODES + 9 * (D / 8)>(base + at_v2),
                                 sizes<N, HALF + CODES + 2 * D>(base + at_v2), sizes<N, HALF + CODES + 17 * (D / 8)>(base + at_v2), sizes<N, HALF + CODES + 3 * D>(base + at_v2),
                                 sizes<N, HALF + CODES + 25 * (D / 8)>(base + at_v2)};
         uint32_t largest = 0;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             mx = fmaxf(mx, m);
             const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(largest & 0xffffu, largest >> 16), bound >> 16));
-            const int power = top == 0 ? 0 : (int)((top + 0x7fu) >> 7) - 127, kept = min(max(power, -20), 20);      // no size is above 2^power
+            const int power = top == 0 ? 0 : (int)((top + 0x7fu) >> 7) - 127, kept = min(max(power, -20), 40);      // no size is above 2^power
             bound = min(top + 0x7fu, 0x7f80u) & 0xff80u;
             bound |= bound << 16;
             const float shift_now = 7.f - (float)kept;
@@ -339,6 +346,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
 #pragma unroll
             for (int i = 0; i < 2 * N; ++i) o[i][0] *= c0, o[i][1] *= c1, o[i][2] *= c0, o[i][3] *= c1;
         }
+        if (wide != 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (uint32_t& y : vs[i].w) y = scaled(y, two_to(wide));
+        }
         const float low = (m == -INFINITY ? 0.f : m) - shift;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - low);
@@ -346,11 +359,6 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         auto values = [&](auto which) {
             constexpr int AT = HALF + decltype(which)::value * GROUP * (D / 2), S = HALF + CODES + decltype(which)::value * GROUP * (D / 8), E = decltype(which)::value * 4;
             const float2 w0 = make_float2(x[E], x[E + 1]), w1 = make_float2(x[E + 2], x[E + 3]);
-            float2 u0 = w0, u1 = w1;
-            if (wide != 0) {
-                const float f = two_to(wide);
-                u0.x *= f, u0.y *= f, u1.x *= f, u1.y *= f;
-            }
             {                                                          // the weights' sums of lows
                 const uint32_t p0 = pack2(w0), p1 = pack2(w1);
                 uint32_t b0 = 0, b1 = 0;
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             }
 #pragma unroll
             for (int c = 0; c < N; ++c) {
-                const float2 y0 = __fmul2_rn(u0, make_float2(size_of(vs[E], c), size_of(vs[E + 1], c))), y1 = __fmul2_rn(u1, make_float2(size_of(vs[E + 2], c), size_of(vs[E + 3], c)));
+                const float2 y0 = __fmul2_rn(w0, make_float2(size_of(vs[E], c), size_of(vs[E + 1], c))), y1 = __fmul2_rn(w1, make_float2(size_of(vs[E + 2], c), size_of(vs[E + 3], c)));
                 uint32_t p0 = pack16(y0.x, y0.y), p1 = pack16(y1.x, y1.y);
                 const uint32_t r0 = rest16(y0, p0, rests), r1 = rest16(y1, p1, rests);
                 if constexpr (TWICE) p0 = r0, p1 = r1;
@@ -390,21 +398,26 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     __syncthreads();
     constexpr int LD = D + 4;
     float *O = reinterpret_cast<float*>(smem), *E = O + WARPS * HEADS * LD;      // [WARPS][HEADS][LD], [WARPS][HEADS][8], over the rings
+    // This warp's share of a head: what its weights are multiplied by for a sum of one over the CTA.  (Averages are what is joined, here and further on: sums of values leave fp32 earlier.)
     auto factor = [&](int head) -> float {
-        float top = part_m[0][head];
+        float top = part_m[0][head], sum = 0.f;
 #pragma unroll
         for (int y = 1; y < WARPS; ++y) top = fmaxf(top, part_m[y][head]);
-        return part_m[w][head] == -INFINITY ? 0.f : ex2(part_m[w][head] - top);
+#pragma unroll
+        for (int y = 0; y < WARPS; ++y) sum += part_l[y][head] == 0.f ? 0.f : part_l[y][head] * ex2(part_m[y][head] - top);
+        return inverse(sum) * (part_m[w][head] == -INFINITY ? 0.f : ex2(part_m[w][head] - top));
     };
-    // (the weights' shift is in l, o and e alike and is taken out here; codes are in units of 2^-24, the odd ones of 2^-20)
-    const float unshift = ex2(-shift), unscale = unshift * two_to(min(24 - wide, 127)), f0 = factor(2 * t) * unscale, f1 = factor(2 * t + 1) * unscale, fg = factor(g) * unshift;
+    // (the weights' shift is in l, o and e alike and is taken out here; codes are in units of 2^-24, the odd ones of 2^-20.  24 - shift - wide is up to 145, for values next to the largest number: two factors)
+    const int back = 24 - (int)shift - wide, some = min(back, 100);
+    const float unshift = ex2(-shift), unscale = two_to(some), more = two_to(back - some), f0 = factor(2 * t), f1 = factor(2 * t + 1), fg = factor(g);
+    auto number = [&](float f, float x) -> float { return f * x * unscale * more; };
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) {
         const int d = i / 2 * 32 + 4 * g + 2 * (i & 1);
-        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t) * LD + d) = make_float2(f0 * o[i][0], f0 * 0.0625f * o[i][2]);
-        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t + 1) * LD + d) = make_float2(f1 * o[i][1], f1 * 0.0625f * o[i][3]);
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t) * LD + d) = make_float2(number(f0, o[i][0]), number(f0 * 0.0625f, o[i][2]));
+        *reinterpret_cast<float2*>(O + (w * HEADS + 2 * t + 1) * LD + d) = make_float2(number(f1, o[i][1]), number(f1 * 0.0625f, o[i][3]));
     }
-    *reinterpret_cast<float2*>(E + (w * HEADS + g) * 8 + 2 * t) = make_float2(fg * (e[0] + e[2]), fg * (e[1] + e[3]));
+    *reinterpret_cast<float2*>(E + (w * HEADS + g) * 8 + 2 * t) = make_float2(fg * (e[0] + e[2]) * unshift, fg * (e[1] + e[3]) * unshift);
     if (threadIdx.x < HEADS) {
         float top = part_m[0][threadIdx.x], sum = 0.f;
 #pragma unroll
@@ -433,10 +446,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         y.x += rest_; y.y += rest_; y.z += rest_; y.w += rest_;
         const long long bh = (long long)b * a.H + h0 + r;
         if (cluster) store4(O + r * LD + d, y);                        // (only this thread reads what lies there)
-        else if (a.splits == 1) {
-            const float inv = inverse(cta_l[r]);
-            *reinterpret_cast<uint2*>((T*)a.out + bh * D + d) = make_uint2(out2<T>(y.x * inv, y.y * inv), out2<T>(y.z * inv, y.w * inv));
-        } else {
+        else if (a.splits == 1) *reinterpret_cast<uint2*>((T*)a.out + bh * D + d) = make_uint2(out2<T>(y.x, y.y), out2<T>(y.z, y.w));
+        else {
             store4(a.part + (bh * a.splits + split) * D + d, y);
             if (d == 0) *reinterpret_cast<float2*>(a.ml + (bh * a.splits + split) * 2) = make_float2(cta_m[r], cta_l[r]);
         }
@@ -453,17 +464,21 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
             ls[c] = c < a.splits ? *cl.map_shared_rank(&cta_l[r], c) : 0.f;
             top = fmaxf(top, ms[c]);
         }
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+            if (ls[c] != 0.f) ls[c] *= ex2(ms[c] - top);
+            sum += ls[c];
+        }
+        const float inv = inverse(sum);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < MAX_CLUSTER; ++c) {
             if (ls[c] == 0.f) continue;
-            const float f = ex2(ms[c] - top);
+            const float f = ls[c] * inv;
             const float4 z = load4(cl.map_shared_rank(O + r * LD + d, c));
-            sum += f * ls[c];
             y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
         }
-        const float inv = inverse(sum);
-        *reinterpret_cast<uint2*>((T*)a.out + ((long long)b * a.H + h0 + r) * D + d) = make_uint2(out2<T>(y.x * inv, y.y * inv), out2<T>(y.z * inv, y.w * inv));
+        *reinterpret_cast<uint2*>((T*)a.out + ((long long)b * a.H + h0 + r) * D + d) = make_uint2(out2<T>(y.x, y.y), out2<T>(y.z, y.w));
     }
     cl.sync();                                                         // the other CTAs have read this one's part
 }
@@ -475,7 +490,6 @@ template <typename T, int N>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) {
     constexpr int D = 32 * N, LANES = N == 3 ? 32 : D / 4, SUB = 32 / LANES;
     __shared__ float4 O[JOIN_WARPS][LANES];
-    __shared__ float L[JOIN_WARPS];
     pdl_wait();
     const int bh = blockIdx.x, b = bh / a.H, w = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LANES * 4;
     const Share sh = share_of(a, b);
@@ -483,41 +497,39 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) int4_join_kernel(StepArgs a) 
     const float* ml = a.ml + (long long)bh * a.splits * 2;
     const float* part = a.part + (long long)bh * a.splits * D + d;
     const bool mine = d < D;
-    float top = -INFINITY;                                             // of all parts, first: then no part waits for the one before it
-    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[2 * s]);
-    top = warp_max(top);
-    float l = 0.f;
+    float seen = -INFINITY, sum = 0.f;                                 // of all parts, first: then no part waits for the one before it
+    for (int s = lane; s < n; s += 32) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
+        const float high = fmaxf(seen, x.x);
+        sum = (sum == 0.f ? 0.f : sum * ex2(seen - high)) + (x.y == 0.f ? 0.f : x.y * ex2(x.x - high));
+        seen = high;
+    }
+    const float top = warp_max(seen), inv = inverse(warp_sum(sum == 0.f ? 0.f : sum * ex2(seen - top)));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int s = w * SUB + lane / LANES; s < n; s += JOIN_WARPS * SUB) {
         const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
         const float4 y = mine ? load4(part + (long long)s * D) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
-        l += x.y * f;
+        const float f = x.y == 0.f ? 0.f : x.y * ex2(x.x - top) * inv;
         o.x += y.x * f; o.y += y.y * f; o.z += y.z * f; o.w += y.w * f;
     }
 #pragma unroll
     for (int x = LANES; x < 32; x <<= 1) {
-        l += __shfl_xor_sync(0xffffffffu, l, x);
         o.x += __shfl_xor_sync(0xffffffffu, o.x, x);
         o.y += __shfl_xor_sync(0xffffffffu, o.y, x);
         o.z += __shfl_xor_sync(0xffffffffu, o.z, x);
         o.w += __shfl_xor_sync(0xffffffffu, o.w, x);
     }
     if (lane < LANES) O[w][lane] = o;
-    if (lane == 0) L[w] = l;
     __syncthreads();
     if (w > 0 || lane >= LANES) return;
-    float sum = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < JOIN_WARPS; ++x) {
         const float4 y = O[x][lane];
-        sum += L[x];
         o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
-    const float inv = inverse(sum);
-    if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * D + d) = make_uint2(out2<T>(o.x * inv, o.y * inv), out2<T>(o.z * inv, o.w * inv));
+    if (mine) *reinterpret_cast<uint2*>((T*)a.out + (long long)bh * D + d) = make_uint2(out2<T>(o.x, o.y), out2<T>(o.z, o.w));
 }
 
 template <typename T, int N, bool TWICE>

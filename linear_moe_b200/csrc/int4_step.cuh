@@ -9,7 +9,7 @@ struct StepArgs {
     const void* q;                        // [B, H, D]
     const unsigned char *k, *v;           // [pages, G, page bytes] twice
     void* out;                            // [B, H, D]
-    float *part, *ml;                     // [B, H, splits, D], [B, H, splits, 2]: (maximum in units of log 2, sum); more parts than a cluster joins
+    float *part, *ml;                     // [B, H, splits, D], averages, and [B, H, splits, 2]: (maximum in units of log 2, sum); more parts than a cluster joins
     const float* slopes;                  // [H] or null
     const int *table, *lengths;           // [B, table_n], [B]
     long long q_b, q_h, table_ld;

@@ -500,3 +500,35 @@ def test_values_of_negative_zeros(H, G, D, dtype):
     for k, v in ((s["k"], s["v"]), pools):
         check(dict(s, k=k, v=v))
         check(dict(s, k=k, v=v), window=20)
+
+
+@gpu
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (8, 1, 64), (6, 2, 96), (2, 1, 32)])
+@pytest.mark.parametrize("size", [1e35, 1e30, 1e-30, 1e-35])
+def test_values_far_from_one(size, H, G, D):
+    """Values whose sizes are powers of two from -118 to 118: scaled for the products and back without leaving 32 bits, also where the largest score so far lags behind (scores of up to 5).  Sums below 2^-126 are zeros: of a
+    warp's rounded, rest and low sums, four warps, up to eight parts, before the division by a sum of weights of one at least, and of the output: 97 times 2^-126 at most."""
+    floor = 97 * 2.0 ** -126
+
+    def check(s, **kw):
+        got = attend(s, **kw).double()
+        want, room = formula(s, **kw)
+        assert got.isfinite().all() and ((got - want).abs() <= 2.0 ** -8 * (want.abs() + room) + room + floor).all()
+        gemm.check_error()
+    for lens, scores in (([300, 20, 1], 1.5), ([200, 33], 4.0)):
+        s = make(lens, H, G, D, size=scores)
+        s["v"] = make(lens, H, G, D, values=lambda gen, n, G, D: torch.randn(n, G, D, generator=gen) * size)["v"]      # (the same pages)
+        check(s)
+        check(s, cap=3.0, window=70)
+    # sizes that grow and shrink by many powers of two on the way
+    s["v"] = make(lens, H, G, D, values=lambda gen, n, G, D: torch.randn(n, G, D, generator=gen) * size * 2.0 ** torch.randint(-20, 3, (n, 1, 1), generator=gen))["v"]
+    check(s)
+
+
+@gpu
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (8, 1, 64)])
+def test_values_near_the_largest_number(H, G, D):
+    """One or two keys' values of up to 1.6 10^38, whose sum 32 bits still hold."""
+    s = make([1, 2, 2], H, G, D)
+    s["v"] = make([1, 2, 2], H, G, D, values=lambda gen, n, G, D: torch.rand(n, G, D, generator=gen) * 3.2e38 - 1.6e38)["v"]
+    check(s)
