@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     uint32_t qa[N][4], sums[3] = {0, 0, 0};
     const bool there = gh < nh;
     const float slope = there && a.slopes != nullptr ? a.slopes[h0 + gh] * LOG2E : 0.f;
-    float unit_q;                                                      // of the scores
+    float unit_q, more_q;                                              // of the scores: up to 2^137, for queries next to the largest number, in two factors
     {
         float q[N][8], most = 0.f;
 #pragma unroll
@@ -217,20 +217,21 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int top = most > 0.f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 116) : 0;      // up to 2^15, the odd codes' numbers up to 2^11
+        const int top = most > 0.f ? max((int)(__float_as_uint(fminf(most, 3.402823466e38f)) >> 23) - 127, -100) : 0;      // up to 2^15, the odd codes' numbers up to 2^11
         const float scale = two_to(14 - top);
-        unit_q = two_to(10 + top);
-        const float back = two_to(-10 - top);
+        unit_q = two_to(10 + min(top, 100));
+        more_q = two_to(max(top - 100, 0));
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 qa[c][i] = pack16(q[c][i] * (i & 1 ? scale * 0.0625f : scale), q[c][i + 4] * (i & 1 ? scale * 0.0625f : scale));
-                sum += q[c][i] * back + q[c][i + 4] * back;
+                sum += q[c][i] * scale + q[c][i + 4] * scale;
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= two_to(-24);                                        // as the codes'
             if (c / 2 == t) {
 #pragma unroll
                 for (int y = 0; y < 3; ++y) {
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
     const uint32_t part = (w >> 1) * PART, codes_at = part + (w & 1) * 2 * GROUP * (D / 2), scales_at = part + (w & 1) * 2 * GROUP * (D / 8);
     const uint32_t at_k = codes_at + g * (D / 2) + place(N, g, 0) * 16 + 4 * t, at_v = codes_at + 2 * t * (D / 2) + place(N, 2 * t, 0) * 16 + 2 * g, at_s = scales_at + g * (D / 8), at_ks = at_s + 4 * t, at_v2 = scales_at + 2 * t * (D / 8), at_vs = at_v2 + 2 * g;
     auto chunk = [](uint32_t a, int c) -> uint32_t { return N == 2 || N == 4 ? a ^ (16u * c) : a + 16u * c; };
+    const bool far = __any_sync(0xffffffffu, more_q != 1.f);
     const float rests = TWICE && g < 4 ? 0.f : -1.f;
     bool alive = true;
     int j = 0;
@@ -306,6 +308,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) int4_step_kernel(const StepA
         };
         scores(std::integral_constant<int, 0>());
         scores(std::integral_constant<int, 1>());
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * more_q);
+        }
         if (a.cap > 0.f) fatc::tanh_of(v, pre);
         float x[8];
 #pragma unroll

@@ -532,3 +532,20 @@ def test_values_near_the_largest_number(H, G, D):
     s = make([1, 2, 2], H, G, D)
     s["v"] = make([1, 2, 2], H, G, D, values=lambda gen, n, G, D: torch.rand(n, G, D, generator=gen) * 3.2e38 - 1.6e38)["v"]
     check(s)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (8, 1, 64), (6, 2, 96)])
+@pytest.mark.parametrize("power", [110, 117, 120, 125, -90, -110])
+def test_queries_far_from_one(power, H, G, D, dtype):
+    """Queries of 2^110 to 2^127 and of 2^-90 to 2^-112 with keys that bring the scores back to a few: the same bounds, which grow with scale, query and key alike."""
+    keys = -power // 2
+    for lens in ([300, 20, 1], [200, 33]):
+        s = make(lens, H, G, D, dtype=dtype)
+        s["k"] = make(lens, H, G, D, values=lambda gen, n, G, D: torch.randn(n, G, D, generator=gen) * 2.0 ** keys)["k"]      # (the same pages)
+        s["q"] = (s["q"].double().clamp(-3.9, 3.9) * 2.0 ** power).to(dtype)
+        scale = D ** -0.5 * 2.0 ** (-power - keys)
+        check(s, scale=scale)
+        check(s, scale=scale, cap=3.0, window=70)
+        check(s, scale=scale, slopes=ops.alibi_slopes(H).cuda())
