@@ -149,7 +149,7 @@ class SelfAttention(nn.Module):
         # position_offset is the absolute position of this call's first token (the cache length when decoding)
         pos0 = position_offset + (cp.rank * T if not cp.is_trivial else 0)
         paged = cache is not None and "table" in cache
-        if self.rope is not None and rotary is not None and rotary[0].shape[0] != B * T:
+        if self.rope is not None and rotary is not None and not (paged and T == 1) and rotary[0].shape[0] != B * T:
             raise ValueError(f"{rotary[0].shape[0]} positions for {B} x {T} tokens")
         if cfg.fused_qkv_heads:
             q, k, v = self._heads(qkv, cache if paged else None, pos0, rotary)

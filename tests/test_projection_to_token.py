@@ -225,3 +225,24 @@ def test_requests_with_top_k_and_top_p():
                     want = G.generate_and_post_process(m, tok, body["prompts"], 6, top_k_sampling=8, top_p_sampling=0.8, temperature=2.0, random_seed=3, fused_sampling=fused, **extra)
                 assert got.status_code == 200 and got.json()["tokens"] == want[1]
             assert c.put("/api", json={**body, "min_p": "x"}).status_code == 400
+
+
+@pytest.mark.parametrize("one_pass", [False, True])
+def test_single_tokens_from_pages_take_their_own_positions(one_pass):
+    """A layer's step over pages turns by the pages' lengths, whatever tables come along; elsewhere these have a row for every token."""
+    m = model(num_layers=1, fused_qkv_heads=one_pass)
+    att = m.decoder.layers[0]._mixer()
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 12, 128, generator=gen)
+    tables = att.rope.get(5, 0, x.device)
+    with torch.no_grad():
+        out = []
+        for rotary in (None, tables):
+            cache = PagedCache(m, 2, 40)
+            cache.advance(11)
+            att(x[:, :11], cache=cache[0])
+            cache.advance(1)
+            out.append(att(x[:, 11:], cache=cache[0], position_offset=11, rotary=rotary))
+        assert torch.equal(*out)
+        with pytest.raises(ValueError, match="positions for"):
+            att(x, rotary=tables)
