@@ -113,7 +113,7 @@ struct Shared {
     uint32_t at_count, total_count;
     u64 at_mass, total_mass;
     uint32_t tied;                                     // of the chosen warp: tokens on the edge, and weight, ahead of it
-    u64 ahead, whole, goal;
+    u64 ahead;
 };
 
 __device__ __forceinline__ u64 up_to(u64 v) {          // inclusive over the lanes
