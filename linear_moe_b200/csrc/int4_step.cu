@@ -10,15 +10,16 @@
 // second ones are one small product each of bf16 numbers, whose other operand is the row's lows as they lie in the cache; Q in three parts, p in two.
 // Queries go in scaled by a power of two per head, which fp16 holds exactly but for what is below 2^-35 of the head's largest number.  p size goes in as two fp16 numbers, what it is rounded to and the rest of it, together
 // 22 bits: where a key head has up to four query heads the columns 4 to 7 of the products, which would be empty, take the heads 0 to 3 once more with the rests, otherwise there are second products.  (The
-// rounded one alone, 11 bits, put one bf16 output in seven on the wrong neighbour of the 64-bit value; 64 requests of up to 8192 keys, replayed: 113 us without the rests, 117 with them.)  A power of two per warp keeps p size at 2^15 at most, where p is 1 and size the largest one seen at 2^7
-// (fp16 tells 2^-24 apart there).
+// rounded one alone, 11 bits, put one bf16 output in seven on the wrong neighbour of the 64-bit value.  64 requests of up to 8192 keys, four heads a key head: 106 us without the rests, 111 with them; eight: 106 and 117.  In three bf16 parts instead of two, p beside
+// the lows changed nothing that could be measured: scores are off by more, 2^-23 of their products' largest part a step of 16.)  A power of two per warp keeps p size at 2^15 at most, where p is 1 and size the largest
+// one seen at 2^7 (fp16 tells 2^-24 apart there).
 //
 // A CTA of four warps takes one key head, up to 8 of its query heads and a range of keys, 128 at a time: a stage of a ring of two, of which a warp reads 32 keys.  The warps take turns in filling the stages by bulk
 // copies, a lane per copy (64 rows of a page lie together: eight copies a stage; pages of other sizes: 32).  Maxima lag by up to 2^8: unless a score runs ahead of that, nothing is exchanged between lanes and nothing rescaled.
 //
-// 64 requests of up to 8192 keys, 32 over 8 heads of 128, capped (390 MB, 59 us at the copy rate): 107 us.  Issue slots are what it runs out of: 390 instructions for 16 keys, half of them on the ALU pipe, with 16 warps
-// per SM.  What took it there: heads as the rows of the score products, codes as 128 + code in bf16 and their sums taken out again 185; keys as the rows, addresses of 32 bits 152; two groups of 16 keys at a time 137; codes
-// as small fp16 numbers 129; rings of the CTA instead of the warps' own (fewer, larger copies) 121; four CTAs per SM with two stages instead of three with three 113.  Two of up to 100001 keys, 16 over 2 heads of 64: 23 us.
+// 64 requests of up to 8192 keys, 32 over 8 heads of 128, capped (390 MB, 59 us at the copy rate): 111 us.  Issue slots are what it runs out of (60 % at 16 warps per SM): 453 instructions of a warp for 16 keys, the CTAs' starts and ends among
+// them, half of them on the ALU pipe.  What took it there (with 11 bits of p size, 106 in the end): heads as the rows of the score products, codes as 128 + code in bf16 and their sums taken out again 185; keys as the rows, addresses of 32 bits 152; two groups of 16 keys at a time 137; codes
+// as small fp16 numbers 129; rings of the CTA instead of the warps' own (fewer, larger copies) 121; four CTAs per SM with two stages instead of three with three 113.  Two of up to 100001 keys, 16 over 2 heads of 64: 21 us.
 // (Keys and values in five places of their own, more of them on their way: 123, for a second wait in every stage.)
 // Rows of a group that are hidden (behind the last key, in front of the window, on a page that is none) are masked, and their values' scales set to zero in the ring, so that nothing stale meets a weight of zero.
 // A NaN score raises no maximum, so what has seen nothing is told by its sum of zero, not by its maximum: a head that sees NaN gives NaN.

@@ -5,9 +5,9 @@
 //
 // Bound by reading the projection once and writing the heads once (backward: the heads' gradients and the normed part of the projection once, its gradient once); the norm's factor is computed again
 // instead of being kept.  32-bit arithmetic, one rounding per number; compiled without approximate functions.
-// 16384 tokens, 32 over 8 heads of 128, bf16: forward 402 MB in 74 us (5.4 TB/s), backward 571 MB in 129 us (4.4 TB/s) and 6 us for the sums of the weights' gradients.  A warp per head with a number every 32nd lane
+// 16384 tokens, 32 over 8 heads of 128, bf16: forward 402 MB in 74 us (5.4 TB/s), backward 571 MB in 130 us (4.4 TB/s) and 7 us for the sums of the weights' gradients.  A warp per head with a number every 32nd lane
 // took 1279 us for both; 16 bytes a thread, blocks of queries, keys and values 365; the next head's numbers loaded ahead, index divisions as products, arithmetic two numbers at a time 209.
-// Two heads ahead, with the norms' weights in shared memory to make room for them, took 276: the forward pass spills at its 64 registers, the backward pass goes from 129 to 144.
+// Two heads ahead, with the norms' weights in shared memory to make room for them, took 276: the forward pass spills at its 64 registers, the backward pass goes from 130 to 144.
 #include <cuda_fp16.h>
 
 #include "common.cuh"

@@ -9,8 +9,9 @@
 // for a factor of two) with the number and the weight of each bin's tokens tells the bin in which the cut lies; histograms over the numbers inside of it tell the logit, and the equal ones are counted
 // by their numbers.  Last, the kept weights are summed up per thread, and a scan finds the thread, and the token, that the random number falls to.
 //
-// One row of 32000 logits 16 us, 17 rows of 50257 with settings of their own 24, 128 rows of 128256 in fp32 with top-p 165 (the logits alone take 10 at the copy rate): what it spends its time on is some 60 instructions
-// around each exponential, once for the histogram and once for what is kept, and the cluster's barriers (about 1 us each, five or six of them).  The first form, a CTA per 65536 logits with branches around its
+// One row of 32000 logits 16 us, 17 rows of 50257 with settings of their own 24, 128 rows of 128256 in fp32 with top-p 165 (the logits alone take 10 at the copy rate).  Of the 60000
+// cycles of such a row's CTAs (four waves of two per SM) 8000 to 13000 are the loads, 9000 the exponentials of the histogram (some 60 instructions each), 6000 its atomics, 2000 what is kept (without a cut, where all of it is: 10000), and
+// about half are barriers of the cluster, five or six of them with what lies between, and the searches over bins.  The first form, a CTA per 65536 logits with branches around its
 // exponentials, took 68, 96 and 273.  CTAs of 768 threads, which leaves 40 registers and spills, take 22, 31 and 182 where 512 threads take 18, 27 and 162 (replayed from a graph).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>

@@ -172,9 +172,9 @@ HEADS, MAX_CLUSTER, MIN_GROUPS = 8, 8, 8                  # csrc/int4_step.cu, .
 def splits_of(B: int, G: int, heads: int, D: int, keys: int) -> Tuple[int, int]:
     """(CTAs that share a key head of a request of up to ``keys`` keys, are the longest requests to come first).
 
-    One wave: as many parts as give every slot of the GPU a CTA, of 128 keys at least (300 keys in three parts 8.5 us, in one 10.5, replayed).  Two of up to 100001 keys, 2 heads of 64: 69 us in 16 parts, 41 in 32, 25 in
-    111, 23 in 148.  Requests that fill more than half of the slots by themselves, but not four waves, go in two parts each, the longest ones first (64 of up to 8192 keys, 8 heads of 128: 131 us, in one part each 156, in four 139; in
-    two unsorted 137)."""
+    One wave: as many parts as give every slot of the GPU a CTA, of 128 keys at least (300 keys in three parts 8.3 us, in one 10.3, replayed).  Two of up to 100001 keys, 2 heads of 64: 77 us in 16 parts, 43 in 32, 25 in
+    111, 23 in 148.  Requests that fill more than half of the slots by themselves, but not four waves, go in two parts each, the longest ones first (64 of up to 8192 keys, 8 heads of 128: 113 us, in one part each 156, in four 130; in
+    two unsorted 144).  The host knows how many pages a request's table has, not how long the request is: a short one with a wide table has parts without keys, and a second launch where there are more than eight."""
     from . import cuda as K
     work, slots = max(1, B * G * -(-heads // HEADS)), 4 * K.num_sms()
     n = slots // work if 2 * work <= slots else 2 if work < 4 * slots else 1
@@ -207,7 +207,11 @@ def _step_plan(q, k_pages, v_pages, table, lengths, scale, window, softcap, slop
 
 def paged_attention_int4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: Optional[int] = None, *,
                          softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``[B, H, D]``: ``ops.paged_attention`` over pools of 4 bits a number, into which the new token's row has been stored (:func:`store_rows_int4`).  Forward only."""
+    """``[B, H, D]``: ``ops.paged_attention`` over pools of 4 bits a number, into which the new token's row has been stored (:func:`store_rows_int4`).  Forward only.
+
+    On CUDA 16-bit queries of up to 128 numbers a head run on the tensor cores: sums in 32 bits, weights times the sizes of values to 22 bits and times their lows to 16 (the error against 64 bits is that of 32-bit
+    arithmetic and one rounding), queries but for what is below 2^-35 of a head's largest number.  Others are computed in 32 bits throughout by a simpler kernel (64 requests of up to 8192 keys, 32 over 8 heads of 128:
+    111 us and, with queries in fp32, 4990)."""
     if torch.is_grad_enabled() and q.requires_grad:
         raise ValueError("one-token attention has no backward pass: use ops.softmax_attention")
     if not q.is_cuda:

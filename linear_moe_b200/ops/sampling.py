@@ -80,8 +80,9 @@ def _sums(w):
 
 
 def _shares(V: int) -> Tuple[int, int]:
-    """(CTAs of a row, logits of each): as many as a cluster has, of 2048 logits at least (one row of 32000: 43 us in one part, 31 in two, 23 in four, 18 in eight; 128 rows of 128256 in fp32, top-p: 197 in two,
-    201 in four, 162 in eight; in bf16 with the 50 largest 133, 107, 125)."""
+    """(CTAs of a row, logits of each): as many as a cluster has, of 2048 logits at least (one row of 32000: 38 us in one part, 26 in two, 18 in four, 15 in eight; 128 rows of 128256 in fp32, top-p: 181 in two,
+    175 in four, 149 in eight; nothing cut off: 90, 98, 86; 20 calls in a graph).  Full batches with a top-k alone would do better in four (bf16, the 50 largest: 121, 101, 119): the rule does not look at the settings, which may
+    lie on the device."""
     parts = 1
     while parts < 8 and parts * 2048 < V:
         parts *= 2
